@@ -17,7 +17,8 @@
  *  - A context owns every device allocation (bins, gradients, quantized gradients,
  *    row permutation buffers, histogram slots, tree buffers).  A context is not
  *    thread-safe (the reference backend is `!Sync`, lib.rs:3840-3846); all calls
- *    on one context are synchronous at the API boundary.
+ *    on one context are synchronous at the API boundary, but for the entries that
+ *    take a stream when they are given one.
  *  - Histogram cells use the reference layout: feature f occupies
  *    [slot_off[f], slot_off[f] + 2*num_bin[f]) of a leaf slot, grad at 2*bin,
  *    hess at 2*bin+1 (crates/lgbm-compute/src/kernels/histogram.rs:64-68,
@@ -709,6 +710,134 @@ int lgbm_hip_predict_early_stop(lgbm_hip_ctx* ctx, const lgbm_hip_model* model, 
                                 int64_t num_rows, int32_t num_cols, int32_t start_iteration,
                                 int32_t num_iteration, int32_t freq, double margin, double* out,
                                 int32_t* iterations);
+
+/* ---- the operators around a forest's leaves ---------------------------------------- */
+
+/* A tree sends every row to a leaf (LGBM_HIP_PREDICT_LEAF), and a leaf may hold a linear
+ * map of its own: one output for the linear leaves of a linear tree, several for experts.
+ * These entries group the rows by leaf, apply the maps, give their gradients, drop
+ * elements or rows at random, and turn class scores into answers.  None has a counterpart
+ * in the reference, which fits linear leaves on the host and has no device path for them.
+ *
+ * All pointers marked d_ are memory of the context's device.  `stream` points to a stream
+ * handle (hipStream_t; the handle 0 is the device's default stream) of the HIP runtime
+ * that this library uses: the work is queued there and the call returns at once, so calls
+ * on one stream follow each other and can be recorded into a graph.  stream NULL: the
+ * context's own stream, and the call returns when the outputs are written; the inputs
+ * have to be complete before the call.  Nothing is allocated: working memory is the
+ * caller's (d_ws, 16-byte aligned, of the size that the _workspace entry gives; unused
+ * after the work is done, and not shared by calls that may run at the same time).
+ * Outputs must not overlap inputs unless an entry says so.  Matrices are row-major with a
+ * row stride in elements (at least the columns); any alignment of the element type.  The
+ * caller's current device is the same after a call.  Results depend neither on the order
+ * in which blocks run nor on the device's number of CUs. */
+#define LGBM_HIP_DTYPE_BF16 2
+#define LGBM_HIP_DTYPE_F16 3
+#define LGBM_HIP_MAX_GROUP_LEAVES 4095 /* of one tree, for lgbm_hip_leaf_groups */
+#define LGBM_HIP_MAX_GROUP_TREES 65535
+
+/* The rows of every leaf from the leaf of every row.  d_leaf: int32 [num_rows][num_trees]
+ * with row stride ld (what LGBM_HIP_PREDICT_LEAF writes); an index outside
+ * [0, num_leaves) means that the row is in no leaf of that tree.  d_order: int32
+ * [num_trees][num_rows], the rows of a tree by leaf, ascending within a leaf, rows in no
+ * leaf last; d_begin, d_count: int32 [num_trees][num_leaves], each leaf's range of its
+ * tree's part of d_order.  A grown tree's layout (lgbm_layout_out: indices, leaf_begin,
+ * leaf_count) has the same form, with one tree. */
+int lgbm_hip_leaf_groups_workspace(int64_t num_rows, int32_t num_trees, int32_t num_leaves,
+                                   size_t* bytes);
+int lgbm_hip_leaf_groups(lgbm_hip_ctx* ctx, const int32_t* d_leaf, int64_t ld, int64_t num_rows,
+                         int32_t num_trees, int32_t num_leaves, int32_t* d_order, int32_t* d_begin,
+                         int32_t* d_count, void* d_ws, size_t ws_bytes, void* const* stream);
+
+/* Grouped rows and the shape of the leaves' maps.  A tree's leaves have to stand in its
+ * part of d_order without overlap, in any order, in front of the rows in no leaf, and a
+ * row may stand there once a tree.  Entries outside [0, num_rows) are passed over and
+ * ranges are held within the order, so a wrong table gives wrong values but reaches no
+ * other memory. */
+typedef struct lgbm_leaf_maps {
+  const int32_t* d_order; /* [num_trees][num_rows] */
+  const int32_t* d_begin; /* [num_trees][num_leaves] */
+  const int32_t* d_count;
+  int64_t num_rows;
+  int32_t num_trees;
+  int32_t num_leaves;
+  int32_t inputs;
+  int32_t outputs;
+  int32_t dtype; /* LGBM_HIP_DTYPE_F32, _BF16 or _F16: x, w, bias, y, dy and dx */
+  int32_t _pad;
+} lgbm_leaf_maps;
+
+#define LGBM_HIP_LEAF_PRODUCT 0
+#define LGBM_HIP_LEAF_PRODUCT_DX 1
+#define LGBM_HIP_LEAF_PRODUCT_DW 2
+int lgbm_hip_leaf_product_workspace(const lgbm_leaf_maps* maps, int32_t what, size_t* bytes);
+/* y[n] = sum over trees t of w[t][leaf] x[n] + bias[t][leaf], in float32 and rounded
+ * once.  d_x [num_rows][inputs], d_w [num_trees * num_leaves][outputs][inputs], d_bias
+ * [num_trees * num_leaves][outputs] or NULL, d_y [num_rows][outputs]; w and bias
+ * contiguous.  A tree that has a row in no leaf adds nothing to it. */
+int lgbm_hip_leaf_product(lgbm_hip_ctx* ctx, const lgbm_leaf_maps* maps, const void* d_x, int64_t ldx,
+                          const void* d_w, const void* d_bias, void* d_y, int64_t ldy, void* d_ws,
+                          size_t ws_bytes, void* const* stream);
+/* dx[n] = sum over trees of w[t][leaf]^T dy[n]. */
+int lgbm_hip_leaf_product_dx(lgbm_hip_ctx* ctx, const lgbm_leaf_maps* maps, const void* d_dy,
+                             int64_t lddy, const void* d_w, void* d_dx, int64_t lddx, void* d_ws,
+                             size_t ws_bytes, void* const* stream);
+/* dw[leaf] = sum over the leaf's rows of dy[n] x[n]^T, db[leaf] = the sum of dy[n], in
+ * float32 whatever the type of x and dy; zeros for a leaf without rows.  d_db may be
+ * NULL.  With dy = [h x | -g] these are the normal equations of linear leaves. */
+int lgbm_hip_leaf_product_dw(lgbm_hip_ctx* ctx, const lgbm_leaf_maps* maps, const void* d_dy,
+                             int64_t lddy, const void* d_x, int64_t ldx, float* d_dw, float* d_db,
+                             void* d_ws, size_t ws_bytes, void* const* stream);
+
+/* out = x with units dropped (0, whatever x holds there) with probability p and the
+ * others divided by the share kept.  A unit is an element, numbered row by row, or with
+ * by_row a whole row (bagging of [g, h] pairs).  Unit e is kept where 16-bit field e % 8
+ * (low half first) of Philox4x32-10's block for counter (e / 8, offset) and key seed is at
+ * least t = round(65536 p); the share kept is 1 - t / 65536.  The mask is nowhere stored:
+ * the gradient is the same call on the outputs' gradient.  dtype as in lgbm_leaf_maps;
+ * d_out may be d_x with the same stride. */
+int lgbm_hip_dropout(lgbm_hip_ctx* ctx, const void* d_x, int64_t ldx, int64_t num_rows,
+                     int64_t num_cols, int32_t dtype, double p, uint64_t seed, uint64_t offset,
+                     int32_t by_row, void* d_out, int64_t ldo, void* const* stream);
+
+/* Class scores to answers.  With c the number of times class j stands in row n's history:
+ *   s = x[n][j];  c > 0: s = (s > 0 ? s / repetition : s * repetition)
+ *                            - frequency * c - presence;
+ *   s += bias[j];  s = -inf where bit j of the row's mask is 0
+ * and out is s (LGBM_HIP_PREDICT_RAW) or the softmax of s over the row
+ * (LGBM_HIP_PREDICT_TRANSFORMED).  A class with s = -inf has probability 0, also in a row
+ * where that is every class; a masked score is never looked at (NaN and infinities
+ * included), while a NaN or +inf that is not masked makes the row's other probabilities
+ * NaN.  Arithmetic is float64 for float64 scores, else float32, rounded once. */
+typedef struct lgbm_score_args {
+  const void* d_x; /* [num_rows][num_classes], row stride ldx */
+  int64_t ldx;
+  int64_t num_rows;
+  int32_t num_classes;
+  int32_t dtype; /* LGBM_HIP_DTYPE_F32, _F64, _BF16 or _F16: x, bias and out */
+  int32_t kind;  /* LGBM_HIP_PREDICT_RAW or _TRANSFORMED */
+  int32_t num_masks;
+  const void* d_bias;         /* [num_classes] or NULL */
+  const uint32_t* d_mask;     /* [num_masks][ceil(num_classes / 32)], bit j % 32 of word
+                                 j / 32: class j may be answered; or NULL */
+  const int32_t* d_mask_rows; /* [num_rows] the mask of every row, outside [0, num_masks):
+                                 no mask; NULL: one mask for all rows or one for each */
+  const int32_t* d_ids;       /* the rows' histories, or NULL; classes outside
+                                 [0, num_classes) are passed over */
+  const int64_t* d_offsets;   /* [num_rows + 1]: row n's history is ids[offsets[n] ..
+                                 offsets[n + 1]) */
+  int64_t num_ids;
+  double repetition; /* > 0; 1: none */
+  double frequency;
+  double presence;
+  const float* d_penalties; /* [num_rows][3] (repetition, frequency, presence) instead of
+                               the three above, or NULL */
+  void* d_out;              /* may be d_x with the same stride */
+  int64_t ldo;
+} lgbm_score_args;
+int lgbm_hip_adjust_scores_workspace(const lgbm_score_args* args, size_t* bytes);
+int lgbm_hip_adjust_scores(lgbm_hip_ctx* ctx, const lgbm_score_args* args, void* d_ws,
+                           size_t ws_bytes, void* const* stream);
 
 /* ---- measurement ------------------------------------------------------------ */
 

@@ -7,3 +7,4 @@ from ._abi import FeatureMeta, GainConfig, SplitInfo, BatchedFeature  # noqa: F4
 from .backend import (HipBackend, HipError, Model, binary_boost_from_score, boost_from_score,  # noqa: F401,E501
                       feature_meta, load_library)
 from .binning import BinMapper, feature_mappers, sample_indices  # noqa: F401
+from .leaves import LeafGroups  # noqa: F401

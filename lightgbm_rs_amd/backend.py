@@ -49,6 +49,7 @@ class HipBackend:
     def __init__(self, device=0):
         self.lib = load_library()
         self.ctx = C.c_void_p()
+        self.device = device
         rc = self.lib.lgbm_hip_ctx_create(C.c_int(device), C.byref(self.ctx))
         if rc != 0:
             raise HipError(rc, self._err(None))
@@ -85,6 +86,11 @@ class HipBackend:
     def _check(self, rc):
         if rc != 0:
             raise HipError(rc, self._err(self.ctx))
+
+    def _check_plain(self, rc):
+        """The status of an entry without a context."""
+        if rc != 0:
+            raise HipError(rc, self._err(None))
 
     def close(self):
         if self.ctx:

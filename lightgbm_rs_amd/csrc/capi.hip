@@ -18,6 +18,7 @@
 
 #include "kernels.h"
 #include "binning.h"
+#include "context.h"
 #include "model.h"
 
 using namespace lgbm;
@@ -351,6 +352,19 @@ int set_err(lgbm_hip_ctx* c, int code, const std::string& m) {
     g_create_err = m;
   return code;
 }
+
+}  // namespace
+
+// What the entries of leaf_capi.hip need of a context.
+namespace lgbm {
+int context_device(const lgbm_hip_ctx* c) { return c->device; }
+hipStream_t context_stream(const lgbm_hip_ctx* c) { return c->stream; }
+int context_error(lgbm_hip_ctx* c, int code, const std::string& message) {
+  return set_err(c, code, message);
+}
+}  // namespace lgbm
+
+namespace {
 
 #define HIPCHK(c, expr)                                                                   \
   do {                                                                                    \

@@ -1,0 +1,146 @@
+"""The operators around a forest's leaves on the GPU: rows by leaf, leaf products and their
+gradients, dropout, class scores, alone and together, on streams and in graphs.  The checks
+are in leaf_ops_checks.py; they run in one child process, which imports torch first."""
+import json
+import os
+import select
+import subprocess
+import sys
+
+import pytest
+
+pytestmark = pytest.mark.gpu
+HERE = os.path.dirname(os.path.abspath(__file__))
+
+
+class Worker:
+    def __init__(self):
+        self.log = []
+        self.p = subprocess.Popen([sys.executable, "-u", os.path.join(HERE, "leaf_ops_worker.py")],
+                                  stdin=subprocess.PIPE, stdout=subprocess.PIPE, text=True)
+        self.answer()
+
+    def answer(self):
+        ready, _, _ = select.select([self.p.stdout], [], [], 110)
+        line = self.p.stdout.readline() if ready else ""
+        if not line:
+            self.p.kill()
+            raise AssertionError("the worker ended" if ready else "the worker gave no answer")
+        return json.loads(line)["error"]
+
+    def __call__(self, name, **args):
+        if self.p.poll() is not None:
+            pytest.fail("the worker ended in an earlier test")
+        self.p.stdin.write(json.dumps({"name": name, "args": args}) + "\n")
+        self.p.stdin.flush()
+        error = self.answer()
+        assert error is None, error
+
+    def close(self):
+        self.p.stdin.close()
+        try:
+            self.p.wait(60)
+        except subprocess.TimeoutExpired:
+            self.p.kill()
+
+
+@pytest.fixture(scope="module")
+def check():
+    w = Worker()
+    yield w
+    w.close()
+
+
+@pytest.mark.parametrize("rows,trees,leaves,shape,pad", [
+    (1, 1, 1, "even", 0), (1, 3, 4095, "one", 0), (63, 1, 2, "even", 0), (64, 100, 31, "even", 0),
+    (65, 7, 31, "lost", 2), (4096, 1, 255, "skew", 0), (4097, 2, 256, "even", 0),
+    (20011, 3, 63, "lost", 1), (100003, 1, 1000, "even", 0), (30000, 1, 4095, "skew", 0),
+    (50000, 1, 1, "lost", 0), (3000, 300, 15, "even", 0), (300007, 2, 31, "one", 0),
+    (1025, 65, 127, "lost", 3)])
+def test_groups(check, rows, trees, leaves, shape, pad):
+    check("groups", rows=rows, trees=trees, leaves=leaves, shape=shape, pad=pad)
+
+
+# one row and one input; outputs and inputs around 16, 32, 64, 128 and 256; rows of a leaf
+# from one to hundreds; several trees; odd strides and addresses
+SHAPES = [
+    (1, 1, 1, 1, 1, "one", 0), (5, 3, 2, 1, 3, "even", 1), (64, 28, 1, 20, 31, "even", 0),
+    (17, 16, 16, 1, 1, "one", 0), (100, 33, 17, 2, 7, "lost", 3), (257, 64, 64, 1, 4, "skew", 8),
+    (300, 100, 10, 1, 31, "even", 0), (129, 128, 130, 1, 2, "even", 8), (500, 200, 96, 3, 5, "lost", 0),
+    (16, 520, 300, 1, 31, "even", 0), (3, 1000, 260, 2, 3, "even", 0), (1000, 70, 257, 1, 3, "skew", 1),
+    (700, 256, 256, 1, 2, "one", 0), (2000, 13, 3, 5, 63, "skew", 0), (40, 2000, 1, 1, 7, "even", 0),
+    (333, 65, 8, 1, 1, "lost", 2), (900, 129, 33, 2, 15, "even", 8), (2500, 40, 10, 1, 2, "one", 0)]
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16", "f16"])
+@pytest.mark.parametrize("rows,inputs,outputs,trees,leaves,shape,pad", SHAPES)
+def test_product(check, rows, inputs, outputs, trees, leaves, shape, pad, dtype):
+    check("product", rows=rows, inputs=inputs, outputs=outputs, trees=trees, leaves=leaves,
+          shape=shape, pad=pad, dtype=dtype, bias=rows % 2 == 0)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16", "f16"])
+@pytest.mark.parametrize("rows,inputs,outputs,trees,leaves,shape,pad", SHAPES)
+def test_gradients(check, rows, inputs, outputs, trees, leaves, shape, pad, dtype):
+    check("grads", rows=rows, inputs=inputs, outputs=outputs, trees=trees, leaves=leaves,
+          shape=shape, pad=pad, dtype=dtype, bias=rows % 2 == 0)
+
+
+@pytest.mark.parametrize("what", ["product", "grads"])
+@pytest.mark.parametrize("rows,inputs,outputs,trees,leaves,dtype", [
+    (9000, 24, 6, 1, 2, "f32"), (9000, 30, 9, 1, 2, "bf16"), (5000, 320, 272, 1, 3, "bf16"),
+    (5000, 272, 320, 1, 3, "f16"), (1500, 600, 512, 2, 2, "bf16"), (40000, 5, 1, 1, 300, "f32")])
+def test_long(check, what, rows, inputs, outputs, trees, leaves, dtype):
+    check(what, rows=rows, inputs=inputs, outputs=outputs, trees=trees, leaves=leaves, dtype=dtype,
+          shape="even")
+
+
+@pytest.mark.parametrize("name", ["differences", "odd_tables", "any_order", "empty", "layouts",
+                                  "scores_history", "refused", "own_stream", "side_stream",
+                                  "captured", "threads", "forest", "learner"])
+def test_plain(check, name):
+    check(name)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16", "f16"])
+@pytest.mark.parametrize("rows,cols,p,by,pad,seed,offset", [
+    (1, 1, 0.5, "element", 0, 1, 0), (7, 9, 0.1, "element", 0, 2 ** 63 + 5, 2 ** 64 - 1),
+    (100, 64, 0.3, "element", 0, 7, 1), (33, 31, 0.5, "element", 5, 8, 0),
+    (1000, 8, 0.05, "element", 8, 9, 2 ** 32), (3, 10000, 0.9, "element", 1, 10, 0),
+    (1000, 2, 0.3, "row", 0, 11, 3), (999, 1, 0.5, "row", 0, 12, 0), (257, 7, 0.2, "row", 1, 13, 0),
+    (130, 100, 0.5, "row", 4, 14, 0), (50, 16, 0.0, "element", 0, 15, 0),
+    (50, 16, 1.0, "element", 0, 16, 0), (50, 3, 1.0, "row", 0, 17, 0),
+    (600, 1024, 0.25, "element", 0, 18, 0), (70000, 2, 0.4, "row", 0, 19, 0)])
+def test_dropout(check, rows, cols, p, by, pad, seed, offset, dtype):
+    check("dropout", rows=rows, cols=cols, p=p, by=by, pad=pad, seed=seed, offset=offset, dtype=dtype)
+
+
+def test_dropout_far(check):
+    check("dropout_far")
+
+
+@pytest.mark.parametrize("kind", ["raw", "transformed"])
+@pytest.mark.parametrize("dtype", ["f64", "f32", "bf16", "f16"])
+@pytest.mark.parametrize("rows,classes,bias,masks,history,per_row,pad", [
+    (1, 1, False, 0, 0, False, 0), (1, 5000, True, 1, 40, False, 0), (300, 2, True, 3, 3, True, 0),
+    (1000, 10, True, 5, 0, False, 0), (257, 31, False, 2, 5, False, 1), (65, 64, True, 2, 70, True, 8),
+    (33, 255, False, 0, 20, True, 3), (5, 1023, True, 3, 500, True, 0), (4, 4097, False, 2, 6000, False, 1),
+    (3, 20001, True, 2, 100, True, 0), (2, 70000, True, 1, 0, False, 0), (130, 33, True, 0, 1, False, 0)])
+def test_scores(check, rows, classes, bias, masks, history, per_row, pad, dtype, kind):
+    check("scores", rows=rows, classes=classes, dtype=dtype, kind=kind, bias=bias, masks=masks,
+          history=history, per_row=per_row, pad=pad, seed=rows)
+
+
+def test_scores_mask_for_each_row(check):
+    check("scores", rows=37, classes=90, dtype="f32", kind="transformed", masks=37, by_row_masks=True)
+
+
+@pytest.mark.parametrize("dtype", ["f64", "f32", "bf16", "f16"])
+def test_scores_edges(check, dtype):
+    check("scores_edges", dtype=dtype)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16", "f16"])
+def test_together(check, dtype):
+    check("together", dtype=dtype)
+
