@@ -3,7 +3,19 @@
 //
 // s = x[n][j]; where class j stands c > 0 times in the row's history, s = (s > 0 ? s / r :
 // s * r) - f c - p; then + bias[j]; -inf (probability 0) where the mask's bit j is not set.
-// Sums, maxima and products are float64 for float64 scores and float32 for the others.
+// Sums, maxima and products are float64 for float64 scores and float32 for the others;
+// what a row's sum is made of is added in a fixed order.
+//
+// Bound by memory: a pass reads and writes every score once.  Three forms, by how many
+// classes a row has:
+//  - up to 32: a row a thread (k_scores_thread): the rows of a block pass through LDS, so
+//    that global accesses are contiguous, and no lane waits for another's maximum;
+//  - up to 4096: the row in registers of a wave or a block (k_scores_row), read once;
+//  - more: chunks of a row, each in a block's registers.  For probabilities the chunks'
+//    maxima and sums are written first (PART) and every chunk is read again to be
+//    written (FINISH); its second read mostly hits the caches.
+// Counts of a row's history are whole numbers in LDS; a chunk looks at the whole history
+// and counts its own classes.
 #include <algorithm>
 
 #include "leaf_ops.h"
@@ -14,7 +26,8 @@ namespace lgbm {
 namespace {
 
 constexpr int THREADS = 256;
-constexpr int CHUNK = 4096;  // classes whose counts a block holds in LDS at a time
+constexpr int THREAD_CLASSES = 32;
+constexpr int NARROW_CLASSES = 256, WAVE_CLASSES = 512, SMALL_CHUNK = 2048, CHUNK = 4096;
 
 template <typename T>
 struct Wide {
@@ -27,95 +40,306 @@ struct Wide<double> {
 
 __device__ __forceinline__ float exp_of(float v) { return expf(v); }
 __device__ __forceinline__ double exp_of(double v) { return exp(v); }
-
-// Maximum and sum of exponentials joined with another's; a maximum of -inf has sum 0.
+// fmax that keeps a NaN
 template <typename A>
-__device__ __forceinline__ void join(A& m, A& s, A m2, A s2) {
-  const A top = m > m2 || m != m ? m : m2;  // NaN stays
-  const A a = m == -INFINITY ? (A)0 : s * exp_of(m - top);
-  const A b = m2 == -INFINITY ? (A)0 : s2 * exp_of(m2 - top);
-  m = top;
-  s = a + b;
+__device__ __forceinline__ A top_of(A a, A b) {
+  return a > b || a != a ? a : b;
 }
 
-// A block a row.
-template <typename T>
-__global__ __launch_bounds__(THREADS) void k_scores(ScoreArgs a) {
-  typedef typename Wide<T>::type A;
-  __shared__ uint32_t count[CHUNK];
-  __shared__ A tops[THREADS / 64], sums[THREADS / 64];
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-  const int V = a.classes, words = (V + 31) / 32;
-  for (int64_t n = blockIdx.x; n < a.rows; n += gridDim.x) {
-    const T* const x = (const T*)a.x + n * a.ldx;
-    T* const out = (T*)a.out + n * a.ldo;
-    const uint32_t* mask = nullptr;
-    if (a.mask) {
-      const int64_t m = a.mask_rows ? a.mask_rows[n] : a.masks == 1 ? 0 : n;
-      if (m >= 0 && m < a.masks) mask = a.mask + m * words;
-    }
-    int64_t h0 = 0, h1 = 0;
-    if (a.ids) {
-      h0 = min(max(a.offsets[n], (int64_t)0), a.num_ids);
-      h1 = min(max(a.offsets[n + 1], h0), a.num_ids);
-    }
-    A rep = (A)a.repetition, fre = (A)a.frequency, pre = (A)a.presence;
+// What a row's scores are adjusted by.
+template <typename A>
+struct Row {
+  const uint32_t* mask;  // null: every class is allowed
+  int64_t h0, h1;        // its history
+  A rep, fre, pre;
+};
+
+template <typename A>
+__device__ __forceinline__ Row<A> row_of(const ScoreArgs& a, int64_t n) {
+  Row<A> r{nullptr, 0, 0, (A)a.repetition, (A)a.frequency, (A)a.presence};
+  if (a.mask) {
+    const int64_t m = a.mask_rows ? a.mask_rows[n] : a.masks == 1 ? 0 : n;
+    if (m >= 0 && m < a.masks) r.mask = a.mask + m * ((a.classes + 31) / 32);
+  }
+  if (a.ids) {
+    r.h0 = min(max(a.offsets[n], (int64_t)0), a.num_ids);
+    r.h1 = min(max(a.offsets[n + 1], r.h0), a.num_ids);
     if (a.penalties) {
-      rep = (A)a.penalties[n * 3];
-      fre = (A)a.penalties[n * 3 + 1];
-      pre = (A)a.penalties[n * 3 + 2];
+      r.rep = (A)a.penalties[n * 3];
+      r.fre = (A)a.penalties[n * 3 + 1];
+      r.pre = (A)a.penalties[n * 3 + 2];
     }
-    A top = -INFINITY, sum = 0;
-    auto value = [&](int j, uint32_t c) {
-      A s = (A)x[j];
-      if (c) s = (s > 0 ? s / rep : s * rep) - fre * (A)c - pre;
-      if (a.bias) s += (A)((const T*)a.bias)[j];
-      if (mask && !((mask[j >> 5] >> (j & 31)) & 1)) s = -INFINITY;
-      return s;
-    };
-    // kind transformed: the first sweep finds the maximum and the sum, the second writes
-    for (int sweep = a.kind == LGBM_HIP_PREDICT_TRANSFORMED ? 0 : 1; sweep < 2; ++sweep) {
-      for (int c0 = 0; c0 < V; c0 += CHUNK) {
-        if (h1 > h0) {
-          __syncthreads();
-          for (int j = tid; j < CHUNK; j += THREADS) count[j] = 0;
-          __syncthreads();
-          for (int64_t h = h0 + tid; h < h1; h += THREADS) {
-            const uint32_t j = (uint32_t)a.ids[h] - (uint32_t)c0;
-            if (j < (uint32_t)CHUNK) atomicAdd(&count[j], 1u);
+  }
+  return r;
+}
+
+template <typename A>
+__device__ __forceinline__ A adjusted(A s, uint32_t count, const Row<A>& r, A bias, bool allowed) {
+  if (count) s = (s > 0 ? s / r.rep : s * r.rep) - r.fre * (A)count - r.pre;
+  s += bias;
+  return allowed ? s : -INFINITY;
+}
+
+// ---- a row a thread ------------------------------------------------------------------------
+
+// LDS: [THREADS][classes | 1] values (odd strides: a wave's rows in different banks), and
+// as many counts where there is a history.
+template <typename T>
+__global__ __launch_bounds__(THREADS) void k_scores_thread(ScoreArgs a, uint32_t inverse) {
+  typedef typename Wide<T>::type A;
+  extern __shared__ __align__(16) char lds[];
+  const int V = a.classes, stride = V | 1, tid = threadIdx.x;
+  A* const values = (A*)lds;
+  uint32_t* const counts = (uint32_t*)(values + THREADS * stride) + tid * stride;
+  A* const mine = values + tid * stride;
+  const T* const bias = (const T*)a.bias;
+  for (int64_t n0 = blockIdx.x * (int64_t)THREADS; n0 < a.rows; n0 += (int64_t)gridDim.x * THREADS) {
+    const int rows = (int)min((int64_t)THREADS, a.rows - n0);
+    const T* const x = (const T*)a.x + n0 * a.ldx;
+    for (int i = tid; i < rows * V; i += THREADS) {
+      const int r = (int)((uint32_t)i * inverse >> 19), j = i - r * V;
+      values[r * stride + j] = (A)x[r * a.ldx + j];
+    }
+    __syncthreads();
+    if (tid < rows) {
+      const Row<A> row = row_of<A>(a, n0 + tid);
+      const uint32_t allowed = row.mask ? row.mask[0] : ~0u;
+      if (a.ids) {
+        for (int j = 0; j < V; ++j) counts[j] = 0;
+        for (int64_t h = row.h0; h < row.h1; ++h) {
+          const uint32_t j = (uint32_t)a.ids[h];
+          if (j < (uint32_t)V) ++counts[j];
+        }
+      }
+      A top = -INFINITY;
+      for (int j = 0; j < V; ++j) {
+        const A s = adjusted(mine[j], a.ids ? counts[j] : 0, row, bias ? (A)bias[j] : (A)0,
+                             (allowed >> j) & 1);
+        mine[j] = s;
+        top = top_of(top, s);
+      }
+      if (a.kind == LGBM_HIP_PREDICT_TRANSFORMED) {
+        A sum = 0;
+        for (int j = 0; j < V; ++j) {
+          const A s = mine[j], e = s == -INFINITY ? (A)0 : exp_of(s - top);
+          mine[j] = e;
+          sum += e;
+        }
+        const A scale = top == -INFINITY ? (A)0 : 1 / sum;
+        for (int j = 0; j < V; ++j) mine[j] = mine[j] == 0 ? (A)0 : mine[j] * scale;
+      }
+    }
+    __syncthreads();
+    T* const out = (T*)a.out + n0 * a.ldo;
+    for (int i = tid; i < rows * V; i += THREADS) {
+      const int r = (int)((uint32_t)i * inverse >> 19), j = i - r * V;
+      out[r * a.ldo + j] = (T)values[r * stride + j];
+    }
+    __syncthreads();
+  }
+}
+
+// ---- a row, or a chunk of one, in registers ----------------------------------------------------
+
+enum { WHOLE, PART, FINISH };
+
+// LANES of one row, each with NV vectors of VW neighbouring classes, LANES * NV * VW classes
+// from c0 on.
+template <typename T, int LANES, int NV, int VW, int MODE>
+__global__ __launch_bounds__(THREADS) void k_scores_row(ScoreArgs a, int chunks) {
+  typedef typename Wide<T>::type A;
+  constexpr int CAP = LANES * NV * VW, TEAMS = THREADS / LANES;
+  __shared__ uint32_t counts[TEAMS * CAP];
+  __shared__ A shared[THREADS / 64];
+  const int lane = threadIdx.x % LANES, team = threadIdx.x / LANES;
+  uint32_t* const count = counts + team * CAP;
+  auto sync = [&] {
+    if (LANES == 64) {
+      __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+      __builtin_amdgcn_wave_barrier();
+    } else {
+      __syncthreads();
+    }
+  };
+  // over the row's lanes; every one gets the result
+  auto reduce = [&](A v, auto join) {
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) v = join(v, (A)__shfl_xor(v, d));
+    if (LANES > 64) {
+      __syncthreads();
+      if (lane % 64 == 0) shared[lane / 64] = v;
+      __syncthreads();
+      v = shared[0];
+#pragma unroll
+      for (int w = 1; w < LANES / 64; ++w) v = join(v, shared[w]);
+    }
+    return v;
+  };
+  const auto larger = [](A p, A q) { return top_of(p, q); };
+  const auto plus = [](A p, A q) { return p + q; };
+  const int64_t tasks = a.rows * chunks;
+  for (int64_t task = blockIdx.x * (int64_t)TEAMS + team; task < tasks;
+       task += (int64_t)gridDim.x * TEAMS) {
+    const int64_t n = task / chunks;
+    const int c0 = (int)(task - n * chunks) * CAP;
+    const int V = min(a.classes - c0, CAP);
+    const T* const x = (const T*)a.x + n * a.ldx + c0;
+    const Row<A> row = row_of<A>(a, n);
+    const T* const bias = a.bias ? (const T*)a.bias + c0 : nullptr;
+    const bool seen = row.h1 > row.h0;
+    A s[NV][VW];
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      const int j = (i * LANES + lane) * VW;
+      T v[VW];
+      if (j + VW <= V)
+        __builtin_memcpy(v, x + j, sizeof(v));
+      else
+#pragma unroll
+        for (int e = 0; e < VW; ++e) v[e] = j + e < V ? x[j + e] : (T)0.0f;
+#pragma unroll
+      for (int e = 0; e < VW; ++e) s[i][e] = (A)v[e];
+    }
+    if (seen) {
+      for (int j = lane; j < V; j += LANES) count[j] = 0;
+      sync();
+      for (int64_t h = row.h0 + lane; h < row.h1; h += LANES) {
+        const uint32_t j = (uint32_t)a.ids[h] - (uint32_t)c0;
+        if (j < (uint32_t)V) atomicAdd(&count[j], 1u);
+      }
+      sync();
+    }
+    A top = -INFINITY;
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      const int j = (i * LANES + lane) * VW;
+      T b[VW];
+      if (bias && j + VW <= V)
+        __builtin_memcpy(b, bias + j, sizeof(b));
+      else
+#pragma unroll
+        for (int e = 0; e < VW; ++e) b[e] = bias && j + e < V ? bias[j + e] : (T)0.0f;
+      // VW divides 32 and c0 is a multiple of 32, so the bits are of one word
+      const uint32_t allowed = row.mask && j < V ? row.mask[(c0 + j) >> 5] >> (j & 31) : ~0u;
+#pragma unroll
+      for (int e = 0; e < VW; ++e) {
+        const bool in = j + e < V;
+        s[i][e] = adjusted(s[i][e], seen && in ? count[j + e] : 0, row, (A)b[e],
+                           in && ((allowed >> e) & 1));
+        top = top_of(top, s[i][e]);
+      }
+    }
+    if (seen) sync();  // the counts are read before the next row's are cleared
+    A scale = 1;
+    const bool probabilities = a.kind == LGBM_HIP_PREDICT_TRANSFORMED;
+    if (probabilities) {
+      A* const parts = (A*)a.ws;  // [rows][chunks]: maximum, sum
+      if (MODE != FINISH) {
+        top = reduce(top, larger);
+        A sum = 0;
+#pragma unroll
+        for (int i = 0; i < NV; ++i)
+#pragma unroll
+          for (int e = 0; e < VW; ++e) {
+            const A ex = s[i][e] == -INFINITY ? (A)0 : exp_of(s[i][e] - top);
+            if (MODE == WHOLE) s[i][e] = ex;
+            sum += ex;
           }
-          __syncthreads();
+        sum = reduce(sum, plus);
+        if (MODE == PART) {
+          if (lane == 0) parts[task * 2] = top, parts[task * 2 + 1] = sum;
+          continue;
         }
-        for (int j = tid; j < CHUNK && c0 + j < V; j += THREADS) {
-          const A s = value(c0 + j, h1 > h0 ? count[j] : 0);
-          if (sweep == 0)
-            join(top, sum, s, (A)1);
-          else if (a.kind == LGBM_HIP_PREDICT_RAW)
-            out[c0 + j] = (T)s;
-          else
-            out[c0 + j] = (T)(top == -INFINITY ? (A)0 : exp_of(s - top) / sum);
+        scale = top == -INFINITY ? (A)0 : 1 / sum;
+      } else {
+        top = -INFINITY;
+        for (int c = lane; c < chunks; c += LANES) top = top_of(top, parts[(n * chunks + c) * 2]);
+        top = reduce(top, larger);
+        A sum = 0;
+        for (int c = lane; c < chunks; c += LANES) {
+          const A m = parts[(n * chunks + c) * 2];
+          if (m != -INFINITY) sum += parts[(n * chunks + c) * 2 + 1] * exp_of(m - top);
         }
+        sum = reduce(sum, plus);
+        scale = top == -INFINITY ? (A)0 : 1 / sum;
+#pragma unroll
+        for (int i = 0; i < NV; ++i)
+#pragma unroll
+          for (int e = 0; e < VW; ++e) s[i][e] = s[i][e] == -INFINITY ? (A)0 : exp_of(s[i][e] - top);
       }
-      if (sweep == 0) {
-        for (int d = 1; d < 64; d <<= 1) join(top, sum, (A)__shfl_xor(top, d), (A)__shfl_xor(sum, d));
-        __syncthreads();
-        if (lane == 0) tops[wave] = top, sums[wave] = sum;
-        __syncthreads();
-        top = -INFINITY, sum = 0;
-        for (int w = 0; w < THREADS / 64; ++w) join(top, sum, tops[w], sums[w]);
-      }
+    }
+    T* const out = (T*)a.out + n * a.ldo + c0;
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      const int j = (i * LANES + lane) * VW;
+      T v[VW];
+#pragma unroll
+      for (int e = 0; e < VW; ++e)  // 0 stays 0 beside a NaN
+        v[e] = (T)(probabilities ? (s[i][e] == 0 ? (A)0 : s[i][e] * scale) : s[i][e]);
+      if (j + VW <= V)
+        __builtin_memcpy(out + j, v, sizeof(v));
+      else
+#pragma unroll
+        for (int e = 0; e < VW; ++e)
+          if (j + e < V) out[j + e] = v[e];
     }
   }
 }
 
+template <typename T, int LANES, int CAP, int VW, int MODE>
+void launch_row(const ScoreArgs& a, int chunks, hipStream_t s) {
+  constexpr int TEAMS = THREADS / LANES;
+  const int64_t blocks = (a.rows * chunks + TEAMS - 1) / TEAMS;
+  k_scores_row<T, LANES, CAP / LANES / VW, VW, MODE>
+      <<<(unsigned)std::min<int64_t>(blocks, 1 << 20), THREADS, 0, s>>>(a, chunks);
+}
+
+int chunk_of(int64_t rows, int32_t classes) {
+  // small chunks where large ones leave half of the CUs without a second block
+  return rows * ((classes + CHUNK - 1) / CHUNK) < 512 ? SMALL_CHUNK : CHUNK;
+}
+
+template <typename T, int CAP>
+void launch_chunks(const ScoreArgs& a, hipStream_t s) {
+  constexpr int VW = 16 / sizeof(T);
+  const int chunks = (a.classes + CAP - 1) / CAP;
+  if (a.kind == LGBM_HIP_PREDICT_RAW) return launch_row<T, THREADS, CAP, VW, WHOLE>(a, chunks, s);
+  launch_row<T, THREADS, CAP, VW, PART>(a, chunks, s);
+  launch_row<T, THREADS, CAP, VW, FINISH>(a, chunks, s);
+}
+
 template <typename T>
 void launch(const ScoreArgs& a, hipStream_t s) {
-  k_scores<T><<<(unsigned)std::min<int64_t>(a.rows, 65536), THREADS, 0, s>>>(a);
+  typedef typename Wide<T>::type A;
+  constexpr int VW = 16 / sizeof(T);
+  const int V = a.classes;
+  if (V <= THREAD_CLASSES) {
+    const size_t lds = (size_t)THREADS * (V | 1) * (sizeof(A) + (a.ids ? 4 : 0));
+    const int64_t blocks = (a.rows + THREADS - 1) / THREADS;
+    const uint32_t inverse = ((1u << 19) + V - 1) / V;  // i / V for i < 256 V: i V < 2^19
+    k_scores_thread<T><<<(unsigned)std::min<int64_t>(blocks, 1 << 20), THREADS, lds, s>>>(a, inverse);
+  } else if (V <= NARROW_CLASSES) {
+    launch_row<T, 64, NARROW_CLASSES, 1, WHOLE>(a, 1, s);
+  } else if (V <= WAVE_CLASSES) {
+    launch_row<T, 64, WAVE_CLASSES, VW, WHOLE>(a, 1, s);
+  } else if (V <= SMALL_CHUNK) {
+    launch_row<T, THREADS, SMALL_CHUNK, VW, WHOLE>(a, 1, s);
+  } else if (V <= CHUNK) {
+    launch_row<T, THREADS, CHUNK, VW, WHOLE>(a, 1, s);
+  } else if (chunk_of(a.rows, V) == SMALL_CHUNK) {
+    launch_chunks<T, SMALL_CHUNK>(a, s);
+  } else {
+    launch_chunks<T, CHUNK>(a, s);
+  }
 }
 
 }  // namespace
 
-size_t adjust_scores_workspace(int64_t rows, int32_t classes, int32_t dtype, int32_t kind) { return 0; }
+size_t adjust_scores_workspace(int64_t rows, int32_t classes, int32_t dtype, int32_t kind) {
+  if (classes <= CHUNK || kind == LGBM_HIP_PREDICT_RAW) return 0;
+  const int chunk = chunk_of(rows, classes);
+  return (size_t)rows * (size_t)((classes + chunk - 1) / chunk) * (dtype == LGBM_HIP_DTYPE_F64 ? 16 : 8);
+}
 
 void launch_adjust_scores(const ScoreArgs& a, hipStream_t s) {
   if (a.dtype == LGBM_HIP_DTYPE_F64)

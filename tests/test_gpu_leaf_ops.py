@@ -125,7 +125,10 @@ def test_dropout_far(check):
     (1, 1, False, 0, 0, False, 0), (1, 5000, True, 1, 40, False, 0), (300, 2, True, 3, 3, True, 0),
     (1000, 10, True, 5, 0, False, 0), (257, 31, False, 2, 5, False, 1), (65, 64, True, 2, 70, True, 8),
     (33, 255, False, 0, 20, True, 3), (5, 1023, True, 3, 500, True, 0), (4, 4097, False, 2, 6000, False, 1),
-    (3, 20001, True, 2, 100, True, 0), (2, 70000, True, 1, 0, False, 0), (130, 33, True, 0, 1, False, 0)])
+    (3, 20001, True, 2, 100, True, 0), (300, 32, True, 2, 9, False, 0), (9, 256, True, 1, 30, False, 1),
+    (9, 257, False, 2, 30, True, 0), (7, 512, True, 0, 60, False, 0), (6, 513, True, 2, 60, False, 3),
+    (5, 2048, False, 1, 90, True, 0), (5, 2049, True, 2, 90, False, 0), (5, 4096, True, 1, 900, False, 1),
+    (150, 8200, True, 3, 50, True, 1), (2, 70000, True, 1, 0, False, 0), (130, 33, True, 0, 1, False, 0)])
 def test_scores(check, rows, classes, bias, masks, history, per_row, pad, dtype, kind):
     check("scores", rows=rows, classes=classes, dtype=dtype, kind=kind, bias=bias, masks=masks,
           history=history, per_row=per_row, pad=pad, seed=rows)
