@@ -807,8 +807,8 @@ int lgbm_hip_dropout(lgbm_hip_ctx* ctx, const void* d_x, int64_t ldx, int64_t nu
  * and out is s (LGBM_HIP_PREDICT_RAW) or the softmax of s over the row
  * (LGBM_HIP_PREDICT_TRANSFORMED).  A class with s = -inf has probability 0, also in a row
  * where that is every class; a masked score is never looked at (NaN and infinities
- * included), while a NaN or +inf that is not masked makes the row's other probabilities
- * NaN.  Arithmetic is float64 for float64 scores, else float32, rounded once. */
+ * included), while a NaN that is not masked makes the row's other probabilities NaN and a
+ * +inf its own.  Arithmetic is float64 for float64 scores, else float32, rounded once. */
 typedef struct lgbm_score_args {
   const void* d_x; /* [num_rows][num_classes], row stride ldx */
   int64_t ldx;

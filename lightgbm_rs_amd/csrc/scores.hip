@@ -10,7 +10,7 @@
 // classes a row has:
 //  - up to 32: a row a thread (k_scores_thread): the rows of a block pass through LDS, so
 //    that global accesses are contiguous, and no lane waits for another's maximum;
-//  - up to 4096: the row in registers of a wave or a block (k_scores_row), read once;
+//  - up to 8192: the row in registers of a wave or a block (k_scores_row), read once;
 //  - more: chunks of a row, each in a block's registers.  For probabilities the chunks'
 //    maxima and sums are written first (PART) and every chunk is read again to be
 //    written (FINISH); its second read mostly hits the caches.
@@ -27,7 +27,7 @@ namespace {
 
 constexpr int THREADS = 256;
 constexpr int THREAD_CLASSES = 32;
-constexpr int NARROW_CLASSES = 256, WAVE_CLASSES = 512, SMALL_CHUNK = 2048, CHUNK = 4096;
+constexpr int NARROW_CLASSES = 256, WAVE_CLASSES = 512, BLOCK_CLASSES = 2048, ROW_CLASSES = 8192;
 
 template <typename T>
 struct Wide {
@@ -38,12 +38,23 @@ struct Wide<double> {
   typedef double type;
 };
 
-__device__ __forceinline__ float exp_of(float v) { return expf(v); }
-__device__ __forceinline__ double exp_of(double v) { return exp(v); }
-// fmax that keeps a NaN
+// e^v.  For 16-bit results the hardware's 2^x is enough: the product with log2(e) is off by
+// |v| 2^-24, far below their rounding wherever e^v is not 0 beside the row's largest.
+template <typename T>
+__device__ __forceinline__ float exp_of(float v) {
+  return sizeof(T) == 2 ? __builtin_amdgcn_exp2f(v * 1.44269504f) : expf(v);
+}
+template <typename T>
+__device__ __forceinline__ double exp_of(double v) {
+  return exp(v);
+}
+// The larger; a NaN is passed over (it comes back through the sum).
+__device__ __forceinline__ float top_of(float a, float b) { return fmaxf(a, b); }
+__device__ __forceinline__ double top_of(double a, double b) { return fmax(a, b); }
+// What the exponentials are relative to: where every class is masked their -inf stays.
 template <typename A>
-__device__ __forceinline__ A top_of(A a, A b) {
-  return a > b || a != a ? a : b;
+__device__ __forceinline__ A base_of(A top) {
+  return top == -INFINITY ? (A)0 : top;
 }
 
 // What a row's scores are adjusted by.
@@ -83,23 +94,40 @@ __device__ __forceinline__ A adjusted(A s, uint32_t count, const Row<A>& r, A bi
 // ---- a row a thread ------------------------------------------------------------------------
 
 // LDS: [THREADS][classes | 1] values (odd strides: a wave's rows in different banks), and
-// as many counts where there is a history.
-template <typename T>
+// as many counts where there is a history.  FLAT: the rows of x and of out follow each
+// other without gaps, so a block's are copied as vectors of 16 bytes.
+template <typename T, bool FLAT>
 __global__ __launch_bounds__(THREADS) void k_scores_thread(ScoreArgs a, uint32_t inverse) {
   typedef typename Wide<T>::type A;
+  constexpr int VE = FLAT ? 16 / (int)sizeof(T) : 1;
   extern __shared__ __align__(16) char lds[];
   const int V = a.classes, stride = V | 1, tid = threadIdx.x;
   A* const values = (A*)lds;
   uint32_t* const counts = (uint32_t*)(values + THREADS * stride) + tid * stride;
   A* const mine = values + tid * stride;
   const T* const bias = (const T*)a.bias;
+  auto at = [&](int i) {  // element i of the block's rows in LDS
+    const int r = (int)((uint32_t)i * inverse >> 19);
+    return r * stride + (i - r * V);
+  };
   for (int64_t n0 = blockIdx.x * (int64_t)THREADS; n0 < a.rows; n0 += (int64_t)gridDim.x * THREADS) {
-    const int rows = (int)min((int64_t)THREADS, a.rows - n0);
+    const int rows = (int)min((int64_t)THREADS, a.rows - n0), total = rows * V;
     const T* const x = (const T*)a.x + n0 * a.ldx;
-    for (int i = tid; i < rows * V; i += THREADS) {
-      const int r = (int)((uint32_t)i * inverse >> 19), j = i - r * V;
-      values[r * stride + j] = (A)x[r * a.ldx + j];
+    T* const out = (T*)a.out + n0 * a.ldo;
+#pragma unroll 4
+    for (int i = tid * VE; i + VE <= total; i += THREADS * VE) {
+      T v[VE];
+      if (FLAT) {
+        __builtin_memcpy(v, x + i, sizeof(v));
+      } else {
+        const int r = (int)((uint32_t)i * inverse >> 19);
+        v[0] = x[r * a.ldx + (i - r * V)];
+      }
+#pragma unroll
+      for (int e = 0; e < VE; ++e) values[at(i + e)] = (A)v[e];
     }
+    const int tail = total - total % VE + tid;
+    if (tail < total) values[at(tail)] = (A)x[tail];  // FLAT only
     __syncthreads();
     if (tid < rows) {
       const Row<A> row = row_of<A>(a, n0 + tid);
@@ -119,22 +147,31 @@ __global__ __launch_bounds__(THREADS) void k_scores_thread(ScoreArgs a, uint32_t
         top = top_of(top, s);
       }
       if (a.kind == LGBM_HIP_PREDICT_TRANSFORMED) {
+        const A base = base_of(top);
         A sum = 0;
         for (int j = 0; j < V; ++j) {
-          const A s = mine[j], e = s == -INFINITY ? (A)0 : exp_of(s - top);
+          const A e = exp_of<T>(mine[j] - base);
           mine[j] = e;
           sum += e;
         }
-        const A scale = top == -INFINITY ? (A)0 : 1 / sum;
+        const A scale = 1 / sum;
         for (int j = 0; j < V; ++j) mine[j] = mine[j] == 0 ? (A)0 : mine[j] * scale;
       }
     }
     __syncthreads();
-    T* const out = (T*)a.out + n0 * a.ldo;
-    for (int i = tid; i < rows * V; i += THREADS) {
-      const int r = (int)((uint32_t)i * inverse >> 19), j = i - r * V;
-      out[r * a.ldo + j] = (T)values[r * stride + j];
+#pragma unroll 4
+    for (int i = tid * VE; i + VE <= total; i += THREADS * VE) {
+      T v[VE];
+#pragma unroll
+      for (int e = 0; e < VE; ++e) v[e] = (T)values[at(i + e)];
+      if (FLAT) {
+        __builtin_memcpy(out + i, v, sizeof(v));
+      } else {
+        const int r = (int)((uint32_t)i * inverse >> 19);
+        out[r * a.ldo + (i - r * V)] = v[0];
+      }
     }
+    if (tail < total) out[tail] = (T)values[at(tail)];
     __syncthreads();
   }
 }
@@ -146,11 +183,11 @@ enum { WHOLE, PART, FINISH };
 // LANES of one row, each with NV vectors of VW neighbouring classes, LANES * NV * VW classes
 // from c0 on.
 template <typename T, int LANES, int NV, int VW, int MODE>
-__global__ __launch_bounds__(THREADS) void k_scores_row(ScoreArgs a, int chunks) {
+__global__ __launch_bounds__(LANES < THREADS ? THREADS : LANES) void k_scores_row(ScoreArgs a, int chunks) {
   typedef typename Wide<T>::type A;
-  constexpr int CAP = LANES * NV * VW, TEAMS = THREADS / LANES;
-  __shared__ uint32_t counts[TEAMS * CAP];
-  __shared__ A shared[THREADS / 64];
+  constexpr int CAP = LANES * NV * VW, TEAMS = LANES < THREADS ? THREADS / LANES : 1;
+  __shared__ __align__(16) uint32_t counts[TEAMS * CAP];
+  __shared__ A shared[LANES / 64];
   const int lane = threadIdx.x % LANES, team = threadIdx.x / LANES;
   uint32_t* const count = counts + team * CAP;
   auto sync = [&] {
@@ -201,8 +238,10 @@ __global__ __launch_bounds__(THREADS) void k_scores_row(ScoreArgs a, int chunks)
       for (int e = 0; e < VW; ++e) s[i][e] = (A)v[e];
     }
     if (seen) {
-      for (int j = lane; j < V; j += LANES) count[j] = 0;
+#pragma unroll
+      for (int i = 0; i < NV; ++i) __builtin_memset(count + (i * LANES + lane) * VW, 0, 4 * VW);
       sync();
+#pragma unroll 4
       for (int64_t h = row.h0 + lane; h < row.h1; h += LANES) {
         const uint32_t j = (uint32_t)a.ids[h] - (uint32_t)c0;
         if (j < (uint32_t)V) atomicAdd(&count[j], 1u);
@@ -213,19 +252,30 @@ __global__ __launch_bounds__(THREADS) void k_scores_row(ScoreArgs a, int chunks)
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
       const int j = (i * LANES + lane) * VW;
+      const bool full = j + VW <= V;
       T b[VW];
-      if (bias && j + VW <= V)
+      if (bias && full)
         __builtin_memcpy(b, bias + j, sizeof(b));
       else
 #pragma unroll
         for (int e = 0; e < VW; ++e) b[e] = bias && j + e < V ? bias[j + e] : (T)0.0f;
       // VW divides 32 and c0 is a multiple of 32, so the bits are of one word
-      const uint32_t allowed = row.mask && j < V ? row.mask[(c0 + j) >> 5] >> (j & 31) : ~0u;
+      uint32_t allowed = row.mask && j < V ? row.mask[(c0 + j) >> 5] >> (j & 31) : ~0u;
+      if (!full) allowed &= j < V ? (1u << (V - j)) - 1 : 0u;
+      if (seen) {
+        uint32_t c[VW], any = 0;
+        __builtin_memcpy(c, count + j, sizeof(c));  // behind V: zeros
+#pragma unroll
+        for (int e = 0; e < VW; ++e) any |= c[e];
+        if (any) {
+#pragma unroll
+          for (int e = 0; e < VW; ++e)
+            if (c[e]) s[i][e] = (s[i][e] > 0 ? s[i][e] / row.rep : s[i][e] * row.rep) - row.fre * (A)c[e] - row.pre;
+        }
+      }
 #pragma unroll
       for (int e = 0; e < VW; ++e) {
-        const bool in = j + e < V;
-        s[i][e] = adjusted(s[i][e], seen && in ? count[j + e] : 0, row, (A)b[e],
-                           in && ((allowed >> e) & 1));
+        s[i][e] = (allowed >> e) & 1 ? s[i][e] + (A)b[e] : -INFINITY;
         top = top_of(top, s[i][e]);
       }
     }
@@ -234,39 +284,30 @@ __global__ __launch_bounds__(THREADS) void k_scores_row(ScoreArgs a, int chunks)
     const bool probabilities = a.kind == LGBM_HIP_PREDICT_TRANSFORMED;
     if (probabilities) {
       A* const parts = (A*)a.ws;  // [rows][chunks]: maximum, sum
-      if (MODE != FINISH) {
-        top = reduce(top, larger);
-        A sum = 0;
-#pragma unroll
-        for (int i = 0; i < NV; ++i)
-#pragma unroll
-          for (int e = 0; e < VW; ++e) {
-            const A ex = s[i][e] == -INFINITY ? (A)0 : exp_of(s[i][e] - top);
-            if (MODE == WHOLE) s[i][e] = ex;
-            sum += ex;
-          }
-        sum = reduce(sum, plus);
-        if (MODE == PART) {
-          if (lane == 0) parts[task * 2] = top, parts[task * 2 + 1] = sum;
-          continue;
-        }
-        scale = top == -INFINITY ? (A)0 : 1 / sum;
-      } else {
+      if (MODE == FINISH) {
         top = -INFINITY;
         for (int c = lane; c < chunks; c += LANES) top = top_of(top, parts[(n * chunks + c) * 2]);
-        top = reduce(top, larger);
-        A sum = 0;
-        for (int c = lane; c < chunks; c += LANES) {
-          const A m = parts[(n * chunks + c) * 2];
-          if (m != -INFINITY) sum += parts[(n * chunks + c) * 2 + 1] * exp_of(m - top);
-        }
-        sum = reduce(sum, plus);
-        scale = top == -INFINITY ? (A)0 : 1 / sum;
-#pragma unroll
-        for (int i = 0; i < NV; ++i)
-#pragma unroll
-          for (int e = 0; e < VW; ++e) s[i][e] = s[i][e] == -INFINITY ? (A)0 : exp_of(s[i][e] - top);
       }
+      top = reduce(top, larger);
+      const A base = base_of(top);
+      A sum = 0;
+#pragma unroll
+      for (int i = 0; i < NV; ++i)
+#pragma unroll
+        for (int e = 0; e < VW; ++e) {
+          s[i][e] = exp_of<T>(s[i][e] - base);
+          if (MODE != FINISH) sum += s[i][e];
+        }
+      if (MODE == FINISH) {
+        for (int c = lane; c < chunks; c += LANES)
+          sum += parts[(n * chunks + c) * 2 + 1] * exp_of<A>(parts[(n * chunks + c) * 2] - base);
+      }
+      sum = reduce(sum, plus);
+      if (MODE == PART) {
+        if (lane == 0) parts[task * 2] = top, parts[task * 2 + 1] = sum;
+        continue;
+      }
+      scale = 1 / sum;
     }
     T* const out = (T*)a.out + n * a.ldo + c0;
 #pragma unroll
@@ -288,24 +329,27 @@ __global__ __launch_bounds__(THREADS) void k_scores_row(ScoreArgs a, int chunks)
 
 template <typename T, int LANES, int CAP, int VW, int MODE>
 void launch_row(const ScoreArgs& a, int chunks, hipStream_t s) {
-  constexpr int TEAMS = THREADS / LANES;
+  constexpr int TEAMS = LANES < THREADS ? THREADS / LANES : 1;
   const int64_t blocks = (a.rows * chunks + TEAMS - 1) / TEAMS;
   k_scores_row<T, LANES, CAP / LANES / VW, VW, MODE>
-      <<<(unsigned)std::min<int64_t>(blocks, 1 << 20), THREADS, 0, s>>>(a, chunks);
+      <<<(unsigned)std::min<int64_t>(blocks, 1 << 20), TEAMS * LANES, 0, s>>>(a, chunks);
 }
 
-int chunk_of(int64_t rows, int32_t classes) {
-  // small chunks where large ones leave half of the CUs without a second block
-  return rows * ((classes + CHUNK - 1) / CHUNK) < 512 ? SMALL_CHUNK : CHUNK;
+// Long rows: chunks of two vectors a lane in blocks of 1024, so that few blocks look at the
+// same history; smaller ones where those would leave CUs without a block.
+constexpr int CHUNK_LANES = 1024, SMALL_LANES = 256, CHUNK_BYTES = 32;
+int chunk_lanes(int64_t rows, int32_t classes, int e) {
+  const int chunk = CHUNK_LANES * (CHUNK_BYTES / e);
+  return rows * ((classes + chunk - 1) / chunk) < 256 ? SMALL_LANES : CHUNK_LANES;
 }
 
-template <typename T, int CAP>
+template <typename T, int LANES>
 void launch_chunks(const ScoreArgs& a, hipStream_t s) {
-  constexpr int VW = 16 / sizeof(T);
+  constexpr int VW = 16 / sizeof(T), CAP = LANES * (CHUNK_BYTES / (int)sizeof(T));
   const int chunks = (a.classes + CAP - 1) / CAP;
-  if (a.kind == LGBM_HIP_PREDICT_RAW) return launch_row<T, THREADS, CAP, VW, WHOLE>(a, chunks, s);
-  launch_row<T, THREADS, CAP, VW, PART>(a, chunks, s);
-  launch_row<T, THREADS, CAP, VW, FINISH>(a, chunks, s);
+  if (a.kind == LGBM_HIP_PREDICT_RAW) return launch_row<T, LANES, CAP, VW, WHOLE>(a, chunks, s);
+  launch_row<T, LANES, CAP, VW, PART>(a, chunks, s);
+  launch_row<T, LANES, CAP, VW, FINISH>(a, chunks, s);
 }
 
 template <typename T>
@@ -317,28 +361,33 @@ void launch(const ScoreArgs& a, hipStream_t s) {
     const size_t lds = (size_t)THREADS * (V | 1) * (sizeof(A) + (a.ids ? 4 : 0));
     const int64_t blocks = (a.rows + THREADS - 1) / THREADS;
     const uint32_t inverse = ((1u << 19) + V - 1) / V;  // i / V for i < 256 V: i V < 2^19
-    k_scores_thread<T><<<(unsigned)std::min<int64_t>(blocks, 1 << 20), THREADS, lds, s>>>(a, inverse);
+    const unsigned grid = (unsigned)std::min<int64_t>(blocks, 1 << 20);
+    if (a.ldx == V && a.ldo == V)
+      k_scores_thread<T, true><<<grid, THREADS, lds, s>>>(a, inverse);
+    else
+      k_scores_thread<T, false><<<grid, THREADS, lds, s>>>(a, inverse);
   } else if (V <= NARROW_CLASSES) {
     launch_row<T, 64, NARROW_CLASSES, 1, WHOLE>(a, 1, s);
   } else if (V <= WAVE_CLASSES) {
     launch_row<T, 64, WAVE_CLASSES, VW, WHOLE>(a, 1, s);
-  } else if (V <= SMALL_CHUNK) {
-    launch_row<T, THREADS, SMALL_CHUNK, VW, WHOLE>(a, 1, s);
-  } else if (V <= CHUNK) {
-    launch_row<T, THREADS, CHUNK, VW, WHOLE>(a, 1, s);
-  } else if (chunk_of(a.rows, V) == SMALL_CHUNK) {
-    launch_chunks<T, SMALL_CHUNK>(a, s);
+  } else if (V <= BLOCK_CLASSES) {
+    launch_row<T, THREADS, BLOCK_CLASSES, VW, WHOLE>(a, 1, s);
+  } else if (V <= ROW_CLASSES) {
+    launch_row<T, 512, ROW_CLASSES, VW, WHOLE>(a, 1, s);
+  } else if (chunk_lanes(a.rows, V, sizeof(T)) == SMALL_LANES) {
+    launch_chunks<T, SMALL_LANES>(a, s);
   } else {
-    launch_chunks<T, CHUNK>(a, s);
+    launch_chunks<T, CHUNK_LANES>(a, s);
   }
 }
 
 }  // namespace
 
 size_t adjust_scores_workspace(int64_t rows, int32_t classes, int32_t dtype, int32_t kind) {
-  if (classes <= CHUNK || kind == LGBM_HIP_PREDICT_RAW) return 0;
-  const int chunk = chunk_of(rows, classes);
-  return (size_t)rows * (size_t)((classes + chunk - 1) / chunk) * (dtype == LGBM_HIP_DTYPE_F64 ? 16 : 8);
+  if (classes <= ROW_CLASSES || kind == LGBM_HIP_PREDICT_RAW) return 0;
+  const int e = dtype == LGBM_HIP_DTYPE_F64 ? 8 : dtype == LGBM_HIP_DTYPE_F32 ? 4 : 2;
+  const int chunk = chunk_lanes(rows, classes, e) * (CHUNK_BYTES / e);
+  return (size_t)rows * (size_t)((classes + chunk - 1) / chunk) * (e == 8 ? 16 : 8);
 }
 
 void launch_adjust_scores(const ScoreArgs& a, hipStream_t s) {
