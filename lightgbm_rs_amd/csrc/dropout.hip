@@ -7,6 +7,13 @@
 // fields, so the ten rounds are shared by eight units; unit e is kept where field e % 8 of
 // block e / 8 is at least threshold = round(65536 p), and what is kept is divided by the
 // share that is really kept, 1 - threshold / 65536.
+//
+// Bound by memory: an element is read and written once; the ten rounds' twenty 32 x 32
+// products for eight elements are below the time that their bytes take.  Elements without
+// gaps between rows are one long row, so any number of columns runs in vectors
+// (k_dropout_flat); rows of which the pairs of a few columns follow each other too
+// (k_dropout_rows: a unit's columns lie in one vector or one run of vectors); the rest goes
+// by element (k_dropout).
 #include <algorithm>
 
 #include "leaf_ops.h"
@@ -40,40 +47,125 @@ __device__ __forceinline__ uint32_t field_of(const uint4& r, int j) {
   return (j & 1) ? w >> 16 : w & 0xffffu;
 }
 
-// A block of eight units a thread.
+struct Dropout {
+  uint32_t threshold;
+  float scale;
+  uint64_t seed, offset;
+};
+
 template <typename T>
-__global__ __launch_bounds__(THREADS) void k_dropout(const T* x, int64_t ldx, int64_t rows, int64_t cols,
-                                                     uint32_t threshold, float scale, uint64_t seed,
-                                                     uint64_t offset, int by_row, T* out, int64_t ldo) {
-  const int64_t units = by_row ? rows : rows * cols;
-  const int64_t blocks = (units + 7) / 8;
+__device__ __forceinline__ T kept(T x, bool keep, float scale) {
+  return keep ? (T)((float)x * scale) : (T)0.0f;
+}
+
+// `total` elements in a row: a block of eight a thread, as 16-byte vectors.
+template <typename T>
+__global__ __launch_bounds__(THREADS) void k_dropout_flat(const T* x, int64_t total, Dropout d, T* out) {
+  const int64_t blocks = (total + 7) / 8;
   for (int64_t b = blockIdx.x * (int64_t)THREADS + threadIdx.x; b < blocks;
        b += (int64_t)gridDim.x * THREADS) {
-    const uint4 r = philox((uint64_t)b, offset, seed);
-    for (int j = 0; j < 8; ++j) {
-      const int64_t e = b * 8 + j;
-      if (e >= units) break;
-      const bool keep = field_of(r, j) >= threshold;
-      if (by_row) {
-        for (int64_t c = 0; c < cols; ++c)
-          out[e * ldo + c] = keep ? (T)((float)x[e * ldx + c] * scale) : (T)0.0f;
-      } else {
-        const int64_t n = e / cols, c = e % cols;
-        out[n * ldo + c] = keep ? (T)((float)x[n * ldx + c] * scale) : (T)0.0f;
+    const uint4 r = philox((uint64_t)b, d.offset, d.seed);
+    T v[8];
+    if (b * 8 + 8 <= total) {
+      __builtin_memcpy(v, x + b * 8, sizeof(v));
+#pragma unroll
+      for (int j = 0; j < 8; ++j) v[j] = kept(v[j], field_of(r, j) >= d.threshold, d.scale);
+      __builtin_memcpy(out + b * 8, v, sizeof(v));
+    } else {
+#pragma unroll
+      for (int j = 0; j < 8; ++j)
+        if (b * 8 + j < total) out[b * 8 + j] = kept(x[b * 8 + j], field_of(r, j) >= d.threshold, d.scale);
+    }
+  }
+}
+
+// Whole rows of 1 << col_bits columns without gaps, a vector a thread.  Eight rows share a
+// block of the generator, so 8 columns / V threads make the same one: no more work than
+// the memory leaves time for.
+template <typename T>
+__global__ __launch_bounds__(THREADS) void k_dropout_rows(const T* x, int64_t total, int col_bits,
+                                                          Dropout d, T* out) {
+  constexpr int V = 16 / (int)sizeof(T);
+  for (int64_t i = (blockIdx.x * (int64_t)THREADS + threadIdx.x) * V; i < total;
+       i += (int64_t)gridDim.x * THREADS * V) {
+    const int64_t row = i >> col_bits;
+    const uint4 r = philox((uint64_t)(row >> 3), d.offset, d.seed);
+    const uint64_t lo = (uint64_t)r.y << 32 | r.x, hi = (uint64_t)r.w << 32 | r.z;
+    // V consecutive elements of rows of a power of two reach over at most 8 rows of one
+    // block: V <= 8, and a block is 8 columns long or a multiple of it
+    T v[V];
+    if (i + V <= total) {
+      __builtin_memcpy(v, x + i, sizeof(v));
+#pragma unroll
+      for (int e = 0; e < V; ++e) {
+        const int j = (int)((i + e) >> col_bits) & 7;
+        const uint32_t f = (uint32_t)((j < 4 ? lo : hi) >> ((j & 3) * 16)) & 0xffffu;
+        v[e] = kept(v[e], f >= d.threshold, d.scale);
+      }
+      __builtin_memcpy(out + i, v, sizeof(v));
+    } else {
+      for (int e = 0; e < V && i + e < total; ++e) {
+        const int j = (int)((i + e) >> col_bits) & 7;
+        const uint32_t f = (uint32_t)((j < 4 ? lo : hi) >> ((j & 3) * 16)) & 0xffffu;
+        out[i + e] = kept(x[i + e], f >= d.threshold, d.scale);
       }
     }
   }
 }
 
+// Any strides: a block of eight units a thread, or a block's eight rows a wave.
 template <typename T>
-void launch(const void* x, int64_t ldx, int64_t rows, int64_t cols, uint32_t threshold, uint64_t seed,
-            uint64_t offset, int by_row, void* out, int64_t ldo, hipStream_t s) {
-  const int64_t blocks = ((by_row ? rows : rows * cols) + 7) / 8;
-  const unsigned grid = (unsigned)std::min<int64_t>((blocks + THREADS - 1) / THREADS, 65536);
-  // threshold 65536 keeps nothing: the scale is then of no effect
-  const float scale = threshold < 65536 ? (float)(65536.0 / (65536.0 - (double)threshold)) : 0.0f;
-  k_dropout<T><<<grid, THREADS, 0, s>>>((const T*)x, ldx, rows, cols, threshold, scale, seed, offset,
-                                        by_row, (T*)out, ldo);
+__global__ __launch_bounds__(THREADS) void k_dropout(const T* x, int64_t ldx, int64_t rows, int64_t cols,
+                                                     Dropout d, int by_row, T* out, int64_t ldo) {
+  if (by_row) {
+    const int lane = threadIdx.x & 63;
+    const int64_t blocks = (rows + 7) / 8, waves = (int64_t)gridDim.x * (THREADS / 64);
+    for (int64_t b = blockIdx.x * (int64_t)(THREADS / 64) + (threadIdx.x >> 6); b < blocks; b += waves) {
+      const uint4 r = philox((uint64_t)b, d.offset, d.seed);
+      const int here = (int)min((int64_t)8, rows - b * 8);
+      for (int j = 0; j < here; ++j) {
+        const bool keep = field_of(r, j) >= d.threshold;
+        const T* const from = x + (b * 8 + j) * ldx;
+        T* const to = out + (b * 8 + j) * ldo;
+        for (int64_t c = lane; c < cols; c += 64) to[c] = kept(from[c], keep, d.scale);
+      }
+    }
+    return;
+  }
+  const int64_t units = rows * cols, blocks = (units + 7) / 8;
+  for (int64_t b = blockIdx.x * (int64_t)THREADS + threadIdx.x; b < blocks;
+       b += (int64_t)gridDim.x * THREADS) {
+    const uint4 r = philox((uint64_t)b, d.offset, d.seed);
+    int64_t n = b * 8 / cols, c = b * 8 - n * cols;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      if (b * 8 + j >= units) break;
+      out[n * ldo + c] = kept(x[n * ldx + c], field_of(r, j) >= d.threshold, d.scale);
+      if (++c == cols) c = 0, ++n;
+    }
+  }
+}
+
+unsigned grid_of(int64_t threads) {
+  return (unsigned)std::max<int64_t>(1, std::min<int64_t>((threads + THREADS - 1) / THREADS, 1 << 20));
+}
+
+template <typename T>
+void launch(const void* x, int64_t ldx, int64_t rows, int64_t cols, const Dropout& d, int by_row,
+            void* out, int64_t ldo, hipStream_t s) {
+  const bool flat = ldx == cols && ldo == cols;
+  constexpr int V = 16 / sizeof(T);
+  if (flat && !by_row) {
+    k_dropout_flat<T><<<grid_of((rows * cols + 7) / 8), THREADS, 0, s>>>((const T*)x, rows * cols, d, (T*)out);
+  } else if (flat && (cols & (cols - 1)) == 0 && cols < ((int64_t)1 << 31)) {
+    int bits = 0;
+    while (((int64_t)1 << bits) < cols) ++bits;
+    k_dropout_rows<T><<<grid_of((rows * cols + V - 1) / V), THREADS, 0, s>>>((const T*)x, rows * cols, bits,
+                                                                             d, (T*)out);
+  } else {
+    const int64_t threads = by_row ? (rows + 7) / 8 * 64 : (rows * cols + 7) / 8;
+    k_dropout<T><<<grid_of(threads), THREADS, 0, s>>>((const T*)x, ldx, rows, cols, d, by_row, (T*)out, ldo);
+  }
 }
 
 }  // namespace
@@ -81,12 +173,15 @@ void launch(const void* x, int64_t ldx, int64_t rows, int64_t cols, uint32_t thr
 void launch_dropout(const void* x, int64_t ldx, int64_t rows, int64_t cols, int32_t dtype,
                     uint32_t threshold, uint64_t seed, uint64_t offset, int by_row, void* out,
                     int64_t ldo, hipStream_t s) {
+  // threshold 65536 keeps nothing: the scale is then of no effect
+  const float scale = threshold < 65536 ? (float)(65536.0 / (65536.0 - (double)threshold)) : 0.0f;
+  const Dropout d{threshold, scale, seed, offset};
   if (dtype == LGBM_HIP_DTYPE_F32)
-    launch<float>(x, ldx, rows, cols, threshold, seed, offset, by_row, out, ldo, s);
+    launch<float>(x, ldx, rows, cols, d, by_row, out, ldo, s);
   else if (dtype == LGBM_HIP_DTYPE_BF16)
-    launch<__bf16>(x, ldx, rows, cols, threshold, seed, offset, by_row, out, ldo, s);
+    launch<__bf16>(x, ldx, rows, cols, d, by_row, out, ldo, s);
   else
-    launch<_Float16>(x, ldx, rows, cols, threshold, seed, offset, by_row, out, ldo, s);
+    launch<_Float16>(x, ldx, rows, cols, d, by_row, out, ldo, s);
 }
 
 }  // namespace lgbm

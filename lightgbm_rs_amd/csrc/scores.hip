@@ -180,6 +180,11 @@ __global__ __launch_bounds__(THREADS) void k_scores_thread(ScoreArgs a, uint32_t
 
 enum { WHOLE, PART, FINISH };
 
+// Long rows: chunks of two vectors a lane in blocks of 1024, so that few blocks look at the
+// same history (64 x 128007 bf16: 37 us; one vector a lane 50 us); blocks of 256 where those
+// would leave CUs without one.
+constexpr int CHUNK_LANES = 1024, SMALL_LANES = 256, CHUNK_BYTES = 32;
+
 // LANES of one row, each with NV vectors of VW neighbouring classes, LANES * NV * VW classes
 // from c0 on.
 template <typename T, int LANES, int NV, int VW, int MODE>
@@ -225,17 +230,25 @@ __global__ __launch_bounds__(LANES < THREADS ? THREADS : LANES) void k_scores_ro
     const T* const bias = a.bias ? (const T*)a.bias + c0 : nullptr;
     const bool seen = row.h1 > row.h0;
     A s[NV][VW];
+    T v[NV][VW], b[NV][VW];
+    uint32_t allowed[NV];
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
       const int j = (i * LANES + lane) * VW;
-      T v[VW];
-      if (j + VW <= V)
-        __builtin_memcpy(v, x + j, sizeof(v));
+      const bool full = j + VW <= V;
+      if (full)
+        __builtin_memcpy(v[i], x + j, sizeof(v[i]));
       else
 #pragma unroll
-        for (int e = 0; e < VW; ++e) v[e] = j + e < V ? x[j + e] : (T)0.0f;
+        for (int e = 0; e < VW; ++e) v[i][e] = j + e < V ? x[j + e] : (T)0.0f;
+      if (bias && full)
+        __builtin_memcpy(b[i], bias + j, sizeof(b[i]));
+      else
 #pragma unroll
-      for (int e = 0; e < VW; ++e) s[i][e] = (A)v[e];
+        for (int e = 0; e < VW; ++e) b[i][e] = bias && j + e < V ? bias[j + e] : (T)0.0f;
+      // VW divides 32 and c0 is a multiple of 32, so the bits are of one word
+      allowed[i] = row.mask && j < V ? row.mask[(c0 + j) >> 5] >> (j & 31) : ~0u;
+      if (!full) allowed[i] &= j < V ? (1u << (V - j)) - 1 : 0u;
     }
     if (seen) {
 #pragma unroll
@@ -252,16 +265,8 @@ __global__ __launch_bounds__(LANES < THREADS ? THREADS : LANES) void k_scores_ro
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
       const int j = (i * LANES + lane) * VW;
-      const bool full = j + VW <= V;
-      T b[VW];
-      if (bias && full)
-        __builtin_memcpy(b, bias + j, sizeof(b));
-      else
 #pragma unroll
-        for (int e = 0; e < VW; ++e) b[e] = bias && j + e < V ? bias[j + e] : (T)0.0f;
-      // VW divides 32 and c0 is a multiple of 32, so the bits are of one word
-      uint32_t allowed = row.mask && j < V ? row.mask[(c0 + j) >> 5] >> (j & 31) : ~0u;
-      if (!full) allowed &= j < V ? (1u << (V - j)) - 1 : 0u;
+      for (int e = 0; e < VW; ++e) s[i][e] = (A)v[i][e];
       if (seen) {
         uint32_t c[VW], any = 0;
         __builtin_memcpy(c, count + j, sizeof(c));  // behind V: zeros
@@ -275,7 +280,7 @@ __global__ __launch_bounds__(LANES < THREADS ? THREADS : LANES) void k_scores_ro
       }
 #pragma unroll
       for (int e = 0; e < VW; ++e) {
-        s[i][e] = (allowed >> e) & 1 ? s[i][e] + (A)b[e] : -INFINITY;
+        s[i][e] = (allowed[i] >> e) & 1 ? s[i][e] + (A)b[i][e] : -INFINITY;
         top = top_of(top, s[i][e]);
       }
     }
@@ -335,9 +340,6 @@ void launch_row(const ScoreArgs& a, int chunks, hipStream_t s) {
       <<<(unsigned)std::min<int64_t>(blocks, 1 << 20), TEAMS * LANES, 0, s>>>(a, chunks);
 }
 
-// Long rows: chunks of two vectors a lane in blocks of 1024, so that few blocks look at the
-// same history; smaller ones where those would leave CUs without a block.
-constexpr int CHUNK_LANES = 1024, SMALL_LANES = 256, CHUNK_BYTES = 32;
 int chunk_lanes(int64_t rows, int32_t classes, int e) {
   const int chunk = CHUNK_LANES * (CHUNK_BYTES / e);
   return rows * ((classes + chunk - 1) / chunk) < 256 ? SMALL_LANES : CHUNK_LANES;
