@@ -56,7 +56,8 @@ def check():
     (65, 7, 31, "lost", 2), (4096, 1, 255, "skew", 0), (4097, 2, 256, "even", 0),
     (20011, 3, 63, "lost", 1), (100003, 1, 1000, "even", 0), (30000, 1, 4095, "skew", 0),
     (50000, 1, 1, "lost", 0), (3000, 300, 15, "even", 0), (300007, 2, 31, "one", 0),
-    (1025, 65, 127, "lost", 3)])
+    (1025, 65, 127, "lost", 3), (8192, 2, 100, "lost", 0), (8193, 2, 100, "skew", 0),
+    (2200001, 1, 255, "lost", 0), (4200000, 1, 3, "even", 1)])
 def test_groups(check, rows, trees, leaves, shape, pad):
     check("groups", rows=rows, trees=trees, leaves=leaves, shape=shape, pad=pad)
 
@@ -110,7 +111,8 @@ def test_plain(check, name):
     (1000, 2, 0.3, "row", 0, 11, 3), (999, 1, 0.5, "row", 0, 12, 0), (257, 7, 0.2, "row", 1, 13, 0),
     (130, 100, 0.5, "row", 4, 14, 0), (50, 16, 0.0, "element", 0, 15, 0),
     (50, 16, 1.0, "element", 0, 16, 0), (50, 3, 1.0, "row", 0, 17, 0),
-    (600, 1024, 0.25, "element", 0, 18, 0), (70000, 2, 0.4, "row", 0, 19, 0)])
+    (600, 1024, 0.25, "element", 0, 18, 0), (1001, 4, 0.2, "row", 0, 20, 0),
+    (515, 8, 0.2, "row", 0, 21, 0), (77, 64, 0.2, "row", 0, 22, 5), (9, 1, 0.2, "row", 0, 23, 0), (70000, 2, 0.4, "row", 0, 19, 0)])
 def test_dropout(check, rows, cols, p, by, pad, seed, offset, dtype):
     check("dropout", rows=rows, cols=cols, p=p, by=by, pad=pad, seed=seed, offset=offset, dtype=dtype)
 

@@ -45,10 +45,10 @@ def groups(lib, leaf=A, ld=3, rows=10, trees=3, leaves=7, order=B, begin=D, coun
     (dict(rows=2 ** 31), CAPABILITY, "2^31"), (dict(trees=65536, ld=65536), CAPABILITY, "65535"),
     (dict(leaves=4096), CAPABILITY, "4095"), (dict(ld=2), INVALID, "stride"),
     (dict(leaf=None), INVALID, "null leaf"), (dict(count=None), INVALID, "null leaf"),
-    (dict(order=B + 2), INVALID, "aligned"), (dict(ws=None), INVALID, "null workspace"),
-    (dict(ws=W + 4), INVALID, "16-byte"), (dict(size=8), MISMATCH, "smaller"),
+    (dict(order=B + 2), INVALID, "aligned"), (dict(rows=10 ** 6, ws=None), INVALID, "null workspace"),
+    (dict(rows=10 ** 6, ws=W + 4), INVALID, "16-byte"), (dict(rows=10 ** 6, size=8), MISMATCH, "smaller"),
     (dict(order=A + 40), INVALID, "overlap"), (dict(count=D + 40), INVALID, "overlap"),
-    (dict(ws=A - 64 + 16), INVALID, "overlap"), (dict(ld=2 ** 41), INVALID, "stride")])
+    (dict(rows=10 ** 6, ws=A - 64), INVALID, "overlap"), (dict(ld=2 ** 41), INVALID, "stride")])
 def test_groups_refused(lib, change, code, text):
     refused(lib, groups(lib, **change), code, text)
 
