@@ -1,0 +1,221 @@
+// leaf_mma.h — what the kernels of the leaves' linear maps share: element types and their
+// matrix instructions, tiles of a leaf's rows, and tiles of operands in LDS.
+#pragma once
+
+#include "leaf_ops.h"
+
+#include "../../include/lgbm_hip.h"
+
+namespace lgbm {
+namespace mma {
+
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef short s16x4 __attribute__((ext_vector_type(4)));
+typedef __bf16 b16x8 __attribute__((ext_vector_type(8)));
+typedef _Float16 h16x8 __attribute__((ext_vector_type(8)));
+typedef unsigned int u32x4 __attribute__((ext_vector_type(4)));
+
+// An element type: how many of them 16 bytes hold, and the matrix instruction over
+// fragments of 16 bytes a lane (lane l: row or column l % 16 and, of a step's 4 chunks of
+// the contraction, chunk l / 16).  Lane l of the result holds rows 4 (l / 16) .. + 4 of the
+// first operand and column l % 16 of the second.  Products and sums are float32; a 16-bit
+// product is exact in it.
+template <typename T>
+struct El;
+template <>
+struct El<float> {
+  static constexpr int V = 4;
+  static __device__ __forceinline__ u32x4 ones() { return u32x4{0x3f800000u, 0x3f800000u, 0x3f800000u, 0x3f800000u}; }
+  static __device__ __forceinline__ f32x4 mfma(u32x4 a, u32x4 b, f32x4 c) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+      c = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(a[j]), __uint_as_float(b[j]), c, 0, 0, 0);
+    return c;
+  }
+};
+template <>
+struct El<__bf16> {
+  static constexpr int V = 8;
+  static __device__ __forceinline__ u32x4 ones() { return u32x4{0x3f803f80u, 0x3f803f80u, 0x3f803f80u, 0x3f803f80u}; }
+  static __device__ __forceinline__ f32x4 mfma(u32x4 a, u32x4 b, f32x4 c) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(b16x8, a),
+                                                   __builtin_bit_cast(b16x8, b), c, 0, 0, 0);
+  }
+};
+template <>
+struct El<_Float16> {
+  static constexpr int V = 8;
+  static __device__ __forceinline__ u32x4 ones() { return u32x4{0x3c003c00u, 0x3c003c00u, 0x3c003c00u, 0x3c003c00u}; }
+  static __device__ __forceinline__ f32x4 mfma(u32x4 a, u32x4 b, f32x4 c) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(h16x8, a),
+                                                  __builtin_bit_cast(h16x8, b), c, 0, 0, 0);
+  }
+};
+
+// 16 bytes of elements p[0 .. valid), zeros behind them; nothing behind `valid` is read.
+// gfx950 loads 16 bytes from any address, so rows need no alignment.
+template <typename T>
+__device__ __forceinline__ u32x4 load16(const T* p, int valid) {
+  u32x4 v = {0, 0, 0, 0};
+  if (valid >= El<T>::V) {
+    __builtin_memcpy(&v, p, 16);
+  } else if (valid > 0) {
+    T e[El<T>::V];
+#pragma unroll
+    for (int j = 0; j < El<T>::V; ++j) e[j] = j < valid ? p[j] : (T)0.0f;
+    __builtin_memcpy(&v, e, 16);
+  }
+  return v;
+}
+
+template <typename T>
+__device__ __forceinline__ u32x4 load16(const T* p) {
+  u32x4 v;
+  __builtin_memcpy(&v, p, 16);
+  return v;
+}
+
+// Four neighbouring results, `valid` of them in the row.
+template <typename T>
+__device__ __forceinline__ void store4(T* p, f32x4 v, int valid) {
+  T e[4];
+#pragma unroll
+  for (int j = 0; j < 4; ++j) e[j] = (T)v[j];
+  if (valid >= 4) {
+    __builtin_memcpy(p, e, sizeof(e));
+  } else {
+#pragma unroll
+    for (int j = 0; j < 3; ++j)
+      if (j < valid) p[j] = e[j];
+  }
+}
+
+// ---- tiles of rows -------------------------------------------------------------------------
+
+struct RowTile {
+  int leaf;   // -1: rows of the tree that are in no leaf
+  int first;  // position in the tree's order
+  int rows;   // 0: there is no such tile
+};
+
+// Tile number `mt` of a tree: the leaves' rows in tiles of `bm`, then the rows in no leaf.
+// Every thread of the block takes part; counts and begins are held within [0, rows], so
+// that a wrong table cannot reach outside the order.
+template <int THREADS>
+__device__ RowTile find_tile(const LeafGroups& g, int tree, int mt, int bm) {
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  __shared__ int wave_tiles[THREADS / 64];
+  __shared__ int wave_rows[THREADS / 64];
+  __shared__ RowTile found;
+  const int32_t* count = g.count + (int64_t)tree * g.leaves;
+  const int32_t* begin = g.begin + (int64_t)tree * g.leaves;
+  int tiles_before = 0;
+  int64_t rows_before = 0;
+  if (tid == 0) found = RowTile{-1, 0, 0};
+  for (int l0 = 0; l0 < g.leaves; l0 += THREADS) {
+    const int l = l0 + tid;
+    int c = 0;
+    if (l < g.leaves) c = min(max(count[l], 0), g.rows);
+    // of 64 leaves at most 2^6 times 2^31 rows: held back to the rows there are, which
+    // only counts that exceed them reach
+    const int tiles = (int)(((int64_t)c + bm - 1) / bm);
+    int incl = tiles, rows = c;
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) {
+      const int up = __shfl_up(incl, d), r = __shfl_xor(rows, d);
+      if (lane >= d) incl += up;
+      rows = (int)min((int64_t)rows + r, (int64_t)g.rows);
+    }
+    __syncthreads();
+    if (lane == 63) {
+      wave_tiles[wave] = incl;
+      wave_rows[wave] = rows;
+    }
+    __syncthreads();
+    int base = tiles_before;
+#pragma unroll
+    for (int w = 0; w < THREADS / 64; ++w) {
+      if (w < wave) base += wave_tiles[w];
+      tiles_before += wave_tiles[w];
+      rows_before += wave_rows[w];
+    }
+    const int excl = base + incl - tiles;
+    if (mt >= excl && mt < excl + tiles) {
+      const int b = min(max(begin[l], 0), g.rows - c), at = (mt - excl) * bm;
+      found = RowTile{l, b + at, min(bm, c - at)};
+    }
+    if (mt < tiles_before) break;
+  }
+  if (mt >= tiles_before && rows_before < g.rows && tid == 0) {
+    const int64_t at = rows_before + (int64_t)(mt - tiles_before) * bm;
+    if (at < g.rows) found = RowTile{-1, (int)at, (int)min((int64_t)bm, g.rows - at)};
+  }
+  __syncthreads();
+  return found;
+}
+
+// Blocks an upper bound of tiles of a tree needs.
+inline int64_t row_tiles(const LeafGroups& g, int64_t bm) { return (g.rows + bm - 1) / bm + g.leaves + 1; }
+
+// The row at a position of a tree's order, -1 for an entry outside the matrix.
+__device__ __forceinline__ int row_at(const LeafGroups& g, int tree, int position) {
+  const int n = g.order[(int64_t)tree * g.rows + position];
+  return n >= 0 && n < g.rows ? n : -1;
+}
+
+// ---- tiles in LDS --------------------------------------------------------------------------
+
+// The swizzle of a contraction-major tile: the rows that a transposing read touches at once
+// land in different banks.
+template <typename T>
+__device__ __forceinline__ int cm_swizzle(int row) {
+  return sizeof(T) == 2 ? ((row & 3) | ((row >> 1) & 4)) : ((row >> 2) & 3);
+}
+
+// Byte of a 16-byte chunk of a tile whose rows hold 128 bytes of the contraction: [ROWS][8].
+__device__ __forceinline__ int kc_at(int row, int chunk) {
+  return row * 128 + ((chunk ^ (row & 7)) << 4);
+}
+// The same for a tile stored with the contraction as the slow index: [128 bytes' worth][COLS].
+template <typename T, int COLS>
+__device__ __forceinline__ int cm_at(int row, int chunk) {
+  constexpr int UNITS = COLS / 16, PER = sizeof(T);  // a unit: 16 columns; its chunks of 16 bytes
+  const int unit = chunk / PER, in = chunk % PER;
+  return row * (COLS * (int)sizeof(T)) + (((unit ^ (cm_swizzle<T>(row) & (UNITS - 1))) * PER + in) << 4);
+}
+
+// A lane's fragment of 16 rows from row0 on, half `step` of the tile's contraction.
+__device__ __forceinline__ u32x4 kc_frag(const char* tile, int row0, int step, int lane) {
+  return *reinterpret_cast<const u32x4*>(tile + kc_at(row0 + (lane & 15), step * 4 + (lane >> 4)));
+}
+
+template <typename T, int COLS>
+__device__ __forceinline__ u32x4 cm_frag(const char* tile, int col0, int step, int lane) {
+  const int q = lane >> 4, l = lane & 15, unit = col0 / 16;
+  constexpr int UNITS = COLS / 16, UB = 16 * (int)sizeof(T), ROW = COLS * (int)sizeof(T);
+  u32x4 out;
+  if constexpr (sizeof(T) == 2) {
+    // a transposing read: within 16 lanes, lane l gives row l / 4, columns 4 (l % 4) .. + 4
+    // and gets column l of the four rows
+    typedef __attribute__((address_space(3))) s16x4* lds_ptr;
+    s16x4 v[2];
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const int row = step * 32 + q * 8 + h * 4 + (l >> 2);
+      const int at = row * ROW + (unit ^ (cm_swizzle<T>(row) & (UNITS - 1))) * UB + (l & 3) * 8;
+      v[h] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_ptr)const_cast<char*>(tile + at));
+    }
+    __builtin_memcpy(&out, v, 16);
+  } else {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const int row = step * 16 + q * 4 + j;
+      const int at = row * ROW + (unit ^ (cm_swizzle<T>(row) & (UNITS - 1))) * UB + l * 4;
+      out[j] = *reinterpret_cast<const uint32_t*>(tile + at);
+    }
+  }
+  return out;
+}
+
+}  // namespace mma
+}  // namespace lgbm

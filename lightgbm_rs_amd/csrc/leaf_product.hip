@@ -4,228 +4,66 @@
 // Rows come grouped by leaf (leaf_groups.hip, or the layout of a grown tree), so every leaf
 // is a matrix product of its own, of as many rows as it holds: a block finds its leaf from
 // the counts on the device and gathers its rows through the order.  One tree writes its
-// rows directly; several write float32 planes [tree][row] that k_sum_trees adds in the
-// trees' order, so results never depend on the order of blocks.
-#include "leaf_ops.h"
-
+// rows directly; several write float32 planes [tree][row] that k_sum_trees adds, so results
+// never depend on the order of blocks.
 #include <algorithm>
 
-#include "../../include/lgbm_hip.h"
+#include "leaf_mma.h"
 
 namespace lgbm {
 namespace {
 
-typedef float f32x4 __attribute__((ext_vector_type(4)));
-typedef short s16x4 __attribute__((ext_vector_type(4)));
-typedef __bf16 b16x8 __attribute__((ext_vector_type(8)));
-typedef _Float16 h16x8 __attribute__((ext_vector_type(8)));
-typedef unsigned int u32x4 __attribute__((ext_vector_type(4)));
+using namespace mma;
 
 constexpr int THREADS = 256;
 
-// An element type: how many of them 16 bytes hold, and the matrix instruction over
-// fragments of 16 bytes a lane (lane l: row or column l % 16 and, of a step's 4 chunks of
-// the contraction, chunk l / 16).  Lane l of the result holds rows 4 (l / 16) .. + 4 of the
-// first operand and column l % 16 of the second.
-template <typename T>
-struct El;
-template <>
-struct El<float> {
-  static constexpr int V = 4;
-  static __device__ __forceinline__ float to(float v) { return v; }
-  static __device__ __forceinline__ float from(float v) { return v; }
-  static __device__ __forceinline__ f32x4 mfma(u32x4 a, u32x4 b, f32x4 c) {
-#pragma unroll
-    for (int j = 0; j < 4; ++j)
-      c = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(a[j]), __uint_as_float(b[j]), c, 0, 0, 0);
-    return c;
-  }
-};
-template <>
-struct El<__bf16> {
-  static constexpr int V = 8;
-  static __device__ __forceinline__ float to(__bf16 v) { return (float)v; }
-  static __device__ __forceinline__ __bf16 from(float v) { return (__bf16)v; }
-  static __device__ __forceinline__ f32x4 mfma(u32x4 a, u32x4 b, f32x4 c) {
-    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(b16x8, a),
-                                                   __builtin_bit_cast(b16x8, b), c, 0, 0, 0);
-  }
-};
-template <>
-struct El<_Float16> {
-  static constexpr int V = 8;
-  static __device__ __forceinline__ float to(_Float16 v) { return (float)v; }
-  static __device__ __forceinline__ _Float16 from(float v) { return (_Float16)v; }
-  static __device__ __forceinline__ f32x4 mfma(u32x4 a, u32x4 b, f32x4 c) {
-    return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(h16x8, a),
-                                                  __builtin_bit_cast(h16x8, b), c, 0, 0, 0);
-  }
-};
-
-// 16 bytes of elements p[0 .. valid), zeros behind them; nothing behind `valid` is read.
-template <typename T, bool VEC>
-__device__ __forceinline__ u32x4 load16(const T* p, int valid) {
-  u32x4 v = {0, 0, 0, 0};
-  if (valid >= El<T>::V) {
-    if (VEC)
-      v = *reinterpret_cast<const u32x4*>(p);
-    else
-      __builtin_memcpy(&v, p, 16);
-  } else if (valid > 0) {
-    T e[El<T>::V];
-#pragma unroll
-    for (int j = 0; j < El<T>::V; ++j) e[j] = j < valid ? p[j] : (T)0.0f;
-    __builtin_memcpy(&v, e, 16);
-  }
-  return v;
-}
-
-// ---- tiles of rows -------------------------------------------------------------------------
-
-struct RowTile {
-  int leaf;   // -1: rows of the tree that are in no leaf
-  int first;  // position in the tree's order
-  int rows;   // 0: there is no such tile
-};
-
-// Tile number `mt` of a tree: the leaves' rows in tiles of BM, then the rows in no leaf.
-// Every thread of the block takes part; counts and begins are held within [0, rows], so
-// that a wrong table cannot reach outside the order.
-template <int BM>
-__device__ RowTile find_tile(const LeafGroups& g, int tree, int mt, RowTile* shared) {
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-  __shared__ int wave_tiles[THREADS / 64];
-  __shared__ int wave_rows[THREADS / 64];
-  const int32_t* count = g.count + (int64_t)tree * g.leaves;
-  const int32_t* begin = g.begin + (int64_t)tree * g.leaves;
-  int tiles_before = 0;
-  int64_t rows_before = 0;
-  if (tid == 0) *shared = RowTile{-1, 0, 0};
-  for (int l0 = 0; l0 < g.leaves; l0 += THREADS) {
-    const int l = l0 + tid;
-    int c = 0;
-    if (l < g.leaves) c = min(max(count[l], 0), g.rows);
-    int tiles = (c + BM - 1) / BM, incl = tiles, rows = c;
-    for (int d = 1; d < 64; d <<= 1) {
-      const int up = __shfl_up(incl, d), r = __shfl_xor(rows, d);
-      if (lane >= d) incl += up;
-      rows += r;  // wraps only where the counts exceed the rows: the rest is then empty
-    }
-    __syncthreads();
-    if (lane == 63) {
-      wave_tiles[wave] = incl;
-      wave_rows[wave] = rows;
-    }
-    __syncthreads();
-    int base = tiles_before;
-    for (int w = 0; w < THREADS / 64; ++w) {
-      if (w < wave) base += wave_tiles[w];
-      tiles_before += wave_tiles[w];
-      rows_before += wave_rows[w];
-    }
-    const int excl = base + incl - tiles;
-    if (mt >= excl && mt < excl + tiles) {
-      const int b = min(max(begin[l], 0), g.rows - c), at = (mt - excl) * BM;
-      *shared = RowTile{l, b + at, min(BM, c - at)};
-    }
-    if (mt < tiles_before) break;
-  }
-  if (mt >= tiles_before && rows_before >= 0 && rows_before < g.rows) {
-    const int64_t at = rows_before + (int64_t)(mt - tiles_before) * BM;
-    if (tid == 0 && at < g.rows) *shared = RowTile{-1, (int)at, (int)min((int64_t)BM, g.rows - at)};
-  }
-  __syncthreads();
-  return *shared;
-}
-
-// Blocks an upper bound of tiles of a tree needs.
-int64_t row_tiles(const LeafGroups& g, int bm) {
-  return ((int64_t)g.rows + bm - 1) / bm + g.leaves + 1;
-}
-
 // ---- products over the inputs (y) and over the outputs (dx) ----------------------------------
 
-// The swizzle of a contraction-major tile: the 16 rows that a transposing read touches at
-// once land in different banks.
+// Where the rows of a product go: the output of one tree, or a tree's plane.
 template <typename T>
-__device__ __forceinline__ int cm_swizzle(int row) {
-  return sizeof(T) == 2 ? ((row & 3) | ((row >> 1) & 4)) : ((row >> 2) & 3);
+__device__ __forceinline__ void store_row(const LeafProduct& p, int tree, int n, int col, int cols, f32x4 v) {
+  if (p.g.trees > 1)
+    store4((float*)p.ws + ((int64_t)tree * p.g.rows + n) * cols + col, v, cols - col);
+  else
+    store4((T*)p.out + (int64_t)n * p.ldo + col, v, cols - col);
 }
 
-// A tile in LDS of which lanes read 16 bytes along the contraction: [ROWS][8 chunks].
-__device__ __forceinline__ int kc_at(int row, int chunk) {
-  return row * 128 + ((chunk ^ (row & 7)) << 4);
-}
-// The same, stored with the contraction as the slow index: [128 bytes' worth][COLS].
-template <typename T, int COLS>
-__device__ __forceinline__ int cm_at(int row, int chunk) {
-  constexpr int UNITS = COLS / 16, PER = sizeof(T);  // a unit: 16 columns; its chunks of 16 bytes
-  const int unit = chunk / PER, in = chunk % PER;
-  return row * (COLS * (int)sizeof(T)) + (((unit ^ (cm_swizzle<T>(row) & (UNITS - 1))) * PER + in) << 4);
-}
-
-__device__ __forceinline__ u32x4 kc_frag(const char* tile, int row0, int step, int lane) {
-  return *reinterpret_cast<const u32x4*>(tile + kc_at(row0 + (lane & 15), step * 4 + (lane >> 4)));
-}
-
-template <typename T, int COLS>
-__device__ __forceinline__ u32x4 cm_frag(const char* tile, int col0, int step, int lane) {
-  const int q = lane >> 4, l = lane & 15, unit = col0 / 16;
-  constexpr int UNITS = COLS / 16, UB = 16 * (int)sizeof(T), ROW = COLS * (int)sizeof(T);
-  if constexpr (sizeof(T) == 2) {
-    // a transposing read: within 16 lanes, lane l gives row l / 4, columns 4 (l % 4) .. + 4
-    // and gets column l of the four rows
-    typedef __attribute__((address_space(3))) s16x4* lds_ptr;
-    s16x4 v[2];
+template <typename T>
+__device__ __forceinline__ f32x4 bias4(const T* bias, int col, int cols) {
+  f32x4 v = {0, 0, 0, 0};
+  if (bias)
 #pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      const int row = step * 32 + q * 8 + h * 4 + (l >> 2);
-      const int at = row * ROW + (unit ^ (cm_swizzle<T>(row) & (UNITS - 1))) * UB + (l & 3) * 8;
-      v[h] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_ptr)const_cast<char*>(tile + at));
-    }
-    u32x4 out;
-    __builtin_memcpy(&out, v, 16);
-    return out;
-  } else {
-    u32x4 out;
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const int row = step * 16 + q * 4 + j;
-      const int at = row * ROW + (unit ^ (cm_swizzle<T>(row) & (UNITS - 1))) * UB + l * 4;
-      out[j] = *reinterpret_cast<const uint32_t*>(tile + at);
-    }
-    return out;
-  }
+    for (int e = 0; e < 4; ++e)
+      if (col + e < cols) v[e] = (float)bias[col + e];
+  return v;
 }
 
 // out[row][col] = sum over c of a[row][c] * B(c, col), rows gathered through the order.
 // DX false: B(c, col) = w[leaf][col][c] (c: inputs, col: outputs); DX true: B(c, col) =
 // w[leaf][c][col] (c: outputs, col: inputs).  BM x BN of the output a block, 128 bytes of the
-// contraction a step through LDS, 4 waves in 2 x 2.
-template <typename T, bool DX, bool VEC, int BM, int BN>
+// contraction a step through LDS, GM x 4 / GM waves.  Rows and columns that a tile has
+// more than the product only make results that are not stored, so their loads are those of
+// the last ones; only the end of the contraction needs zeros.
+template <typename T, bool DX, int BM, int BN, int GM>
 __global__ __launch_bounds__(THREADS) void k_leaf_tile(LeafProduct p, int length, int cols,
                                                        int col_tiles) {
   constexpr int V = El<T>::V, BK = 8 * V;  // elements of the contraction a step
-  constexpr int WM = BM / 2, WN = BN / 2;
+  constexpr int GN = 4 / GM, WM = BM / GM, WN = BN / GN;
   constexpr int ACH = BM * 8 / THREADS, BCH = BN * 8 / THREADS;
   __shared__ __align__(16) char lds[2][(BM + BN) * 128];
   __shared__ int32_t row_of[BM];
-  __shared__ RowTile tile;
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const int tree = blockIdx.y;
   const int mt = blockIdx.x / col_tiles, c0 = (blockIdx.x % col_tiles) * BN;
-  const RowTile rt = find_tile<BM>(p.g, tree, mt, &tile);
+  const RowTile rt = find_tile<THREADS>(p.g, tree, mt, BM);
   if (rt.rows == 0) return;
-  for (int r = tid; r < BM; r += THREADS) {
-    int n = -1;
-    if (r < rt.rows) n = p.g.order[(int64_t)tree * p.g.rows + rt.first + r];
-    row_of[r] = (n >= 0 && n < p.g.rows) ? n : -1;
-  }
+  for (int r = tid; r < BM; r += THREADS) row_of[r] = r < rt.rows ? row_at(p.g, tree, rt.first + r) : -1;
   __syncthreads();
   const int64_t leaf = (int64_t)tree * p.g.leaves + rt.leaf;
   const T* const w = (const T*)p.w + (rt.leaf < 0 ? 0 : leaf * p.outputs * (int64_t)p.inputs);
   const T* const src = (const T*)(DX ? p.dy : p.x);
-  const int64_t lds_src = DX ? p.lddy : p.ldx;
+  const int64_t ld = DX ? p.lddy : p.ldx;
+  const int m0 = (wave / GN) * WM, n0 = (wave % GN) * WN;
 
   f32x4 acc[WM / 16][WN / 16];
 #pragma unroll
@@ -235,28 +73,26 @@ __global__ __launch_bounds__(THREADS) void k_leaf_tile(LeafProduct p, int length
 
   if (rt.leaf >= 0) {
     u32x4 ra[ACH], rb[BCH];
-    const T* arow[ACH];
+    const T *arow[ACH], *brow[BCH];
 #pragma unroll
-    for (int i = 0; i < ACH; ++i) {
-      const int n = row_of[(tid + i * THREADS) >> 3];
-      arow[i] = n < 0 ? nullptr : src + (int64_t)n * lds_src;
-    }
+    for (int i = 0; i < ACH; ++i) arow[i] = src + (int64_t)max(row_of[(tid + i * THREADS) >> 3], 0) * ld;
+    if (!DX)
+#pragma unroll
+      for (int i = 0; i < BCH; ++i)
+        brow[i] = w + (int64_t)min(c0 + ((tid + i * THREADS) >> 3), cols - 1) * length;
     auto load = [&](int k0) {
+      const int k = k0 + (tid & 7) * V;
+      const bool whole = k0 + BK <= length;
 #pragma unroll
-      for (int i = 0; i < ACH; ++i) {
-        const int k = k0 + (tid & 7) * V;
-        ra[i] = load16<T, VEC>(arow[i] + k, arow[i] ? length - k : 0);
-      }
+      for (int i = 0; i < ACH; ++i) ra[i] = whole ? load16(arow[i] + k) : load16(arow[i] + k, length - k);
 #pragma unroll
       for (int i = 0; i < BCH; ++i) {
-        const int at = tid + i * THREADS;
         if (DX) {
           constexpr int CH = BN / V;  // chunks a row
-          const int row = k0 + at / CH, col = c0 + at % CH * V;
-          rb[i] = load16<T, VEC>(w + (int64_t)row * cols + col, row < length ? cols - col : 0);
+          const int at = tid + i * THREADS, row = k0 + at / CH, col = c0 + at % CH * V;
+          rb[i] = load16(w + (int64_t)row * cols + col, row < length ? cols - col : 0);
         } else {
-          const int col = c0 + (at >> 3), k = k0 + (at & 7) * V;
-          rb[i] = load16<T, VEC>(w + (int64_t)col * length + k, col < cols ? length - k : 0);
+          rb[i] = whole ? load16(brow[i] + k) : load16(brow[i] + k, length - k);
         }
       }
     };
@@ -274,7 +110,6 @@ __global__ __launch_bounds__(THREADS) void k_leaf_tile(LeafProduct p, int length
         *reinterpret_cast<u32x4*>(buf + BM * 128 + to) = rb[i];
       }
     };
-    const int m0 = (wave >> 1) * WM, n0 = (wave & 1) * WN;
     load(0);
     store(lds[0]);
     __syncthreads();
@@ -284,6 +119,7 @@ __global__ __launch_bounds__(THREADS) void k_leaf_tile(LeafProduct p, int length
       const char *ta = lds[b], *tb = lds[b] + BM * 128;
 #pragma unroll
       for (int step = 0; step < 2; ++step) {
+        if (step == 1 && k0 + BK / 2 >= length) break;
         u32x4 fa[WM / 16], fb[WN / 16];
 #pragma unroll
         for (int i = 0; i < WM / 16; ++i) fa[i] = kc_frag(ta, m0 + 16 * i, step, lane);
@@ -301,120 +137,257 @@ __global__ __launch_bounds__(THREADS) void k_leaf_tile(LeafProduct p, int length
   }
 
   // lane: output row lane % 16, columns 4 (lane / 16) .. + 4 of each 16 x 16
-  const bool planes = p.g.trees > 1;
-  float* const plane = (float*)p.ws + (int64_t)tree * p.g.rows * cols;
   const T* const bias = (!DX && p.b && rt.leaf >= 0) ? (const T*)p.b + leaf * cols : nullptr;
 #pragma unroll
-  for (int i = 0; i < WM / 16; ++i) {
-    const int n = row_of[(wave >> 1) * WM + i * 16 + (lane & 15)];
-    if (n < 0) continue;
+  for (int j = 0; j < WN / 16; ++j) {
+    const int col = c0 + n0 + j * 16 + (lane >> 4) * 4;
+    if (col >= cols) continue;
+    const f32x4 b = bias4(bias, col, cols);
 #pragma unroll
-    for (int j = 0; j < WN / 16; ++j) {
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const int col = c0 + (wave & 1) * WN + j * 16 + (lane >> 4) * 4 + e;
-        if (col >= cols) continue;
-        const float v = acc[i][j][e] + (bias ? El<T>::to(bias[col]) : 0.0f);
-        if (planes)
-          plane[(int64_t)n * cols + col] = v;
-        else
-          ((T*)p.out)[(int64_t)n * p.ldo + col] = El<T>::from(v);
-      }
+    for (int i = 0; i < WM / 16; ++i) {
+      const int n = row_of[m0 + i * 16 + (lane & 15)];
+      if (n >= 0) store_row<T>(p, tree, n, col, cols, acc[i][j] + b);
     }
   }
 }
 
-// The trees' planes added in their order, rounded once.
+// The same for up to 16 NB outputs of a leaf: bound by reading x, which no wave shares with
+// another, so lanes load their fragments straight from memory (16 rows x 64 bytes an
+// instruction; w from the caches), UNROLL steps at a time and without a barrier.  A wave
+// takes ROUNDS times 32 rows.
+template <typename T, int NB>
+__global__ __launch_bounds__(THREADS) void k_leaf_narrow(LeafProduct p) {
+  constexpr int V = El<T>::V, UNROLL = 4, ROUNDS = 2, BM = 4 * 32 * ROUNDS;
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, r = lane & 15, q = lane >> 4;
+  const int tree = blockIdx.y, length = p.inputs, cols = p.outputs;
+  const RowTile rt = find_tile<THREADS>(p.g, tree, blockIdx.x, BM);
+  const int64_t leaf = (int64_t)tree * p.g.leaves + rt.leaf;
+  const T* const w = (const T*)p.w + (rt.leaf < 0 ? 0 : leaf * cols * (int64_t)length);
+  const T* wrow[NB];
+#pragma unroll
+  for (int j = 0; j < NB; ++j) wrow[j] = w + (int64_t)min(j * 16 + r, cols - 1) * length;
+  const T* const bias = (p.b && rt.leaf >= 0) ? (const T*)p.b + leaf * cols : nullptr;
+  f32x4 b[NB];
+#pragma unroll
+  for (int j = 0; j < NB; ++j) b[j] = bias4(bias, j * 16 + q * 4, cols);
+  int n[ROUNDS][2];
+#pragma unroll
+  for (int t = 0; t < ROUNDS; ++t)
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const int at = (t * 4 + wave) * 32 + i * 16 + r;
+      n[t][i] = at < rt.rows ? row_at(p.g, tree, rt.first + at) : -1;
+    }
+#pragma unroll
+  for (int t = 0; t < ROUNDS; ++t) {
+    if ((t * 4 + wave) * 32 >= rt.rows) break;
+    f32x4 acc[2][NB];
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+#pragma unroll
+      for (int j = 0; j < NB; ++j) acc[i][j] = b[j];
+    if (rt.leaf >= 0) {
+      const T* xrow[2];
+#pragma unroll
+      for (int i = 0; i < 2; ++i) xrow[i] = (const T*)p.x + (int64_t)max(n[t][i], 0) * p.ldx;
+      for (int k0 = 0; k0 < length; k0 += 4 * V * UNROLL) {
+        u32x4 fa[UNROLL][2], fb[UNROLL][NB];
+        if (k0 + 4 * V * UNROLL <= length) {
+#pragma unroll
+          for (int u = 0; u < UNROLL; ++u) {
+            const int k = k0 + (u * 4 + q) * V;
+#pragma unroll
+            for (int i = 0; i < 2; ++i) fa[u][i] = load16(xrow[i] + k);
+#pragma unroll
+            for (int j = 0; j < NB; ++j) fb[u][j] = load16(wrow[j] + k);
+          }
+        } else {
+#pragma unroll
+          for (int u = 0; u < UNROLL; ++u) {
+            const int k = k0 + (u * 4 + q) * V;
+#pragma unroll
+            for (int i = 0; i < 2; ++i) fa[u][i] = load16(xrow[i] + k, length - k);
+#pragma unroll
+            for (int j = 0; j < NB; ++j) fb[u][j] = load16(wrow[j] + k, length - k);
+          }
+        }
+#pragma unroll
+        for (int u = 0; u < UNROLL; ++u) {
+          if (k0 + u * 4 * V >= length) break;
+#pragma unroll
+          for (int i = 0; i < 2; ++i)
+#pragma unroll
+            for (int j = 0; j < NB; ++j) acc[i][j] = El<T>::mfma(fb[u][j], fa[u][i], acc[i][j]);
+        }
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+#pragma unroll
+      for (int j = 0; j < NB; ++j) {
+        const int col = j * 16 + q * 4;
+        if (n[t][i] >= 0 && col < cols) store_row<T>(p, tree, n[t][i], col, cols, acc[i][j]);
+      }
+  }
+}
+
+// The trees' planes added, rounded once: 64 elements a block, a quarter of the trees a wave;
+// in float64, since a forest has hundreds of trees.
 template <typename T>
 __global__ __launch_bounds__(THREADS) void k_sum_trees(const float* planes, int64_t rows, int cols,
                                                        int trees, T* out, int64_t ldo) {
+  __shared__ double part[4][64];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int64_t total = rows * cols;
+  const int t0 = (int)((int64_t)trees * wave / 4), t1 = (int)((int64_t)trees * (wave + 1) / 4);
+  for (int64_t e0 = blockIdx.x * (int64_t)64; e0 < total; e0 += (int64_t)gridDim.x * 64) {
+    const int64_t e = e0 + lane;
+    double v = 0;
+    if (e < total) {
+#pragma unroll 8
+      for (int t = t0; t < t1; ++t) v += (double)planes[t * total + e];
+    }
+    part[wave][lane] = v;
+    __syncthreads();
+    if (wave == 0 && e < total)
+      out[e / cols * ldo + e % cols] = (T)(float)(part[0][lane] + part[1][lane] + part[2][lane] + part[3][lane]);
+    __syncthreads();
+  }
+}
+// Few trees: a thread an element.
+template <typename T>
+__global__ __launch_bounds__(THREADS) void k_sum_few_trees(const float* planes, int64_t rows, int cols,
+                                                           int trees, T* out, int64_t ldo) {
   const int64_t total = rows * cols;
   for (int64_t e = blockIdx.x * (int64_t)THREADS + threadIdx.x; e < total;
        e += (int64_t)gridDim.x * THREADS) {
-    float v = 0.0f;
-    for (int t = 0; t < trees; ++t) v += planes[t * total + e];
-    out[e / cols * ldo + e % cols] = El<T>::from(v);
+    double v = 0;
+#pragma unroll 4
+    for (int t = 0; t < trees; ++t) v += (double)planes[t * total + e];
+    out[e / cols * ldo + e % cols] = (T)(float)v;
   }
 }
 
 // ---- gradients of the maps -------------------------------------------------------------------
 
+// Rows a block sums at most, 0: a leaf's rows are not split.  Split sums go to slots in the
+// workspace, [tree][slots][outputs * inputs + outputs], and k_sum_slots adds them.  Leaves
+// differ in size and may be fewer than the CUs, so blocks take about a thousandth of the
+// work; in float32 also no more than 8192 rows, to keep a sum's rounding at that of its
+// slots.
+struct Split {
+  int rows;
+  int64_t slots;  // a tree
+};
+Split dw_split(const LeafProduct& p, int64_t tiles) {
+  const int64_t work = (int64_t)p.g.rows * p.g.trees * tiles;
+  int64_t rows = (work / 1024 + 255) / 256 * 256;
+  rows = std::max<int64_t>(rows, 512);
+  if (p.dtype == LGBM_HIP_DTYPE_F32) rows = std::min<int64_t>(rows, 8192);
+  if (rows >= p.g.rows) return {0, 0};
+  return {(int)rows, row_tiles(p.g, rows)};
+}
+
 // dw[leaf][m][k] = sum over the leaf's rows of dy[row][m] * x[row][k]; db[leaf][m] their sum.
-template <typename T, bool VEC, int BM, int BN>
-__global__ __launch_bounds__(THREADS) void k_leaf_dw(LeafProduct p, int m_tiles, int k_tiles) {
+// BM x BN of a leaf's outputs x inputs a block, 128 bytes' worth of rows a step.
+template <typename T, int BM, int BN, int GM>
+__global__ __launch_bounds__(THREADS) void k_leaf_dw(LeafProduct p, int m_tiles, int k_tiles, Split split) {
   constexpr int V = El<T>::V, BK = 8 * V;  // rows a step
-  constexpr int WM = BM / 2, WN = BN / 2;
-  constexpr int ACH = BM * 8 / THREADS, BCH = BN * 8 / THREADS;
+  constexpr int GN = 4 / GM, WM = BM / GM, WN = BN / GN;
+  constexpr int ACH = (BM * 8 + THREADS - 1) / THREADS, BCH = (BN * 8 + THREADS - 1) / THREADS;
+  constexpr int CA = BM / V, CB = BN / V;  // chunks a row
   __shared__ __align__(16) char lds[2][(BM + BN) * 128];
+  __shared__ int32_t row_of[2][BK];
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-  const int64_t id = blockIdx.x;
-  const int k0 = (int)(id % k_tiles) * BN, m0 = (int)(id / k_tiles % m_tiles) * BM;
-  const int64_t leaf = id / ((int64_t)k_tiles * m_tiles);
-  const int tree = (int)(leaf / p.g.leaves);
-  const int count = min(max(p.g.count[leaf], 0), p.g.rows);
-  const int first = min(max(p.g.begin[leaf], 0), p.g.rows - count);
-  const int32_t* const order = p.g.order + (int64_t)tree * p.g.rows + first;
+  const int tiles = m_tiles * k_tiles, tile = (int)(blockIdx.x % tiles);
+  const int k0 = tile % k_tiles * BN, m0 = tile / k_tiles * BM;
+  const int id = (int)(blockIdx.x / tiles);
+  int tree, first, count;
+  float *dw, *db = nullptr;
+  const int64_t size = (int64_t)p.outputs * p.inputs;
+  if (split.rows) {
+    tree = blockIdx.y;
+    const RowTile rt = find_tile<THREADS>(p.g, tree, id, split.rows);
+    if (rt.rows == 0 || rt.leaf < 0) return;
+    first = rt.first, count = rt.rows;
+    dw = (float*)p.ws + (tree * split.slots + id) * (size + p.outputs);
+    if (p.db) db = dw + size;
+  } else {
+    tree = id / p.g.leaves;
+    count = min(max(p.g.count[id], 0), p.g.rows);
+    first = min(max(p.g.begin[id], 0), p.g.rows - count);
+    dw = p.dw + id * size;
+    if (p.db) db = p.db + (int64_t)id * p.outputs;
+  }
 
   f32x4 acc[WM / 16][WN / 16];
 #pragma unroll
   for (int i = 0; i < WM / 16; ++i)
 #pragma unroll
     for (int j = 0; j < WN / 16; ++j) acc[i][j] = f32x4{0, 0, 0, 0};
-  float bias = 0.0f;
+  f32x4 bias[WM / 16];
+#pragma unroll
+  for (int i = 0; i < WM / 16; ++i) bias[i] = f32x4{0, 0, 0, 0};
+  const bool sums = db && k0 == 0 && wave % GN == 0;  // a product with ones
 
+  // rows of step s in row_of[s & 1]; the loads of a step are two steps behind its rows
+  auto rows = [&](int r0) {
+    if (tid < BK) row_of[(r0 / BK) & 1][tid] = r0 + tid < count ? row_at(p.g, tree, first + r0 + tid) : -1;
+  };
   u32x4 ra[ACH], rb[BCH];
-  auto row_at = [&](int i) {
-    if (i >= count) return -1;
-    const int n = order[i];
-    return n >= 0 && n < p.g.rows ? n : -1;
-  };
   auto load = [&](int r0) {
-    constexpr int CA = BM / V, CB = BN / V;
-#pragma unroll
-    for (int i = 0; i < ACH; ++i) {
-      const int at = tid + i * THREADS, n = row_at(r0 + at / CA), m = m0 + at % CA * V;
-      ra[i] = load16<T, VEC>((const T*)p.dy + (int64_t)n * p.lddy + m, n < 0 ? 0 : p.outputs - m);
-    }
-#pragma unroll
-    for (int i = 0; i < BCH; ++i) {
-      const int at = tid + i * THREADS, n = row_at(r0 + at / CB), k = k0 + at % CB * V;
-      rb[i] = load16<T, VEC>((const T*)p.x + (int64_t)n * p.ldx + k, n < 0 ? 0 : p.inputs - k);
-    }
-  };
-  auto store = [&](char* buf) {
-    constexpr int CA = BM / V, CB = BN / V;
+    const int32_t* const of = row_of[(r0 / BK) & 1];
 #pragma unroll
     for (int i = 0; i < ACH; ++i) {
       const int at = tid + i * THREADS;
+      if (BM * 8 % THREADS != 0 && at >= BM * 8) break;
+      const int n = of[at / CA], m = m0 + at % CA * V;
+      ra[i] = load16((const T*)p.dy + (int64_t)max(n, 0) * p.lddy + m, n < 0 ? 0 : p.outputs - m);
+    }
+#pragma unroll
+    for (int i = 0; i < BCH; ++i) {
+      const int at = tid + i * THREADS;
+      if (BN * 8 % THREADS != 0 && at >= BN * 8) break;
+      const int n = of[at / CB], k = k0 + at % CB * V;
+      rb[i] = load16((const T*)p.x + (int64_t)max(n, 0) * p.ldx + k, n < 0 ? 0 : p.inputs - k);
+    }
+  };
+  auto store = [&](char* buf) {
+#pragma unroll
+    for (int i = 0; i < ACH; ++i) {
+      const int at = tid + i * THREADS;
+      if (BM * 8 % THREADS != 0 && at >= BM * 8) break;
       *reinterpret_cast<u32x4*>(buf + cm_at<T, BM>(at / CA, at % CA)) = ra[i];
     }
 #pragma unroll
     for (int i = 0; i < BCH; ++i) {
       const int at = tid + i * THREADS;
+      if (BN * 8 % THREADS != 0 && at >= BN * 8) break;
       *reinterpret_cast<u32x4*>(buf + BM * 128 + cm_at<T, BN>(at / CB, at % CB)) = rb[i];
     }
   };
   if (count > 0) {
+    rows(0);
+    __syncthreads();
     load(0);
+    rows(BK);
     store(lds[0]);
     __syncthreads();
     for (int r0 = 0, b = 0; r0 < count; r0 += BK, b ^= 1) {
       const bool more = r0 + BK < count;
       if (more) load(r0 + BK);
+      rows(r0 + 2 * BK);  // into the half whose rows are loaded already
       const char *ta = lds[b], *tb = lds[b] + BM * 128;
-      if (p.db && k0 == 0 && tid < BM) {
-        for (int r = 0; r < BK; ++r)
-          bias += El<T>::to(*reinterpret_cast<const T*>(ta + cm_at<T, BM>(r, tid / V) + tid % V * sizeof(T)));
-      }
 #pragma unroll
       for (int step = 0; step < 2; ++step) {
         u32x4 fa[WM / 16], fb[WN / 16];
 #pragma unroll
-        for (int i = 0; i < WM / 16; ++i)
-          fa[i] = cm_frag<T, BM>(ta, (wave >> 1) * WM + 16 * i, step, lane);
+        for (int i = 0; i < WM / 16; ++i) fa[i] = cm_frag<T, BM>(ta, (wave / GN) * WM + 16 * i, step, lane);
 #pragma unroll
-        for (int j = 0; j < WN / 16; ++j)
-          fb[j] = cm_frag<T, BN>(tb, (wave & 1) * WN + 16 * j, step, lane);
+        for (int j = 0; j < WN / 16; ++j) fb[j] = cm_frag<T, BN>(tb, (wave % GN) * WN + 16 * j, step, lane);
+        if (sums)
+#pragma unroll
+          for (int i = 0; i < WM / 16; ++i) bias[i] = El<T>::mfma(El<T>::ones(), fa[i], bias[i]);
 #pragma unroll
         for (int i = 0; i < WM / 16; ++i)
 #pragma unroll
@@ -424,82 +397,150 @@ __global__ __launch_bounds__(THREADS) void k_leaf_dw(LeafProduct p, int m_tiles,
       __syncthreads();
     }
   }
-  float* const dw = p.dw + leaf * p.outputs * (int64_t)p.inputs;
 #pragma unroll
   for (int i = 0; i < WM / 16; ++i) {
-    const int m = m0 + (wave >> 1) * WM + i * 16 + (lane & 15);
+    const int m = m0 + (wave / GN) * WM + i * 16 + (lane & 15);
     if (m >= p.outputs) continue;
+    if (sums && lane < 16) db[m] = bias[i][0];
 #pragma unroll
-    for (int j = 0; j < WN / 16; ++j)
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const int k = k0 + (wave & 1) * WN + j * 16 + (lane >> 4) * 4 + e;
-        if (k < p.inputs) dw[(int64_t)m * p.inputs + k] = acc[i][j][e];
-      }
+    for (int j = 0; j < WN / 16; ++j) {
+      const int k = k0 + (wave % GN) * WN + j * 16 + (lane >> 4) * 4;
+      if (k < p.inputs) store4(dw + (int64_t)m * p.inputs + k, acc[i][j], p.inputs - k);
+    }
   }
-  if (p.db && k0 == 0 && tid < BM && m0 + tid < p.outputs) p.db[leaf * p.outputs + m0 + tid] = bias;
 }
 
-template <typename T, bool VEC>
-void launch(const LeafProduct& p, int what, hipStream_t s) {
-  constexpr int B = 64;
-  if (what == LEAF_PRODUCT_DW) {
-    const int mt = (p.outputs + B - 1) / B, kt = (p.inputs + B - 1) / B;
-    const int64_t blocks = (int64_t)mt * kt * p.g.trees * p.g.leaves;
-    k_leaf_dw<T, VEC, B, B><<<dim3((unsigned)blocks), THREADS, 0, s>>>(p, mt, kt);
+// A leaf's slots added in their order, by `parts` blocks a leaf.
+__global__ __launch_bounds__(THREADS) void k_sum_slots(LeafProduct p, Split split, int parts) {
+  __shared__ int before[THREADS / 64];
+  const int64_t at = blockIdx.x / parts;  // leaf of the forest
+  const int tree = (int)(at / p.g.leaves), leaf = (int)(at - (int64_t)tree * p.g.leaves);
+  const int32_t* const counts = p.g.count + (int64_t)tree * p.g.leaves;
+  int tiles = 0;
+  for (int l = threadIdx.x; l < leaf; l += THREADS)
+    tiles += (int)(((int64_t)min(max(counts[l], 0), p.g.rows) + split.rows - 1) / split.rows);
+#pragma unroll
+  for (int d = 1; d < 64; d <<= 1) tiles += __shfl_xor(tiles, d);
+  if ((threadIdx.x & 63) == 0) before[threadIdx.x >> 6] = tiles;
+  __syncthreads();
+  const int64_t from = (int64_t)before[0] + before[1] + before[2] + before[3];
+  const int64_t num = ((int64_t)min(max(counts[leaf], 0), p.g.rows) + split.rows - 1) / split.rows;
+  const int64_t to = min(from + num, split.slots);
+  const int64_t map = (int64_t)p.outputs * p.inputs, size = map + p.outputs;
+  const int64_t used = p.db ? size : map;
+  const float* const slots = (const float*)p.ws + tree * split.slots * size;
+  for (int64_t e = blockIdx.x % parts * (int64_t)THREADS + threadIdx.x; e < used; e += (int64_t)parts * THREADS) {
+    float v = 0.0f;
+#pragma unroll 4
+    for (int64_t s = from; s < to; ++s) v += slots[s * size + e];
+    if (e < map)
+      p.dw[at * map + e] = v;
+    else
+      p.db[at * p.outputs + (e - map)] = v;
+  }
+}
+
+// ---- which kernel ------------------------------------------------------------------------------
+
+// The tile of outputs x inputs of a leaf that a block of k_leaf_dw sums.
+struct DwShape {
+  int bm, bn;
+};
+DwShape dw_shape(const LeafProduct& p) {
+  if (p.outputs <= 16) return {16, 128};
+  if (p.inputs <= 16) return {128, 16};
+  return {64, 64};
+}
+
+template <typename T, int BM, int BN, int GM>
+void launch_dw(const LeafProduct& p, hipStream_t s) {
+  const int mt = (p.outputs + BM - 1) / BM, kt = (p.inputs + BN - 1) / BN;
+  const Split split = dw_split(p, (int64_t)mt * kt);
+  if (split.rows == 0) {
+    k_leaf_dw<T, BM, BN, GM><<<(unsigned)((int64_t)mt * kt * p.g.trees * p.g.leaves), THREADS, 0, s>>>(p, mt, kt, split);
     return;
   }
-  const bool dx = what == LEAF_PRODUCT_DX;
-  const int length = dx ? p.outputs : p.inputs, cols = dx ? p.inputs : p.outputs;
-  const int ct = (cols + B - 1) / B;
-  const dim3 grid((unsigned)(row_tiles(p.g, B) * ct), (unsigned)p.g.trees);
-  if (dx)
-    k_leaf_tile<T, true, VEC, B, B><<<grid, THREADS, 0, s>>>(p, length, cols, ct);
-  else
-    k_leaf_tile<T, false, VEC, B, B><<<grid, THREADS, 0, s>>>(p, length, cols, ct);
-  if (p.g.trees > 1) {
-    const int64_t total = (int64_t)p.g.rows * cols;
-    const unsigned blocks = (unsigned)std::min<int64_t>((total + THREADS - 1) / THREADS, 4096);
-    k_sum_trees<T><<<blocks, THREADS, 0, s>>>((const float*)p.ws, p.g.rows, cols, p.g.trees,
-                                              (T*)p.out, p.ldo);
-  }
+  k_leaf_dw<T, BM, BN, GM><<<dim3((unsigned)(split.slots * mt * kt), p.g.trees), THREADS, 0, s>>>(p, mt, kt, split);
+  const int64_t size = (int64_t)p.outputs * (p.inputs + 1);
+  const int64_t leaves = (int64_t)p.g.trees * p.g.leaves;
+  const int parts = (int)std::max<int64_t>(1, std::min((size + THREADS - 1) / THREADS, (1 << 16) / leaves));
+  k_sum_slots<<<(unsigned)(leaves * parts), THREADS, 0, s>>>(p, split, parts);
 }
 
-// 16-byte loads: every row of every operand starts on 16 bytes.
-bool aligned16(const LeafProduct& p, int what, size_t e) {
-  auto ok = [&](const void* q, int64_t ld) { return ((uintptr_t)q | (uintptr_t)(ld * (int64_t)e)) % 16 == 0; };
-  if (what == LEAF_PRODUCT_DW) return ok(p.dy, p.lddy) && ok(p.x, p.ldx);
-  return ok(p.w, p.inputs) && (what == LEAF_PRODUCT_DX ? ok(p.dy, p.lddy) : ok(p.x, p.ldx));
+template <typename T, bool DX, int BM, int BN, int GM>
+void launch_tile(const LeafProduct& p, hipStream_t s) {
+  const int length = DX ? p.outputs : p.inputs, cols = DX ? p.inputs : p.outputs;
+  const int ct = (cols + BN - 1) / BN;
+  const dim3 grid((unsigned)(row_tiles(p.g, BM) * ct), (unsigned)p.g.trees);
+  k_leaf_tile<T, DX, BM, BN, GM><<<grid, THREADS, 0, s>>>(p, length, cols, ct);
 }
 
 template <typename T>
-void launch_type(const LeafProduct& p, int what, hipStream_t s) {
-  if (aligned16(p, what, sizeof(T)))
-    launch<T, true>(p, what, s);
-  else
-    launch<T, false>(p, what, s);
+void launch(const LeafProduct& p, int what, hipStream_t s) {
+  if (what == LEAF_PRODUCT_DW) {
+    const DwShape d = dw_shape(p);
+    if (d.bm == 16)
+      launch_dw<T, 16, 128, 1>(p, s);
+    else if (d.bn == 16)
+      launch_dw<T, 128, 16, 4>(p, s);
+    else
+      launch_dw<T, 64, 64, 2>(p, s);
+    return;
+  }
+  const bool dx = what == LEAF_PRODUCT_DX;
+  const int cols = dx ? p.inputs : p.outputs;
+  if (dx) {
+    launch_tile<T, true, 64, 64, 2>(p, s);
+  } else if (cols <= 32) {
+    const dim3 grid((unsigned)row_tiles(p.g, 256), (unsigned)p.g.trees);
+    if (cols <= 16)
+      k_leaf_narrow<T, 1><<<grid, THREADS, 0, s>>>(p);
+    else
+      k_leaf_narrow<T, 2><<<grid, THREADS, 0, s>>>(p);
+  } else {
+    launch_tile<T, false, 64, 64, 2>(p, s);
+  }
+  if (p.g.trees > 1) {
+    const int64_t total = (int64_t)p.g.rows * cols;
+    if (p.g.trees >= 16)
+      k_sum_trees<T><<<(unsigned)std::min<int64_t>((total + 63) / 64, 1 << 20), THREADS, 0, s>>>(
+          (const float*)p.ws, p.g.rows, cols, p.g.trees, (T*)p.out, p.ldo);
+    else
+      k_sum_few_trees<T><<<(unsigned)std::min<int64_t>((total + THREADS - 1) / THREADS, 1 << 16), THREADS, 0, s>>>(
+          (const float*)p.ws, p.g.rows, cols, p.g.trees, (T*)p.out, p.ldo);
+  }
 }
 
 }  // namespace
 
 size_t leaf_product_workspace(const LeafProduct& p, int what) {
-  if (what == LEAF_PRODUCT_DW || p.g.trees <= 1) return 0;
+  if (what == LEAF_PRODUCT_DW) {
+    const DwShape d = dw_shape(p);
+    const Split split = dw_split(p, (int64_t)((p.outputs + d.bm - 1) / d.bm) * ((p.inputs + d.bn - 1) / d.bn));
+    return (size_t)p.g.trees * (size_t)split.slots * (size_t)p.outputs * (size_t)(p.inputs + 1) * 4;
+  }
+  if (p.g.trees <= 1) return 0;
   return (size_t)p.g.trees * (size_t)p.g.rows * (size_t)(what == LEAF_PRODUCT_DX ? p.inputs : p.outputs) * 4;
 }
 
 int64_t leaf_product_blocks(const LeafProduct& p, int what) {
-  const int64_t kt = (p.inputs + 63) / 64, mt = (p.outputs + 63) / 64;
-  if (what == LEAF_PRODUCT_DW) return kt * mt * p.g.trees * p.g.leaves;
-  return row_tiles(p.g, 64) * (what == LEAF_PRODUCT_DX ? kt : mt);
+  if (what == LEAF_PRODUCT_DW) {
+    const DwShape d = dw_shape(p);
+    const int64_t tiles = (int64_t)((p.outputs + d.bm - 1) / d.bm) * ((p.inputs + d.bn - 1) / d.bn);
+    const Split split = dw_split(p, tiles);
+    const int64_t leaves = (int64_t)p.g.trees * p.g.leaves;
+    return split.rows ? std::max(tiles * split.slots, leaves) : tiles * leaves;
+  }
+  return row_tiles(p.g, 64) * (((what == LEAF_PRODUCT_DX ? p.inputs : p.outputs) + 63) / 64);
 }
 
 void launch_leaf_product(const LeafProduct& p, int what, hipStream_t s) {
   if (p.dtype == LGBM_HIP_DTYPE_F32)
-    launch_type<float>(p, what, s);
+    launch<float>(p, what, s);
   else if (p.dtype == LGBM_HIP_DTYPE_BF16)
-    launch_type<__bf16>(p, what, s);
+    launch<__bf16>(p, what, s);
   else
-    launch_type<_Float16>(p, what, s);
+    launch<_Float16>(p, what, s);
 }
 
 }  // namespace lgbm
