@@ -154,6 +154,31 @@ __device__ RowTile find_tile(const LeafGroups& g, int tree, int mt, int bm) {
   return found;
 }
 
+// How many tiles a tree has.
+template <int THREADS>
+__device__ int count_tiles(const LeafGroups& g, int tree, int bm) {
+  __shared__ int64_t wave_tiles[THREADS / 64], wave_rows[THREADS / 64];
+  const int32_t* count = g.count + (int64_t)tree * g.leaves;
+  int64_t tiles = 0, rows = 0;
+  for (int l = threadIdx.x; l < g.leaves; l += THREADS) {
+    const int c = min(max(count[l], 0), g.rows);
+    tiles += ((int64_t)c + bm - 1) / bm;
+    rows += c;
+  }
+#pragma unroll
+  for (int d = 1; d < 64; d <<= 1) {
+    tiles += __shfl_xor(tiles, d);
+    rows += __shfl_xor(rows, d);
+  }
+  if ((threadIdx.x & 63) == 0) wave_tiles[threadIdx.x >> 6] = tiles, wave_rows[threadIdx.x >> 6] = rows;
+  __syncthreads();
+  tiles = rows = 0;
+#pragma unroll
+  for (int w = 0; w < THREADS / 64; ++w) tiles += wave_tiles[w], rows += wave_rows[w];
+  if (rows < g.rows) tiles += (g.rows - rows + bm - 1) / bm;
+  return (int)min(tiles, (int64_t)0x7fffffff);
+}
+
 // Blocks an upper bound of tiles of a tree needs.
 inline int64_t row_tiles(const LeafGroups& g, int64_t bm) { return (g.rows + bm - 1) / bm + g.leaves + 1; }
 
@@ -161,6 +186,25 @@ inline int64_t row_tiles(const LeafGroups& g, int64_t bm) { return (g.rows + bm 
 __device__ __forceinline__ int row_at(const LeafGroups& g, int tree, int position) {
   const int n = g.order[(int64_t)tree * g.rows + position];
   return n >= 0 && n < g.rows ? n : -1;
+}
+
+// Where the rows of a product go: the output of one tree, or a tree's plane.
+template <typename T>
+__device__ __forceinline__ void store_row(const LeafProduct& p, int tree, int n, int col, int cols, f32x4 v) {
+  if (p.g.trees > 1)
+    store4((float*)p.ws + ((int64_t)tree * p.g.rows + n) * cols + col, v, cols - col);
+  else
+    store4((T*)p.out + (int64_t)n * p.ldo + col, v, cols - col);
+}
+
+template <typename T>
+__device__ __forceinline__ f32x4 bias4(const T* bias, int col, int cols) {
+  f32x4 v = {0, 0, 0, 0};
+  if (bias)
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+      if (col + e < cols) v[e] = (float)bias[col + e];
+  return v;
 }
 
 // ---- tiles in LDS --------------------------------------------------------------------------

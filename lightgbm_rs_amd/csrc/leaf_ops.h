@@ -53,6 +53,10 @@ struct LeafProduct {
 size_t leaf_product_workspace(const LeafProduct& p, int what);
 int64_t leaf_product_blocks(const LeafProduct& p, int what);  // along x of its largest launch
 void launch_leaf_product(const LeafProduct& p, int what, hipStream_t s);
+// leaf_big.hip: 16-bit products of large tiles
+bool leaf_big_fits(const LeafProduct& p, int what);
+int64_t leaf_big_blocks(const LeafProduct& p, int what);
+void launch_leaf_big(const LeafProduct& p, int what, hipStream_t s);
 
 // ---- dropout ---------------------------------------------------------------------------
 

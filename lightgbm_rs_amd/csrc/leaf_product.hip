@@ -19,25 +19,6 @@ constexpr int THREADS = 256;
 
 // ---- products over the inputs (y) and over the outputs (dx) ----------------------------------
 
-// Where the rows of a product go: the output of one tree, or a tree's plane.
-template <typename T>
-__device__ __forceinline__ void store_row(const LeafProduct& p, int tree, int n, int col, int cols, f32x4 v) {
-  if (p.g.trees > 1)
-    store4((float*)p.ws + ((int64_t)tree * p.g.rows + n) * cols + col, v, cols - col);
-  else
-    store4((T*)p.out + (int64_t)n * p.ldo + col, v, cols - col);
-}
-
-template <typename T>
-__device__ __forceinline__ f32x4 bias4(const T* bias, int col, int cols) {
-  f32x4 v = {0, 0, 0, 0};
-  if (bias)
-#pragma unroll
-    for (int e = 0; e < 4; ++e)
-      if (col + e < cols) v[e] = (float)bias[col + e];
-  return v;
-}
-
 // out[row][col] = sum over c of a[row][c] * B(c, col), rows gathered through the order.
 // DX false: B(c, col) = w[leaf][col][c] (c: inputs, col: outputs); DX true: B(c, col) =
 // w[leaf][c][col] (c: outputs, col: inputs).  BM x BN of the output a block, 128 bytes of the
@@ -478,6 +459,7 @@ void launch_tile(const LeafProduct& p, hipStream_t s) {
 template <typename T>
 void launch(const LeafProduct& p, int what, hipStream_t s) {
   if (what == LEAF_PRODUCT_DW) {
+    if (leaf_big_fits(p, what)) return launch_leaf_big(p, what, s);
     const DwShape d = dw_shape(p);
     if (d.bm == 16)
       launch_dw<T, 16, 128, 1>(p, s);
@@ -489,7 +471,9 @@ void launch(const LeafProduct& p, int what, hipStream_t s) {
   }
   const bool dx = what == LEAF_PRODUCT_DX;
   const int cols = dx ? p.inputs : p.outputs;
-  if (dx) {
+  if (leaf_big_fits(p, what)) {
+    launch_leaf_big(p, what, s);
+  } else if (dx) {
     launch_tile<T, true, 64, 64, 2>(p, s);
   } else if (cols <= 32) {
     const dim3 grid((unsigned)row_tiles(p.g, 256), (unsigned)p.g.trees);
@@ -515,6 +499,7 @@ void launch(const LeafProduct& p, int what, hipStream_t s) {
 
 size_t leaf_product_workspace(const LeafProduct& p, int what) {
   if (what == LEAF_PRODUCT_DW) {
+    // whatever the pointers' alignment, which may turn the large tiles down
     const DwShape d = dw_shape(p);
     const Split split = dw_split(p, (int64_t)((p.outputs + d.bm - 1) / d.bm) * ((p.inputs + d.bn - 1) / d.bn));
     return (size_t)p.g.trees * (size_t)split.slots * (size_t)p.outputs * (size_t)(p.inputs + 1) * 4;
@@ -524,6 +509,7 @@ size_t leaf_product_workspace(const LeafProduct& p, int what) {
 }
 
 int64_t leaf_product_blocks(const LeafProduct& p, int what) {
+  if (leaf_big_fits(p, what)) return leaf_big_blocks(p, what);
   if (what == LEAF_PRODUCT_DW) {
     const DwShape d = dw_shape(p);
     const int64_t tiles = (int64_t)((p.outputs + d.bm - 1) / d.bm) * ((p.inputs + d.bn - 1) / d.bn);
