@@ -1,11 +1,13 @@
 // leaf_big.hip — the leaves' linear maps in 16 bits where leaves hold hundreds of rows and
 // wide maps: bound by the matrix cores.
 //
-// A block of 8 waves makes 256 x 256 of a result, a wave 128 x 64 of it in registers.  64
-// elements of the contraction a step pass through LDS, in two buffers: while the matrix
-// instructions work on one, loads that go to LDS directly fill the other (rows and chunks
-// are addressed a lane, so the gather through the order costs nothing and the swizzle is
-// made by the addresses).  A lane beyond the operand reads zeros.
+// A block of four waves makes 256 x 256 of a result, a wave 128 x 128 of it in registers (a
+// smaller wave tile reads LDS for as long as it multiplies).  64 elements of the
+// contraction a stage pass through LDS, in two buffers: 128 bytes of a row, since the
+// caches fetch no less (32 elements a stage: 64 KB from L2 take 1.2 us a CU instead of
+// 0.8).  Two more stages are on their way in registers, which the accumulators in the other
+// half of the register file leave free.  Every lane gives its own address, so the gather
+// through the order costs nothing, and what is beyond an operand reads zeros.
 #include <algorithm>
 
 #include "leaf_mma.h"
@@ -15,192 +17,350 @@ namespace {
 
 using namespace mma;
 
-constexpr int THREADS = 512, BM = 256, BN = 256, BK = 64, WM = 128, WN = 64;
+constexpr int THREADS = 256, BM = 256, BN = 256, BK = 64, WM = 128, WN = 128;
+constexpr int A_BYTES = BM * BK * 2, STAGE = (BM + BN) * BK * 2;
+constexpr int LOADS = 8;  // of 1 KB a wave, operand and stage
 
 __device__ __align__(16) unsigned int zeros[4];
 
-typedef const __attribute__((address_space(1))) void* global_ptr;
-typedef __attribute__((address_space(3))) void* lds_ptr;
+typedef const __attribute__((address_space(4))) int32_t* const_ints;
+typedef const __attribute__((address_space(1))) u32x4* global_vec;
 
-// 64 lanes x 16 bytes to `to` (wave-uniform) and the 1 KB behind it.
-__device__ __forceinline__ void load_lds(const void* from, char* to) {
-  __builtin_amdgcn_global_load_lds((global_ptr)from, (lds_ptr)to, 16, 0, 0);
+// The wave's LDS accesses are done, then the block's.
+__device__ __forceinline__ void turn() {
+  asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+  __builtin_amdgcn_s_barrier();
+  asm volatile("" ::: "memory");
+}
+
+typedef float f32x16 __attribute__((ext_vector_type(16)));
+
+// 32 x 32 of a result, 16 of the contraction: a lane's fragment is 16 bytes of row lane % 32,
+// chunk lane / 32 of two.  Lane l of the result holds column l % 32 (of the second operand)
+// and in element 4 a + b row 8 a + 4 (l / 32) + b (of the first).
+template <typename T>
+__device__ __forceinline__ f32x16 mfma32(u32x4 a, u32x4 b, f32x16 c) {
+  if constexpr (__is_same(T, __bf16))
+    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(b16x8, a), __builtin_bit_cast(b16x8, b), c,
+                                                   0, 0, 0);
+  else
+    return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(h16x8, a), __builtin_bit_cast(h16x8, b), c,
+                                                  0, 0, 0);
+}
+
+// The first operand is the columns' (B), taken in the order that leaves a lane with 16
+// neighbouring columns of one row: fragment row 8 a + 4 h + b is column 16 h + 4 a + b.
+__device__ __forceinline__ int column_of(int r) { return ((r >> 2) & 1) * 16 + (r >> 3) * 4 + (r & 3); }
+
+// Stages in LDS.  Along the contraction: [256 rows][8 chunks of 16 bytes], the chunks
+// swizzled so that the eight rows that are read together lie in different banks.
+template <bool COLUMNS>
+__device__ __forceinline__ int kc_swizzle(int row) {
+  return COLUMNS ? (row & 3) | ((row >> 2) & 4) : row & 7;
+}
+template <bool COLUMNS>
+__device__ __forceinline__ u32x4 kc_frag32(const char* tile, int base, int step, int lane) {
+  const int r = lane & 31, row = base + (COLUMNS ? column_of(r) : r);
+  return *reinterpret_cast<const u32x4*>(
+      tile + row * 128 + (((step * 2 + (lane >> 5)) ^ kc_swizzle<COLUMNS>(row)) << 4));
+}
+// Contraction-major: [64][256 columns], in units of 16 columns (32 bytes), pairs of units
+// swizzled.  Transposing reads: within 16 lanes, lane l gives four columns of row l / 4 and
+// gets column l of the four rows.
+__device__ __forceinline__ int cm_swizzle32(int row) { return ((row & 3) | ((row >> 1) & 4)) << 1; }
+template <bool COLUMNS>
+__device__ __forceinline__ u32x4 cm_frag32(const char* tile, int base, int step, int lane) {
+  typedef __attribute__((address_space(3))) s16x4* tr_ptr;
+  const int g = lane >> 4, l = lane & 15, piece = l & 3;
+  const int col = base + (COLUMNS ? (piece & 1) * 16 + (g & 1) * 8 + (piece >> 1) * 4 : (g & 1) * 16 + piece * 4);
+  s16x4 v[2];
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    const int row = step * 16 + (g >> 1) * 8 + h * 4 + (l >> 2);
+    const int at = row * 512 + (((col >> 4) ^ cm_swizzle32(row)) << 5) + (col & 15) * 2;
+    v[h] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((tr_ptr) const_cast<char*>(tile + at));
+  }
+  u32x4 out;
+  __builtin_memcpy(&out, v, 16);
+  return out;
 }
 
 // MODE LEAF_PRODUCT_Y: a = x rows [k], b = w[leaf] [col][k]; _DX: a = dy rows [m], b = w[leaf]
-// [m][col]; _DW: a = dy [row][m], b = x [row][k] over a leaf's rows.
+// [m][col]; _DW: a = dy [row][m], b = x [row][k] over a leaf's rows.  Y and DX: one block a
+// CU takes tile after tile, so that what it stores drains while the next tile begins; DW:
+// a block a tile, since leaves differ in length.
 template <typename T, int MODE>
-__global__ __launch_bounds__(THREADS) void k_leaf_big(LeafProduct p, int col_tiles) {
+__global__ __launch_bounds__(THREADS, 1) void k_leaf_big(LeafProduct p, int col_tiles) {
   constexpr bool DW = MODE == LEAF_PRODUCT_DW, ACM = DW, BCM = MODE != LEAF_PRODUCT_Y;
-  __shared__ __align__(1024) char a0[BM * 128], b0[BN * 128], a1[BM * 128], b1[BN * 128];
+  constexpr int FM = WM / 32, FN = WN / 32, STEPS = BK / 16, ITEMS = STEPS * FM, RING = 4, TURN = ITEMS - 2, AHEAD = 1;
+  __shared__ __align__(1024) char lds[2][STAGE];
   __shared__ int32_t row_of[DW ? 1 : BM];
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-  const int wm = (wave >> 2) * WM, wn = (wave & 3) * WN;
-
-  // the block's part of the result, and the length of the contraction
-  int tree, first = 0, length, m0 = 0, c0, cols, rows = BM;
-  int64_t leaf;
-  if (DW) {
-    const int tiles = (p.outputs + BM - 1) / BM * col_tiles, tile = (int)(blockIdx.x % tiles);
-    leaf = blockIdx.x / tiles;
-    tree = (int)(leaf / p.g.leaves);
-    length = min(max(p.g.count[leaf], 0), p.g.rows);
-    first = min(max(p.g.begin[leaf], 0), p.g.rows - length);
-    m0 = tile / col_tiles * BM, c0 = tile % col_tiles * BN, cols = p.inputs;
-  } else {
-    tree = blockIdx.y;
-    length = MODE == LEAF_PRODUCT_Y ? p.inputs : p.outputs;
-    cols = MODE == LEAF_PRODUCT_Y ? p.outputs : p.inputs;
-    // neighbouring tiles to one XCD, which shares their rows and maps in its L2
-    const int tiles = count_tiles<THREADS>(p.g, tree, BM) * col_tiles, share = (tiles + 7) / 8;
-    const int slot = (int)(blockIdx.x >> 3), id = (int)(blockIdx.x & 7) * share + slot;
-    if (slot >= share || id >= tiles) return;
-    const RowTile rt = find_tile<THREADS>(p.g, tree, id / col_tiles, BM);
-    c0 = id % col_tiles * BN;
-    if (rt.rows == 0) return;
-    rows = rt.rows;
-    leaf = rt.leaf < 0 ? -1 : (int64_t)tree * p.g.leaves + rt.leaf;
-    if (tid < BM) row_of[tid] = tid < rows ? row_at(p.g, tree, rt.first + tid) : -1;
-    __syncthreads();
-    if (leaf < 0) length = 0;
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int wm = (wave >> 1) * WM, wn = (wave & 1) * WN;
+  const int tree_y = blockIdx.y;
+  // neighbouring tiles to one XCD, which shares their rows and maps in its L2
+  int tiles = 0, share = 0;
+  if (!DW) {
+    tiles = count_tiles<THREADS>(p.g, tree_y, BM) * col_tiles;
+    share = (tiles + 7) / 8;
   }
-  const T* const w = (const T*)p.w + (DW || leaf < 0 ? 0 : leaf * p.outputs * (int64_t)p.inputs);
 
-  // a lane's addresses: four loads of each operand a step.  Along the contraction: row
-  // 8 (4 wave + j) + lane / 8, chunk lane % 8 (swizzled); contraction-major: row 2 (4 wave +
-  // j) + lane / 32, 16 bytes lane % 32 (swizzled).
-  const int kc_row = wave * 32 + (lane >> 3), cm_row = wave * 8 + (lane >> 5);
-  const T *abase[4], *bbase[4];
-  int acol[4], bcol[4];
-#pragma unroll
-  for (int j = 0; j < 4; ++j) {
-    const int row = cm_row + 2 * j, sw = cm_swizzle<T>(row);
-    const int unit = ((lane & 31) >> 1) ^ sw, in = (unit * 2 + (lane & 1)) * 8;
-    const int kr = kc_row + 8 * j, kchunk = ((lane & 7) ^ (kr & 7)) * 8;
-    if (ACM) {
-      acol[j] = m0 + in;
+  for (int slot = blockIdx.x >> 3;; slot += gridDim.x >> 3) {
+    // the block's part of the result, and the length of the contraction
+    int tree = tree_y, first = 0, length, m0 = 0, c0, cols;
+    int64_t leaf;
+    if (DW) {
+      const int of = (p.outputs + BM - 1) / BM * col_tiles, tile = (int)(blockIdx.x % of);
+      leaf = blockIdx.x / of;
+      tree = (int)(leaf / p.g.leaves);
+      length = min(max(p.g.count[leaf], 0), p.g.rows);
+      first = min(max(p.g.begin[leaf], 0), p.g.rows - length);
+      m0 = tile / col_tiles * BM, c0 = tile % col_tiles * BN, cols = p.inputs;
     } else {
-      acol[j] = kchunk;
-      const T* const src = (const T*)(MODE == LEAF_PRODUCT_Y ? p.x : p.dy);
-      abase[j] = src + (int64_t)max(row_of[DW ? 0 : kr], 0) * (MODE == LEAF_PRODUCT_Y ? p.ldx : p.lddy) + kchunk;
+      length = MODE == LEAF_PRODUCT_Y ? p.inputs : p.outputs;
+      cols = MODE == LEAF_PRODUCT_Y ? p.outputs : p.inputs;
+      const int id = (int)(blockIdx.x & 7) * share + slot;
+      if (slot >= share || id >= tiles) return;
+      const RowTile rt = find_tile<THREADS>(p.g, tree, id / col_tiles, BM);
+      c0 = id % col_tiles * BN;
+      if (rt.rows == 0) return;
+      leaf = rt.leaf < 0 ? -1 : (int64_t)tree * p.g.leaves + rt.leaf;
+      row_of[tid] = tid < rt.rows ? row_at(p.g, tree, rt.first + tid) : -1;
+      __syncthreads();
+      if (leaf < 0) length = 0;
     }
-    if (BCM) {
-      bcol[j] = c0 + in;
-    } else {
-      bcol[j] = kchunk;
-      bbase[j] = w + (int64_t)min(c0 + kr, cols - 1) * length + kchunk;
-    }
-  }
-  int next_row[4];  // DW: the rows of the step that is loaded next
-  auto fetch_rows = [&](int k0) {
+    const T* const w = (const T*)p.w + (DW || leaf < 0 ? 0 : leaf * p.outputs * (int64_t)p.inputs);
+
+    // A lane's addresses.  Along the contraction: row 8 (8 wave + j) + lane / 8, chunk lane %
+    // 8 (swizzled); contraction-major: row 2 (8 wave + j) + lane / 32, 16 bytes lane % 32
+    // (swizzled).
+    const int kc_row = wave * 64 + (lane >> 3), cm_row = wave * 16 + (lane >> 5);
+    const int achunk = ((lane & 7) ^ kc_swizzle<false>(kc_row)) * 8;
+    // Offsets are in 16 bytes, which rows are whole ones of: 32 bits reach 64 GB.
+    uint32_t aoff[LOADS], boff[LOADS];
+    int bchunk[LOADS], cm_col[LOADS];
+    const uint32_t ld16 = (uint32_t)((MODE == LEAF_PRODUCT_Y ? p.ldx : p.lddy) / 8);
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const int at = k0 + cm_row + 2 * j;
-      next_row[j] = at < length ? row_at(p.g, tree, first + at) : -1;
+    for (int j = 0; j < LOADS; ++j) {
+      const int unit = ((lane & 31) >> 1) ^ cm_swizzle32(cm_row + 2 * j);
+      cm_col[j] = (unit * 2 + (lane & 1)) * 8;
+      bchunk[j] = ((lane & 7) ^ kc_swizzle<true>(kc_row + 8 * j)) * 8;
+      if (!ACM) aoff[j] = (uint32_t)max(row_of[DW ? 0 : kc_row + 8 * j], 0) * ld16 + achunk / 8;
+      if (MODE == LEAF_PRODUCT_Y)
+        boff[j] = (uint32_t)min(c0 + kc_row + 8 * j, cols - 1) * (uint32_t)(length / 8) + bchunk[j] / 8;
+      if (MODE == LEAF_PRODUCT_DX) boff[j] = (uint32_t)(cm_row + 2 * j) * (uint32_t)(cols / 8) + (c0 + cm_col[j]) / 8;
     }
-  };
-  auto load = [&](int k0, char* a, char* b) {
+    // DW: the rows of the stage that is loaded next, by scalar loads, which do not count
+    // among the loads to LDS
+    int next_row[DW ? 2 * LOADS : 1];
+    auto fetch_rows = [&](int k0) {
+      const const_ints order = (const_ints)(uintptr_t)(p.g.order + (int64_t)tree * p.g.rows);
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const void *from_a, *from_b;
-      if (DW) {
-        const int n = next_row[j];
-        from_a = n >= 0 && acol[j] < p.outputs ? (const T*)p.dy + n * p.lddy + acol[j] : (const void*)zeros;
-        from_b = n >= 0 && bcol[j] < cols ? (const T*)p.x + n * p.ldx + bcol[j] : (const void*)zeros;
-      } else {
-        from_a = k0 + acol[j] < length ? abase[j] + k0 : (const void*)zeros;
-        if (BCM) {
-          const int m = k0 + cm_row + 2 * j;
-          from_b = m < length && bcol[j] < cols ? w + (int64_t)m * cols + bcol[j] : (const void*)zeros;
-        } else {
-          from_b = k0 + bcol[j] < length ? bbase[j] + k0 : (const void*)zeros;
-        }
+      for (int j = 0; j < 2 * LOADS; ++j) {
+        const int at = k0 + wave * 16 + j;
+        const int n = order[min(first + at, p.g.rows - 1)];
+        next_row[DW ? j : 0] = at < length && n >= 0 && n < p.g.rows ? n : -1;
       }
-      load_lds(from_a, a + (wave * 4 + j) * 1024);
-      load_lds(from_b, b + (wave * 4 + j) * 1024);
-    }
-    if (DW) fetch_rows(k0 + BK);
-  };
+    };
+    // The j-th loads of the stage at k0, and their place in its buffer.  The stage's addresses
+    // are scalars that the compiler takes as new ones, or it would keep a lane's 32 in
+    // registers.
+    const T* const src = (const T*)(MODE == LEAF_PRODUCT_Y ? p.x : p.dy);
+    const uint64_t zero_at = (uint64_t)(uintptr_t)zeros;
+    struct Stage {
+      uint64_t a, b;
+    };
+    auto stage_at = [&](int k0) {
+      Stage g{(uint64_t)(uintptr_t)(src + k0),
+              (uint64_t)(uintptr_t)(w + (MODE == LEAF_PRODUCT_Y ? (int64_t)k0 : (int64_t)k0 * cols))};
+      if (!DW) asm("" : "+s"(g.a), "+s"(g.b));
+      return g;
+    };
+    auto load_a = [&](const Stage& g, int k0, int j) {
+      uint64_t from;
+      bool in;
+      if (DW) {
+        const int n = lane < 32 ? next_row[DW ? 2 * j : 0] : next_row[DW ? 2 * j + 1 : 0], m = m0 + cm_col[j];
+        in = n >= 0 && m < p.outputs;
+        from = (uint64_t)(uintptr_t)((const T*)p.dy + n * p.lddy + m);
+      } else {
+        in = k0 + achunk < length;
+        from = g.a + (uint64_t)aoff[j] * 16;
+      }
+      return *(global_vec)(in ? from : zero_at);
+    };
+    auto load_b = [&](const Stage& g, int k0, int j) {
+      uint64_t from;
+      bool in;
+      if (DW) {
+        const int n = lane < 32 ? next_row[DW ? 2 * j : 0] : next_row[DW ? 2 * j + 1 : 0], k = c0 + cm_col[j];
+        in = n >= 0 && k < cols;
+        from = (uint64_t)(uintptr_t)((const T*)p.x + n * p.ldx + k);
+      } else {
+        in = BCM ? k0 + cm_row + 2 * j < length && c0 + cm_col[j] < cols : k0 + bchunk[j] < length;
+        from = g.b + (uint64_t)boff[j] * 16;
+      }
+      return *(global_vec)(in ? from : zero_at);
+    };
+    auto place = [&](char* buf, int j) { return (u32x4*)(buf + (wave * LOADS + j) * 1024 + lane * 16); };
 
-  f32x4 acc[WM / 16][WN / 16];
-  float bias[DW ? WM / 16 : 1];  // of the lane's chunks
+    f32x16 acc[FM][FN];
 #pragma unroll
-  for (int i = 0; i < WM / 16; ++i)
+    for (int i = 0; i < FM; ++i)
 #pragma unroll
-    for (int j = 0; j < WN / 16; ++j) acc[i][j] = f32x4{0, 0, 0, 0};
+      for (int j = 0; j < FN; ++j)
 #pragma unroll
-  for (int i = 0; i < (DW ? WM / 16 : 1); ++i) bias[i] = 0.0f;
-  const bool sums = DW && p.db && c0 == 0 && wn == 0;
+        for (int e = 0; e < 16; ++e) acc[i][j][e] = 0.0f;
+    float bias[DW ? FM : 1];  // of the lane's chunks
+#pragma unroll
+    for (int i = 0; i < (DW ? FM : 1); ++i) bias[i] = 0.0f;
+    const bool sums = DW && p.db && c0 == 0 && wn == 0;
 
-  auto compute = [&](const char* a, const char* b) {
+    // item: step FM + i of a stage
+    auto frag_a = [&](const char* buf, int item) {
+      const int base = wm + 32 * (item % FM), step = item / FM;
+      return ACM ? cm_frag32<false>(buf, base, step, lane) : kc_frag32<false>(buf, base, step, lane);
+    };
+    auto frag_b = [&](const char* buf, int j, int step) {
+      return BCM ? cm_frag32<true>(buf + A_BYTES, wn + 32 * j, step, lane)
+                 : kc_frag32<true>(buf + A_BYTES, wn + 32 * j, step, lane);
+    };
+    u32x4 fa[RING], fb[2][FN], ahead[AHEAD][2 * LOADS];
+    // A stage is 16 items: a fragment of rows times the four of columns, for each 16 of the
+    // stage's contraction.  Fragments of rows are read three items ahead, the columns' four.
+    // During items 0 to 7 the next stage goes from registers to the other buffer, and the
+    // registers are loaded with the stage AHEAD further on.  Behind item 13 the wave has
+    // read all of its buffer: the block turns and the first fragments of the next stage are
+    // read.
+    const auto share_of = [](int t) constexpr {  // the eight shares, over items 0 to 11
+      for (int j = 0; j < LOADS; ++j)
+        if (j * 13 / 8 == t) return j;
+      return -1;
+    };
+    auto stage = [&](int k0, int set, char* cur, char* next) {
+      const Stage from = stage_at(k0 + (AHEAD + 1) * BK);
 #pragma unroll
-    for (int step = 0; step < 2; ++step) {
-      u32x4 fa[WM / 16], fb[WN / 16];
+      for (int t = 0; t < ITEMS; ++t) {
+        const int i = t % FM, step = t / FM;
+        if (t == TURN) {
+          turn();
 #pragma unroll
-      for (int j = 0; j < WN / 16; ++j)
-        fb[j] = BCM ? cm_frag<T, BN>(b, wn + 16 * j, step, lane) : kc_frag(b, wn + 16 * j, step, lane);
-#pragma unroll
-      for (int i = 0; i < WM / 16; ++i)
-        fa[i] = ACM ? cm_frag<T, BM>(a, wm + 16 * i, step, lane) : kc_frag(a, wm + 16 * i, step, lane);
-      if (DW && sums)
-#pragma unroll
-        for (int i = 0; i < WM / 16; ++i) {
+          for (int j = 0; j < FN; ++j) fb[0][j] = frag_b(next, j, 0);
+        }
+        if (t < TURN - 1)
+          fa[(t + RING - 1) % RING] = frag_a(cur, t + RING - 1);
+        else if (t >= TURN)
+          for (int u = t == TURN ? 0 : 2; u < (t == TURN ? 2 : 3); ++u) fa[u] = frag_a(next, u);
+        if (step + 1 < STEPS) fb[(step + 1) % 2][i] = frag_b(cur, i, step + 1);
+        const u32x4 f = fa[t % RING];
+        if (DW && sums) {
           T e[8];
-          __builtin_memcpy(e, &fa[i], 16);
+          __builtin_memcpy(e, &f, 16);
 #pragma unroll
           for (int k = 0; k < 8; ++k) bias[DW ? i : 0] += (float)e[k];
         }
+        if (share_of(t) >= 0) {
+          const int l = share_of(t);
+          *place(next, l) = ahead[set][2 * l];
+          *place(next + A_BYTES, l) = ahead[set][2 * l + 1];
+          ahead[set][2 * l] = load_a(from, k0 + (AHEAD + 1) * BK, l);
+        }
+        __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-      for (int i = 0; i < WM / 16; ++i)
+        for (int j = 0; j < FN / 2; ++j) acc[i][j] = mfma32<T>(fb[step % 2][j], f, acc[i][j]);
+        __builtin_amdgcn_sched_barrier(0);
+        if (t > 0 && share_of(t - 1) >= 0) {
+          const int l = share_of(t - 1);
+          ahead[set][2 * l + 1] = load_b(from, k0 + (AHEAD + 1) * BK, l);
+        }
 #pragma unroll
-        for (int j = 0; j < WN / 16; ++j) acc[i][j] = El<T>::mfma(fb[j], fa[i], acc[i][j]);
-      __builtin_amdgcn_sched_barrier(0);
-    }
-  };
-
-  if (DW) fetch_rows(0);
-  if (length > 0) load(0, a0, b0);
-  for (int k0 = 0; k0 < length; k0 += 2 * BK) {
-    __syncthreads();  // the loads are there, and the other buffer has been read
-    load(k0 + BK, a1, b1);  // behind the end: zeros
-    compute(a0, b0);
-    __syncthreads();
-    if (k0 + 2 * BK < length) load(k0 + 2 * BK, a0, b0);
-    compute(a1, b1);
-  }
-
-  // lane: row lane % 16, columns 4 (lane / 16) .. + 4 of each 16 x 16
-  if (DW) {
-    float* const dw = p.dw + leaf * p.outputs * (int64_t)p.inputs;
-#pragma unroll
-    for (int i = 0; i < WM / 16; ++i) {
-      const int m = m0 + wm + i * 16 + (lane & 15);
-      if (m >= p.outputs) continue;
-      if (sums) {
-        float b = bias[DW ? i : 0];
-        b += __shfl_xor(b, 16);
-        b += __shfl_xor(b, 32);
-        if (lane < 16) p.db[leaf * p.outputs + m] = b;
+        for (int j = FN / 2; j < FN; ++j) acc[i][j] = mfma32<T>(fb[step % 2][j], f, acc[i][j]);
+        __builtin_amdgcn_sched_barrier(0);
+        if (t == TURN && DW) fetch_rows(k0 + (AHEAD + 2) * BK);
       }
+    };
+
+    if (length > 0) {
+      // stage 0 to the first buffer, the AHEAD behind it on their way
 #pragma unroll
-      for (int j = 0; j < WN / 16; ++j) {
-        const int k = c0 + wn + j * 16 + (lane >> 4) * 4;
-        if (k < cols) store4(dw + (int64_t)m * cols + k, acc[i][j], cols - k);
+      for (int s = 0; s <= AHEAD; ++s) {
+        if (DW) fetch_rows(s * BK);
+#pragma unroll
+        for (int j = 0; j < LOADS; ++j) {
+          ahead[s % AHEAD][2 * j] = load_a(stage_at(s * BK), s * BK, j);
+          ahead[s % AHEAD][2 * j + 1] = load_b(stage_at(s * BK), s * BK, j);
+        }
+        if (s == 0)
+#pragma unroll
+          for (int j = 0; j < LOADS; ++j)
+            *place(lds[0], j) = ahead[0][2 * j], *place(lds[0] + A_BYTES, j) = ahead[0][2 * j + 1];
+      }
+      if (DW) fetch_rows((AHEAD + 1) * BK);
+      turn();
+#pragma unroll
+      for (int j = 0; j < FN; ++j) fb[0][j] = frag_b(lds[0], j, 0);
+#pragma unroll
+      for (int u = 0; u < RING - 1; ++u) fa[u] = frag_a(lds[0], u);
+      int cur = 0;
+      for (int k0 = 0; k0 < length; k0 += BK, cur ^= 1) stage(k0, 0, lds[cur], lds[cur ^ 1]);
+    }
+
+    // lane: of each 32 x 32, row lane % 32 and columns 16 (lane / 32) .. + 16
+    if (DW) {
+      float* const dw = p.dw + leaf * p.outputs * (int64_t)p.inputs;
+#pragma unroll
+      for (int i = 0; i < FM; ++i) {
+        const int m = m0 + wm + i * 32 + (lane & 31);
+        if (sums) {
+          const float b = bias[DW ? i : 0] + __shfl_xor(bias[DW ? i : 0], 32);
+          if (lane < 32 && m < p.outputs) p.db[leaf * p.outputs + m] = b;
+        }
+        if (m >= p.outputs) continue;
+#pragma unroll
+        for (int j = 0; j < FN; ++j) {
+          const int k = c0 + wn + j * 32 + (lane >> 5) * 16;
+          float* const to = dw + (int64_t)m * cols + k;
+#pragma unroll
+          for (int e = 0; e < 16; e += 4)  // columns come in eights
+            if (k + e < cols) __builtin_memcpy(to + e, (const float*)&acc[i][j] + e, 16);
+        }
+      }
+      return;
+    }
+    const T* const bias_of = MODE == LEAF_PRODUCT_Y && p.b && leaf >= 0 ? (const T*)p.b + leaf * cols : nullptr;
+    const bool planes = p.g.trees > 1;
+#pragma unroll
+    for (int j = 0; j < FN; ++j) {
+#pragma unroll
+      for (int half = 0; half < 16; half += 8) {
+        const int col = c0 + wn + j * 32 + (lane >> 5) * 16 + half;
+        if (col >= cols) continue;  // columns come in eights
+        float b[8] = {0, 0, 0, 0, 0, 0, 0, 0};
+        if (bias_of) {
+          T e[8];
+          __builtin_memcpy(e, bias_of + col, sizeof(e));
+#pragma unroll
+          for (int k = 0; k < 8; ++k) b[k] = (float)e[k];
+        }
+#pragma unroll
+        for (int i = 0; i < FM; ++i) {
+          const int n = row_of[DW ? 0 : wm + i * 32 + (lane & 31)];
+          if (n < 0) continue;
+          float v[8];
+#pragma unroll
+          for (int k = 0; k < 8; ++k) v[k] = acc[i][j][half + k] + b[k];
+          if (planes) {
+            __builtin_memcpy((float*)p.ws + ((int64_t)tree * p.g.rows + n) * cols + col, v, 32);
+          } else {
+            T e[8];
+#pragma unroll
+            for (int k = 0; k < 8; ++k) e[k] = (T)v[k];
+            __builtin_memcpy((T*)p.out + (int64_t)n * p.ldo + col, e, 16);
+          }
+        }
       }
     }
-    return;
-  }
-  const T* const bias_of = MODE == LEAF_PRODUCT_Y && p.b && leaf >= 0 ? (const T*)p.b + leaf * cols : nullptr;
-#pragma unroll
-  for (int j = 0; j < WN / 16; ++j) {
-    const int col = c0 + wn + j * 16 + (lane >> 4) * 4;
-    if (col >= cols) continue;
-    const f32x4 b = bias4(bias_of, col, cols);
-#pragma unroll
-    for (int i = 0; i < WM / 16; ++i) {
-      const int n = row_of[DW ? 0 : wm + i * 16 + (lane & 15)];
-      if (n >= 0) store_row<T>(p, tree, n, col, cols, acc[i][j] + b);
-    }
+    __syncthreads();  // row_of is read before the next tile's
   }
 }
 
@@ -221,7 +381,7 @@ void launch(const LeafProduct& p, int what, hipStream_t s) {
 int64_t leaf_big_blocks(const LeafProduct& p, int what) {
   const int64_t ct = ((what == LEAF_PRODUCT_Y ? p.outputs : p.inputs) + BN - 1) / BN;
   if (what == LEAF_PRODUCT_DW) return (p.outputs + BM - 1) / BM * ct * p.g.trees * p.g.leaves;
-  return (row_tiles(p.g, BM) * ct + 7) / 8 * 8;
+  return std::min<int64_t>((row_tiles(p.g, BM) * ct + 7) / 8 * 8, 256);  // one a CU
 }
 
 // Rows and maps that make whole tiles of 256 x 256 worthwhile, and 16-byte chunks that do not
@@ -230,6 +390,7 @@ bool leaf_big_fits(const LeafProduct& p, int what) {
   if (p.dtype == LGBM_HIP_DTYPE_F32) return false;
   if (p.inputs % 8 || p.outputs % 8 || p.inputs < 192 || p.outputs < 192) return false;
   if ((int64_t)p.g.rows < 192 * (int64_t)p.g.leaves) return false;
+  if (p.g.rows * std::max(p.ldx, p.lddy) >> 35 || (int64_t)p.inputs * p.outputs >> 35) return false;  // 64 GB
   auto ok = [](const void* q, int64_t ld) { return (((uintptr_t)q) | (uintptr_t)(ld * 2)) % 16 == 0; };
   if (what == LEAF_PRODUCT_Y) return ok(p.x, p.ldx) && ok(p.w, p.inputs);
   if (what == LEAF_PRODUCT_DX) return ok(p.dy, p.lddy) && ok(p.w, p.inputs);
