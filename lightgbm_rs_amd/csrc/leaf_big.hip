@@ -9,6 +9,7 @@
 // half of the register file leave free.  Every lane gives its own address, so the gather
 // through the order costs nothing, and what is beyond an operand reads zeros.
 #include <algorithm>
+#include <type_traits>
 
 #include "leaf_mma.h"
 
@@ -24,6 +25,8 @@ constexpr int LOADS = 8;  // of 1 KB a wave, operand and stage
 __device__ __align__(16) unsigned int zeros[4];
 
 typedef const __attribute__((address_space(4))) int32_t* const_ints;
+typedef int i32x16 __attribute__((ext_vector_type(16), aligned(4)));
+typedef const __attribute__((address_space(4))) i32x16* const_ints16;
 typedef const __attribute__((address_space(1))) u32x4* global_vec;
 
 // The wave's LDS accesses are done, then the block's.
@@ -152,15 +155,31 @@ __global__ __launch_bounds__(THREADS, 1) void k_leaf_big(LeafProduct p, int col_
     }
     // DW: the rows of the stage that is loaded next, by scalar loads, which do not count
     // among the loads to LDS
-    int next_row[DW ? 2 * LOADS : 1];
+    // (offset of dy's row, of x's; a bit a load and half wave: whether there is a row)
+    uint32_t row_a[DW ? 2 * LOADS : 1], row_b[DW ? 2 * LOADS : 1], there = 0;
     auto fetch_rows = [&](int k0) {
       const const_ints order = (const_ints)(uintptr_t)(p.g.order + (int64_t)tree * p.g.rows);
+      const int at = k0 + wave * 16, from = first + at;
+      i32x16 n;
+      if (from + 16 <= p.g.rows) {
+        n = *(const_ints16)(order + from);
+      } else {
 #pragma unroll
-      for (int j = 0; j < 2 * LOADS; ++j) {
-        const int at = k0 + wave * 16 + j;
-        const int n = order[min(first + at, p.g.rows - 1)];
-        next_row[DW ? j : 0] = at < length && n >= 0 && n < p.g.rows ? n : -1;
+        for (int j = 0; j < 16; ++j) n[j] = order[min(from + j, p.g.rows - 1)];
       }
+      there = 0;
+#pragma unroll
+      for (int j = 0; j < 16; ++j) {
+        const bool ok = at + j < length && (uint32_t)n[j] < (uint32_t)p.g.rows;
+        there |= (uint32_t)ok << j;
+        const uint32_t row = ok ? (uint32_t)n[j] : 0u;
+        row_a[DW ? j : 0] = row * (uint32_t)(p.lddy / 8);
+        row_b[DW ? j : 0] = row * (uint32_t)(p.ldx / 8);
+      }
+    };
+    // of a lane's load j: its half wave's value
+    auto half_of = [&](const uint32_t (&v)[DW ? 2 * LOADS : 1], int j) {
+      return lane < 32 ? v[DW ? 2 * j : 0] : v[DW ? 2 * j + 1 : 0];
     };
     // The j-th loads of the stage at k0, and their place in its buffer.  The stage's addresses
     // are scalars that the compiler takes as new ones, or it would keep a lane's 32 in
@@ -171,18 +190,18 @@ __global__ __launch_bounds__(THREADS, 1) void k_leaf_big(LeafProduct p, int col_
       uint64_t a, b;
     };
     auto stage_at = [&](int k0) {
+      if (DW) return Stage{(uint64_t)(uintptr_t)p.dy, (uint64_t)(uintptr_t)p.x};
       Stage g{(uint64_t)(uintptr_t)(src + k0),
               (uint64_t)(uintptr_t)(w + (MODE == LEAF_PRODUCT_Y ? (int64_t)k0 : (int64_t)k0 * cols))};
-      if (!DW) asm("" : "+s"(g.a), "+s"(g.b));
+      asm("" : "+s"(g.a), "+s"(g.b));
       return g;
     };
     auto load_a = [&](const Stage& g, int k0, int j) {
       uint64_t from;
       bool in;
       if (DW) {
-        const int n = lane < 32 ? next_row[DW ? 2 * j : 0] : next_row[DW ? 2 * j + 1 : 0], m = m0 + cm_col[j];
-        in = n >= 0 && m < p.outputs;
-        from = (uint64_t)(uintptr_t)((const T*)p.dy + n * p.lddy + m);
+        in = (there >> (2 * j + (lane >> 5)) & 1) && m0 + cm_col[j] < p.outputs;
+        from = g.a + (uint64_t)(half_of(row_a, j) + (m0 + cm_col[j]) / 8) * 16;
       } else {
         in = k0 + achunk < length;
         from = g.a + (uint64_t)aoff[j] * 16;
@@ -193,9 +212,8 @@ __global__ __launch_bounds__(THREADS, 1) void k_leaf_big(LeafProduct p, int col_
       uint64_t from;
       bool in;
       if (DW) {
-        const int n = lane < 32 ? next_row[DW ? 2 * j : 0] : next_row[DW ? 2 * j + 1 : 0], k = c0 + cm_col[j];
-        in = n >= 0 && k < cols;
-        from = (uint64_t)(uintptr_t)((const T*)p.x + n * p.ldx + k);
+        in = (there >> (2 * j + (lane >> 5)) & 1) && c0 + cm_col[j] < cols;
+        from = g.b + (uint64_t)(half_of(row_b, j) + (c0 + cm_col[j]) / 8) * 16;
       } else {
         in = BCM ? k0 + cm_row + 2 * j < length && c0 + cm_col[j] < cols : k0 + bchunk[j] < length;
         from = g.b + (uint64_t)boff[j] * 16;
@@ -214,8 +232,7 @@ __global__ __launch_bounds__(THREADS, 1) void k_leaf_big(LeafProduct p, int col_
     float bias[DW ? FM : 1];  // of the lane's chunks
 #pragma unroll
     for (int i = 0; i < (DW ? FM : 1); ++i) bias[i] = 0.0f;
-    const bool sums = DW && p.db && c0 == 0 && wn == 0;
-
+    
     // item: step FM + i of a stage
     auto frag_a = [&](const char* buf, int item) {
       const int base = wm + 32 * (item % FM), step = item / FM;
@@ -237,7 +254,7 @@ __global__ __launch_bounds__(THREADS, 1) void k_leaf_big(LeafProduct p, int col_
         if (j * 13 / 8 == t) return j;
       return -1;
     };
-    auto stage = [&](int k0, int set, char* cur, char* next) {
+    auto stage = [&](auto sums, int k0, int set, char* cur, char* next) {
       const Stage from = stage_at(k0 + (AHEAD + 1) * BK);
 #pragma unroll
       for (int t = 0; t < ITEMS; ++t) {
@@ -253,7 +270,7 @@ __global__ __launch_bounds__(THREADS, 1) void k_leaf_big(LeafProduct p, int col_
           for (int u = t == TURN ? 0 : 2; u < (t == TURN ? 2 : 3); ++u) fa[u] = frag_a(next, u);
         if (step + 1 < STEPS) fb[(step + 1) % 2][i] = frag_b(cur, i, step + 1);
         const u32x4 f = fa[t % RING];
-        if (DW && sums) {
+        if (sums) {
           T e[8];
           __builtin_memcpy(e, &f, 16);
 #pragma unroll
@@ -302,7 +319,14 @@ __global__ __launch_bounds__(THREADS, 1) void k_leaf_big(LeafProduct p, int col_
 #pragma unroll
       for (int u = 0; u < RING - 1; ++u) fa[u] = frag_a(lds[0], u);
       int cur = 0;
-      for (int k0 = 0; k0 < length; k0 += BK, cur ^= 1) stage(k0, 0, lds[cur], lds[cur ^ 1]);
+      // sums of dy's columns cost as much again as what else the matrix instructions hide: only
+      // the blocks of the first columns make them
+      if (DW && p.db && c0 == 0) {
+        for (int k0 = 0; k0 < length; k0 += BK, cur ^= 1)
+          stage(std::integral_constant<bool, DW>(), k0, 0, lds[cur], lds[cur ^ 1]);
+      } else {
+        for (int k0 = 0; k0 < length; k0 += BK, cur ^= 1) stage(std::false_type(), k0, 0, lds[cur], lds[cur ^ 1]);
+      }
     }
 
     // lane: of each 32 x 32, row lane % 32 and columns 16 (lane / 32) .. + 16
@@ -311,7 +335,7 @@ __global__ __launch_bounds__(THREADS, 1) void k_leaf_big(LeafProduct p, int col_
 #pragma unroll
       for (int i = 0; i < FM; ++i) {
         const int m = m0 + wm + i * 32 + (lane & 31);
-        if (sums) {
+        if (p.db && c0 == 0 && wn == 0) {
           const float b = bias[DW ? i : 0] + __shfl_xor(bias[DW ? i : 0], 32);
           if (lane < 32 && m < p.outputs) p.db[leaf * p.outputs + m] = b;
         }
