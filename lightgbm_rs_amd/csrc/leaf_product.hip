@@ -212,6 +212,65 @@ __global__ __launch_bounds__(THREADS) void k_leaf_narrow(LeafProduct p) {
   }
 }
 
+// dx for up to 32 outputs of a leaf: bound by writing dx.  A wave keeps the leaf's map of 128
+// inputs in registers, turned as the matrix instruction takes it, and runs over its rows, 16
+// at a time: one load of dy's rows, then a product and a store of 16 x 16 for each 16
+// inputs.
+template <typename T>
+__global__ __launch_bounds__(THREADS) void k_leaf_dx_narrow(LeafProduct p, int col_tiles, int steps) {
+  constexpr int V = El<T>::V, MAX_STEPS = sizeof(T) == 2 ? 1 : 2, FN = 8, BM = 512;
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, r = lane & 15, q = lane >> 4;
+  const int tree = blockIdx.y, cols = p.inputs, length = p.outputs;
+  const int c0 = (int)(blockIdx.x % col_tiles) * (16 * FN);
+  const RowTile rt = find_tile<THREADS>(p.g, tree, blockIdx.x / col_tiles, BM);
+  if (wave * 16 >= rt.rows) return;
+  const int64_t leaf = (int64_t)tree * p.g.leaves + rt.leaf;
+  const T* const w = (const T*)p.w + (rt.leaf < 0 ? 0 : leaf * length * (int64_t)cols);
+  u32x4 fw[MAX_STEPS][FN];
+#pragma unroll
+  for (int s = 0; s < MAX_STEPS; ++s)
+#pragma unroll
+    for (int j = 0; j < FN; ++j) {
+      T e[V];
+#pragma unroll
+      for (int v = 0; v < V; ++v) {
+        const int m = (s * 4 + q) * V + v, k = c0 + j * 16 + r;
+        e[v] = rt.leaf >= 0 && m < length && k < cols ? w[(int64_t)m * cols + k] : (T)0.0f;
+      }
+      __builtin_memcpy(&fw[s][j], e, 16);
+    }
+  constexpr int UNROLL = 2;
+  for (int r0 = wave * 16; r0 < rt.rows; r0 += 64 * UNROLL) {
+    int n[UNROLL];
+    u32x4 f[UNROLL][MAX_STEPS];
+#pragma unroll
+    for (int u = 0; u < UNROLL; ++u) {
+      const int at = r0 + u * 64 + r;
+      n[u] = at < rt.rows ? row_at(p.g, tree, rt.first + at) : -1;
+    }
+#pragma unroll
+    for (int u = 0; u < UNROLL; ++u)
+#pragma unroll
+      for (int s = 0; s < MAX_STEPS; ++s) {
+        const int m = (s * 4 + q) * V;
+        f[u][s] = load16((const T*)p.dy + (int64_t)max(n[u], 0) * p.lddy + m,
+                         n[u] < 0 || rt.leaf < 0 ? 0 : length - m);
+      }
+#pragma unroll
+    for (int u = 0; u < UNROLL; ++u)
+#pragma unroll
+      for (int j = 0; j < FN; ++j) {
+        const int col = c0 + j * 16 + q * 4;
+        if (c0 + j * 16 >= cols) break;
+        f32x4 acc = {0, 0, 0, 0};
+#pragma unroll
+        for (int s = 0; s < MAX_STEPS; ++s)
+          if (s < steps) acc = El<T>::mfma(fw[s][j], f[u][s], acc);
+        if (n[u] >= 0 && col < cols) store_row<T>(p, tree, n[u], col, cols, acc);
+      }
+  }
+}
+
 // The trees' planes added, rounded once: 64 elements a block, a quarter of the trees a wave;
 // in float64, since a forest has hundreds of trees.
 template <typename T>
@@ -235,17 +294,25 @@ __global__ __launch_bounds__(THREADS) void k_sum_trees(const float* planes, int6
     __syncthreads();
   }
 }
-// Few trees: a thread an element.
-template <typename T>
+// Few trees: a thread an element, or four of rows without gaps.
+template <typename T, int V>
 __global__ __launch_bounds__(THREADS) void k_sum_few_trees(const float* planes, int64_t rows, int cols,
                                                            int trees, T* out, int64_t ldo) {
   const int64_t total = rows * cols;
-  for (int64_t e = blockIdx.x * (int64_t)THREADS + threadIdx.x; e < total;
-       e += (int64_t)gridDim.x * THREADS) {
-    double v = 0;
+  for (int64_t e = (blockIdx.x * (int64_t)THREADS + threadIdx.x) * V; e < total;
+       e += (int64_t)gridDim.x * THREADS * V) {
+    double v[V] = {};
 #pragma unroll 4
-    for (int t = 0; t < trees; ++t) v += (double)planes[t * total + e];
-    out[e / cols * ldo + e % cols] = (T)(float)v;
+    for (int t = 0; t < trees; ++t) {
+      float x[V];
+      __builtin_memcpy(x, planes + t * total + e, sizeof(x));
+#pragma unroll
+      for (int i = 0; i < V; ++i) v[i] += (double)x[i];
+    }
+    T o[V];
+#pragma unroll
+    for (int i = 0; i < V; ++i) o[i] = (T)(float)v[i];
+    __builtin_memcpy(out + (V > 1 ? e : e / cols * ldo + e % cols), o, sizeof(o));
   }
 }
 
@@ -473,6 +540,10 @@ void launch(const LeafProduct& p, int what, hipStream_t s) {
   const int cols = dx ? p.inputs : p.outputs;
   if (leaf_big_fits(p, what)) {
     launch_leaf_big(p, what, s);
+  } else if (dx && p.outputs <= 32) {
+    const int ct = (cols + 127) / 128, steps = (p.outputs + 4 * El<T>::V - 1) / (4 * El<T>::V);
+    const dim3 grid((unsigned)(row_tiles(p.g, 512) * ct), (unsigned)p.g.trees);
+    k_leaf_dx_narrow<T><<<grid, THREADS, 0, s>>>(p, ct, steps);
   } else if (dx) {
     launch_tile<T, true, 64, 64, 2>(p, s);
   } else if (cols <= 32) {
@@ -489,9 +560,12 @@ void launch(const LeafProduct& p, int what, hipStream_t s) {
     if (p.g.trees >= 16)
       k_sum_trees<T><<<(unsigned)std::min<int64_t>((total + 63) / 64, 1 << 20), THREADS, 0, s>>>(
           (const float*)p.ws, p.g.rows, cols, p.g.trees, (T*)p.out, p.ldo);
+    else if (p.ldo == cols && total % 4 == 0)
+      k_sum_few_trees<T, 4><<<(unsigned)std::min<int64_t>((total / 4 + THREADS - 1) / THREADS, 1 << 16), THREADS, 0,
+                              s>>>((const float*)p.ws, p.g.rows, cols, p.g.trees, (T*)p.out, p.ldo);
     else
-      k_sum_few_trees<T><<<(unsigned)std::min<int64_t>((total + THREADS - 1) / THREADS, 1 << 16), THREADS, 0, s>>>(
-          (const float*)p.ws, p.g.rows, cols, p.g.trees, (T*)p.out, p.ldo);
+      k_sum_few_trees<T, 1><<<(unsigned)std::min<int64_t>((total + THREADS - 1) / THREADS, 1 << 16), THREADS, 0,
+                              s>>>((const float*)p.ws, p.g.rows, cols, p.g.trees, (T*)p.out, p.ldo);
   }
 }
 
