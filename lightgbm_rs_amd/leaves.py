@@ -16,9 +16,9 @@ from typing import Any, NamedTuple
 
 import numpy as np
 
-from .backend import PREDICT_KINDS, HipBackend
+from .backend import PREDICT_KINDS, HipBackend, load_library
 
-_DTYPES = {"float32": 0, "float64": 1, "bfloat16": 2, "float16": 3}
+_DTYPES = {}  # torch's element types -> LGBM_HIP_DTYPE_*
 _PRODUCT, _DX, _DW = 0, 1, 2
 
 
@@ -59,32 +59,62 @@ class LeafGroups(NamedTuple):
         return cls(up(layout["indices"]), up(layout["leaf_begin"]), up(layout["leaf_count"]))
 
 
+_torch = None  # the module, once a method has been called
+
+
+def _module():
+    """torch, the library's entries with their argument types declared, and the element types:
+    set up by the first call, so that the package itself does not need torch."""
+    global _torch
+    if _torch is None:
+        import torch
+        p, i32, i64, u64, size = C.c_void_p, C.c_int32, C.c_int64, C.c_uint64, C.c_size_t
+        lib = load_library()
+        for name, types in (
+                ("leaf_groups_workspace", (i64, i32, i32, p)),
+                ("leaf_groups", (p, p, i64, i64, i32, i32, p, p, p, p, size, p)),
+                ("leaf_product_workspace", (p, i32, p)),
+                ("leaf_product", (p, p, p, i64, p, p, p, i64, p, size, p)),
+                ("leaf_product_dx", (p, p, p, i64, p, p, i64, p, size, p)),
+                ("leaf_product_dw", (p, p, p, i64, p, i64, p, p, p, size, p)),
+                ("dropout", (p, p, i64, i64, i64, i32, C.c_double, u64, u64, i32, p, i64, p)),
+                ("adjust_scores_workspace", (p, p)),
+                ("adjust_scores", (p, p, p, size, p))):
+            getattr(lib, "lgbm_hip_" + name).argtypes = types
+        for name, code in (("float32", 0), ("float64", 1), ("bfloat16", 2), ("float16", 3)):
+            _DTYPES[getattr(torch, name)] = code
+        _torch = torch
+    return _torch
+
+
 def _stream(self, torch):
     """The `stream` argument: torch's current stream of the backend's device."""
     return C.byref(C.c_void_p(torch.cuda.current_stream(self.device).cuda_stream))
 
 
-def _dtype(t, what, names=("float32", "bfloat16", "float16")):
-    name = str(t.dtype)[6:]
-    if name not in names:
-        raise ValueError(f"{what} is {name}: one of {', '.join(names)} is needed")
-    return _DTYPES[name]
+def _dtype(t, what, double=False):
+    code = _DTYPES.get(t.dtype)
+    if code is None or (code == 1 and not double):
+        raise ValueError(f"{what} is {t.dtype}: a floating-point type of the device is needed"
+                         + ("" if double else ", of at most 32 bits"))
+    return code
 
 
 def _here(self, **tensors):
     for name, t in tensors.items():
-        if t is not None and (not t.is_cuda or t.device.index != self.device):
+        if t is not None and (not t.is_cuda or t.get_device() != self.device):
             raise ValueError(f"{name} is on {t.device}: cuda:{self.device} is needed")
 
 
 def _shape(t, shape, what):
-    if tuple(t.shape) != tuple(shape):
+    if t.shape != shape:
         raise ValueError(f"{what} has shape {tuple(t.shape)}: {tuple(shape)} is needed")
 
 
-def _ints(t, what, name="int32"):
-    if str(t.dtype)[6:] != name:
-        raise ValueError(f"{what} is {str(t.dtype)[6:]}: {name} is needed")
+def _typed(t, what, dtype):
+    """t without gaps, of a type."""
+    if t.dtype is not dtype:
+        raise ValueError(f"{what} is {t.dtype}: {dtype} is needed")
     return t.contiguous()
 
 
@@ -95,62 +125,60 @@ def _ld(t):
 
 def _rows(t):
     """t with unit column stride and rows that do not overlap."""
-    rows, cols = t.shape
-    if (cols > 1 and t.stride(1) != 1) or (rows > 1 and t.stride(0) < cols):
-        t = t.contiguous()
+    if not t.is_contiguous():
+        rows, cols = t.shape
+        if (cols > 1 and t.stride(1) != 1) or (rows > 1 and t.stride(0) < cols):
+            t = t.contiguous()
     return t
 
 
-def _out(out, like, shape, dtype=None):
+def _out(out, like, shape):
     """The output: the caller's, checked, or a new tensor."""
     if out is None:
-        return like.new_empty(shape, dtype=dtype or like.dtype)
+        return like.new_empty(shape)
     _shape(out, shape, "out")
-    if out.dtype != (dtype or like.dtype):
-        raise ValueError(f"out is {out.dtype}: {dtype or like.dtype} is needed")
+    if out.dtype is not like.dtype:
+        raise ValueError(f"out is {out.dtype}: {like.dtype} is needed")
     if _rows(out) is not out:
         raise ValueError("out has strided columns or rows that overlap")
     return out
 
 
-def _workspace(self, torch, size):
-    """(pointer, bytes, the tensor that holds them)"""
-    if not size:
+def _workspace(self, torch, entry, *args):
+    """(pointer, bytes, the tensor that holds them) of an entry's working memory."""
+    size = C.c_size_t(0)
+    self._check_plain(entry(*args, C.byref(size)))
+    if not size.value:
         return None, 0, None
-    t = torch.empty(size, dtype=torch.uint8, device=f"cuda:{self.device}")
-    return t.data_ptr(), size, t
+    t = torch.empty(size.value, dtype=torch.uint8, device=f"cuda:{self.device}")
+    return t.data_ptr(), size.value, t
 
 
 def _leaf_groups(self, leaf, num_leaves):
     """The rows of every leaf (`lgbm_hip_leaf_groups`) from leaf int32 [rows, trees] or
     [rows], as `predict(kind="leaf")` gives it; an index outside [0, num_leaves) means that
     the row is in no leaf of that tree.  Returns LeafGroups."""
-    import torch
+    torch = _module()
     if leaf.dim() == 1:
         leaf = leaf[:, None]
     if leaf.dim() != 2 or leaf.shape[1] == 0:
         raise ValueError("leaf has to be [rows, trees]")
-    if leaf.dtype != torch.int32:
+    if leaf.dtype is not torch.int32:
         raise ValueError(f"leaf is {leaf.dtype}: int32 is needed")
     _here(self, leaf=leaf)
     leaf = _rows(leaf)
     rows, trees = leaf.shape
-    size = C.c_size_t(0)
-    self._check_plain(self.lib.lgbm_hip_leaf_groups_workspace(
-        C.c_int64(rows), C.c_int32(trees), C.c_int32(num_leaves), C.byref(size)))
+    ws, nbytes, hold = _workspace(self, torch, self.lib.lgbm_hip_leaf_groups_workspace, rows,
+                                  trees, num_leaves)
     order = leaf.new_empty((trees, rows))
-    begin = leaf.new_empty((trees, num_leaves))
-    count = leaf.new_empty((trees, num_leaves))
-    ws, nbytes, keep = _workspace(self, torch, size.value)
+    begin, count = leaf.new_empty((2, trees, num_leaves))
     self._check(self.lib.lgbm_hip_leaf_groups(
-        self.ctx, C.c_void_p(leaf.data_ptr()), C.c_int64(_ld(leaf)), C.c_int64(rows),
-        C.c_int32(trees), C.c_int32(num_leaves), C.c_void_p(order.data_ptr()),
-        C.c_void_p(begin.data_ptr()), C.c_void_p(count.data_ptr()), C.c_void_p(ws),
-        C.c_size_t(nbytes), _stream(self, torch)))
+        self.ctx, leaf.data_ptr(), _ld(leaf), rows, trees, num_leaves, order.data_ptr(),
+        begin.data_ptr(), count.data_ptr(), ws, nbytes, _stream(self, torch)))
     return LeafGroups(order, begin, count)
 
 
-def _maps(self, rows, inputs, outputs, dtype, groups, leaves=None):
+def _maps(self, torch, rows, inputs, outputs, dtype, groups, leaves=None):
     """(lgbm_leaf_maps, the tensors it points to)"""
     order, begin, count = groups
     trees, num = begin.shape
@@ -158,18 +186,9 @@ def _maps(self, rows, inputs, outputs, dtype, groups, leaves=None):
     _shape(count, (trees, num), "count")
     if leaves is not None and leaves != trees * num:
         raise ValueError(f"weights of {leaves} leaves for {trees} x {num}")
-    order, begin, count = _ints(order, "order"), _ints(begin, "begin"), _ints(count, "count")
+    hold = [_typed(t, n, torch.int32) for t, n in ((order, "order"), (begin, "begin"), (count, "count"))]
     _here(self, order=order, begin=begin, count=count)
-    m = _Maps(order.data_ptr(), begin.data_ptr(), count.data_ptr(), rows, trees, num, inputs,
-              outputs, dtype, 0)
-    return m, (order, begin, count)
-
-
-def _product_workspace(self, torch, m, what):
-    size = C.c_size_t(0)
-    self._check_plain(self.lib.lgbm_hip_leaf_product_workspace(C.byref(m), C.c_int32(what),
-                                                               C.byref(size)))
-    return _workspace(self, torch, size.value)
+    return _Maps(*[t.data_ptr() for t in hold], rows, trees, num, inputs, outputs, dtype, 0), hold
 
 
 def _leaf_product(self, x, weight, groups, bias=None, out=None):
@@ -177,7 +196,7 @@ def _leaf_product(self, x, weight, groups, bias=None, out=None):
     (`lgbm_hip_leaf_product`): x [rows, inputs], weight [trees * leaves, outputs, inputs],
     bias [trees * leaves, outputs] or None, all float32, bfloat16 or float16.  Returns y
     [rows, outputs]."""
-    import torch
+    torch = _module()
     if x.dim() != 2 or weight.dim() != 3:
         raise ValueError("x has to be [rows, inputs], weight [leaves, outputs, inputs]")
     dtype, (rows, inputs) = _dtype(x, "x"), x.shape
@@ -189,13 +208,13 @@ def _leaf_product(self, x, weight, groups, bias=None, out=None):
         _shape(bias, (leaves, outputs), "bias")
         bias = bias.contiguous()
     _here(self, x=x, weight=weight, bias=bias, out=out)
-    m, keep = _maps(self, rows, inputs, outputs, dtype, groups, leaves)
+    m, keep = _maps(self, torch, rows, inputs, outputs, dtype, groups, leaves)
     x, weight, out = _rows(x), weight.contiguous(), _out(out, x, (rows, outputs))
-    ws, nbytes, hold = _product_workspace(self, torch, m, _PRODUCT)
+    ws, nbytes, hold = _workspace(self, torch, self.lib.lgbm_hip_leaf_product_workspace,
+                                  C.byref(m), _PRODUCT)
     self._check(self.lib.lgbm_hip_leaf_product(
-        self.ctx, C.byref(m), C.c_void_p(x.data_ptr()), C.c_int64(_ld(x)),
-        C.c_void_p(weight.data_ptr()), C.c_void_p(None if bias is None else bias.data_ptr()),
-        C.c_void_p(out.data_ptr()), C.c_int64(_ld(out)), C.c_void_p(ws), C.c_size_t(nbytes),
+        self.ctx, C.byref(m), x.data_ptr(), _ld(x), weight.data_ptr(),
+        None if bias is None else bias.data_ptr(), out.data_ptr(), _ld(out), ws, nbytes,
         _stream(self, torch)))
     return out
 
@@ -203,7 +222,7 @@ def _leaf_product(self, x, weight, groups, bias=None, out=None):
 def _leaf_product_dx(self, dy, weight, groups, out=None):
     """The gradient of `leaf_product`'s x (`lgbm_hip_leaf_product_dx`): dy [rows, outputs]
     gives dx [rows, inputs], the sum over the trees."""
-    import torch
+    torch = _module()
     if dy.dim() != 2 or weight.dim() != 3:
         raise ValueError("dy has to be [rows, outputs], weight [leaves, outputs, inputs]")
     dtype, (rows, outputs) = _dtype(dy, "dy"), dy.shape
@@ -212,13 +231,13 @@ def _leaf_product_dx(self, dy, weight, groups, out=None):
     if weight.dtype != dy.dtype:
         raise ValueError("dy and weight differ in type")
     _here(self, dy=dy, weight=weight, out=out)
-    m, keep = _maps(self, rows, inputs, outputs, dtype, groups, leaves)
+    m, keep = _maps(self, torch, rows, inputs, outputs, dtype, groups, leaves)
     dy, weight, out = _rows(dy), weight.contiguous(), _out(out, dy, (rows, inputs))
-    ws, nbytes, hold = _product_workspace(self, torch, m, _DX)
+    ws, nbytes, hold = _workspace(self, torch, self.lib.lgbm_hip_leaf_product_workspace,
+                                  C.byref(m), _DX)
     self._check(self.lib.lgbm_hip_leaf_product_dx(
-        self.ctx, C.byref(m), C.c_void_p(dy.data_ptr()), C.c_int64(_ld(dy)),
-        C.c_void_p(weight.data_ptr()), C.c_void_p(out.data_ptr()), C.c_int64(_ld(out)),
-        C.c_void_p(ws), C.c_size_t(nbytes), _stream(self, torch)))
+        self.ctx, C.byref(m), dy.data_ptr(), _ld(dy), weight.data_ptr(), out.data_ptr(), _ld(out),
+        ws, nbytes, _stream(self, torch)))
     return out
 
 
@@ -226,7 +245,7 @@ def _leaf_product_dw(self, dy, x, groups, bias=True, out=None, bias_out=None):
     """The gradients of `leaf_product`'s weight and bias (`lgbm_hip_leaf_product_dw`):
     dw [trees * leaves, outputs, inputs] and db [trees * leaves, outputs] (None without
     `bias`), float32 whatever the type of dy [rows, outputs] and x [rows, inputs]."""
-    import torch
+    torch = _module()
     if dy.dim() != 2 or x.dim() != 2:
         raise ValueError("dy has to be [rows, outputs], x [rows, inputs]")
     dtype, (rows, outputs) = _dtype(dy, "dy"), dy.shape
@@ -237,7 +256,7 @@ def _leaf_product_dw(self, dy, x, groups, bias=True, out=None, bias_out=None):
     if bias_out is not None and not bias:
         raise ValueError("bias_out without bias")
     _here(self, dy=dy, x=x, out=out, bias_out=bias_out)
-    m, keep = _maps(self, rows, inputs, outputs, dtype, groups)
+    m, keep = _maps(self, torch, rows, inputs, outputs, dtype, groups)
     leaves = m.num_trees * m.num_leaves
     for name, t, shape in (("out", out, (leaves, outputs, inputs)),
                            ("bias_out", bias_out, (leaves, outputs))):
@@ -250,12 +269,11 @@ def _leaf_product_dw(self, dy, x, groups, bias=True, out=None, bias_out=None):
     if bias and db is None:
         db = dy.new_empty((leaves, outputs), dtype=torch.float32)
     dy, x = _rows(dy), _rows(x)
-    ws, nbytes, hold = _product_workspace(self, torch, m, _DW)
+    ws, nbytes, hold = _workspace(self, torch, self.lib.lgbm_hip_leaf_product_workspace,
+                                  C.byref(m), _DW)
     self._check(self.lib.lgbm_hip_leaf_product_dw(
-        self.ctx, C.byref(m), C.c_void_p(dy.data_ptr()), C.c_int64(_ld(dy)),
-        C.c_void_p(x.data_ptr()), C.c_int64(_ld(x)), C.c_void_p(dw.data_ptr()),
-        C.c_void_p(None if db is None else db.data_ptr()), C.c_void_p(ws), C.c_size_t(nbytes),
-        _stream(self, torch)))
+        self.ctx, C.byref(m), dy.data_ptr(), _ld(dy), x.data_ptr(), _ld(x), dw.data_ptr(),
+        None if db is None else db.data_ptr(), ws, nbytes, _stream(self, torch)))
     return dw, db
 
 
@@ -264,7 +282,7 @@ def _dropout(self, x, p, seed, offset=0, by="element", out=None):
     others divided by the share kept (`lgbm_hip_dropout`): the mask follows from seed and
     offset (64 bits each), so the gradient is the same call on the outputs' gradient.
     x [rows, cols] or [rows] float32, bfloat16 or float16; out may be x."""
-    import torch
+    torch = _module()
     if by not in ("element", "row"):
         raise ValueError("by is neither 'element' nor 'row'")
     if x.dim() not in (1, 2):
@@ -280,10 +298,8 @@ def _dropout(self, x, p, seed, offset=0, by="element", out=None):
         raise ValueError("out has strided columns or rows that overlap")
     dst = _out(out, x, tuple(x.shape))
     self._check(self.lib.lgbm_hip_dropout(
-        self.ctx, C.c_void_p(src.data_ptr()), C.c_int64(_ld(src)), C.c_int64(x.shape[0]),
-        C.c_int64(x.shape[1]), C.c_int32(dtype), C.c_double(p), C.c_uint64(seed & (2 ** 64 - 1)),
-        C.c_uint64(offset & (2 ** 64 - 1)), C.c_int32(by == "row"), C.c_void_p(dst.data_ptr()),
-        C.c_int64(_ld(dst)), _stream(self, torch)))
+        self.ctx, src.data_ptr(), _ld(src), x.shape[0], x.shape[1], dtype, p, seed & (2 ** 64 - 1),
+        offset & (2 ** 64 - 1), by == "row", dst.data_ptr(), _ld(dst), _stream(self, torch)))
     return dst
 
 
@@ -299,12 +315,12 @@ def _adjust_scores(self, scores, kind="raw", bias=None, mask=None, mask_rows=Non
     int32 [rows] the mask of every row (-1: none; left out: one mask, or one for each row);
     ids int32 and offsets int64 [rows + 1]: row n's history is ids[offsets[n]:offsets[n +
     1]]; penalties float32 [rows, 3] instead of the three numbers.  out may be scores."""
-    import torch
+    torch = _module()
     if scores.dim() != 2:
         raise ValueError("scores has to be [rows, classes]")
     if kind not in ("raw", "transformed"):
         raise ValueError("kind is neither 'raw' nor 'transformed'")
-    dtype, (rows, classes) = _dtype(scores, "scores", tuple(_DTYPES)), scores.shape
+    dtype, (rows, classes) = _dtype(scores, "scores", True), scores.shape
     if bias is not None:
         _shape(bias, (classes,), "bias")
         if bias.dtype != scores.dtype:
@@ -314,21 +330,21 @@ def _adjust_scores(self, scores, kind="raw", bias=None, mask=None, mask_rows=Non
         if mask.dim() == 1:
             mask = mask[None]
         _shape(mask, (mask.shape[0], (classes + 31) // 32), "mask")
-        mask = _ints(mask, "mask")
+        mask = _typed(mask, "mask", torch.int32)
     elif mask_rows is not None:
         raise ValueError("mask_rows without mask")
     if mask_rows is not None:
         _shape(mask_rows, (rows,), "mask_rows")
-        mask_rows = _ints(mask_rows, "mask_rows")
+        mask_rows = _typed(mask_rows, "mask_rows", torch.int32)
     if (ids is None) != (offsets is None):
         raise ValueError("a history needs ids and offsets")
     if ids is not None:
         _shape(ids, (ids.numel(),), "ids")
         _shape(offsets, (rows + 1,), "offsets")
-        ids, offsets = _ints(ids, "ids"), _ints(offsets, "offsets", "int64")
+        ids, offsets = _typed(ids, "ids", torch.int32), _typed(offsets, "offsets", torch.int64)
     if penalties is not None:
         _shape(penalties, (rows, 3), "penalties")
-        penalties = _ints(penalties, "penalties", "float32")
+        penalties = _typed(penalties, "penalties", torch.float32)
     _here(self, scores=scores, bias=bias, mask=mask, mask_rows=mask_rows, ids=ids,
           offsets=offsets, penalties=penalties, out=out)
     src = _rows(scores)
@@ -340,11 +356,9 @@ def _adjust_scores(self, scores, kind="raw", bias=None, mask=None, mask_rows=Non
                 0 if mask is None else mask.shape[0], at(bias), at(mask), at(mask_rows), at(ids),
                 at(offsets), 0 if ids is None else ids.numel(), repetition, frequency, presence,
                 at(penalties), at(out), _ld(out))
-    size = C.c_size_t(0)
-    self._check_plain(self.lib.lgbm_hip_adjust_scores_workspace(C.byref(a), C.byref(size)))
-    ws, nbytes, hold = _workspace(self, torch, size.value)
-    self._check(self.lib.lgbm_hip_adjust_scores(self.ctx, C.byref(a), C.c_void_p(ws),
-                                                C.c_size_t(nbytes), _stream(self, torch)))
+    ws, nbytes, hold = _workspace(self, torch, self.lib.lgbm_hip_adjust_scores_workspace, C.byref(a))
+    self._check(self.lib.lgbm_hip_adjust_scores(self.ctx, C.byref(a), ws, nbytes,
+                                                _stream(self, torch)))
     return out
 
 
