@@ -12,8 +12,8 @@ using namespace lgbm;
 
 namespace {
 
-// hipLaunch's limit of work items along x, in blocks of the largest size used here.
-constexpr int64_t MAX_GRID_X = (int64_t)0xffffffff / 1024;
+// The limit of work items along x, in blocks of the products' size.
+constexpr int64_t MAX_GRID_X = (int64_t)0xffffffff / 256;
 
 int bad(lgbm_hip_ctx* c, const char* what) {
   return context_error(c, LGBM_HIP_ERR_INVALID_ARGUMENT, what);
@@ -191,6 +191,7 @@ int lgbm_hip_leaf_product(lgbm_hip_ctx* c, const lgbm_leaf_maps* m, const void* 
     return bad(c, "a pointer is not aligned to its type");
   LeafProduct p = product_of(m);
   const size_t need = leaf_product_workspace(p, LEAF_PRODUCT_Y);
+  p.x = d_x, p.ldx = ldx, p.w = d_w, p.b = d_bias, p.out = d_y, p.ldo = ldy, p.ws = d_ws;
   if ((rc = check_ws(c, d_ws, ws_bytes, need)) || (rc = check_grid(c, p, LEAF_PRODUCT_Y))) return rc;
   const Span y = matrix(d_y, rows, m->outputs, ldy, e), ws{d_ws, (int64_t)need};
   const Span x = matrix(d_x, rows, m->inputs, ldx, e), w = weights(m, d_w, e), b = biases(m, d_bias, e);
@@ -198,7 +199,6 @@ int lgbm_hip_leaf_product(lgbm_hip_ctx* c, const lgbm_leaf_maps* m, const void* 
       overlaps(ws, {x, w, b, order_of(m), table(m, m->d_begin), table(m, m->d_count)}))
     return bad(c, "y or the workspace overlaps an input");
   if (rows == 0) return c ? LGBM_HIP_OK : bad(c, "null context");
-  p.x = d_x, p.ldx = ldx, p.w = d_w, p.b = d_bias, p.out = d_y, p.ldo = ldy, p.ws = d_ws;
   return queue(c, stream, [&](hipStream_t s) { launch_leaf_product(p, LEAF_PRODUCT_Y, s); });
 }
 
@@ -215,6 +215,7 @@ int lgbm_hip_leaf_product_dx(lgbm_hip_ctx* c, const lgbm_leaf_maps* m, const voi
     return bad(c, "a pointer is not aligned to its type");
   LeafProduct p = product_of(m);
   const size_t need = leaf_product_workspace(p, LEAF_PRODUCT_DX);
+  p.dy = d_dy, p.lddy = lddy, p.w = d_w, p.out = d_dx, p.ldo = lddx, p.ws = d_ws;
   if ((rc = check_ws(c, d_ws, ws_bytes, need)) || (rc = check_grid(c, p, LEAF_PRODUCT_DX))) return rc;
   const Span dx = matrix(d_dx, rows, m->inputs, lddx, e), ws{d_ws, (int64_t)need};
   const Span dy = matrix(d_dy, rows, m->outputs, lddy, e), w = weights(m, d_w, e);
@@ -222,7 +223,6 @@ int lgbm_hip_leaf_product_dx(lgbm_hip_ctx* c, const lgbm_leaf_maps* m, const voi
       overlaps(ws, {dy, w, order_of(m), table(m, m->d_begin), table(m, m->d_count)}))
     return bad(c, "dx or the workspace overlaps an input");
   if (rows == 0) return c ? LGBM_HIP_OK : bad(c, "null context");
-  p.dy = d_dy, p.lddy = lddy, p.w = d_w, p.out = d_dx, p.ldo = lddx, p.ws = d_ws;
   return queue(c, stream, [&](hipStream_t s) { launch_leaf_product(p, LEAF_PRODUCT_DX, s); });
 }
 
@@ -239,6 +239,7 @@ int lgbm_hip_leaf_product_dw(lgbm_hip_ctx* c, const lgbm_leaf_maps* m, const voi
     return bad(c, "a pointer is not aligned to its type");
   LeafProduct p = product_of(m);
   const size_t need = leaf_product_workspace(p, LEAF_PRODUCT_DW);
+  p.dy = d_dy, p.lddy = lddy, p.x = d_x, p.ldx = ldx, p.dw = d_dw, p.db = d_db, p.ws = d_ws;
   if ((rc = check_ws(c, d_ws, ws_bytes, need)) || (rc = check_grid(c, p, LEAF_PRODUCT_DW))) return rc;
   const Span dw = weights(m, d_dw, 4), db = biases(m, d_db, 4), ws{d_ws, (int64_t)need};
   const Span dy = matrix(d_dy, rows, m->outputs, lddy, e), x = matrix(d_x, rows, m->inputs, ldx, e);
@@ -246,7 +247,6 @@ int lgbm_hip_leaf_product_dw(lgbm_hip_ctx* c, const lgbm_leaf_maps* m, const voi
       overlaps(db, {dy, x, order_of(m), table(m, m->d_begin), table(m, m->d_count), ws}) ||
       overlaps(ws, {dy, x, order_of(m), table(m, m->d_begin), table(m, m->d_count)}))
     return bad(c, "dw, db or the workspace overlaps an input or one another");
-  p.dy = d_dy, p.lddy = lddy, p.x = d_x, p.ldx = ldx, p.dw = d_dw, p.db = d_db, p.ws = d_ws;
   return queue(c, stream, [&](hipStream_t s) { launch_leaf_product(p, LEAF_PRODUCT_DW, s); });
 }
 

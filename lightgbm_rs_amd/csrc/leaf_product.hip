@@ -135,13 +135,14 @@ __global__ __launch_bounds__(THREADS) void k_leaf_tile(LeafProduct p, int length
 // The same for up to 16 NB outputs of a leaf: bound by reading x, which no wave shares with
 // another, so lanes load their fragments straight from memory (16 rows x 64 bytes an
 // instruction; w from the caches), UNROLL steps at a time and without a barrier.  A wave
-// takes ROUNDS times 32 rows.
-template <typename T, int NB>
-__global__ __launch_bounds__(THREADS) void k_leaf_narrow(LeafProduct p) {
-  constexpr int V = El<T>::V, UNROLL = 4, ROUNDS = 2, BM = 4 * 32 * ROUNDS;
+// takes ROUNDS times 32 rows; blocks of one wave where leaves hold few rows.
+template <typename T, int NB, int WAVES>
+__global__ __launch_bounds__(WAVES * 64) void k_leaf_narrow(LeafProduct p) {
+  constexpr int V = El<T>::V, UNROLL = 4, ROUNDS = 2, BM = WAVES * 32 * ROUNDS;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, r = lane & 15, q = lane >> 4;
   const int tree = blockIdx.y, length = p.inputs, cols = p.outputs;
-  const RowTile rt = find_tile<THREADS>(p.g, tree, blockIdx.x, BM);
+  const RowTile rt = find_tile<WAVES * 64>(p.g, tree, blockIdx.x, BM);
+  if (rt.rows == 0) return;
   const int64_t leaf = (int64_t)tree * p.g.leaves + rt.leaf;
   const T* const w = (const T*)p.w + (rt.leaf < 0 ? 0 : leaf * cols * (int64_t)length);
   const T* wrow[NB];
@@ -156,12 +157,12 @@ __global__ __launch_bounds__(THREADS) void k_leaf_narrow(LeafProduct p) {
   for (int t = 0; t < ROUNDS; ++t)
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
-      const int at = (t * 4 + wave) * 32 + i * 16 + r;
+      const int at = (t * WAVES + wave) * 32 + i * 16 + r;
       n[t][i] = at < rt.rows ? row_at(p.g, tree, rt.first + at) : -1;
     }
 #pragma unroll
   for (int t = 0; t < ROUNDS; ++t) {
-    if ((t * 4 + wave) * 32 >= rt.rows) break;
+    if ((t * WAVES + wave) * 32 >= rt.rows) break;
     f32x4 acc[2][NB];
 #pragma unroll
     for (int i = 0; i < 2; ++i)
@@ -209,6 +210,49 @@ __global__ __launch_bounds__(THREADS) void k_leaf_narrow(LeafProduct p) {
         const int col = j * 16 + q * 4;
         if (n[t][i] >= 0 && col < cols) store_row<T>(p, tree, n[t][i], col, cols, acc[i][j]);
       }
+  }
+}
+
+// y where leaves hold few rows and the inputs are many: bound by reading the maps.  A block
+// makes 16 x 16 of a leaf's result; its waves take every fourth part of the inputs, straight
+// from memory, and their sums are added in LDS.
+template <typename T>
+__global__ __launch_bounds__(THREADS) void k_leaf_few(LeafProduct p, int col_tiles) {
+  constexpr int V = El<T>::V, UNROLL = 4, PART = 4 * V * UNROLL;
+  __shared__ f32x4 sums[4][64];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, r = lane & 15, q = lane >> 4;
+  const int tree = blockIdx.y, length = p.inputs, cols = p.outputs;
+  const int c0 = (int)(blockIdx.x % col_tiles) * 16;
+  const RowTile rt = find_tile<THREADS>(p.g, tree, blockIdx.x / col_tiles, 16);
+  if (rt.rows == 0) return;
+  const int64_t leaf = (int64_t)tree * p.g.leaves + rt.leaf;
+  const int n = r < rt.rows ? row_at(p.g, tree, rt.first + r) : -1;
+  f32x4 acc = {0, 0, 0, 0};
+  if (rt.leaf >= 0) {
+    const T* const xrow = (const T*)p.x + (int64_t)max(n, 0) * p.ldx;
+    const T* const wrow = (const T*)p.w + (leaf * cols + min(c0 + r, cols - 1)) * (int64_t)length;
+    for (int k0 = wave * PART; k0 < length; k0 += 4 * PART) {
+      u32x4 fx[UNROLL], fw[UNROLL];
+      const bool whole = k0 + PART <= length;
+#pragma unroll
+      for (int u = 0; u < UNROLL; ++u) {
+        const int k = k0 + (u * 4 + q) * V;
+        fw[u] = whole ? load16(wrow + k) : load16(wrow + k, length - k);
+        fx[u] = whole ? load16(xrow + k) : load16(xrow + k, length - k);
+      }
+#pragma unroll
+      for (int u = 0; u < UNROLL; ++u) acc = El<T>::mfma(fw[u], fx[u], acc);
+    }
+  }
+  sums[wave][lane] = acc;
+  __syncthreads();
+  const int col = c0 + q * 4;
+  if (wave == 0 && n >= 0 && col < cols) {
+    const T* const bias = (p.b && rt.leaf >= 0) ? (const T*)p.b + leaf * cols : nullptr;
+    acc += bias4(bias, col, cols);
+#pragma unroll
+    for (int v = 1; v < 4; ++v) acc += sums[v][lane];
+    store_row<T>(p, tree, n, col, cols, acc);
   }
 }
 
@@ -500,6 +544,9 @@ DwShape dw_shape(const LeafProduct& p) {
   return {64, 64};
 }
 
+// Leaves of 16 rows at most, on average.
+bool few_rows(const LeafProduct& p) { return p.g.rows <= 16 * (int64_t)p.g.leaves; }
+
 template <typename T, int BM, int BN, int GM>
 void launch_dw(const LeafProduct& p, hipStream_t s) {
   const int mt = (p.outputs + BM - 1) / BM, kt = (p.inputs + BN - 1) / BN;
@@ -546,12 +593,20 @@ void launch(const LeafProduct& p, int what, hipStream_t s) {
     k_leaf_dx_narrow<T><<<grid, THREADS, 0, s>>>(p, ct, steps);
   } else if (dx) {
     launch_tile<T, true, 64, 64, 2>(p, s);
+  } else if (few_rows(p) && p.inputs >= 512) {
+    const int ct = (cols + 15) / 16;
+    k_leaf_few<T><<<dim3((unsigned)(row_tiles(p.g, 16) * ct), (unsigned)p.g.trees), THREADS, 0, s>>>(p, ct);
   } else if (cols <= 32) {
-    const dim3 grid((unsigned)row_tiles(p.g, 256), (unsigned)p.g.trees);
-    if (cols <= 16)
-      k_leaf_narrow<T, 1><<<grid, THREADS, 0, s>>>(p);
+    const bool one = few_rows(p);
+    const dim3 grid((unsigned)row_tiles(p.g, one ? 64 : 256), (unsigned)p.g.trees);
+    if (cols <= 16 && one)
+      k_leaf_narrow<T, 1, 1><<<grid, 64, 0, s>>>(p);
+    else if (cols <= 16)
+      k_leaf_narrow<T, 1, 4><<<grid, 256, 0, s>>>(p);
+    else if (one)
+      k_leaf_narrow<T, 2, 1><<<grid, 64, 0, s>>>(p);
     else
-      k_leaf_narrow<T, 2><<<grid, THREADS, 0, s>>>(p);
+      k_leaf_narrow<T, 2, 4><<<grid, 256, 0, s>>>(p);
   } else {
     launch_tile<T, false, 64, 64, 2>(p, s);
   }
@@ -591,7 +646,10 @@ int64_t leaf_product_blocks(const LeafProduct& p, int what) {
     const int64_t leaves = (int64_t)p.g.trees * p.g.leaves;
     return split.rows ? std::max(tiles * split.slots, leaves) : tiles * leaves;
   }
-  return row_tiles(p.g, 64) * (((what == LEAF_PRODUCT_DX ? p.inputs : p.outputs) + 63) / 64);
+  const int64_t cols = what == LEAF_PRODUCT_DX ? p.inputs : p.outputs;
+  if (what == LEAF_PRODUCT_DX && p.outputs <= 32) return row_tiles(p.g, 512) * ((cols + 127) / 128);
+  if (what == LEAF_PRODUCT_Y && few_rows(p) && p.inputs >= 512) return row_tiles(p.g, 16) * ((cols + 15) / 16);
+  return row_tiles(p.g, 64) * ((cols + 63) / 64);
 }
 
 void launch_leaf_product(const LeafProduct& p, int what, hipStream_t s) {
