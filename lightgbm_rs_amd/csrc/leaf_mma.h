@@ -52,6 +52,33 @@ struct El<_Float16> {
   }
 };
 
+// The sums of a stretch of the contraction.  In float32 they start at zero and are added to
+// the whole ones afterwards, so that a rounding is of a short sum's size: a chain over 1000
+// elements was off by ten times as much.  With 16-bit operands the rounding of the result
+// hides that, and the stretch goes on in place.
+template <typename T, int M, int N>
+struct Parts {
+  f32x4 (&at)[M][N];
+  __device__ __forceinline__ Parts(f32x4 (&sums)[M][N]) : at(sums) {}
+  __device__ __forceinline__ void add_to(f32x4 (&)[M][N]) {}
+};
+template <int M, int N>
+struct Parts<float, M, N> {
+  f32x4 at[M][N];
+  __device__ __forceinline__ Parts(f32x4 (&)[M][N]) {
+#pragma unroll
+    for (int i = 0; i < M; ++i)
+#pragma unroll
+      for (int j = 0; j < N; ++j) at[i][j] = f32x4{0, 0, 0, 0};
+  }
+  __device__ __forceinline__ void add_to(f32x4 (&sums)[M][N]) {
+#pragma unroll
+    for (int i = 0; i < M; ++i)
+#pragma unroll
+      for (int j = 0; j < N; ++j) sums[i][j] += at[i][j];
+  }
+};
+
 // 16 bytes of elements p[0 .. valid), zeros behind them; nothing behind `valid` is read.
 // gfx950 loads 16 bytes from any address, so rows need no alignment.
 template <typename T>

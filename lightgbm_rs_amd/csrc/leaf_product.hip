@@ -98,6 +98,7 @@ __global__ __launch_bounds__(THREADS) void k_leaf_tile(LeafProduct p, int length
       const bool more = k0 + BK < length;
       if (more) load(k0 + BK);
       const char *ta = lds[b], *tb = lds[b] + BM * 128;
+      Parts<T, WM / 16, WN / 16> part(acc);
 #pragma unroll
       for (int step = 0; step < 2; ++step) {
         if (step == 1 && k0 + BK / 2 >= length) break;
@@ -110,8 +111,9 @@ __global__ __launch_bounds__(THREADS) void k_leaf_tile(LeafProduct p, int length
 #pragma unroll
         for (int i = 0; i < WM / 16; ++i)
 #pragma unroll
-          for (int j = 0; j < WN / 16; ++j) acc[i][j] = El<T>::mfma(fb[j], fa[i], acc[i][j]);
+          for (int j = 0; j < WN / 16; ++j) part.at[i][j] = El<T>::mfma(fb[j], fa[i], part.at[i][j]);
       }
+      part.add_to(acc);
       if (more) store(lds[b ^ 1]);
       __syncthreads();
     }
@@ -193,14 +195,16 @@ __global__ __launch_bounds__(WAVES * 64) void k_leaf_narrow(LeafProduct p) {
             for (int j = 0; j < NB; ++j) fb[u][j] = load16(wrow[j] + k, length - k);
           }
         }
+        Parts<T, 2, NB> part(acc);
 #pragma unroll
         for (int u = 0; u < UNROLL; ++u) {
           if (k0 + u * 4 * V >= length) break;
 #pragma unroll
           for (int i = 0; i < 2; ++i)
 #pragma unroll
-            for (int j = 0; j < NB; ++j) acc[i][j] = El<T>::mfma(fb[u][j], fa[u][i], acc[i][j]);
+            for (int j = 0; j < NB; ++j) part.at[i][j] = El<T>::mfma(fb[u][j], fa[u][i], part.at[i][j]);
         }
+        part.add_to(acc);
       }
     }
 #pragma unroll
@@ -227,7 +231,7 @@ __global__ __launch_bounds__(THREADS) void k_leaf_few(LeafProduct p, int col_til
   if (rt.rows == 0) return;
   const int64_t leaf = (int64_t)tree * p.g.leaves + rt.leaf;
   const int n = r < rt.rows ? row_at(p.g, tree, rt.first + r) : -1;
-  f32x4 acc = {0, 0, 0, 0};
+  f32x4 acc[1][1] = {{f32x4{0, 0, 0, 0}}};
   if (rt.leaf >= 0) {
     const T* const xrow = (const T*)p.x + (int64_t)max(n, 0) * p.ldx;
     const T* const wrow = (const T*)p.w + (leaf * cols + min(c0 + r, cols - 1)) * (int64_t)length;
@@ -240,19 +244,21 @@ __global__ __launch_bounds__(THREADS) void k_leaf_few(LeafProduct p, int col_til
         fw[u] = whole ? load16(wrow + k) : load16(wrow + k, length - k);
         fx[u] = whole ? load16(xrow + k) : load16(xrow + k, length - k);
       }
+      Parts<T, 1, 1> part(acc);
 #pragma unroll
-      for (int u = 0; u < UNROLL; ++u) acc = El<T>::mfma(fw[u], fx[u], acc);
+      for (int u = 0; u < UNROLL; ++u) part.at[0][0] = El<T>::mfma(fw[u], fx[u], part.at[0][0]);
+      part.add_to(acc);
     }
   }
-  sums[wave][lane] = acc;
+  sums[wave][lane] = acc[0][0];
   __syncthreads();
   const int col = c0 + q * 4;
   if (wave == 0 && n >= 0 && col < cols) {
     const T* const bias = (p.b && rt.leaf >= 0) ? (const T*)p.b + leaf * cols : nullptr;
-    acc += bias4(bias, col, cols);
+    f32x4 y = acc[0][0] + bias4(bias, col, cols);
 #pragma unroll
-    for (int v = 1; v < 4; ++v) acc += sums[v][lane];
-    store_row<T>(p, tree, n, col, cols, acc);
+    for (int v = 1; v < 4; ++v) y += sums[v][lane];
+    store_row<T>(p, tree, n, col, cols, y);
   }
 }
 
@@ -470,6 +476,7 @@ __global__ __launch_bounds__(THREADS) void k_leaf_dw(LeafProduct p, int m_tiles,
       if (more) load(r0 + BK);
       rows(r0 + 2 * BK);  // into the half whose rows are loaded already
       const char *ta = lds[b], *tb = lds[b] + BM * 128;
+      Parts<T, WM / 16, WN / 16> part(acc);
 #pragma unroll
       for (int step = 0; step < 2; ++step) {
         u32x4 fa[WM / 16], fb[WN / 16];
@@ -483,8 +490,9 @@ __global__ __launch_bounds__(THREADS) void k_leaf_dw(LeafProduct p, int m_tiles,
 #pragma unroll
         for (int i = 0; i < WM / 16; ++i)
 #pragma unroll
-          for (int j = 0; j < WN / 16; ++j) acc[i][j] = El<T>::mfma(fb[j], fa[i], acc[i][j]);
+          for (int j = 0; j < WN / 16; ++j) part.at[i][j] = El<T>::mfma(fb[j], fa[i], part.at[i][j]);
       }
+      part.add_to(acc);
       if (more) store(lds[b ^ 1]);
       __syncthreads();
     }
