@@ -555,6 +555,21 @@ DwShape dw_shape(const LeafProduct& p) {
 // Leaves of 16 rows at most, on average.
 bool few_rows(const LeafProduct& p) { return p.g.rows <= 16 * (int64_t)p.g.leaves; }
 
+// k_leaf_few: leaves of few rows, or few outputs of so few rows that blocks of 256 would leave
+// CUs without work (3000 x 2000 float32 to 10 outputs: 68 us by k_leaf_narrow, 14).
+bool by_maps(const LeafProduct& p) {
+  return p.inputs >= 512 && (few_rows(p) || (p.outputs <= 32 && p.g.rows < 65536));
+}
+
+// Tiles of 128 x 128, where leaves fill them and there is one for every CU: 16-bit products
+// that are not for leaf_big.hip (40000 x 2001 to 2047 bf16 by 9 leaves: y 690 us instead of
+// 965, dx 945 instead of 1004).  float32 is slower by them (20000 x 1000 to 1000 by 7: 454 us,
+// 423 by 64 x 64), and so are the gradients of the maps (bf16 as above: 2518 us, 1371).
+bool wide_tiles(const LeafProduct& p, int cols) {
+  return p.dtype != LGBM_HIP_DTYPE_F32 && cols >= 128 && p.g.rows >= 128 * (int64_t)p.g.leaves &&
+         (int64_t)p.g.rows / 128 * ((cols + 127) / 128) * p.g.trees >= 256;
+}
+
 template <typename T, int BM, int BN, int GM>
 void launch_dw(const LeafProduct& p, hipStream_t s) {
   const int mt = (p.outputs + BM - 1) / BM, kt = (p.inputs + BN - 1) / BN;
@@ -570,12 +585,20 @@ void launch_dw(const LeafProduct& p, hipStream_t s) {
   k_sum_slots<<<(unsigned)(leaves * parts), THREADS, 0, s>>>(p, split, parts);
 }
 
-template <typename T, bool DX, int BM, int BN, int GM>
+template <typename T, bool DX, int BM, int BN>
 void launch_tile(const LeafProduct& p, hipStream_t s) {
   const int length = DX ? p.outputs : p.inputs, cols = DX ? p.inputs : p.outputs;
   const int ct = (cols + BN - 1) / BN;
   const dim3 grid((unsigned)(row_tiles(p.g, BM) * ct), (unsigned)p.g.trees);
-  k_leaf_tile<T, DX, BM, BN, GM><<<grid, THREADS, 0, s>>>(p, length, cols, ct);
+  k_leaf_tile<T, DX, BM, BN, 2><<<grid, THREADS, 0, s>>>(p, length, cols, ct);
+}
+
+template <typename T, bool DX>
+void launch_tiles(const LeafProduct& p, int cols, hipStream_t s) {
+  if constexpr (sizeof(T) == 2) {
+    if (wide_tiles(p, cols)) return launch_tile<T, DX, 128, 128>(p, s);
+  }
+  launch_tile<T, DX, 64, 64>(p, s);
 }
 
 template <typename T>
@@ -600,8 +623,8 @@ void launch(const LeafProduct& p, int what, hipStream_t s) {
     const dim3 grid((unsigned)(row_tiles(p.g, 512) * ct), (unsigned)p.g.trees);
     k_leaf_dx_narrow<T><<<grid, THREADS, 0, s>>>(p, ct, steps);
   } else if (dx) {
-    launch_tile<T, true, 64, 64, 2>(p, s);
-  } else if (few_rows(p) && p.inputs >= 512) {
+    launch_tiles<T, true>(p, cols, s);
+  } else if (by_maps(p)) {
     const int ct = (cols + 15) / 16;
     k_leaf_few<T><<<dim3((unsigned)(row_tiles(p.g, 16) * ct), (unsigned)p.g.trees), THREADS, 0, s>>>(p, ct);
   } else if (cols <= 32) {
@@ -616,7 +639,7 @@ void launch(const LeafProduct& p, int what, hipStream_t s) {
     else
       k_leaf_narrow<T, 2, 4><<<grid, 256, 0, s>>>(p);
   } else {
-    launch_tile<T, false, 64, 64, 2>(p, s);
+    launch_tiles<T, false>(p, cols, s);
   }
   if (p.g.trees > 1) {
     const int64_t total = (int64_t)p.g.rows * cols;
@@ -656,7 +679,7 @@ int64_t leaf_product_blocks(const LeafProduct& p, int what) {
   }
   const int64_t cols = what == LEAF_PRODUCT_DX ? p.inputs : p.outputs;
   if (what == LEAF_PRODUCT_DX && p.outputs <= 32) return row_tiles(p.g, 512) * ((cols + 127) / 128);
-  if (what == LEAF_PRODUCT_Y && few_rows(p) && p.inputs >= 512) return row_tiles(p.g, 16) * ((cols + 15) / 16);
+  if (what == LEAF_PRODUCT_Y && by_maps(p)) return row_tiles(p.g, 16) * ((cols + 15) / 16);
   return row_tiles(p.g, 64) * ((cols + 63) / 64);
 }
 

@@ -69,7 +69,7 @@ SHAPES = [
     (17, 16, 16, 1, 1, "one", 0), (100, 33, 17, 2, 7, "lost", 3), (257, 64, 64, 1, 4, "skew", 8),
     (300, 100, 10, 1, 31, "even", 0), (129, 128, 130, 1, 2, "even", 8), (500, 200, 96, 3, 5, "lost", 0),
     (16, 520, 300, 1, 31, "even", 0), (3, 1000, 260, 2, 3, "even", 0), (1000, 70, 257, 1, 3, "skew", 1),
-    (700, 256, 256, 1, 2, "one", 0), (2000, 13, 3, 5, 63, "skew", 0), (40, 2000, 1, 1, 7, "even", 0),
+    (700, 256, 256, 1, 2, "one", 0), (2000, 13, 3, 5, 63, "skew", 0), (40, 2000, 1, 1, 7, "even", 0), (600, 530, 20, 1, 2, "skew", 0),
     (333, 65, 8, 1, 1, "lost", 2), (900, 129, 33, 2, 15, "even", 8), (2500, 40, 10, 1, 2, "one", 0)]
 
 
@@ -90,7 +90,9 @@ def test_gradients(check, rows, inputs, outputs, trees, leaves, shape, pad, dtyp
 @pytest.mark.parametrize("what", ["product", "grads"])
 @pytest.mark.parametrize("rows,inputs,outputs,trees,leaves,dtype", [
     (9000, 24, 6, 1, 2, "f32"), (9000, 30, 9, 1, 2, "bf16"), (5000, 320, 272, 1, 3, "bf16"),
-    (5000, 272, 320, 1, 3, "f16"), (1500, 600, 512, 2, 2, "bf16"), (40000, 5, 1, 1, 300, "f32")])
+    (5000, 272, 320, 1, 3, "f16"), (1500, 600, 512, 2, 2, "bf16"), (40000, 5, 1, 1, 300, "f32"),
+    (9000, 65, 513, 1, 3, "bf16"), (9000, 515, 33, 1, 3, "f16"), (3000, 200, 1100, 5, 2, "f16"),
+    (2000, 264, 520, 1, 5, "bf16"), (70000, 600, 20, 1, 2, "bf16"), (1000, 2048, 256, 1, 1, "bf16")])
 def test_long(check, what, rows, inputs, outputs, trees, leaves, dtype):
     check(what, rows=rows, inputs=inputs, outputs=outputs, trees=trees, leaves=leaves, dtype=dtype,
           shape="even")
