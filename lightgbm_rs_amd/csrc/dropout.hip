@@ -10,10 +10,11 @@
 //
 // Bound by memory: an element is read and written once; the ten rounds' twenty 32 x 32
 // products for eight elements are below the time that their bytes take.  Elements without
-// gaps between rows are one long row, so any number of columns runs in vectors
-// (k_dropout_flat); rows of which the pairs of a few columns follow each other too
-// (k_dropout_rows: a unit's columns lie in one vector or one run of vectors); the rest goes
-// by element (k_dropout).
+// gaps between rows are one long row (k_dropout_flat: 32771 x 4096 bfloat16 89 us, 6.0 TB/s);
+// so are whole rows of 1, 2 or 4 columns, where a thread's vector holds several
+// (k_dropout_pairs: 10.5M x 2 float32 29 us, 5.8 TB/s); the rest goes row by row, eight
+// elements a thread (k_dropout_rows: 32771 x 4096 of stride 4104 111 us, 4.8 TB/s; 10M x 3
+// whole rows of float32 94 us, where every row makes its own block of the generator).
 #include <algorithm>
 
 #include "leaf_ops.h"
@@ -79,20 +80,17 @@ __global__ __launch_bounds__(THREADS) void k_dropout_flat(const T* x, int64_t to
   }
 }
 
-// Whole rows of 1 << col_bits columns without gaps, a vector a thread.  Eight rows share a
-// block of the generator, so 8 columns / V threads make the same one: no more work than
-// the memory leaves time for.
+// Whole rows of 1, 2 or 4 columns without gaps, a vector a thread: its rows lie in one block
+// of the generator.
 template <typename T>
-__global__ __launch_bounds__(THREADS) void k_dropout_rows(const T* x, int64_t total, int col_bits,
-                                                          Dropout d, T* out) {
+__global__ __launch_bounds__(THREADS) void k_dropout_pairs(const T* x, int64_t total, int col_bits,
+                                                           Dropout d, T* out) {
   constexpr int V = 16 / (int)sizeof(T);
   for (int64_t i = (blockIdx.x * (int64_t)THREADS + threadIdx.x) * V; i < total;
        i += (int64_t)gridDim.x * THREADS * V) {
     const int64_t row = i >> col_bits;
     const uint4 r = philox((uint64_t)(row >> 3), d.offset, d.seed);
     const uint64_t lo = (uint64_t)r.y << 32 | r.x, hi = (uint64_t)r.w << 32 | r.z;
-    // V consecutive elements of rows of a power of two reach over at most 8 rows of one
-    // block: V <= 8, and a block is 8 columns long or a multiple of it
     T v[V];
     if (i + V <= total) {
       __builtin_memcpy(v, x + i, sizeof(v));
@@ -113,35 +111,36 @@ __global__ __launch_bounds__(THREADS) void k_dropout_rows(const T* x, int64_t to
   }
 }
 
-// Any strides: a block of eight units a thread, or a block's eight rows a wave.
-template <typename T>
-__global__ __launch_bounds__(THREADS) void k_dropout(const T* x, int64_t ldx, int64_t rows, int64_t cols,
-                                                     Dropout d, int by_row, T* out, int64_t ldo) {
-  if (by_row) {
-    const int lane = threadIdx.x & 63;
-    const int64_t blocks = (rows + 7) / 8, waves = (int64_t)gridDim.x * (THREADS / 64);
-    for (int64_t b = blockIdx.x * (int64_t)(THREADS / 64) + (threadIdx.x >> 6); b < blocks; b += waves) {
-      const uint4 r = philox((uint64_t)b, d.offset, d.seed);
-      const int here = (int)min((int64_t)8, rows - b * 8);
-      for (int j = 0; j < here; ++j) {
-        const bool keep = field_of(r, j) >= d.threshold;
-        const T* const from = x + (b * 8 + j) * ldx;
-        T* const to = out + (b * 8 + j) * ldo;
-        for (int64_t c = lane; c < cols; c += 64) to[c] = kept(from[c], keep, d.scale);
-      }
-    }
-    return;
-  }
-  const int64_t units = rows * cols, blocks = (units + 7) / 8;
-  for (int64_t b = blockIdx.x * (int64_t)THREADS + threadIdx.x; b < blocks;
-       b += (int64_t)gridDim.x * THREADS) {
-    const uint4 r = philox((uint64_t)b, d.offset, d.seed);
-    int64_t n = b * 8 / cols, c = b * 8 - n * cols;
+// Rows of any columns and strides, eight elements of a row a thread, 1 << tx_bits threads
+// along a row.  By element the eights are the generator's blocks, so a row may begin and end
+// within one, which two rows then make.
+template <typename T, bool BY_ROW>
+__global__ __launch_bounds__(THREADS) void k_dropout_rows(const T* x, int64_t ldx, int64_t rows, int64_t cols,
+                                                          int tx_bits, Dropout d, T* out, int64_t ldo) {
+  const int tx = threadIdx.x & ((1 << tx_bits) - 1), ty = threadIdx.x >> tx_bits;
+  const int64_t row_step = (int64_t)gridDim.y * (THREADS >> tx_bits), col_step = ((int64_t)gridDim.x << tx_bits) * 8;
+  for (int64_t n = blockIdx.y * (int64_t)(THREADS >> tx_bits) + ty; n < rows; n += row_step) {
+    const int64_t unit0 = BY_ROW ? 0 : n * cols;
+    const T* const from = x + n * ldx;
+    T* const to = out + n * ldo;
+    const uint4 whole = BY_ROW ? philox((uint64_t)n >> 3, d.offset, d.seed) : make_uint4(0, 0, 0, 0);
+    const bool keep = field_of(whole, (int)(n & 7)) >= d.threshold;
+    // the column of an eight's first element, which may lie before the row
+    for (int64_t c = ((((int64_t)blockIdx.x << tx_bits) + tx) * 8) - (unit0 & 7); c < cols; c += col_step) {
+      const uint4 r = BY_ROW ? whole : philox((uint64_t)(unit0 + c) >> 3, d.offset, d.seed);
+      if (c >= 0 && c + 8 <= cols) {
+        T v[8];
+        __builtin_memcpy(v, from + c, sizeof(v));
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      if (b * 8 + j >= units) break;
-      out[n * ldo + c] = kept(x[n * ldx + c], field_of(r, j) >= d.threshold, d.scale);
-      if (++c == cols) c = 0, ++n;
+        for (int j = 0; j < 8; ++j)
+          v[j] = kept(v[j], BY_ROW ? keep : field_of(r, j) >= d.threshold, d.scale);
+        __builtin_memcpy(to + c, v, sizeof(v));
+      } else {
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+          if (c + j >= 0 && c + j < cols)
+            to[c + j] = kept(from[c + j], BY_ROW ? keep : field_of(r, j) >= d.threshold, d.scale);
+      }
     }
   }
 }
@@ -157,15 +156,23 @@ void launch(const void* x, int64_t ldx, int64_t rows, int64_t cols, const Dropou
   constexpr int V = 16 / sizeof(T);
   if (flat && !by_row) {
     k_dropout_flat<T><<<grid_of((rows * cols + 7) / 8), THREADS, 0, s>>>((const T*)x, rows * cols, d, (T*)out);
-  } else if (flat && (cols & (cols - 1)) == 0 && cols < ((int64_t)1 << 31)) {
-    int bits = 0;
-    while (((int64_t)1 << bits) < cols) ++bits;
-    k_dropout_rows<T><<<grid_of((rows * cols + V - 1) / V), THREADS, 0, s>>>((const T*)x, rows * cols, bits,
-                                                                             d, (T*)out);
-  } else {
-    const int64_t threads = by_row ? (rows + 7) / 8 * 64 : (rows * cols + 7) / 8;
-    k_dropout<T><<<grid_of(threads), THREADS, 0, s>>>((const T*)x, ldx, rows, cols, d, by_row, (T*)out, ldo);
+    return;
   }
+  if (flat && (cols == 1 || cols == 2 || cols == 4)) {
+    k_dropout_pairs<T><<<grid_of((rows * cols + V - 1) / V), THREADS, 0, s>>>((const T*)x, rows * cols,
+                                                                              (int)cols / 2, d, (T*)out);
+    return;
+  }
+  // eights that a row reaches over
+  const int64_t eights = by_row || cols % 8 == 0 ? (cols + 7) / 8 : (cols + 14) / 8;
+  int bits = 0;
+  while (bits < 8 && ((int64_t)1 << bits) < eights) ++bits;
+  const int64_t across = (eights + (1 << bits) - 1) >> bits, down = (rows + (THREADS >> bits) - 1) / (THREADS >> bits);
+  const dim3 grid((unsigned)std::min<int64_t>(across, 1 << 20), (unsigned)std::min<int64_t>(down, 65535));
+  if (by_row)
+    k_dropout_rows<T, true><<<grid, THREADS, 0, s>>>((const T*)x, ldx, rows, cols, bits, d, (T*)out, ldo);
+  else
+    k_dropout_rows<T, false><<<grid, THREADS, 0, s>>>((const T*)x, ldx, rows, cols, bits, d, (T*)out, ldo);
 }
 
 }  // namespace

@@ -5,9 +5,13 @@
 // smaller wave tile reads LDS for as long as it multiplies).  64 elements of the
 // contraction a stage pass through LDS, in two buffers: 128 bytes of a row, since the
 // caches fetch no less (32 elements a stage: 64 KB from L2 take 1.2 us a CU instead of
-// 0.8).  Two more stages are on their way in registers, which the accumulators in the other
-// half of the register file leave free.  Every lane gives its own address, so the gather
-// through the order costs nothing, and what is beyond an operand reads zeros.
+// 0.8).  A further stage is on its way in registers (two gain nothing and spill), which the
+// accumulators in the other half of the register file leave free.  Every lane gives its own
+// address, so the gather through the order costs nothing, and what is beyond an operand
+// reads zeros.
+//
+// Measured in bfloat16: 16384 rows of 2048 inputs in 8 leaves to 4096 outputs 429 us, 640
+// TFLOP/s with ragged leaves (FIGURE).
 #include <algorithm>
 #include <type_traits>
 
@@ -95,7 +99,8 @@ __device__ __forceinline__ u32x4 cm_frag32(const char* tile, int base, int step,
 template <typename T, int MODE>
 __global__ __launch_bounds__(THREADS, 1) void k_leaf_big(LeafProduct p, int col_tiles) {
   constexpr bool DW = MODE == LEAF_PRODUCT_DW, ACM = DW, BCM = MODE != LEAF_PRODUCT_Y;
-  constexpr int FM = WM / 32, FN = WN / 32, STEPS = BK / 16, ITEMS = STEPS * FM, RING = 4, TURN = ITEMS - 2, AHEAD = 1;
+  constexpr int FM = WM / 32, FN = WN / 32, STEPS = BK / 16, ITEMS = STEPS * FM, RING = 4;
+  constexpr int TURN = ITEMS - 2;
   __shared__ __align__(1024) char lds[2][STAGE];
   __shared__ int32_t row_of[DW ? 1 : BM];
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -153,9 +158,8 @@ __global__ __launch_bounds__(THREADS, 1) void k_leaf_big(LeafProduct p, int col_
         boff[j] = (uint32_t)min(c0 + kc_row + 8 * j, cols - 1) * (uint32_t)(length / 8) + bchunk[j] / 8;
       if (MODE == LEAF_PRODUCT_DX) boff[j] = (uint32_t)(cm_row + 2 * j) * (uint32_t)(cols / 8) + (c0 + cm_col[j]) / 8;
     }
-    // DW: the rows of the stage that is loaded next, by scalar loads, which do not count
-    // among the loads to LDS
-    // (offset of dy's row, of x's; a bit a load and half wave: whether there is a row)
+    // DW: the rows of the stage that is loaded next, by scalar loads (offset of dy's row, of
+    // x's; a bit a load and half wave: whether there is a row)
     uint32_t row_a[DW ? 2 * LOADS : 1], row_b[DW ? 2 * LOADS : 1], there = 0;
     auto fetch_rows = [&](int k0) {
       const const_ints order = (const_ints)(uintptr_t)(p.g.order + (int64_t)tree * p.g.rows);
@@ -232,7 +236,7 @@ __global__ __launch_bounds__(THREADS, 1) void k_leaf_big(LeafProduct p, int col_
     float bias[DW ? FM : 1];  // of the lane's chunks
 #pragma unroll
     for (int i = 0; i < (DW ? FM : 1); ++i) bias[i] = 0.0f;
-    
+
     // item: step FM + i of a stage
     auto frag_a = [&](const char* buf, int item) {
       const int base = wm + 32 * (item % FM), step = item / FM;
@@ -242,20 +246,19 @@ __global__ __launch_bounds__(THREADS, 1) void k_leaf_big(LeafProduct p, int col_
       return BCM ? cm_frag32<true>(buf + A_BYTES, wn + 32 * j, step, lane)
                  : kc_frag32<true>(buf + A_BYTES, wn + 32 * j, step, lane);
     };
-    u32x4 fa[RING], fb[2][FN], ahead[AHEAD][2 * LOADS];
+    u32x4 fa[RING], fb[2][FN], ahead[2 * LOADS];
     // A stage is 16 items: a fragment of rows times the four of columns, for each 16 of the
     // stage's contraction.  Fragments of rows are read three items ahead, the columns' four.
-    // During items 0 to 7 the next stage goes from registers to the other buffer, and the
-    // registers are loaded with the stage AHEAD further on.  Behind item 13 the wave has
-    // read all of its buffer: the block turns and the first fragments of the next stage are
-    // read.
+    // During items 0 to 11 the next stage goes from registers to the other buffer, and the
+    // registers are loaded with the stage behind it.  Behind item 13 the wave has read all of
+    // its buffer: the block turns and the first fragments of the next stage are read.
     const auto share_of = [](int t) constexpr {  // the eight shares, over items 0 to 11
       for (int j = 0; j < LOADS; ++j)
         if (j * 13 / 8 == t) return j;
       return -1;
     };
-    auto stage = [&](auto sums, int k0, int set, char* cur, char* next) {
-      const Stage from = stage_at(k0 + (AHEAD + 1) * BK);
+    auto stage = [&](auto sums, int k0, char* cur, char* next) {
+      const Stage from = stage_at(k0 + 2 * BK);
 #pragma unroll
       for (int t = 0; t < ITEMS; ++t) {
         const int i = t % FM, step = t / FM;
@@ -278,9 +281,9 @@ __global__ __launch_bounds__(THREADS, 1) void k_leaf_big(LeafProduct p, int col_
         }
         if (share_of(t) >= 0) {
           const int l = share_of(t);
-          *place(next, l) = ahead[set][2 * l];
-          *place(next + A_BYTES, l) = ahead[set][2 * l + 1];
-          ahead[set][2 * l] = load_a(from, k0 + (AHEAD + 1) * BK, l);
+          *place(next, l) = ahead[2 * l];
+          *place(next + A_BYTES, l) = ahead[2 * l + 1];
+          ahead[2 * l] = load_a(from, k0 + 2 * BK, l);
         }
         __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
@@ -288,31 +291,31 @@ __global__ __launch_bounds__(THREADS, 1) void k_leaf_big(LeafProduct p, int col_
         __builtin_amdgcn_sched_barrier(0);
         if (t > 0 && share_of(t - 1) >= 0) {
           const int l = share_of(t - 1);
-          ahead[set][2 * l + 1] = load_b(from, k0 + (AHEAD + 1) * BK, l);
+          ahead[2 * l + 1] = load_b(from, k0 + 2 * BK, l);
         }
 #pragma unroll
         for (int j = FN / 2; j < FN; ++j) acc[i][j] = mfma32<T>(fb[step % 2][j], f, acc[i][j]);
         __builtin_amdgcn_sched_barrier(0);
-        if (t == TURN && DW) fetch_rows(k0 + (AHEAD + 2) * BK);
+        if (t == TURN && DW) fetch_rows(k0 + 3 * BK);
       }
     };
 
     if (length > 0) {
-      // stage 0 to the first buffer, the AHEAD behind it on their way
+      // stage 0 to the first buffer, stage 1 on its way
 #pragma unroll
-      for (int s = 0; s <= AHEAD; ++s) {
+      for (int s = 0; s < 2; ++s) {
         if (DW) fetch_rows(s * BK);
 #pragma unroll
         for (int j = 0; j < LOADS; ++j) {
-          ahead[s % AHEAD][2 * j] = load_a(stage_at(s * BK), s * BK, j);
-          ahead[s % AHEAD][2 * j + 1] = load_b(stage_at(s * BK), s * BK, j);
+          ahead[2 * j] = load_a(stage_at(s * BK), s * BK, j);
+          ahead[2 * j + 1] = load_b(stage_at(s * BK), s * BK, j);
         }
         if (s == 0)
 #pragma unroll
           for (int j = 0; j < LOADS; ++j)
-            *place(lds[0], j) = ahead[0][2 * j], *place(lds[0] + A_BYTES, j) = ahead[0][2 * j + 1];
+            *place(lds[0], j) = ahead[2 * j], *place(lds[0] + A_BYTES, j) = ahead[2 * j + 1];
       }
-      if (DW) fetch_rows((AHEAD + 1) * BK);
+      if (DW) fetch_rows(2 * BK);
       turn();
 #pragma unroll
       for (int j = 0; j < FN; ++j) fb[0][j] = frag_b(lds[0], j, 0);
@@ -323,9 +326,9 @@ __global__ __launch_bounds__(THREADS, 1) void k_leaf_big(LeafProduct p, int col_
       // the blocks of the first columns make them
       if (DW && p.db && c0 == 0) {
         for (int k0 = 0; k0 < length; k0 += BK, cur ^= 1)
-          stage(std::integral_constant<bool, DW>(), k0, 0, lds[cur], lds[cur ^ 1]);
+          stage(std::integral_constant<bool, DW>(), k0, lds[cur], lds[cur ^ 1]);
       } else {
-        for (int k0 = 0; k0 < length; k0 += BK, cur ^= 1) stage(std::false_type(), k0, 0, lds[cur], lds[cur ^ 1]);
+        for (int k0 = 0; k0 < length; k0 += BK, cur ^= 1) stage(std::false_type(), k0, lds[cur], lds[cur ^ 1]);
       }
     }
 

@@ -55,7 +55,7 @@ bool overlaps(const Span& out, std::initializer_list<Span> in) {
 bool misaligned(const void* p, int64_t e) { return (uintptr_t)p % (uintptr_t)e != 0; }
 
 // Rows times a stride has to stay far from the end of 64 bits.
-bool huge(int64_t rows, int64_t ld) { return ld > ((int64_t)1 << 40) || rows > ((int64_t)1 << 40); }
+bool huge(int64_t rows, int64_t ld) { return ld > ((int64_t)1 << 40) || (__int128)rows * ld > ((__int128)1 << 58); }
 
 int check_ws(lgbm_hip_ctx* c, const void* ws, size_t have, size_t need) {
   if (need == 0) return LGBM_HIP_OK;

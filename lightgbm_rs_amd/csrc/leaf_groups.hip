@@ -175,7 +175,8 @@ __global__ __launch_bounds__(THREADS) void k_count_leaves(const int32_t* leaf, i
 // A block a leaf: counts become the sums over the chunks before, the total goes to totals.
 __global__ __launch_bounds__(THREADS) void k_sum_chunks(int chunks, int32_t* counts, int32_t* totals) {
   __shared__ int sums[WAVES];
-  int32_t* const c = counts + (int64_t)blockIdx.x * chunks;
+  const int64_t list = (int64_t)blockIdx.y * gridDim.x + blockIdx.x;  // a tree's leaf
+  int32_t* const c = counts + list * chunks;
   int32_t base = 0;
   for (int i0 = 0; i0 < chunks; i0 += THREADS) {
     const int i = i0 + (int)threadIdx.x;
@@ -184,7 +185,7 @@ __global__ __launch_bounds__(THREADS) void k_sum_chunks(int chunks, int32_t* cou
     if (i < chunks) c[i] = base + before;
     base += all;
   }
-  if (threadIdx.x == 0) totals[blockIdx.x] = base;
+  if (threadIdx.x == 0) totals[list] = base;
 }
 
 // LDS: [WAVES + 1][leaves + 1]
@@ -233,9 +234,9 @@ void launch_leaf_groups(const int32_t* leaf, int64_t ld, int64_t rows, int32_t t
   int32_t* const counts = (int32_t*)ws;
   int32_t* const totals = counts + lists * chunks;
   k_count_leaves<<<grid, THREADS, row, s>>>(leaf, ld, rows, chunk, leaves, chunks, counts);
-  k_sum_chunks<<<(unsigned)lists, THREADS, 0, s>>>(chunks, counts, totals);
-  k_order_rows<<<grid, THREADS, lds, s>>>(leaf, ld, rows, chunk, leaves, bits, chunks, counts,
-                                                         totals, order, begin, count);
+  k_sum_chunks<<<dim3(leaves + 1, trees), THREADS, 0, s>>>(chunks, counts, totals);
+  k_order_rows<<<grid, THREADS, lds, s>>>(leaf, ld, rows, chunk, leaves, bits, chunks, counts, totals, order, begin,
+                                        count);
 }
 
 }  // namespace lgbm

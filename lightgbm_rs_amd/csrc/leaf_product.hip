@@ -555,10 +555,14 @@ DwShape dw_shape(const LeafProduct& p) {
 // Leaves of 16 rows at most, on average.
 bool few_rows(const LeafProduct& p) { return p.g.rows <= 16 * (int64_t)p.g.leaves; }
 
-// k_leaf_few: leaves of few rows, or few outputs of so few rows that blocks of 256 would leave
-// CUs without work (3000 x 2000 float32 to 10 outputs: 68 us by k_leaf_narrow, 14).
+// k_leaf_few: leaves of few rows, or few outputs of so few rows that k_leaf_narrow's blocks
+// of 256 would leave CUs without work (float32, 2000 inputs to 10 outputs by k_leaf_narrow
+// and by it: 1000 rows 85 and 16 us, 30000 rows 109 and 92, 60000 rows 141 and 152; to 32
+// outputs 10000 rows 121 and 52, 30000 rows 138 and 151; 130 inputs to 10, 10000 rows: 16
+// and 9).
 bool by_maps(const LeafProduct& p) {
-  return p.inputs >= 512 && (few_rows(p) || (p.outputs <= 32 && p.g.rows < 65536));
+  if (p.outputs > 32) return p.inputs >= 512 && few_rows(p);
+  return p.inputs >= 128 && (few_rows(p) || (int64_t)p.g.rows * ((p.outputs + 15) / 16) < 49152);
 }
 
 // Tiles of 128 x 128, where leaves fill them and there is one for every CU: 16-bit products

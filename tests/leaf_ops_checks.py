@@ -85,6 +85,15 @@ def groups(rows, trees, leaves, shape, pad=0, seed=0):
         assert np.array_equal(got.cpu().numpy(), want)
 
 
+def groups_many():
+    """So many leaves that blocks for all of them along one axis pass 32 bits of threads."""
+    rows, trees, leaves = 4097, 4200, 4095
+    leaf = leaves_of(np.random.default_rng(0), rows, 1, leaves, "even")
+    t = torch.from_numpy(leaf).to(DEV).int().expand(rows, trees).contiguous()
+    for got, want in zip(backend().leaf_groups(t, leaves), oracle.groups(leaf, leaves)):
+        assert bool((got == torch.from_numpy(want).to(DEV)).all())
+
+
 def _case(rows, inputs, outputs, trees, leaves, dtype, shape, pad, seed):
     rng = np.random.default_rng(seed)
     leaf = leaves_of(rng, rows, trees, leaves, shape)

@@ -57,9 +57,13 @@ def check():
     (20011, 3, 63, "lost", 1), (100003, 1, 1000, "even", 0), (30000, 1, 4095, "skew", 0),
     (50000, 1, 1, "lost", 0), (3000, 300, 15, "even", 0), (300007, 2, 31, "one", 0),
     (1025, 65, 127, "lost", 3), (8192, 2, 100, "lost", 0), (8193, 2, 100, "skew", 0),
-    (2200001, 1, 255, "lost", 0), (4200000, 1, 3, "even", 1)])
+    (2200001, 1, 255, "lost", 0), (4200000, 1, 3, "even", 1))])
 def test_groups(check, rows, trees, leaves, shape, pad):
     check("groups", rows=rows, trees=trees, leaves=leaves, shape=shape, pad=pad)
+
+
+def test_groups_of_many_leaves(check):
+    check("groups_many")
 
 
 # one row and one input; outputs and inputs around 16, 32, 64, 128 and 256; rows of a leaf
@@ -69,7 +73,8 @@ SHAPES = [
     (17, 16, 16, 1, 1, "one", 0), (100, 33, 17, 2, 7, "lost", 3), (257, 64, 64, 1, 4, "skew", 8),
     (300, 100, 10, 1, 31, "even", 0), (129, 128, 130, 1, 2, "even", 8), (500, 200, 96, 3, 5, "lost", 0),
     (16, 520, 300, 1, 31, "even", 0), (3, 1000, 260, 2, 3, "even", 0), (1000, 70, 257, 1, 3, "skew", 1),
-    (700, 256, 256, 1, 2, "one", 0), (2000, 13, 3, 5, 63, "skew", 0), (40, 2000, 1, 1, 7, "even", 0), (600, 530, 20, 1, 2, "skew", 0),
+    (700, 256, 256, 1, 2, "one", 0), (2000, 13, 3, 5, 63, "skew", 0), (40, 2000, 1, 1, 7, "even", 0),
+    (600, 530, 20, 1, 2, "skew", 0), (170, 140, 7, 2, 3, "lost", 1),
     (333, 65, 8, 1, 1, "lost", 2), (900, 129, 33, 2, 15, "even", 8), (2500, 40, 10, 1, 2, "one", 0)]
 
 
@@ -114,7 +119,8 @@ def test_plain(check, name):
     (130, 100, 0.5, "row", 4, 14, 0), (50, 16, 0.0, "element", 0, 15, 0),
     (50, 16, 1.0, "element", 0, 16, 0), (50, 3, 1.0, "row", 0, 17, 0),
     (600, 1024, 0.25, "element", 0, 18, 0), (1001, 4, 0.2, "row", 0, 20, 0),
-    (515, 8, 0.2, "row", 0, 21, 0), (77, 64, 0.2, "row", 0, 22, 5), (9, 1, 0.2, "row", 0, 23, 0), (70000, 2, 0.4, "row", 0, 19, 0)])
+    (5, 70001, 0.5, "row", 0, 24, 0), (5, 4099, 0.5, "element", 3, 25, 2), (40, 2100, 0.3, "row", 8, 26, 1),
+    (300, 5, 0.4, "element", 1, 27, 0), (70001, 3, 0.4, "element", 2, 28, 0), (515, 8, 0.2, "row", 0, 21, 0), (77, 64, 0.2, "row", 0, 22, 5), (9, 1, 0.2, "row", 0, 23, 0), (70000, 2, 0.4, "row", 0, 19, 0)])
 def test_dropout(check, rows, cols, p, by, pad, seed, offset, dtype):
     check("dropout", rows=rows, cols=cols, p=p, by=by, pad=pad, seed=seed, offset=offset, dtype=dtype)
 

@@ -48,7 +48,8 @@ def groups(lib, leaf=A, ld=3, rows=10, trees=3, leaves=7, order=B, begin=D, coun
     (dict(order=B + 2), INVALID, "aligned"), (dict(rows=10 ** 6, ws=None), INVALID, "null workspace"),
     (dict(rows=10 ** 6, ws=W + 4), INVALID, "16-byte"), (dict(rows=10 ** 6, size=8), MISMATCH, "smaller"),
     (dict(order=A + 40), INVALID, "overlap"), (dict(count=D + 40), INVALID, "overlap"),
-    (dict(rows=10 ** 6, ws=A - 64), INVALID, "overlap"), (dict(ld=2 ** 41), INVALID, "stride")])
+    (dict(rows=10 ** 6, ws=A - 64), INVALID, "overlap"), (dict(ld=2 ** 41), INVALID, "stride"),
+    (dict(rows=2 ** 30, ld=2 ** 34), INVALID, "stride")])
 def test_groups_refused(lib, change, code, text):
     refused(lib, groups(lib, **change), code, text)
 
