@@ -57,7 +57,7 @@ def check():
     (20011, 3, 63, "lost", 1), (100003, 1, 1000, "even", 0), (30000, 1, 4095, "skew", 0),
     (50000, 1, 1, "lost", 0), (3000, 300, 15, "even", 0), (300007, 2, 31, "one", 0),
     (1025, 65, 127, "lost", 3), (8192, 2, 100, "lost", 0), (8193, 2, 100, "skew", 0),
-    (2200001, 1, 255, "lost", 0), (4200000, 1, 3, "even", 1))])
+    (2200001, 1, 255, "lost", 0), (4200000, 1, 3, "even", 1)])
 def test_groups(check, rows, trees, leaves, shape, pad):
     check("groups", rows=rows, trees=trees, leaves=leaves, shape=shape, pad=pad)
 
