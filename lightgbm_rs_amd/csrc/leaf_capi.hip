@@ -309,7 +309,7 @@ int lgbm_hip_adjust_scores_workspace(const lgbm_score_args* a, size_t* bytes) {
   const int rc = check_scores(nullptr, a);
   if (rc) return rc;
   if (!bytes) return bad(nullptr, "null bytes");
-  *bytes = adjust_scores_workspace(a->num_rows, a->num_classes, a->dtype, a->kind);
+  *bytes = adjust_scores_workspace(a->num_rows, a->num_classes, a->dtype, a->kind, a->num_ids > 0);
   return LGBM_HIP_OK;
 }
 
@@ -317,7 +317,7 @@ int lgbm_hip_adjust_scores(lgbm_hip_ctx* c, const lgbm_score_args* a, void* d_ws
                            void* const* stream) {
   int rc = check_scores(c, a);
   if (rc) return rc;
-  const size_t need = adjust_scores_workspace(a->num_rows, a->num_classes, a->dtype, a->kind);
+  const size_t need = adjust_scores_workspace(a->num_rows, a->num_classes, a->dtype, a->kind, a->num_ids > 0);
   if ((rc = check_ws(c, d_ws, ws_bytes, need))) return rc;
   const int64_t e = type_size(a->dtype), rows = a->num_rows, V = a->num_classes;
   const Span x = matrix(a->d_x, rows, V, a->ldx, e), out = matrix(a->d_out, rows, V, a->ldo, e);

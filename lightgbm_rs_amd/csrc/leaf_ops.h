@@ -83,7 +83,7 @@ struct ScoreArgs {
   int64_t ldo;
   void* ws;
 };
-size_t adjust_scores_workspace(int64_t rows, int32_t classes, int32_t dtype, int32_t kind);
+size_t adjust_scores_workspace(int64_t rows, int32_t classes, int32_t dtype, int32_t kind, bool history);
 void launch_adjust_scores(const ScoreArgs& a, hipStream_t s);
 
 }  // namespace lgbm

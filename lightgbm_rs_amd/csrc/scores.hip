@@ -51,6 +51,14 @@ __device__ __forceinline__ double exp_of(double v) {
 // The larger; a NaN is passed over (it comes back through the sum).
 __device__ __forceinline__ float top_of(float a, float b) { return fmaxf(a, b); }
 __device__ __forceinline__ double top_of(double a, double b) { return fmax(a, b); }
+// s, or -inf where bit e is set.
+__device__ __forceinline__ float unless(uint32_t bits, int e, float s) {
+  const uint32_t m = (uint32_t)((int32_t)(bits << (31 - e)) >> 31);
+  return __uint_as_float((m & 0xff800000u) | (~m & __float_as_uint(s)));
+}
+__device__ __forceinline__ double unless(uint32_t bits, int e, double s) {
+  return (bits >> e) & 1 ? -INFINITY : s;
+}
 // What the exponentials are relative to: where every class is masked their -inf stays.
 template <typename A>
 __device__ __forceinline__ A base_of(A top) {
@@ -180,10 +188,8 @@ __global__ __launch_bounds__(THREADS) void k_scores_thread(ScoreArgs a, uint32_t
 
 enum { WHOLE, PART, FINISH };
 
-// Long rows: chunks of two vectors a lane in blocks of 1024, so that few blocks look at the
-// same history (64 x 128007 bf16: 37 us; one vector a lane 50 us); blocks of 256 where those
-// would leave CUs without one.
-constexpr int CHUNK_LANES = 1024, SMALL_LANES = 256, CHUNK_BYTES = 32;
+// Long rows: chunks of 32 bytes a lane.
+constexpr int CHUNK_BYTES = 32;
 
 // LANES of one row, each with NV vectors of VW neighbouring classes, LANES * NV * VW classes
 // from c0 on.
@@ -192,7 +198,7 @@ __global__ __launch_bounds__(LANES < THREADS ? THREADS : LANES) void k_scores_ro
   typedef typename Wide<T>::type A;
   constexpr int CAP = LANES * NV * VW, TEAMS = LANES < THREADS ? THREADS / LANES : 1;
   __shared__ __align__(16) uint32_t counts[TEAMS * CAP];
-  __shared__ A shared[LANES / 64];
+  __shared__ A shared[LANES / 64], sums[LANES / 64];
   const int lane = threadIdx.x % LANES, team = threadIdx.x / LANES;
   uint32_t* const count = counts + team * CAP;
   auto sync = [&] {
@@ -204,9 +210,13 @@ __global__ __launch_bounds__(LANES < THREADS ? THREADS : LANES) void k_scores_ro
     }
   };
   // over the row's lanes; every one gets the result
-  auto reduce = [&](A v, auto join) {
+  auto of_wave = [&](A v, auto join) {
 #pragma unroll
     for (int d = 1; d < 64; d <<= 1) v = join(v, (A)__shfl_xor(v, d));
+    return v;
+  };
+  auto reduce = [&](A v, auto join) {
+    v = of_wave(v, join);
     if (LANES > 64) {
       __syncthreads();
       if (lane % 64 == 0) shared[lane / 64] = v;
@@ -226,12 +236,9 @@ __global__ __launch_bounds__(LANES < THREADS ? THREADS : LANES) void k_scores_ro
     const int c0 = (int)(task - n * chunks) * CAP;
     const int V = min(a.classes - c0, CAP);
     const T* const x = (const T*)a.x + n * a.ldx + c0;
-    const Row<A> row = row_of<A>(a, n);
     const T* const bias = a.bias ? (const T*)a.bias + c0 : nullptr;
-    const bool seen = row.h1 > row.h0;
     A s[NV][VW];
     T v[NV][VW], b[NV][VW];
-    uint32_t allowed[NV];
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
       const int j = (i * LANES + lane) * VW;
@@ -246,9 +253,17 @@ __global__ __launch_bounds__(LANES < THREADS ? THREADS : LANES) void k_scores_ro
       else
 #pragma unroll
         for (int e = 0; e < VW; ++e) b[i][e] = bias && j + e < V ? bias[j + e] : (T)0.0f;
+    }
+    const Row<A> row = row_of<A>(a, n);
+    const bool seen = row.h1 > row.h0;
+    const bool masked = row.mask || V < CAP;  // else every class is allowed
+    uint32_t refused[NV];
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      const int j = (i * LANES + lane) * VW;
       // VW divides 32 and c0 is a multiple of 32, so the bits are of one word
-      allowed[i] = row.mask && j < V ? row.mask[(c0 + j) >> 5] >> (j & 31) : ~0u;
-      if (!full) allowed[i] &= j < V ? (1u << (V - j)) - 1 : 0u;
+      refused[i] = row.mask && j < V ? ~(row.mask[(c0 + j) >> 5] >> (j & 31)) : 0u;
+      if (j + VW > V) refused[i] |= j < V ? ~0u << (V - j) : ~0u;
     }
     if (seen) {
 #pragma unroll
@@ -279,10 +294,12 @@ __global__ __launch_bounds__(LANES < THREADS ? THREADS : LANES) void k_scores_ro
         }
       }
 #pragma unroll
-      for (int e = 0; e < VW; ++e) {
-        s[i][e] = (allowed[i] >> e) & 1 ? s[i][e] + (A)b[i][e] : -INFINITY;
-        top = top_of(top, s[i][e]);
-      }
+      for (int e = 0; e < VW; ++e) s[i][e] += (A)b[i][e];
+      if (masked)
+#pragma unroll
+        for (int e = 0; e < VW; ++e) s[i][e] = unless(refused[i], e, s[i][e]);
+#pragma unroll
+      for (int e = 0; e < VW; ++e) top = top_of(top, s[i][e]);
     }
     if (seen) sync();  // the counts are read before the next row's are cleared
     A scale = 1;
@@ -293,7 +310,8 @@ __global__ __launch_bounds__(LANES < THREADS ? THREADS : LANES) void k_scores_ro
         top = -INFINITY;
         for (int c = lane; c < chunks; c += LANES) top = top_of(top, parts[(n * chunks + c) * 2]);
       }
-      top = reduce(top, larger);
+      // a part's waves are joined at its end, in one turn of the block
+      top = MODE == PART ? of_wave(top, larger) : reduce(top, larger);
       const A base = base_of(top);
       A sum = 0;
 #pragma unroll
@@ -307,12 +325,28 @@ __global__ __launch_bounds__(LANES < THREADS ? THREADS : LANES) void k_scores_ro
         for (int c = lane; c < chunks; c += LANES)
           sum += parts[(n * chunks + c) * 2 + 1] * exp_of<A>(parts[(n * chunks + c) * 2] - base);
       }
-      sum = reduce(sum, plus);
       if (MODE == PART) {
-        if (lane == 0) parts[task * 2] = top, parts[task * 2 + 1] = sum;
+        sum = of_wave(sum, plus);
+        __syncthreads();
+        if (lane % 64 == 0) shared[lane / 64] = top, sums[lane / 64] = sum;
+        __syncthreads();
+        if (lane < 64) {
+          A t = lane < LANES / 64 ? shared[lane] : (A)-INFINITY;
+          top = of_wave(t, larger);
+          sum = of_wave(lane < LANES / 64 ? sums[lane] * exp_of<A>(t - base_of(top)) : (A)0, plus);
+          if (lane == 0) parts[task * 2] = top, parts[task * 2 + 1] = sum;
+        }
         continue;
       }
+      sum = reduce(sum, plus);
       scale = 1 / sum;
+    }
+    if (!(scale <= 1)) {  // of a NaN, or of no class: 0 stays 0 beside it
+#pragma unroll
+      for (int i = 0; i < NV; ++i)
+#pragma unroll
+        for (int e = 0; e < VW; ++e) s[i][e] = s[i][e] == 0 ? (A)0 : s[i][e] * scale;
+      scale = 1;
     }
     T* const out = (T*)a.out + n * a.ldo + c0;
 #pragma unroll
@@ -320,8 +354,7 @@ __global__ __launch_bounds__(LANES < THREADS ? THREADS : LANES) void k_scores_ro
       const int j = (i * LANES + lane) * VW;
       T v[VW];
 #pragma unroll
-      for (int e = 0; e < VW; ++e)  // 0 stays 0 beside a NaN
-        v[e] = (T)(probabilities ? (s[i][e] == 0 ? (A)0 : s[i][e] * scale) : s[i][e]);
+      for (int e = 0; e < VW; ++e) v[e] = (T)(s[i][e] * scale);
       if (j + VW <= V)
         __builtin_memcpy(out + j, v, sizeof(v));
       else
@@ -340,9 +373,15 @@ void launch_row(const ScoreArgs& a, int chunks, hipStream_t s) {
       <<<(unsigned)std::min<int64_t>(blocks, 1 << 20), TEAMS * LANES, 0, s>>>(a, chunks);
 }
 
-int chunk_lanes(int64_t rows, int32_t classes, int e) {
-  const int chunk = CHUNK_LANES * (CHUNK_BYTES / e);
-  return rows * ((classes + chunk - 1) / chunk) < 256 ? SMALL_LANES : CHUNK_LANES;
+// Lanes of a chunk.  Small blocks overlap best (bfloat16 x 128007 without histories: 256 rows
+// 90 us by 256 lanes, 97 by 512, 106 by 1024), but every block of a row looks at its whole
+// history (1000 ids a row: 134, 136 and 147 us; 64 rows 39, 39 and 37), so where all blocks
+// of 1024 fit the card at once those are taken; and 256 lanes where CUs would be without
+// work.
+int chunk_lanes(int64_t rows, int32_t classes, int e, bool history) {
+  const int chunk = 1024 * (CHUNK_BYTES / e);
+  const int64_t blocks = rows * ((classes + chunk - 1) / chunk);
+  return !history || blocks < 256 ? 256 : blocks <= 512 ? 1024 : 512;
 }
 
 template <typename T, int LANES>
@@ -376,19 +415,23 @@ void launch(const ScoreArgs& a, hipStream_t s) {
     launch_row<T, THREADS, BLOCK_CLASSES, VW, WHOLE>(a, 1, s);
   } else if (V <= ROW_CLASSES) {
     launch_row<T, 512, ROW_CLASSES, VW, WHOLE>(a, 1, s);
-  } else if (chunk_lanes(a.rows, V, sizeof(T)) == SMALL_LANES) {
-    launch_chunks<T, SMALL_LANES>(a, s);
   } else {
-    launch_chunks<T, CHUNK_LANES>(a, s);
+    const int lanes = chunk_lanes(a.rows, V, sizeof(T), a.num_ids > 0);
+    if (lanes == 256)
+      launch_chunks<T, 256>(a, s);
+    else if (lanes == 512)
+      launch_chunks<T, 512>(a, s);
+    else
+      launch_chunks<T, 1024>(a, s);
   }
 }
 
 }  // namespace
 
-size_t adjust_scores_workspace(int64_t rows, int32_t classes, int32_t dtype, int32_t kind) {
+size_t adjust_scores_workspace(int64_t rows, int32_t classes, int32_t dtype, int32_t kind, bool history) {
   if (classes <= ROW_CLASSES || kind == LGBM_HIP_PREDICT_RAW) return 0;
   const int e = dtype == LGBM_HIP_DTYPE_F64 ? 8 : dtype == LGBM_HIP_DTYPE_F32 ? 4 : 2;
-  const int chunk = chunk_lanes(rows, classes, e) * (CHUNK_BYTES / e);
+  const int chunk = chunk_lanes(rows, classes, e, history) * (CHUNK_BYTES / e);
   return (size_t)rows * (size_t)((classes + chunk - 1) / chunk) * (e == 8 ? 16 : 8);
 }
 

@@ -138,7 +138,8 @@ def test_dropout_far(check):
     (3, 20001, True, 2, 100, True, 0), (300, 32, True, 2, 9, False, 0), (9, 256, True, 1, 30, False, 1),
     (9, 257, False, 2, 30, True, 0), (7, 512, True, 0, 60, False, 0), (6, 513, True, 2, 60, False, 3),
     (5, 2048, False, 1, 90, True, 0), (5, 2049, True, 2, 90, False, 0), (5, 4096, True, 1, 900, False, 1),
-    (150, 8200, True, 3, 50, True, 1), (2, 70000, True, 1, 0, False, 0), (130, 33, True, 0, 1, False, 0)])
+    (150, 8200, True, 3, 50, True, 1), (2, 70000, True, 1, 0, False, 0),
+    (90, 70003, False, 2, 30, True, 0), (301, 33000, True, 0, 20, False, 0), (130, 33, True, 0, 1, False, 0)])
 def test_scores(check, rows, classes, bias, masks, history, per_row, pad, dtype, kind):
     check("scores", rows=rows, classes=classes, dtype=dtype, kind=kind, bias=bias, masks=masks,
           history=history, per_row=per_row, pad=pad, seed=rows)
