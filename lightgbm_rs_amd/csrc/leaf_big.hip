@@ -26,12 +26,10 @@ constexpr int THREADS = 256, BM = 256, BN = 256, BK = 64, WM = 128, WN = 128;
 constexpr int A_BYTES = BM * BK * 2, STAGE = (BM + BN) * BK * 2;
 constexpr int LOADS = 8;  // of 1 KB a wave, operand and stage
 
-__device__ __align__(16) unsigned int zeros[4];
+__device__ __align__(16) unsigned int zeros[BN / 2];  // what a row that is not there reads
 
-typedef const __attribute__((address_space(4))) int32_t* const_ints;
-typedef int i32x16 __attribute__((ext_vector_type(16), aligned(4)));
-typedef const __attribute__((address_space(4))) i32x16* const_ints16;
 typedef const __attribute__((address_space(1))) u32x4* global_vec;
+typedef unsigned long long u64x2 __attribute__((ext_vector_type(2)));
 
 // The wave's LDS accesses are done, then the block's.
 __device__ __forceinline__ void turn() {
@@ -103,6 +101,7 @@ __global__ __launch_bounds__(THREADS, 1) void k_leaf_big(LeafProduct p, int col_
   constexpr int TURN = ITEMS - 2;
   __shared__ __align__(1024) char lds[2][STAGE];
   __shared__ int32_t row_of[DW ? 1 : BM];
+  __shared__ __align__(16) uint64_t rows_at[DW ? THREADS / 64 : 1][DW ? 16 : 1][2];
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int wm = (wave >> 1) * WM, wn = (wave & 1) * WN;
   const int tree_y = blockIdx.y;
@@ -158,33 +157,25 @@ __global__ __launch_bounds__(THREADS, 1) void k_leaf_big(LeafProduct p, int col_
         boff[j] = (uint32_t)min(c0 + kc_row + 8 * j, cols - 1) * (uint32_t)(length / 8) + bchunk[j] / 8;
       if (MODE == LEAF_PRODUCT_DX) boff[j] = (uint32_t)(cm_row + 2 * j) * (uint32_t)(cols / 8) + (c0 + cm_col[j]) / 8;
     }
-    // DW: the rows of the stage that is loaded next, by scalar loads (offset of dy's row, of
-    // x's; a bit a load and half wave: whether there is a row)
-    uint32_t row_a[DW ? 2 * LOADS : 1], row_b[DW ? 2 * LOADS : 1], there = 0;
-    auto fetch_rows = [&](int k0) {
-      const const_ints order = (const_ints)(uintptr_t)(p.g.order + (int64_t)tree * p.g.rows);
-      const int at = k0 + wave * 16, from = first + at;
-      i32x16 n;
-      if (from + 16 <= p.g.rows) {
-        n = *(const_ints16)(order + from);
-      } else {
-#pragma unroll
-        for (int j = 0; j < 16; ++j) n[j] = order[min(from + j, p.g.rows - 1)];
-      }
-      there = 0;
-#pragma unroll
-      for (int j = 0; j < 16; ++j) {
-        const bool ok = at + j < length && (uint32_t)n[j] < (uint32_t)p.g.rows;
-        there |= (uint32_t)ok << j;
-        const uint32_t row = ok ? (uint32_t)n[j] : 0u;
-        row_a[DW ? j : 0] = row * (uint32_t)(p.lddy / 8);
-        row_b[DW ? j : 0] = row * (uint32_t)(p.ldx / 8);
-      }
+    // DW: where the 16 rows of a wave's loads begin, in dy and in x at the block's columns.
+    // Lanes 0 to 15 and 32 to 47 make dy's, the others x's; a load's half waves take theirs
+    // from LDS, and every lane adds its column.  Columns behind the last only make results
+    // that are not stored, so they read the last ones.
+    const int half = lane >> 5, op = (lane >> 4) & 1;
+    const uint64_t base_of_op = op ? (uint64_t)(uintptr_t)((const T*)p.x + c0) : (uint64_t)(uintptr_t)((const T*)p.dy + m0);
+    const uint32_t ld_of_op = (uint32_t)(op ? p.ldx : p.lddy) * 2;
+    const uint32_t a_col = (uint32_t)(min(m0 + (lane & 31) * 8, p.outputs - 8) - m0) * 2;
+    const uint32_t b_col = (uint32_t)(min(c0 + (lane & 31) * 8, cols - 8) - c0) * 2;
+    auto order_of = [&](int k0) {
+      return p.g.order[(int64_t)tree * p.g.rows + min(first + k0 + wave * 16 + (lane & 15), p.g.rows - 1)];
     };
-    // of a lane's load j: its half wave's value
-    auto half_of = [&](const uint32_t (&v)[DW ? 2 * LOADS : 1], int j) {
-      return lane < 32 ? v[DW ? 2 * j : 0] : v[DW ? 2 * j + 1 : 0];
+    auto put_rows = [&](int n, int k0) {
+      const bool there = k0 + wave * 16 + (lane & 15) < length && (uint32_t)n < (uint32_t)p.g.rows;
+      const uint64_t at = base_of_op + (uint64_t)(uint32_t)n * ld_of_op;
+      rows_at[DW ? wave : 0][DW ? lane & 15 : 0][op] = there ? at : (uint64_t)(uintptr_t)zeros;
     };
+    auto get_rows = [&](int j) { return *(const u64x2*)rows_at[DW ? wave : 0][DW ? 2 * j + half : 0]; };
+    u64x2 at_row[2];
     // The j-th loads of the stage at k0, and their place in its buffer.  The stage's addresses
     // are scalars that the compiler takes as new ones, or it would keep a lane's 32 in
     // registers.
@@ -203,28 +194,24 @@ __global__ __launch_bounds__(THREADS, 1) void k_leaf_big(LeafProduct p, int col_
     auto load_a = [&](const Stage& g, int k0, int j) {
       uint64_t from;
       bool in;
-      if (DW) {
-        in = (there >> (2 * j + (lane >> 5)) & 1) && m0 + cm_col[j] < p.outputs;
-        from = g.a + (uint64_t)(half_of(row_a, j) + (m0 + cm_col[j]) / 8) * 16;
-      } else {
-        in = k0 + achunk < length;
-        from = g.a + (uint64_t)aoff[j] * 16;
-      }
+      if (DW) return *(global_vec)(at_row[j & 1].x + a_col);
+      in = k0 + achunk < length;
+      from = g.a + (uint64_t)aoff[j] * 16;
       return *(global_vec)(in ? from : zero_at);
     };
     auto load_b = [&](const Stage& g, int k0, int j) {
       uint64_t from;
       bool in;
-      if (DW) {
-        in = (there >> (2 * j + (lane >> 5)) & 1) && c0 + cm_col[j] < cols;
-        from = g.b + (uint64_t)(half_of(row_b, j) + (c0 + cm_col[j]) / 8) * 16;
-      } else {
-        in = BCM ? k0 + cm_row + 2 * j < length && c0 + cm_col[j] < cols : k0 + bchunk[j] < length;
-        from = g.b + (uint64_t)boff[j] * 16;
-      }
+      if (DW) return *(global_vec)(at_row[j & 1].y + b_col);
+      in = BCM ? k0 + cm_row + 2 * j < length && c0 + cm_col[j] < cols : k0 + bchunk[j] < length;
+      from = g.b + (uint64_t)boff[j] * 16;
       return *(global_vec)(in ? from : zero_at);
     };
-    auto place = [&](char* buf, int j) { return (u32x4*)(buf + (wave * LOADS + j) * 1024 + lane * 16); };
+    // (DW: the column's unit swizzled by bits 0, 1 and 3 of the row, 16 wave + 2 j + half)
+    const int lane_at = DW ? half * 512 + (((lane & 31) * 16) ^ (half << 6)) : lane * 16;
+    auto place = [&](char* buf, int j) {
+      return (u32x4*)(buf + (wave * LOADS + j) * 1024 + (DW ? lane_at ^ ((j & 1) << 7 | (j >> 2) << 8) : lane_at));
+    };
 
     f32x16 acc[FM][FN];
 #pragma unroll
@@ -247,6 +234,10 @@ __global__ __launch_bounds__(THREADS, 1) void k_leaf_big(LeafProduct p, int col_
                  : kc_frag32<true>(buf + A_BYTES, wn + 32 * j, step, lane);
     };
     u32x4 fa[RING], fb[2][FN], ahead[2 * LOADS];
+    int next_rows = 0;  // DW: what put_rows takes next
+    // sums of dy's columns cost as much again as what else the matrix instructions hide: only
+    // the blocks of the first columns make them
+    const bool sums = DW && p.db && c0 == 0;
     // A stage is 16 items: a fragment of rows times the four of columns, for each 16 of the
     // stage's contraction.  Fragments of rows are read three items ahead, the columns' four.
     // During items 0 to 11 the next stage goes from registers to the other buffer, and the
@@ -257,7 +248,7 @@ __global__ __launch_bounds__(THREADS, 1) void k_leaf_big(LeafProduct p, int col_
         if (j * 13 / 8 == t) return j;
       return -1;
     };
-    auto stage = [&](auto sums, int k0, char* cur, char* next) {
+    auto stage = [&](int k0, char* cur, char* next) {
       const Stage from = stage_at(k0 + 2 * BK);
 #pragma unroll
       for (int t = 0; t < ITEMS; ++t) {
@@ -273,7 +264,7 @@ __global__ __launch_bounds__(THREADS, 1) void k_leaf_big(LeafProduct p, int col_
           for (int u = t == TURN ? 0 : 2; u < (t == TURN ? 2 : 3); ++u) fa[u] = frag_a(next, u);
         if (step + 1 < STEPS) fb[(step + 1) % 2][i] = frag_b(cur, i, step + 1);
         const u32x4 f = fa[t % RING];
-        if (sums) {
+        if (DW && sums) {
           T e[8];
           __builtin_memcpy(e, &f, 16);
 #pragma unroll
@@ -292,44 +283,66 @@ __global__ __launch_bounds__(THREADS, 1) void k_leaf_big(LeafProduct p, int col_
         if (t > 0 && share_of(t - 1) >= 0) {
           const int l = share_of(t - 1);
           ahead[2 * l + 1] = load_b(from, k0 + 2 * BK, l);
+          if (DW && l + 2 < LOADS) at_row[l & 1] = get_rows(l + 2);
         }
 #pragma unroll
         for (int j = FN / 2; j < FN; ++j) acc[i][j] = mfma32<T>(fb[step % 2][j], f, acc[i][j]);
         __builtin_amdgcn_sched_barrier(0);
-        if (t == TURN && DW) fetch_rows(k0 + 3 * BK);
+        if (t == TURN && DW) {
+          put_rows(next_rows, k0 + 3 * BK);
+          next_rows = order_of(k0 + 4 * BK);
+          at_row[0] = get_rows(0), at_row[1] = get_rows(1);
+        }
       }
     };
 
     if (length > 0) {
-      // stage 0 to the first buffer, stage 1 on its way
+      // stage 0 to the first buffer, then stage 1 on its way, loaded in the order of a stage:
+      // the compiler's waits in the loop count the loads that are younger on every way to it
+      int order[3];
+      if (DW) {
 #pragma unroll
-      for (int s = 0; s < 2; ++s) {
-        if (DW) fetch_rows(s * BK);
-#pragma unroll
-        for (int j = 0; j < LOADS; ++j) {
-          ahead[2 * j] = load_a(stage_at(s * BK), s * BK, j);
-          ahead[2 * j + 1] = load_b(stage_at(s * BK), s * BK, j);
-        }
-        if (s == 0)
-#pragma unroll
-          for (int j = 0; j < LOADS; ++j)
-            *place(lds[0], j) = ahead[2 * j], *place(lds[0] + A_BYTES, j) = ahead[2 * j + 1];
+        for (int i = 0; i < 3; ++i) order[i] = order_of(i * BK);
+        next_rows = order_of(3 * BK);
+        put_rows(order[0], 0);
       }
-      if (DW) fetch_rows(2 * BK);
+      const Stage first_stage = stage_at(0), second = stage_at(BK);
+#pragma unroll
+      for (int j = 0; j < LOADS; ++j) {
+        if (DW) at_row[j & 1] = get_rows(j);
+        ahead[2 * j] = load_a(first_stage, 0, j);
+        ahead[2 * j + 1] = load_b(first_stage, 0, j);
+      }
+#pragma unroll
+      for (int j = 0; j < LOADS; ++j)
+        *place(lds[0], j) = ahead[2 * j], *place(lds[0] + A_BYTES, j) = ahead[2 * j + 1];
+      if (DW) {
+        put_rows(order[1], BK);
+        at_row[0] = get_rows(0), at_row[1] = get_rows(1);
+      }
+#pragma unroll
+      for (int t = 0; t < ITEMS; ++t) {
+        __builtin_amdgcn_sched_barrier(0);
+        if (share_of(t) >= 0) ahead[2 * share_of(t)] = load_a(second, BK, share_of(t));
+        __builtin_amdgcn_sched_barrier(0);
+        if (t > 0 && share_of(t - 1) >= 0) {
+          const int l = share_of(t - 1);
+          ahead[2 * l + 1] = load_b(second, BK, l);
+          if (DW && l + 2 < LOADS) at_row[l & 1] = get_rows(l + 2);
+        }
+      }
+      __builtin_amdgcn_sched_barrier(0);
+      if (DW) {
+        put_rows(order[2], 2 * BK);
+        at_row[0] = get_rows(0), at_row[1] = get_rows(1);
+      }
       turn();
 #pragma unroll
       for (int j = 0; j < FN; ++j) fb[0][j] = frag_b(lds[0], j, 0);
 #pragma unroll
       for (int u = 0; u < RING - 1; ++u) fa[u] = frag_a(lds[0], u);
       int cur = 0;
-      // sums of dy's columns cost as much again as what else the matrix instructions hide: only
-      // the blocks of the first columns make them
-      if (DW && p.db && c0 == 0) {
-        for (int k0 = 0; k0 < length; k0 += BK, cur ^= 1)
-          stage(std::integral_constant<bool, DW>(), k0, lds[cur], lds[cur ^ 1]);
-      } else {
-        for (int k0 = 0; k0 < length; k0 += BK, cur ^= 1) stage(std::false_type(), k0, lds[cur], lds[cur ^ 1]);
-      }
+      for (int k0 = 0; k0 < length; k0 += BK, cur ^= 1) stage(k0, lds[cur], lds[cur ^ 1]);
     }
 
     // lane: of each 32 x 32, row lane % 32 and columns 16 (lane / 32) .. + 16
