@@ -53,31 +53,19 @@ __device__ __forceinline__ f32x16 mfma32(u32x4 a, u32x4 b, f32x16 c) {
                                                   0, 0, 0);
 }
 
-// The first operand is the columns' (B), taken in the order that leaves a lane with 16
-// neighbouring columns of one row: fragment row 8 a + 4 h + b is column 16 h + 4 a + b.
-__device__ __forceinline__ int column_of(int r) { return ((r >> 2) & 1) * 16 + (r >> 3) * 4 + (r & 3); }
-
 // Stages in LDS.  Along the contraction: [256 rows][8 chunks of 16 bytes], the chunks
 // swizzled so that the eight rows that are read together lie in different banks.
-template <bool COLUMNS>
-__device__ __forceinline__ int kc_swizzle(int row) {
-  return COLUMNS ? (row & 3) | ((row >> 2) & 4) : row & 7;
-}
-template <bool COLUMNS>
 __device__ __forceinline__ u32x4 kc_frag32(const char* tile, int base, int step, int lane) {
-  const int r = lane & 31, row = base + (COLUMNS ? column_of(r) : r);
-  return *reinterpret_cast<const u32x4*>(
-      tile + row * 128 + (((step * 2 + (lane >> 5)) ^ kc_swizzle<COLUMNS>(row)) << 4));
+  const int row = base + (lane & 31);
+  return *reinterpret_cast<const u32x4*>(tile + row * 128 + (((step * 2 + (lane >> 5)) ^ (row & 7)) << 4));
 }
 // Contraction-major: [64][256 columns], in units of 16 columns (32 bytes), pairs of units
 // swizzled.  Transposing reads: within 16 lanes, lane l gives four columns of row l / 4 and
 // gets column l of the four rows.
 __device__ __forceinline__ int cm_swizzle32(int row) { return ((row & 3) | ((row >> 1) & 4)) << 1; }
-template <bool COLUMNS>
 __device__ __forceinline__ u32x4 cm_frag32(const char* tile, int base, int step, int lane) {
   typedef __attribute__((address_space(3))) s16x4* tr_ptr;
-  const int g = lane >> 4, l = lane & 15, piece = l & 3;
-  const int col = base + (COLUMNS ? (piece & 1) * 16 + (g & 1) * 8 + (piece >> 1) * 4 : (g & 1) * 16 + piece * 4);
+  const int g = lane >> 4, l = lane & 15, col = base + (g & 1) * 16 + (l & 3) * 4;
   s16x4 v[2];
 #pragma unroll
   for (int h = 0; h < 2; ++h) {
@@ -88,6 +76,17 @@ __device__ __forceinline__ u32x4 cm_frag32(const char* tile, int base, int step,
   u32x4 out;
   __builtin_memcpy(&out, v, 16);
   return out;
+}
+
+// Two results of neighbouring rows, as the 16 bits of two neighbouring columns of one: even
+// lanes take the first row, odd ones the second.
+template <typename T>
+__device__ __forceinline__ uint32_t pair_of(float first, float second, uint32_t select) {
+  const T e[2] = {(T)first, (T)second};
+  uint32_t mine;
+  __builtin_memcpy(&mine, e, 4);
+  const uint32_t other = (uint32_t)__builtin_amdgcn_mov_dpp((int)mine, 0xb1, 0xf, 0xf, true);  // lane ^ 1
+  return __builtin_amdgcn_perm(other, mine, select);
 }
 
 // MODE LEAF_PRODUCT_Y: a = x rows [k], b = w[leaf] [col][k]; _DX: a = dy rows [m], b = w[leaf]
@@ -142,19 +141,18 @@ __global__ __launch_bounds__(THREADS, 1) void k_leaf_big(LeafProduct p, int col_
     // 8 (swizzled); contraction-major: row 2 (8 wave + j) + lane / 32, 16 bytes lane % 32
     // (swizzled).
     const int kc_row = wave * 64 + (lane >> 3), cm_row = wave * 16 + (lane >> 5);
-    const int achunk = ((lane & 7) ^ kc_swizzle<false>(kc_row)) * 8;
+    const int achunk = ((lane & 7) ^ (kc_row & 7)) * 8;
     // Offsets are in 16 bytes, which rows are whole ones of: 32 bits reach 64 GB.
     uint32_t aoff[LOADS], boff[LOADS];
-    int bchunk[LOADS], cm_col[LOADS];
+    int cm_col[LOADS];
     const uint32_t ld16 = (uint32_t)((MODE == LEAF_PRODUCT_Y ? p.ldx : p.lddy) / 8);
 #pragma unroll
     for (int j = 0; j < LOADS; ++j) {
       const int unit = ((lane & 31) >> 1) ^ cm_swizzle32(cm_row + 2 * j);
       cm_col[j] = (unit * 2 + (lane & 1)) * 8;
-      bchunk[j] = ((lane & 7) ^ kc_swizzle<true>(kc_row + 8 * j)) * 8;
       if (!ACM) aoff[j] = (uint32_t)max(row_of[DW ? 0 : kc_row + 8 * j], 0) * ld16 + achunk / 8;
       if (MODE == LEAF_PRODUCT_Y)
-        boff[j] = (uint32_t)min(c0 + kc_row + 8 * j, cols - 1) * (uint32_t)(length / 8) + bchunk[j] / 8;
+        boff[j] = (uint32_t)min(c0 + kc_row + 8 * j, cols - 1) * (uint32_t)(length / 8) + achunk / 8;
       if (MODE == LEAF_PRODUCT_DX) boff[j] = (uint32_t)(cm_row + 2 * j) * (uint32_t)(cols / 8) + (c0 + cm_col[j]) / 8;
     }
     // DW: where the 16 rows of a wave's loads begin, in dy and in x at the block's columns.
@@ -203,7 +201,7 @@ __global__ __launch_bounds__(THREADS, 1) void k_leaf_big(LeafProduct p, int col_
       uint64_t from;
       bool in;
       if (DW) return *(global_vec)(at_row[j & 1].y + b_col);
-      in = BCM ? k0 + cm_row + 2 * j < length && c0 + cm_col[j] < cols : k0 + bchunk[j] < length;
+      in = BCM ? k0 + cm_row + 2 * j < length && c0 + cm_col[j] < cols : k0 + achunk < length;
       from = g.b + (uint64_t)boff[j] * 16;
       return *(global_vec)(in ? from : zero_at);
     };
@@ -227,11 +225,11 @@ __global__ __launch_bounds__(THREADS, 1) void k_leaf_big(LeafProduct p, int col_
     // item: step FM + i of a stage
     auto frag_a = [&](const char* buf, int item) {
       const int base = wm + 32 * (item % FM), step = item / FM;
-      return ACM ? cm_frag32<false>(buf, base, step, lane) : kc_frag32<false>(buf, base, step, lane);
+      return ACM ? cm_frag32(buf, base, step, lane) : kc_frag32(buf, base, step, lane);
     };
     auto frag_b = [&](const char* buf, int j, int step) {
-      return BCM ? cm_frag32<true>(buf + A_BYTES, wn + 32 * j, step, lane)
-                 : kc_frag32<true>(buf + A_BYTES, wn + 32 * j, step, lane);
+      return BCM ? cm_frag32(buf + A_BYTES, wn + 32 * j, step, lane)
+                 : kc_frag32(buf + A_BYTES, wn + 32 * j, step, lane);
     };
     u32x4 fa[RING], fb[2][FN], ahead[2 * LOADS];
     int next_rows = 0;  // DW: what put_rows takes next
@@ -278,7 +276,7 @@ __global__ __launch_bounds__(THREADS, 1) void k_leaf_big(LeafProduct p, int col_
         }
         __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-        for (int j = 0; j < FN / 2; ++j) acc[i][j] = mfma32<T>(fb[step % 2][j], f, acc[i][j]);
+        for (int j = 0; j < FN / 2; ++j) acc[i][j] = mfma32<T>(f, fb[step % 2][j], acc[i][j]);
         __builtin_amdgcn_sched_barrier(0);
         if (t > 0 && share_of(t - 1) >= 0) {
           const int l = share_of(t - 1);
@@ -286,7 +284,7 @@ __global__ __launch_bounds__(THREADS, 1) void k_leaf_big(LeafProduct p, int col_
           if (DW && l + 2 < LOADS) at_row[l & 1] = get_rows(l + 2);
         }
 #pragma unroll
-        for (int j = FN / 2; j < FN; ++j) acc[i][j] = mfma32<T>(fb[step % 2][j], f, acc[i][j]);
+        for (int j = FN / 2; j < FN; ++j) acc[i][j] = mfma32<T>(f, fb[step % 2][j], acc[i][j]);
         __builtin_amdgcn_sched_barrier(0);
         if (t == TURN && DW) {
           put_rows(next_rows, k0 + 3 * BK);
@@ -345,61 +343,61 @@ __global__ __launch_bounds__(THREADS, 1) void k_leaf_big(LeafProduct p, int col_
       for (int k0 = 0; k0 < length; k0 += BK, cur ^= 1) stage(k0, lds[cur], lds[cur ^ 1]);
     }
 
-    // lane: of each 32 x 32, row lane % 32 and columns 16 (lane / 32) .. + 16
+    // A lane has column lane % 32 of each 32 x 32, so that a store's lanes fill 64 or 128 bytes
+    // of a row (16 bytes each of 64 rows: FIGURE).
+    const int col0 = c0 + wn + (lane & 31), row4 = (lane >> 5) * 4;
     if (DW) {
       float* const dw = p.dw + leaf * p.outputs * (int64_t)p.inputs;
 #pragma unroll
       for (int i = 0; i < FM; ++i) {
-        const int m = m0 + wm + i * 32 + (lane & 31);
-        if (p.db && c0 == 0 && wn == 0) {
+        const int mi = m0 + wm + i * 32;
+        if (sums && wn == 0) {
           const float b = bias[DW ? i : 0] + __shfl_xor(bias[DW ? i : 0], 32);
-          if (lane < 32 && m < p.outputs) p.db[leaf * p.outputs + m] = b;
+          if (lane < 32 && mi + lane < p.outputs) p.db[leaf * p.outputs + mi + lane] = b;
         }
-        if (m >= p.outputs) continue;
 #pragma unroll
-        for (int j = 0; j < FN; ++j) {
-          const int k = c0 + wn + j * 32 + (lane >> 5) * 16;
-          float* const to = dw + (int64_t)m * cols + k;
+        for (int e = 0; e < 16; ++e) {
+          const int m = mi + (e >> 2) * 8 + row4 + (e & 3);
+          if (m >= p.outputs) continue;
 #pragma unroll
-          for (int e = 0; e < 16; e += 4)  // columns come in eights
-            if (k + e < cols) __builtin_memcpy(to + e, (const float*)&acc[i][j] + e, 16);
+          for (int j = 0; j < FN; ++j)
+            if (col0 + j * 32 < cols) dw[(int64_t)m * cols + col0 + j * 32] = acc[i][j][e];
         }
       }
       return;
     }
-    const T* const bias_of = MODE == LEAF_PRODUCT_Y && p.b && leaf >= 0 ? (const T*)p.b + leaf * cols : nullptr;
-    const bool planes = p.g.trees > 1;
+    float b[FN];
 #pragma unroll
     for (int j = 0; j < FN; ++j) {
+      const bool has = MODE == LEAF_PRODUCT_Y && p.b && leaf >= 0 && col0 + j * 32 < cols;
+      b[j] = has ? (float)((const T*)p.b)[leaf * cols + col0 + j * 32] : 0.0f;
+    }
+    const uint32_t select = lane & 1 ? 0x03020706u : 0x05040100u;
 #pragma unroll
-      for (int half = 0; half < 16; half += 8) {
-        const int col = c0 + wn + j * 32 + (lane >> 5) * 16 + half;
-        if (col >= cols) continue;  // columns come in eights
-        float b[8] = {0, 0, 0, 0, 0, 0, 0, 0};
-        if (bias_of) {
-          T e[8];
-          __builtin_memcpy(e, bias_of + col, sizeof(e));
+    for (int i = 0; i < FM; ++i)
 #pragma unroll
-          for (int k = 0; k < 8; ++k) b[k] = (float)e[k];
-        }
+      for (int e = 0; e < 16; e += 2) {
+        const int r = wm + i * 32 + (e >> 2) * 8 + row4 + (e & 3);
+        const int n[2] = {row_of[DW ? 0 : r], row_of[DW ? 0 : r + 1]};
+        if (p.g.trees > 1) {
 #pragma unroll
-        for (int i = 0; i < FM; ++i) {
-          const int n = row_of[DW ? 0 : wm + i * 32 + (lane & 31)];
-          if (n < 0) continue;
-          float v[8];
+          for (int k = 0; k < 2; ++k) {
+            if (n[k] < 0) continue;
+            float* const to = (float*)p.ws + ((int64_t)tree * p.g.rows + n[k]) * cols + col0;
 #pragma unroll
-          for (int k = 0; k < 8; ++k) v[k] = acc[i][j][half + k] + b[k];
-          if (planes) {
-            __builtin_memcpy((float*)p.ws + ((int64_t)tree * p.g.rows + n) * cols + col, v, 32);
-          } else {
-            T e[8];
+            for (int j = 0; j < FN; ++j)
+              if (col0 + j * 32 < cols) to[j * 32] = acc[i][j][e + k] + b[j];
+          }
+        } else {
+          const int row = n[lane & 1];
+          T* const to = (T*)p.out + (int64_t)max(row, 0) * p.ldo + (col0 & ~1);
 #pragma unroll
-            for (int k = 0; k < 8; ++k) e[k] = (T)v[k];
-            __builtin_memcpy((T*)p.out + (int64_t)n * p.ldo + col, e, 16);
+          for (int j = 0; j < FN; ++j) {
+            const uint32_t v = pair_of<T>(acc[i][j][e] + b[j], acc[i][j][e + 1] + b[j], select);
+            if (row >= 0 && col0 + j * 32 < cols) __builtin_memcpy(to + j * 32, &v, 4);
           }
         }
       }
-    }
     __syncthreads();  // row_of is read before the next tile's
   }
 }
