@@ -97,7 +97,8 @@ def test_gradients(check, rows, inputs, outputs, trees, leaves, shape, pad, dtyp
     (9000, 24, 6, 1, 2, "f32"), (9000, 30, 9, 1, 2, "bf16"), (5000, 320, 272, 1, 3, "bf16"),
     (5000, 272, 320, 1, 3, "f16"), (1500, 600, 512, 2, 2, "bf16"), (40000, 5, 1, 1, 300, "f32"),
     (9000, 65, 513, 1, 3, "bf16"), (9000, 515, 33, 1, 3, "f16"), (3000, 200, 1100, 5, 2, "f16"),
-    (2000, 264, 520, 1, 5, "bf16"), (70000, 600, 20, 1, 2, "bf16"), (1000, 2048, 256, 1, 1, "bf16")])
+    (2000, 264, 520, 1, 5, "bf16"), (70000, 600, 20, 1, 2, "bf16"),
+    (400, 200, 192, 70, 2, "f16"), (200, 192, 200, 1030, 1, "bf16"), (1000, 2048, 256, 1, 1, "bf16")])
 def test_long(check, what, rows, inputs, outputs, trees, leaves, dtype):
     check(what, rows=rows, inputs=inputs, outputs=outputs, trees=trees, leaves=leaves, dtype=dtype,
           shape="even")
