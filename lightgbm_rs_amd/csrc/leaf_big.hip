@@ -89,6 +89,23 @@ __device__ __forceinline__ uint32_t pair_of(float first, float second, uint32_t 
   return __builtin_amdgcn_perm(other, mine, select);
 }
 
+// The leaf of the forest that is the `rank`-th by rows, of at most THREADS: the long blocks
+// begin first, and the short ones fill the end (both gradients of two trees of 15 leaves, 16389 rows
+// of 2048 to 2048: 824 us in their order, 789).
+__device__ __forceinline__ int leaf_of_rank(const LeafGroups& g, int leaves, int rank) {
+  __shared__ int counts[THREADS];
+  __shared__ int found;
+  const int tid = threadIdx.x, mine = tid < leaves ? g.count[tid] : 0;
+  counts[tid] = mine;
+  __syncthreads();
+  int before = 0;
+#pragma unroll 8
+  for (int l = 0; l < leaves; ++l) before += counts[l] > mine || (counts[l] == mine && l < tid);
+  if (tid < leaves && before == rank) found = tid;
+  __syncthreads();
+  return found;
+}
+
 // MODE LEAF_PRODUCT_Y: a = x rows [k], b = w[leaf] [col][k]; _DX: a = dy rows [m], b = w[leaf]
 // [m][col]; _DW: a = dy [row][m], b = x [row][k] over a leaf's rows.  Y and DX: one block a
 // CU takes tile after tile, so that what it stores drains while the next tile begins; DW:
@@ -118,6 +135,7 @@ __global__ __launch_bounds__(THREADS, 1) void k_leaf_big(LeafProduct p, int col_
     if (DW) {
       const int of = (p.outputs + BM - 1) / BM * col_tiles, tile = (int)(blockIdx.x % of);
       leaf = blockIdx.x / of;
+      if (p.g.trees * (int64_t)p.g.leaves <= THREADS) leaf = leaf_of_rank(p.g, p.g.trees * p.g.leaves, (int)leaf);
       tree = (int)(leaf / p.g.leaves);
       length = min(max(p.g.count[leaf], 0), p.g.rows);
       first = min(max(p.g.begin[leaf], 0), p.g.rows - length);
