@@ -163,32 +163,37 @@ def differences():
         assert abs(change - want) <= 2 * 32 * U * 16 * size, (name, change, want, size)
 
 
-def odd_tables():
+def odd_tables(scale=1, inputs=8, outputs=4, dtype="f32"):
     """Tables that do not hold: ranges outside the order and rows outside the matrix are held
     back or passed over, and rows that stand nowhere are left as they were."""
-    be = backend()
+    be, dt, rows = backend(), TYPES[dtype], 50 * scale
     rng = np.random.default_rng(2)
-    x = matrix(rng, 50, 8, torch.float32)
-    w = matrix(rng, 3 * 4, 8, torch.float32).view(3, 4, 8)
-    dy = matrix(rng, 50, 4, torch.float32)
-    order = torch.arange(50, dtype=torch.int32)
-    order[7], order[8], order[9] = -5, 50, 2 ** 31 - 1
-    for begin, count in (([0, 20, 30], [20, 10, 20]), ([-4, 90, 30], [10, 10, 2000]),
-                         ([0, 0, 0], [-3, 50, 0]), ([2 ** 31 - 1] * 3, [2 ** 31 - 1] * 3)):
+    x = matrix(rng, rows, inputs, dt)
+    w = matrix(rng, 3 * outputs, inputs, dt).view(3, outputs, inputs)
+    dy = matrix(rng, rows, outputs, dt)
+    order = torch.arange(rows, dtype=torch.int32)
+    order[7], order[8], order[9] = -5, rows, 2 ** 31 - 1
+    sizes = [20 * scale, 10 * scale, 20 * scale]
+    for begin, count in (([0, 20 * scale, 30 * scale], sizes), ([-4, 90 * scale, 30], [10, 10, 2000 * scale]),
+                         ([0, 0, 0], [-3, rows, 0]), ([2 ** 31 - 1] * 3, [2 ** 31 - 1] * 3)):
         g = LeafGroups(order[None].to(DEV), torch.tensor([begin], dtype=torch.int32, device=DEV),
                        torch.tensor([count], dtype=torch.int32, device=DEV))
-        y = be.leaf_product(x, w, g, out=torch.full((50, 4), 5.0, device=DEV))
+        y = be.leaf_product(x, w, g, out=torch.full((rows, outputs), 5.0, device=DEV, dtype=dt))
         dw, db = be.leaf_product_dw(dy, x, g)
         be.leaf_product_dx(dy, w, g)
-        if begin == [0, 20, 30]:
-            leaf = np.repeat([0, 1, 2], (20, 10, 20))[:, None].astype(np.int32)
+        if count == sizes:
+            leaf = np.repeat([0, 1, 2], sizes)[:, None].astype(np.int32)
             leaf[7:10] = -1
             want, size = oracle.product(wide(x), wide(w), None, leaf, 3)
             want[7:10] = 5.0
-            near(y, want, size, 8, torch.float32, "y")
+            near(y, want, size, inputs, dt, "y")
             w_want, w_size, b_want, b_size = oracle.product_dw(wide(dy), wide(x), leaf, 3)
-            near(dw, w_want, w_size, 50, torch.float32, "dw")
-            near(db, b_want, b_size, 50, torch.float32, "db")
+            near(dw, w_want, w_size, rows, torch.float32, "dw")
+            near(db, b_want, b_size, rows, torch.float32, "db")
+
+
+def odd_tables_large():
+    odd_tables(16, 200, 192, "bf16")
 
 
 def any_order():

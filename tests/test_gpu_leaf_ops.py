@@ -104,7 +104,7 @@ def test_long(check, what, rows, inputs, outputs, trees, leaves, dtype):
           shape="even")
 
 
-@pytest.mark.parametrize("name", ["differences", "odd_tables", "any_order", "empty", "layouts",
+@pytest.mark.parametrize("name", ["differences", "odd_tables", "odd_tables_large", "any_order", "empty", "layouts",
                                   "scores_history", "refused", "own_stream", "side_stream",
                                   "captured", "threads", "forest", "learner"])
 def test_plain(check, name):
