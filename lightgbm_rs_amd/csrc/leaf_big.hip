@@ -80,17 +80,6 @@ __device__ __forceinline__ u32x4 cm_frag32(const char* tile, int base, int step,
   return out;
 }
 
-// Two results of neighbouring rows, as the 16 bits of two neighbouring columns of one: even
-// lanes take the first row, odd ones the second.
-template <typename T>
-__device__ __forceinline__ uint32_t pair_of(float first, float second, uint32_t select) {
-  const T e[2] = {(T)first, (T)second};
-  uint32_t mine;
-  __builtin_memcpy(&mine, e, 4);
-  const uint32_t other = (uint32_t)__builtin_amdgcn_mov_dpp((int)mine, 0xb1, 0xf, 0xf, true);  // lane ^ 1
-  return __builtin_amdgcn_perm(other, mine, select);
-}
-
 // The leaf of the forest that is the `rank`-th by rows, of at most THREADS: the long blocks
 // begin first, and the short ones fill the end (both gradients of two trees of 15 leaves, 16389 rows
 // of 2048 to 2048: 824 us in their order, 789).
@@ -393,7 +382,6 @@ __global__ __launch_bounds__(THREADS, 1) void k_leaf_big(LeafProduct p, int col_
       const bool has = MODE == LEAF_PRODUCT_Y && p.b && leaf >= 0 && col0 + j * 32 < cols;
       b[j] = has ? (float)((const T*)p.b)[leaf * cols + col0 + j * 32] : 0.0f;
     }
-    const uint32_t select = lane & 1 ? 0x03020706u : 0x05040100u;
 #pragma unroll
     for (int i = 0; i < FM; ++i)
 #pragma unroll
@@ -414,7 +402,7 @@ __global__ __launch_bounds__(THREADS, 1) void k_leaf_big(LeafProduct p, int col_
           T* const to = (T*)p.out + (int64_t)max(row, 0) * p.ldo + (col0 & ~1);
 #pragma unroll
           for (int j = 0; j < FN; ++j) {
-            const uint32_t v = pair_of<T>(acc[i][j][e] + b[j], acc[i][j][e + 1] + b[j], select);
+            const uint32_t v = pair_of<T>(acc[i][j][e] + b[j], acc[i][j][e + 1] + b[j]);
             if (row >= 0 && col0 + j * 32 < cols) __builtin_memcpy(to + j * 32, &v, 4);
           }
         }

@@ -32,7 +32,7 @@ __global__ __launch_bounds__(THREADS) void k_leaf_tile(LeafProduct p, int length
   constexpr int GN = 4 / GM, WM = BM / GM, WN = BN / GN;
   constexpr int ACH = BM * 8 / THREADS, BCH = BN * 8 / THREADS;
   __shared__ __align__(16) char lds[2][(BM + BN) * 128];
-  __shared__ int32_t row_of[BM];
+  __shared__ __align__(16) int32_t row_of[BM];
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const int tree = blockIdx.y;
   const int mt = blockIdx.x / col_tiles, c0 = (blockIdx.x % col_tiles) * BN;
@@ -111,7 +111,7 @@ __global__ __launch_bounds__(THREADS) void k_leaf_tile(LeafProduct p, int length
 #pragma unroll
         for (int i = 0; i < WM / 16; ++i)
 #pragma unroll
-          for (int j = 0; j < WN / 16; ++j) part.at[i][j] = El<T>::mfma(fb[j], fa[i], part.at[i][j]);
+          for (int j = 0; j < WN / 16; ++j) part.at[i][j] = El<T>::mfma(fa[i], fb[j], part.at[i][j]);
       }
       part.add_to(acc);
       if (more) store(lds[b ^ 1]);
@@ -119,17 +119,18 @@ __global__ __launch_bounds__(THREADS) void k_leaf_tile(LeafProduct p, int length
     }
   }
 
-  // lane: output row lane % 16, columns 4 (lane / 16) .. + 4 of each 16 x 16
+  // lane: rows 4 (lane / 16) .. + 4, column lane % 16 of each 16 x 16
   const T* const bias = (!DX && p.b && rt.leaf >= 0) ? (const T*)p.b + leaf * cols : nullptr;
 #pragma unroll
   for (int j = 0; j < WN / 16; ++j) {
-    const int col = c0 + n0 + j * 16 + (lane >> 4) * 4;
-    if (col >= cols) continue;
-    const f32x4 b = bias4(bias, col, cols);
+    if (c0 + n0 + j * 16 >= cols) continue;
+    const int col = c0 + n0 + j * 16 + (lane & 15);
+    const float b = bias_at(bias, col, cols);
 #pragma unroll
     for (int i = 0; i < WM / 16; ++i) {
-      const int n = row_of[m0 + i * 16 + (lane & 15)];
-      if (n >= 0) store_row<T>(p, tree, n, col, cols, acc[i][j] + b);
+      int n[4];
+      __builtin_memcpy(n, row_of + m0 + i * 16 + (lane >> 4) * 4, sizeof(n));
+      store_rows<T>(p, tree, n, col, cols, acc[i][j] + b);
     }
   }
 }
@@ -151,9 +152,9 @@ __global__ __launch_bounds__(WAVES * 64) void k_leaf_narrow(LeafProduct p) {
 #pragma unroll
   for (int j = 0; j < NB; ++j) wrow[j] = w + (int64_t)min(j * 16 + r, cols - 1) * length;
   const T* const bias = (p.b && rt.leaf >= 0) ? (const T*)p.b + leaf * cols : nullptr;
-  f32x4 b[NB];
+  float b[NB];
 #pragma unroll
-  for (int j = 0; j < NB; ++j) b[j] = bias4(bias, j * 16 + q * 4, cols);
+  for (int j = 0; j < NB; ++j) b[j] = bias_at(bias, j * 16 + r, cols);
   int n[ROUNDS][2];
 #pragma unroll
   for (int t = 0; t < ROUNDS; ++t)
@@ -169,7 +170,7 @@ __global__ __launch_bounds__(WAVES * 64) void k_leaf_narrow(LeafProduct p) {
 #pragma unroll
     for (int i = 0; i < 2; ++i)
 #pragma unroll
-      for (int j = 0; j < NB; ++j) acc[i][j] = b[j];
+      for (int j = 0; j < NB; ++j) acc[i][j] = f32x4{b[j], b[j], b[j], b[j]};
     if (rt.leaf >= 0) {
       const T* xrow[2];
 #pragma unroll
@@ -202,18 +203,18 @@ __global__ __launch_bounds__(WAVES * 64) void k_leaf_narrow(LeafProduct p) {
 #pragma unroll
           for (int i = 0; i < 2; ++i)
 #pragma unroll
-            for (int j = 0; j < NB; ++j) part.at[i][j] = El<T>::mfma(fb[u][j], fa[u][i], part.at[i][j]);
+            for (int j = 0; j < NB; ++j) part.at[i][j] = El<T>::mfma(fa[u][i], fb[u][j], part.at[i][j]);
         }
         part.add_to(acc);
       }
     }
 #pragma unroll
-    for (int i = 0; i < 2; ++i)
+    for (int i = 0; i < 2; ++i) {
+      int rows[4];
+      rows_of(n[t][i], lane, rows);
 #pragma unroll
-      for (int j = 0; j < NB; ++j) {
-        const int col = j * 16 + q * 4;
-        if (n[t][i] >= 0 && col < cols) store_row<T>(p, tree, n[t][i], col, cols, acc[i][j]);
-      }
+      for (int j = 0; j < NB; ++j) store_rows<T>(p, tree, rows, j * 16 + r, cols, acc[i][j]);
+    }
   }
 }
 
@@ -246,19 +247,20 @@ __global__ __launch_bounds__(THREADS) void k_leaf_few(LeafProduct p, int col_til
       }
       Parts<T, 1, 1> part(acc);
 #pragma unroll
-      for (int u = 0; u < UNROLL; ++u) part.at[0][0] = El<T>::mfma(fw[u], fx[u], part.at[0][0]);
+      for (int u = 0; u < UNROLL; ++u) part.at[0][0] = El<T>::mfma(fx[u], fw[u], part.at[0][0]);
       part.add_to(acc);
     }
   }
   sums[wave][lane] = acc[0][0];
   __syncthreads();
-  const int col = c0 + q * 4;
-  if (wave == 0 && n >= 0 && col < cols) {
+  if (wave == 0) {
     const T* const bias = (p.b && rt.leaf >= 0) ? (const T*)p.b + leaf * cols : nullptr;
-    f32x4 y = acc[0][0] + bias4(bias, col, cols);
+    f32x4 y = acc[0][0] + bias_at(bias, c0 + r, cols);
 #pragma unroll
     for (int v = 1; v < 4; ++v) y += sums[v][lane];
-    store_row<T>(p, tree, n, col, cols, y);
+    int rows[4];
+    rows_of(n, lane, rows);
+    store_rows<T>(p, tree, rows, c0 + r, cols, y);
   }
 }
 
@@ -266,9 +268,9 @@ __global__ __launch_bounds__(THREADS) void k_leaf_few(LeafProduct p, int col_til
 // inputs in registers, turned as the matrix instruction takes it, and runs over its rows, 16
 // at a time: one load of dy's rows, then a product and a store of 16 x 16 for each 16
 // inputs.
-template <typename T>
-__global__ __launch_bounds__(THREADS) void k_leaf_dx_narrow(LeafProduct p, int col_tiles, int steps) {
-  constexpr int V = El<T>::V, MAX_STEPS = sizeof(T) == 2 ? 1 : 2, FN = 8, BM = 512;
+template <typename T, int STEPS>
+__global__ __launch_bounds__(THREADS) void k_leaf_dx_narrow(LeafProduct p, int col_tiles) {
+  constexpr int V = El<T>::V, FN = 8, BM = 512;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, r = lane & 15, q = lane >> 4;
   const int tree = blockIdx.y, cols = p.inputs, length = p.outputs;
   const int c0 = (int)(blockIdx.x % col_tiles) * (16 * FN);
@@ -276,9 +278,9 @@ __global__ __launch_bounds__(THREADS) void k_leaf_dx_narrow(LeafProduct p, int c
   if (wave * 16 >= rt.rows) return;
   const int64_t leaf = (int64_t)tree * p.g.leaves + rt.leaf;
   const T* const w = (const T*)p.w + (rt.leaf < 0 ? 0 : leaf * length * (int64_t)cols);
-  u32x4 fw[MAX_STEPS][FN];
+  u32x4 fw[STEPS][FN];
 #pragma unroll
-  for (int s = 0; s < MAX_STEPS; ++s)
+  for (int s = 0; s < STEPS; ++s)
 #pragma unroll
     for (int j = 0; j < FN; ++j) {
       T e[V];
@@ -289,10 +291,10 @@ __global__ __launch_bounds__(THREADS) void k_leaf_dx_narrow(LeafProduct p, int c
       }
       __builtin_memcpy(&fw[s][j], e, 16);
     }
-  constexpr int UNROLL = 2;
+  constexpr int UNROLL = 4;
   for (int r0 = wave * 16; r0 < rt.rows; r0 += 64 * UNROLL) {
     int n[UNROLL];
-    u32x4 f[UNROLL][MAX_STEPS];
+    u32x4 f[UNROLL][STEPS];
 #pragma unroll
     for (int u = 0; u < UNROLL; ++u) {
       const int at = r0 + u * 64 + r;
@@ -301,23 +303,25 @@ __global__ __launch_bounds__(THREADS) void k_leaf_dx_narrow(LeafProduct p, int c
 #pragma unroll
     for (int u = 0; u < UNROLL; ++u)
 #pragma unroll
-      for (int s = 0; s < MAX_STEPS; ++s) {
+      for (int s = 0; s < STEPS; ++s) {
         const int m = (s * 4 + q) * V;
         f[u][s] = load16((const T*)p.dy + (int64_t)max(n[u], 0) * p.lddy + m,
                          n[u] < 0 || rt.leaf < 0 ? 0 : length - m);
       }
 #pragma unroll
-    for (int u = 0; u < UNROLL; ++u)
+    for (int u = 0; u < UNROLL; ++u) {
+      int rows[4];
+      rows_of(n[u], lane, rows);
 #pragma unroll
       for (int j = 0; j < FN; ++j) {
-        const int col = c0 + j * 16 + q * 4;
         if (c0 + j * 16 >= cols) break;
         f32x4 acc = {0, 0, 0, 0};
 #pragma unroll
-        for (int s = 0; s < MAX_STEPS; ++s)
-          if (s < steps) acc = El<T>::mfma(fw[s][j], f[u][s], acc);
-        if (n[u] >= 0 && col < cols) store_row<T>(p, tree, n[u], col, cols, acc);
+        for (int s = 0; s < STEPS; ++s)
+          acc = El<T>::mfma(f[u][s], fw[s][j], acc);
+        store_rows<T>(p, tree, rows, c0 + j * 16 + r, cols, acc);
       }
+    }
   }
 }
 
@@ -490,7 +494,7 @@ __global__ __launch_bounds__(THREADS) void k_leaf_dw(LeafProduct p, int m_tiles,
 #pragma unroll
         for (int i = 0; i < WM / 16; ++i)
 #pragma unroll
-          for (int j = 0; j < WN / 16; ++j) part.at[i][j] = El<T>::mfma(fb[j], fa[i], part.at[i][j]);
+          for (int j = 0; j < WN / 16; ++j) part.at[i][j] = El<T>::mfma(fa[i], fb[j], part.at[i][j]);
       }
       part.add_to(acc);
       if (more) store(lds[b ^ 1]);
@@ -499,13 +503,16 @@ __global__ __launch_bounds__(THREADS) void k_leaf_dw(LeafProduct p, int m_tiles,
   }
 #pragma unroll
   for (int i = 0; i < WM / 16; ++i) {
-    const int m = m0 + (wave / GN) * WM + i * 16 + (lane & 15);
-    if (m >= p.outputs) continue;
-    if (sums && lane < 16) db[m] = bias[i][0];
+    const int mi = m0 + (wave / GN) * WM + i * 16;
+    if (sums && lane < 16 && mi + lane < p.outputs) db[mi + lane] = bias[i][0];
 #pragma unroll
-    for (int j = 0; j < WN / 16; ++j) {
-      const int k = k0 + (wave % GN) * WN + j * 16 + (lane >> 4) * 4;
-      if (k < p.inputs) store4(dw + (int64_t)m * p.inputs + k, acc[i][j], p.inputs - k);
+    for (int e = 0; e < 4; ++e) {
+      const int m = mi + (lane >> 4) * 4 + e;
+#pragma unroll
+      for (int j = 0; j < WN / 16; ++j) {
+        const int k = k0 + (wave % GN) * WN + j * 16 + (lane & 15);
+        if (m < p.outputs && k < p.inputs) dw[(int64_t)m * p.inputs + k] = acc[i][j][e];
+      }
     }
   }
 }
@@ -623,9 +630,12 @@ void launch(const LeafProduct& p, int what, hipStream_t s) {
   if (leaf_big_fits(p, what)) {
     launch_leaf_big(p, what, s);
   } else if (dx && p.outputs <= 32) {
-    const int ct = (cols + 127) / 128, steps = (p.outputs + 4 * El<T>::V - 1) / (4 * El<T>::V);
+    const int ct = (cols + 127) / 128;
     const dim3 grid((unsigned)(row_tiles(p.g, 512) * ct), (unsigned)p.g.trees);
-    k_leaf_dx_narrow<T><<<grid, THREADS, 0, s>>>(p, ct, steps);
+    if (p.outputs <= 4 * El<T>::V)
+      k_leaf_dx_narrow<T, 1><<<grid, THREADS, 0, s>>>(p, ct);
+    else if constexpr (sizeof(T) == 4)
+      k_leaf_dx_narrow<T, 2><<<grid, THREADS, 0, s>>>(p, ct);
   } else if (dx) {
     launch_tiles<T, true>(p, cols, s);
   } else if (by_maps(p)) {
