@@ -7,6 +7,7 @@
 // rows directly; several write float32 planes [tree][row] that k_sum_trees adds, so results
 // never depend on the order of blocks.
 #include <algorithm>
+#include <type_traits>
 
 #include "leaf_mma.h"
 
@@ -270,7 +271,8 @@ __global__ __launch_bounds__(THREADS) void k_leaf_few(LeafProduct p, int col_til
 // inputs.
 template <typename T, int STEPS>
 __global__ __launch_bounds__(THREADS) void k_leaf_dx_narrow(LeafProduct p, int col_tiles) {
-  constexpr int V = El<T>::V, FN = 8, BM = 512;
+  constexpr int V = El<T>::V, FN = 8, BM = 512, PITCH = 16 * FN + 4;
+  __shared__ __align__(16) float lds[THREADS / 64][16 * PITCH];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, r = lane & 15, q = lane >> 4;
   const int tree = blockIdx.y, cols = p.inputs, length = p.outputs;
   const int c0 = (int)(blockIdx.x % col_tiles) * (16 * FN);
@@ -291,6 +293,27 @@ __global__ __launch_bounds__(THREADS) void k_leaf_dx_narrow(LeafProduct p, int c
       }
       __builtin_memcpy(&fw[s][j], e, 16);
     }
+  float* const mine = lds[wave];
+  // 16 rows from LDS, 16 bytes a lane
+  auto store_tile = [&](auto* out, int64_t ld, int valid, int row, const float* from) {
+    typedef std::remove_reference_t<decltype(*out)> O;
+    constexpr int CH = 16 / (int)sizeof(O), ACROSS = 16 * FN / CH;
+    const int col = lane % ACROSS * CH;
+#pragma unroll
+    for (int i = 0; i < 16; i += 64 / ACROSS) {
+      const int at = i + lane / ACROSS, n = __shfl(row, at);
+      O v[CH];
+#pragma unroll
+      for (int e = 0; e < CH; ++e) v[e] = (O)from[at * PITCH + col + e];
+      if (n >= 0 && col + CH <= valid) {
+        __builtin_memcpy(out + n * ld + col, v, 16);
+      } else if (n >= 0) {
+#pragma unroll
+        for (int e = 0; e < CH; ++e)
+          if (col + e < valid) out[n * ld + col + e] = v[e];
+      }
+    }
+  };
   constexpr int UNROLL = 4;
   for (int r0 = wave * 16; r0 < rt.rows; r0 += 64 * UNROLL) {
     int n[UNROLL];
@@ -310,17 +333,22 @@ __global__ __launch_bounds__(THREADS) void k_leaf_dx_narrow(LeafProduct p, int c
       }
 #pragma unroll
     for (int u = 0; u < UNROLL; ++u) {
-      int rows[4];
-      rows_of(n[u], lane, rows);
 #pragma unroll
       for (int j = 0; j < FN; ++j) {
         if (c0 + j * 16 >= cols) break;
         f32x4 acc = {0, 0, 0, 0};
 #pragma unroll
-        for (int s = 0; s < STEPS; ++s)
-          acc = El<T>::mfma(f[u][s], fw[s][j], acc);
-        store_rows<T>(p, tree, rows, c0 + j * 16 + r, cols, acc);
+        for (int s = 0; s < STEPS; ++s) acc = El<T>::mfma(f[u][s], fw[s][j], acc);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) mine[(q * 4 + e) * PITCH + j * 16 + r] = acc[e];
       }
+      __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+      __builtin_amdgcn_wave_barrier();
+      if (p.g.trees > 1)
+        store_tile((float*)p.ws + (int64_t)tree * p.g.rows * cols + c0, cols, cols - c0, n[u], mine);
+      else
+        store_tile((T*)p.out + c0, p.ldo, cols - c0, n[u], mine);
+      __builtin_amdgcn_wave_barrier();
     }
   }
 }
