@@ -104,6 +104,17 @@ def test_long(check, what, rows, inputs, outputs, trees, leaves, dtype):
           shape="even")
 
 
+# narrow products over tables beyond the caches
+@pytest.mark.parametrize("what", ["product", "grads"])
+@pytest.mark.parametrize("rows,inputs,outputs,trees,leaves,shape,pad,dtype", [
+    (300000, 61, 10, 1, 3, "lost", 1, "f32"), (270001, 140, 3, 2, 5, "skew", 0, "bf16"),
+    (150000, 120, 31, 1, 7, "even", 8, "f32"), (140000, 300, 20, 1, 1, "lost", 0, "f16"),
+    (200000, 90, 1, 1, 2, "one", 0, "f32")])
+def test_tables(check, what, rows, inputs, outputs, trees, leaves, shape, pad, dtype):
+    check(what, rows=rows, inputs=inputs, outputs=outputs, trees=trees, leaves=leaves, shape=shape,
+          pad=pad, dtype=dtype)
+
+
 @pytest.mark.parametrize("name", ["differences", "odd_tables", "odd_tables_large", "any_order", "empty", "layouts",
                                   "scores_history", "refused", "own_stream", "side_stream",
                                   "captured", "threads", "forest", "learner"])
