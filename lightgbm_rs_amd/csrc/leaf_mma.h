@@ -202,8 +202,12 @@ __device__ int count_tiles(const LeafGroups& g, int tree, int bm) {
   return (int)min(tiles, (int64_t)0x7fffffff);
 }
 
-// Blocks an upper bound of tiles of a tree needs.
-inline int64_t row_tiles(const LeafGroups& g, int64_t bm) { return (g.rows + bm - 1) / bm + g.leaves + 1; }
+// A bound of a tree's tiles: whole ones, an end for every leaf and for the rows in none, and
+// no tile without a row.
+inline int64_t row_tiles(const LeafGroups& g, int64_t bm) {
+  const int64_t tiles = (g.rows + bm - 1) / bm + g.leaves + 1;
+  return tiles < g.rows ? tiles : g.rows;
+}
 
 // The row at a position of a tree's order, -1 for an entry outside the matrix.
 __device__ __forceinline__ int row_at(const LeafGroups& g, int tree, int position) {

@@ -448,6 +448,19 @@ __global__ __launch_bounds__(THREADS) void k_leaf_dw(LeafProduct p, int m_tiles,
     first = min(max(p.g.begin[id], 0), p.g.rows - count);
     dw = p.dw + id * size;
     if (p.db) db = p.db + (int64_t)id * p.outputs;
+    if (count == 0) {  // the leaf's zeros, in one piece a block
+      const int64_t piece = ((size + tiles - 1) / tiles + 3) / 4 * 4, to = min(size, (tile + 1) * piece);
+      for (int64_t e = tile * piece + tid * 4; e < to; e += THREADS * 4) {
+        if (e + 4 <= to) {
+          const f32x4 none = {0, 0, 0, 0};
+          __builtin_memcpy(dw + e, &none, 16);
+        } else {
+          for (int64_t k = e; k < to; ++k) dw[k] = 0.0f;
+        }
+      }
+      for (int m = tile * THREADS + tid; db && m < p.outputs; m += tiles * THREADS) db[m] = 0.0f;
+      return;
+    }
   }
 
   f32x4 acc[WM / 16][WN / 16];
