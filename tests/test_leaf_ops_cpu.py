@@ -83,7 +83,8 @@ def calls(lib, m, p1=D, ld1=5, p2=E, p3=None, out=F, ldo=3, ws=W, size=1 << 40):
     (dict(), dict(out=E - 400), INVALID, "overlaps"), (dict(), dict(out=A + 396), INVALID, "overlaps"),
     (dict(), dict(out=B + 4096), INVALID, "overlaps"),
     (dict(leaves=2 ** 30, outputs=4096, inputs=4096), dict(ld1=4096, ldo=4096), CAPABILITY, "2^48"),
-    (dict(leaves=2 ** 24, outputs=4096, inputs=4096), dict(ld1=4096, ldo=4096), CAPABILITY, "one launch")])
+    (dict(rows=8192, leaves=8192, outputs=2 ** 17, inputs=2 ** 17), dict(ld1=2 ** 17, ldo=2 ** 17),
+     CAPABILITY, "one launch")])
 def test_products_refused(lib, m, change, code, text):
     for rc in calls(lib, None if m is None else maps(**m), **change):
         refused(lib, rc, code, text)
