@@ -402,8 +402,10 @@ __global__ __launch_bounds__(THREADS) void k_sum_few_trees(const float* planes, 
 
 // Rows a block sums at most, 0: a leaf's rows are not split.  Split sums go to slots in the
 // workspace, [tree][slots][outputs * inputs + outputs], and k_sum_slots adds them.  Leaves
-// differ in size and may be fewer than the CUs, so blocks take about a thousandth of the
-// work; in float32 also no more than 8192 rows, to keep a sum's rounding at that of its
+// differ in size and may be fewer than the CUs, so blocks take about a 2048th of the work (a
+// thousandth is one round of blocks and a few more: ragged leaves of 2M rows, 100 float32
+// inputs, 10 outputs 382 us instead of 283), or of many tiles a thousandth (40000 x 2001 to
+// 2047 bfloat16: 1370 us instead of 1480); in float32 also no more than 8192 rows, to keep a sum's rounding at that of its
 // slots.
 struct Split {
   int rows;
@@ -411,7 +413,7 @@ struct Split {
 };
 Split dw_split(const LeafProduct& p, int64_t tiles) {
   const int64_t work = (int64_t)p.g.rows * p.g.trees * tiles;
-  int64_t rows = (work / 1024 + 255) / 256 * 256;
+  int64_t rows = (work / (tiles <= 64 ? 2048 : 1024) + 255) / 256 * 256;
   rows = std::max<int64_t>(rows, 512);
   if (p.dtype == LGBM_HIP_DTYPE_F32) rows = std::min<int64_t>(rows, 8192);
   if (rows >= p.g.rows) return {0, 0};
@@ -579,7 +581,7 @@ __global__ __launch_bounds__(THREADS) void k_sum_slots(LeafProduct p, Split spli
   const float* const slots = (const float*)p.ws + tree * split.slots * size;
   for (int64_t e = blockIdx.x % parts * (int64_t)THREADS + threadIdx.x; e < used; e += (int64_t)parts * THREADS) {
     float v = 0.0f;
-#pragma unroll 4
+#pragma unroll 16
     for (int64_t s = from; s < to; ++s) v += slots[s * size + e];
     if (e < map)
       p.dw[at * map + e] = v;

@@ -563,6 +563,41 @@ def captured():
                 assert torch.equal(a, b)
 
 
+def captured_large():
+    """The forms for large tiles, many rows and long rows of scores, replayed from one graph."""
+    be = backend()
+    rng = np.random.default_rng(8)
+    dt = torch.bfloat16
+    leaf = torch.from_numpy(leaves_of(rng, 1300, 2, 3, "lost")).to(DEV).int()
+    x, dy = matrix(rng, 1300, 264, dt), matrix(rng, 1300, 200, dt)
+    w = matrix(rng, 6 * 200, 264, dt).view(6, 200, 264)
+    long_leaf = torch.from_numpy(leaves_of(rng, 30000, 1, 9, "skew")).to(DEV).int()
+    scores = matrix(rng, 5, 20000, torch.float32)
+
+    def run():
+        g = be.leaf_groups(leaf, 3)
+        dw, db = be.leaf_product_dw(dy, x, g)
+        return (be.leaf_product(x, w, g), be.leaf_product_dx(dy, w, g), dw, db,
+                *be.leaf_groups(long_leaf, 9), be.adjust_scores(scores, "transformed"))
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):
+        run()
+    torch.cuda.current_stream().wait_stream(s)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = run()
+    for turn in range(3):
+        x.copy_(matrix(rng, 1300, 264, dt))
+        scores.copy_(matrix(rng, 5, 20000, torch.float32))
+        leaf.copy_(torch.from_numpy(leaves_of(rng, 1300, 2, 3, "lost")).to(DEV).int())
+        graph.replay()
+        want = run()
+        torch.cuda.synchronize()
+        for a, b in zip(out, want):
+            assert torch.equal(a, b)
+
+
 def learner():
     """With the learner: bagged gradients grow a tree, its layout groups the rows, the normal
     equations of linear leaves come from one product, and the fitted leaves lower the squared

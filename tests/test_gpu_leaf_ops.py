@@ -117,7 +117,7 @@ def test_tables(check, what, rows, inputs, outputs, trees, leaves, shape, pad, d
 
 @pytest.mark.parametrize("name", ["differences", "odd_tables", "odd_tables_large", "any_order", "empty", "layouts",
                                   "scores_history", "refused", "own_stream", "side_stream",
-                                  "captured", "threads", "forest", "learner"])
+                                  "captured", "captured_large", "threads", "forest", "learner"])
 def test_plain(check, name):
     check(name)
 
