@@ -405,8 +405,8 @@ __global__ __launch_bounds__(THREADS) void k_sum_few_trees(const float* planes, 
 // differ in size and may be fewer than the CUs, so blocks take about a 2048th of the work (a
 // thousandth is one round of blocks and a few more: ragged leaves of 2M rows, 100 float32
 // inputs, 10 outputs 382 us instead of 283), or of many tiles a thousandth (40000 x 2001 to
-// 2047 bfloat16: 1370 us instead of 1480); in float32 also no more than 8192 rows, to keep a sum's rounding at that of its
-// slots.
+// 2047 bfloat16: 1370 us instead of 1480); in float32 also no more than 8192 rows, to keep
+// a sum's rounding at that of its slots.
 struct Split {
   int rows;
   int64_t slots;  // a tree
@@ -418,6 +418,24 @@ Split dw_split(const LeafProduct& p, int64_t tiles) {
   if (p.dtype == LGBM_HIP_DTYPE_F32) rows = std::min<int64_t>(rows, 8192);
   if (rows >= p.g.rows) return {0, 0};
   return {(int)rows, row_tiles(p.g, rows)};
+}
+
+// What block number `id` of a tile sums, and where to.
+struct DwPart {
+  int tree, first, count;  // count -1: nothing
+  float *dw, *db;
+};
+__device__ __forceinline__ DwPart dw_part(const LeafProduct& p, const Split& split, int id) {
+  const int64_t size = (int64_t)p.outputs * p.inputs;
+  if (split.rows) {
+    const int tree = blockIdx.y;
+    const RowTile rt = find_tile<THREADS>(p.g, tree, id, split.rows);
+    float* const dw = (float*)p.ws + (tree * split.slots + id) * (size + p.outputs);
+    return {tree, rt.first, rt.rows == 0 || rt.leaf < 0 ? -1 : rt.rows, dw, p.db ? dw + size : nullptr};
+  }
+  const int count = min(max(p.g.count[id], 0), p.g.rows);
+  return {id / p.g.leaves, min(max(p.g.begin[id], 0), p.g.rows - count), count, p.dw + id * size,
+          p.db ? p.db + (int64_t)id * p.outputs : nullptr};
 }
 
 // dw[leaf][m][k] = sum over the leaf's rows of dy[row][m] * x[row][k]; db[leaf][m] their sum.
@@ -433,36 +451,23 @@ __global__ __launch_bounds__(THREADS) void k_leaf_dw(LeafProduct p, int m_tiles,
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const int tiles = m_tiles * k_tiles, tile = (int)(blockIdx.x % tiles);
   const int k0 = tile % k_tiles * BN, m0 = tile / k_tiles * BM;
-  const int id = (int)(blockIdx.x / tiles);
-  int tree, first, count;
-  float *dw, *db = nullptr;
-  const int64_t size = (int64_t)p.outputs * p.inputs;
-  if (split.rows) {
-    tree = blockIdx.y;
-    const RowTile rt = find_tile<THREADS>(p.g, tree, id, split.rows);
-    if (rt.rows == 0 || rt.leaf < 0) return;
-    first = rt.first, count = rt.rows;
-    dw = (float*)p.ws + (tree * split.slots + id) * (size + p.outputs);
-    if (p.db) db = dw + size;
-  } else {
-    tree = id / p.g.leaves;
-    count = min(max(p.g.count[id], 0), p.g.rows);
-    first = min(max(p.g.begin[id], 0), p.g.rows - count);
-    dw = p.dw + id * size;
-    if (p.db) db = p.db + (int64_t)id * p.outputs;
-    if (count == 0) {  // the leaf's zeros, in one piece a block
-      const int64_t piece = ((size + tiles - 1) / tiles + 3) / 4 * 4, to = min(size, (tile + 1) * piece);
-      for (int64_t e = tile * piece + tid * 4; e < to; e += THREADS * 4) {
-        if (e + 4 <= to) {
-          const f32x4 none = {0, 0, 0, 0};
-          __builtin_memcpy(dw + e, &none, 16);
-        } else {
-          for (int64_t k = e; k < to; ++k) dw[k] = 0.0f;
-        }
+  const DwPart part_of = dw_part(p, split, (int)(blockIdx.x / tiles));
+  const int tree = part_of.tree, first = part_of.first, count = part_of.count;
+  float *const dw = part_of.dw, *const db = part_of.db;
+  if (count < 0) return;
+  if (count == 0) {  // the leaf's zeros, in one piece a block
+    const int64_t size = (int64_t)p.outputs * p.inputs;
+    const int64_t piece = ((size + tiles - 1) / tiles + 3) / 4 * 4, to = min(size, (tile + 1) * piece);
+    for (int64_t e = tile * piece + tid * 4; e < to; e += THREADS * 4) {
+      if (e + 4 <= to) {
+        const f32x4 none = {0, 0, 0, 0};
+        __builtin_memcpy(dw + e, &none, 16);
+      } else {
+        for (int64_t k = e; k < to; ++k) dw[k] = 0.0f;
       }
-      for (int m = tile * THREADS + tid; db && m < p.outputs; m += tiles * THREADS) db[m] = 0.0f;
-      return;
     }
+    for (int m = tile * THREADS + tid; db && m < p.outputs; m += tiles * THREADS) db[m] = 0.0f;
+    return;
   }
 
   f32x4 acc[WM / 16][WN / 16];
@@ -560,6 +565,83 @@ __global__ __launch_bounds__(THREADS) void k_leaf_dw(LeafProduct p, int m_tiles,
   }
 }
 
+// The same for up to 16 outputs and 16 NB inputs: bound by reading x, so waves take rows of
+// their own straight from memory, 16 neighbouring columns of a row a load, without a barrier
+// until their sums are added (float32, 500000 x 28 to 1 by 5 trees of 31 leaves: 121 us, by
+// k_leaf_dw 273; 1M x 60 to 10 by 63: 86 and 128).
+template <typename T, int NB>
+__global__ __launch_bounds__(THREADS) void k_leaf_dw_small(LeafProduct p, Split split) {
+  constexpr int V = El<T>::V, STEP = 4 * V, UNROLL = 2;
+  __shared__ f32x4 sums[THREADS / 64][NB + 1][64];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, r = lane & 15, q = lane >> 4;
+  const DwPart part_of = dw_part(p, split, (int)blockIdx.x);
+  if (part_of.count < 0) return;
+  f32x4 acc[1][NB + 1];  // the last: with ones
+#pragma unroll
+  for (int j = 0; j <= NB; ++j) acc[0][j] = f32x4{0, 0, 0, 0};
+  // columns behind the last only make results that are not stored
+  const T* const dy = (const T*)p.dy + min(r, p.outputs - 1);
+  const T* x[NB];
+#pragma unroll
+  for (int j = 0; j < NB; ++j) x[j] = (const T*)p.x + min(j * 16 + r, p.inputs - 1);
+  for (int r0 = wave * (STEP * UNROLL); r0 < part_of.count; r0 += THREADS / 64 * (STEP * UNROLL)) {
+    T fa[UNROLL][V], fb[UNROLL][NB][V];
+    int n[UNROLL][V];
+#pragma unroll
+    for (int u = 0; u < UNROLL; ++u)
+#pragma unroll
+      for (int e = 0; e < V; ++e) {
+        const int at = r0 + u * STEP + q * V + e;
+        n[u][e] = at < part_of.count ? row_at(p.g, part_of.tree, part_of.first + at) : -1;
+      }
+#pragma unroll
+    for (int u = 0; u < UNROLL; ++u)
+#pragma unroll
+      for (int e = 0; e < V; ++e) {
+        const int64_t row = max(n[u][e], 0);
+        fa[u][e] = dy[row * p.lddy];
+#pragma unroll
+        for (int j = 0; j < NB; ++j) fb[u][j][e] = x[j][row * p.ldx];
+      }
+    Parts<T, 1, NB + 1> part(acc);
+#pragma unroll
+    for (int u = 0; u < UNROLL; ++u) {
+      u32x4 a, b[NB];
+#pragma unroll
+      for (int e = 0; e < V; ++e) {
+        if (n[u][e] >= 0) continue;
+        fa[u][e] = (T)0.0f;
+#pragma unroll
+        for (int j = 0; j < NB; ++j) fb[u][j][e] = (T)0.0f;
+      }
+      __builtin_memcpy(&a, fa[u], 16);
+#pragma unroll
+      for (int j = 0; j < NB; ++j) {
+        __builtin_memcpy(&b[j], fb[u][j], 16);
+        part.at[0][j] = El<T>::mfma(a, b[j], part.at[0][j]);
+      }
+      if (part_of.db) part.at[0][NB] = El<T>::mfma(El<T>::ones(), a, part.at[0][NB]);
+    }
+    part.add_to(acc);
+  }
+#pragma unroll
+  for (int j = 0; j <= NB; ++j) sums[wave][j][lane] = acc[0][j];
+  __syncthreads();
+  for (int j = wave; j <= NB; j += THREADS / 64) {
+    f32x4 v = sums[0][j][lane];
+#pragma unroll
+    for (int w = 1; w < THREADS / 64; ++w) v += sums[w][j][lane];
+    if (j == NB) {
+      if (part_of.db && lane < p.outputs && lane < 16) part_of.db[lane] = v[0];
+      continue;
+    }
+    const int k = j * 16 + r;
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+      if (q * 4 + e < p.outputs && k < p.inputs) part_of.dw[(q * 4 + e) * p.inputs + k] = v[e];
+  }
+}
+
 // A leaf's slots added in their order, by `parts` blocks a leaf.
 __global__ __launch_bounds__(THREADS) void k_sum_slots(LeafProduct p, Split split, int parts) {
   __shared__ int before[THREADS / 64];
@@ -597,6 +679,7 @@ struct DwShape {
   int bm, bn;
 };
 DwShape dw_shape(const LeafProduct& p) {
+  if (p.outputs <= 16 && p.inputs <= 64) return {16, 64};
   if (p.outputs <= 16) return {16, 128};
   if (p.inputs <= 16) return {128, 16};
   return {64, 64};
@@ -628,11 +711,17 @@ template <typename T, int BM, int BN, int GM>
 void launch_dw(const LeafProduct& p, hipStream_t s) {
   const int mt = (p.outputs + BM - 1) / BM, kt = (p.inputs + BN - 1) / BN;
   const Split split = dw_split(p, (int64_t)mt * kt);
-  if (split.rows == 0) {
-    k_leaf_dw<T, BM, BN, GM><<<(unsigned)((int64_t)mt * kt * p.g.trees * p.g.leaves), THREADS, 0, s>>>(p, mt, kt, split);
-    return;
+  const dim3 grid = split.rows ? dim3((unsigned)(split.slots * mt * kt), p.g.trees)
+                               : dim3((unsigned)((int64_t)mt * kt * p.g.trees * p.g.leaves));
+  if constexpr (BM == 16 && BN == 64) {
+    if (p.inputs <= 32)
+      k_leaf_dw_small<T, 2><<<grid, THREADS, 0, s>>>(p, split);
+    else
+      k_leaf_dw_small<T, 4><<<grid, THREADS, 0, s>>>(p, split);
+  } else {
+    k_leaf_dw<T, BM, BN, GM><<<grid, THREADS, 0, s>>>(p, mt, kt, split);
   }
-  k_leaf_dw<T, BM, BN, GM><<<dim3((unsigned)(split.slots * mt * kt), p.g.trees), THREADS, 0, s>>>(p, mt, kt, split);
+  if (split.rows == 0) return;
   const int64_t size = (int64_t)p.outputs * (p.inputs + 1);
   const int64_t leaves = (int64_t)p.g.trees * p.g.leaves;
   const int parts = (int)std::max<int64_t>(1, std::min((size + THREADS - 1) / THREADS, (1 << 16) / leaves));
@@ -660,7 +749,9 @@ void launch(const LeafProduct& p, int what, hipStream_t s) {
   if (what == LEAF_PRODUCT_DW) {
     if (leaf_big_fits(p, what)) return launch_leaf_big(p, what, s);
     const DwShape d = dw_shape(p);
-    if (d.bm == 16)
+    if (d.bm == 16 && d.bn == 64)
+      launch_dw<T, 16, 64, 1>(p, s);
+    else if (d.bm == 16)
       launch_dw<T, 16, 128, 1>(p, s);
     else if (d.bn == 16)
       launch_dw<T, 128, 16, 4>(p, s);
