@@ -568,10 +568,10 @@ __global__ __launch_bounds__(THREADS) void k_leaf_dw(LeafProduct p, int m_tiles,
 // The same for up to 16 outputs and 16 NB inputs: bound by reading x, so waves take rows of
 // their own straight from memory, 16 neighbouring columns of a row a load, without a barrier
 // until their sums are added (float32, 500000 x 28 to 1 by 5 trees of 31 leaves: 121 us, by
-// k_leaf_dw 273; 1M x 60 to 10 by 63: 86 and 128).
+// k_leaf_dw 273; 1M x 60 to 10 by 63: 86 and 128; 1M x 100 to 10: 135 and 150).
 template <typename T, int NB>
 __global__ __launch_bounds__(THREADS) void k_leaf_dw_small(LeafProduct p, Split split) {
-  constexpr int V = El<T>::V, STEP = 4 * V, UNROLL = 2;
+  constexpr int V = El<T>::V, STEP = 4 * V, UNROLL = NB == 8 ? 1 : 2;
   __shared__ f32x4 sums[THREADS / 64][NB + 1][64];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, r = lane & 15, q = lane >> 4;
   const DwPart part_of = dw_part(p, split, (int)blockIdx.x);
@@ -674,15 +674,17 @@ __global__ __launch_bounds__(THREADS) void k_sum_slots(LeafProduct p, Split spli
 
 // ---- which kernel ------------------------------------------------------------------------------
 
-// The tile of outputs x inputs of a leaf that a block of k_leaf_dw sums.
+// The tile of outputs x inputs of a leaf that a block of k_leaf_dw sums, or the whole of it by
+// k_leaf_dw_small (1M rows of 128 float16 inputs to 1 by that: 72 us instead of 59, so 16
+// bits stop at 64).
 struct DwShape {
   int bm, bn;
+  bool small;
 };
 DwShape dw_shape(const LeafProduct& p) {
-  if (p.outputs <= 16 && p.inputs <= 64) return {16, 64};
-  if (p.outputs <= 16) return {16, 128};
-  if (p.inputs <= 16) return {128, 16};
-  return {64, 64};
+  if (p.outputs <= 16) return {16, 128, p.inputs <= (p.dtype == LGBM_HIP_DTYPE_F32 ? 128 : 64)};
+  if (p.inputs <= 16) return {128, 16, false};
+  return {64, 64, false};
 }
 
 // Leaves of 16 rows at most, on average.
@@ -707,23 +709,28 @@ bool wide_tiles(const LeafProduct& p, int cols) {
          (int64_t)p.g.rows / 128 * ((cols + 127) / 128) * p.g.trees >= 256;
 }
 
-template <typename T, int BM, int BN, int GM>
+template <typename T>
 void launch_dw(const LeafProduct& p, hipStream_t s) {
-  const int mt = (p.outputs + BM - 1) / BM, kt = (p.inputs + BN - 1) / BN;
+  const DwShape d = dw_shape(p);
+  const int mt = (p.outputs + d.bm - 1) / d.bm, kt = (p.inputs + d.bn - 1) / d.bn;
   const Split split = dw_split(p, (int64_t)mt * kt);
+  const int64_t leaves = (int64_t)p.g.trees * p.g.leaves;
   const dim3 grid = split.rows ? dim3((unsigned)(split.slots * mt * kt), p.g.trees)
-                               : dim3((unsigned)((int64_t)mt * kt * p.g.trees * p.g.leaves));
-  if constexpr (BM == 16 && BN == 64) {
-    if (p.inputs <= 32)
-      k_leaf_dw_small<T, 2><<<grid, THREADS, 0, s>>>(p, split);
-    else
-      k_leaf_dw_small<T, 4><<<grid, THREADS, 0, s>>>(p, split);
-  } else {
-    k_leaf_dw<T, BM, BN, GM><<<grid, THREADS, 0, s>>>(p, mt, kt, split);
-  }
+                               : dim3((unsigned)((int64_t)mt * kt * leaves));
+  if (d.small && p.inputs <= 32)
+    k_leaf_dw_small<T, 2><<<grid, THREADS, 0, s>>>(p, split);
+  else if (d.small && p.inputs <= 64)
+    k_leaf_dw_small<T, 4><<<grid, THREADS, 0, s>>>(p, split);
+  else if (d.small && sizeof(T) == 4)
+    k_leaf_dw_small<float, 8><<<grid, THREADS, 0, s>>>(p, split);
+  else if (d.bm == 16)
+    k_leaf_dw<T, 16, 128, 1><<<grid, THREADS, 0, s>>>(p, mt, kt, split);
+  else if (d.bn == 16)
+    k_leaf_dw<T, 128, 16, 4><<<grid, THREADS, 0, s>>>(p, mt, kt, split);
+  else
+    k_leaf_dw<T, 64, 64, 2><<<grid, THREADS, 0, s>>>(p, mt, kt, split);
   if (split.rows == 0) return;
   const int64_t size = (int64_t)p.outputs * (p.inputs + 1);
-  const int64_t leaves = (int64_t)p.g.trees * p.g.leaves;
   const int parts = (int)std::max<int64_t>(1, std::min((size + THREADS - 1) / THREADS, (1 << 16) / leaves));
   k_sum_slots<<<(unsigned)(leaves * parts), THREADS, 0, s>>>(p, split, parts);
 }
@@ -748,16 +755,7 @@ template <typename T>
 void launch(const LeafProduct& p, int what, hipStream_t s) {
   if (what == LEAF_PRODUCT_DW) {
     if (leaf_big_fits(p, what)) return launch_leaf_big(p, what, s);
-    const DwShape d = dw_shape(p);
-    if (d.bm == 16 && d.bn == 64)
-      launch_dw<T, 16, 64, 1>(p, s);
-    else if (d.bm == 16)
-      launch_dw<T, 16, 128, 1>(p, s);
-    else if (d.bn == 16)
-      launch_dw<T, 128, 16, 4>(p, s);
-    else
-      launch_dw<T, 64, 64, 2>(p, s);
-    return;
+    return launch_dw<T>(p, s);
   }
   const bool dx = what == LEAF_PRODUCT_DX;
   const int cols = dx ? p.inputs : p.outputs;
