@@ -126,7 +126,8 @@ __global__ __launch_bounds__(THREADS, 1) void k_leaf_big(LeafProduct p, int col_
     if (DW) {
       const int of = (p.outputs + BM - 1) / BM * col_tiles, tile = (int)(blockIdx.x % of);
       leaf = blockIdx.x / of;
-      if (p.g.trees * (int64_t)p.g.leaves <= THREADS) leaf = leaf_of_rank(p.g, p.g.trees * p.g.leaves, (int)leaf);
+      if (p.g.trees * (int64_t)p.g.leaves <= THREADS)
+        leaf = leaf_of_rank(p.g, p.g.trees * p.g.leaves, (int)leaf);
       tree = (int)(leaf / p.g.leaves);
       length = min(max(p.g.count[leaf], 0), p.g.rows);
       first = min(max(p.g.begin[leaf], 0), p.g.rows - length);
@@ -169,7 +170,7 @@ __global__ __launch_bounds__(THREADS, 1) void k_leaf_big(LeafProduct p, int col_
     // from LDS, and every lane adds its column.  Columns behind the last only make results
     // that are not stored, so they read the last ones.
     const int half = lane >> 5, op = (lane >> 4) & 1;
-    const uint64_t base_of_op = op ? (uint64_t)(uintptr_t)((const T*)p.x + c0) : (uint64_t)(uintptr_t)((const T*)p.dy + m0);
+    const T* const base = op ? (const T*)p.x + c0 : (const T*)p.dy + m0;
     const uint32_t ld_of_op = (uint32_t)(op ? p.ldx : p.lddy) * 2;
     const uint32_t a_col = (uint32_t)(min(m0 + (lane & 31) * 8, p.outputs - 8) - m0) * 2;
     const uint32_t b_col = (uint32_t)(min(c0 + (lane & 31) * 8, cols - 8) - c0) * 2;
@@ -178,7 +179,7 @@ __global__ __launch_bounds__(THREADS, 1) void k_leaf_big(LeafProduct p, int col_
     };
     auto put_rows = [&](int n, int k0) {
       const bool there = k0 + wave * 16 + (lane & 15) < length && (uint32_t)n < (uint32_t)p.g.rows;
-      const uint64_t at = base_of_op + (uint64_t)(uint32_t)n * ld_of_op;
+      const uint64_t at = (uint64_t)(uintptr_t)base + (uint64_t)(uint32_t)n * ld_of_op;
       rows_at[DW ? wave : 0][DW ? lane & 15 : 0][op] = there ? at : (uint64_t)(uintptr_t)zeros;
     };
     auto get_rows = [&](int j) { return *(const u64x2*)rows_at[DW ? wave : 0][DW ? 2 * j + half : 0]; };

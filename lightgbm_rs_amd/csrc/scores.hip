@@ -14,6 +14,8 @@
 //  - more: chunks of a row, each in a block's registers.  For probabilities the chunks'
 //    maxima and sums are written first (PART) and every chunk is read again to be
 //    written (FINISH); its second read mostly hits the caches.
+// 2M x 10 float64 to probabilities 94 us (3.5 TB/s); 64 x 128007 bfloat16 with histories of 1000 ids
+// 37 us, most of it the latency of two launches.
 // Counts of a row's history are whole numbers in LDS; a chunk looks at the whole history
 // and counts its own classes.
 #include <algorithm>

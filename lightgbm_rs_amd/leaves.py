@@ -290,8 +290,11 @@ def _dropout(self, x, p, seed, offset=0, by="element", out=None):
     dtype = _dtype(x, "x")
     _here(self, x=x, out=out)
     if x.dim() == 1:
-        return _dropout(self, x[:, None], p, seed, offset, by,
-                        None if out is None else out[:, None])[:, 0]
+        if out is not None:
+            _shape(out, x.shape, "out")
+            _dropout(self, x[:, None], p, seed, offset, by, out[:, None])
+            return out
+        return _dropout(self, x[:, None], p, seed, offset, by)[:, 0]
     inplace = out is x
     src = _rows(x)
     if inplace and src is not x:

@@ -258,6 +258,12 @@ def dropout(rows, cols, p, by="element", dtype="f32", pad=0, seed=1, offset=0):
     inner = room[:, 1:1 + cols]
     assert be.dropout(inner, p, seed, offset, by=by, out=inner) is inner
     assert torch.equal(inner, want) and bool((room[:, 0] == 7).all()) and bool((room[:, 1 + cols:] == 7).all())
+    if cols == 1 or by == "element":  # a vector, in place as well
+        line = bad.reshape(-1)
+        flat = want.reshape(-1)
+        assert torch.equal(be.dropout(line, p, seed, offset, by=by), flat)
+        assert be.dropout(line, p, seed, offset, by=by, out=line) is line
+        assert torch.equal(line, flat)
 
 
 def dropout_far():
