@@ -80,29 +80,51 @@ __device__ __forceinline__ u32x4 cm_frag32(const char* tile, int base, int step,
   return out;
 }
 
-// The leaf of the forest that is the `rank`-th by rows, of at most THREADS: the long blocks
-// begin first, and the short ones fill the end (both gradients of two trees of 15 leaves, 16389 rows
+// The part of the gradients that is the `rank`-th by rows, in a forest of at most THREADS
+// leaves: whole parts first, then the leaves' ends by their length.  So the long blocks begin
+// first, and the short ones fill the end (both gradients of two trees of 15 leaves, 16389 rows
 // of 2048 to 2048: 824 us in their order, 789).
-__device__ __forceinline__ int leaf_of_rank(const LeafGroups& g, int leaves, int rank) {
-  __shared__ int counts[THREADS];
-  __shared__ int found;
-  const int tid = threadIdx.x, mine = tid < leaves ? g.count[tid] : 0;
-  counts[tid] = mine;
+__device__ __forceinline__ DwPart part_of_rank(const LeafProduct& p, const Split& split, int rank) {
+  __shared__ int fulls[THREADS], ends[THREADS];
+  __shared__ int found[4];  // leaf of the forest, -1: none; first row, rows, slot
+  const int tid = threadIdx.x, leaves = p.g.trees * p.g.leaves, tree0 = tid / p.g.leaves * p.g.leaves;
+  const int count = tid < leaves ? min(max(p.g.count[tid], 0), p.g.rows) : 0;
+  const int full = split.rows ? count / split.rows : 0, end = count - full * split.rows;
+  fulls[tid] = full, ends[tid] = end;
+  if (tid == 0) found[0] = -1;
   __syncthreads();
-  int before = 0;
+  int longer = 0, before = 0, all = 0, slot = 0;
 #pragma unroll 8
-  for (int l = 0; l < leaves; ++l) before += counts[l] > mine || (counts[l] == mine && l < tid);
-  if (tid < leaves && before == rank) found = tid;
+  for (int l = 0; l < leaves; ++l) {
+    const int f = fulls[l], e = ends[l];
+    longer += e > end || (e == end && l < tid);
+    all += f;
+    before += l < tid ? f : 0;
+    slot += l >= tree0 && l < tid ? f + (e > 0) : 0;
+  }
+  // a leaf without rows is a part where leaves are not split: its zeros
+  const bool in_full = rank >= before && rank < before + full;
+  if (tid < leaves && (in_full || (rank == all + longer && (end > 0 || split.rows == 0)))) {
+    const int skip = in_full ? rank - before : full;
+    found[0] = tid;
+    found[1] = min(max(p.g.begin[tid], 0), p.g.rows - count) + skip * split.rows;
+    found[2] = in_full ? split.rows : end;
+    found[3] = slot + skip;
+  }
   __syncthreads();
-  return found;
+  const int at = __builtin_amdgcn_readfirstlane(found[0]);
+  // a table whose counts exceed its rows may ask for more slots than there are
+  if (at < 0 || (split.rows && found[3] >= split.slots)) return {0, 0, -1, nullptr, nullptr};
+  return dw_part_of(p, split, at / p.g.leaves, at % p.g.leaves, __builtin_amdgcn_readfirstlane(found[1]),
+                    __builtin_amdgcn_readfirstlane(found[2]), __builtin_amdgcn_readfirstlane(found[3]));
 }
 
 // MODE LEAF_PRODUCT_Y: a = x rows [k], b = w[leaf] [col][k]; _DX: a = dy rows [m], b = w[leaf]
 // [m][col]; _DW: a = dy [row][m], b = x [row][k] over a leaf's rows.  Y and DX: one block a
 // CU takes tile after tile, so that what it stores drains while the next tile begins; DW:
-// a block a tile, since leaves differ in length.
+// a block a tile of a part, since leaves differ in length.
 template <typename T, int MODE>
-__global__ __launch_bounds__(THREADS, 1) void k_leaf_big(LeafProduct p, int col_tiles) {
+__global__ __launch_bounds__(THREADS, 1) void k_leaf_big(LeafProduct p, int col_tiles, Split split) {
   constexpr bool DW = MODE == LEAF_PRODUCT_DW, ACM = DW, BCM = MODE != LEAF_PRODUCT_Y;
   constexpr int FM = WM / 32, FN = WN / 32, STEPS = BK / 16, ITEMS = STEPS * FM, RING = 4;
   constexpr int TURN = ITEMS - 2;
@@ -123,14 +145,16 @@ __global__ __launch_bounds__(THREADS, 1) void k_leaf_big(LeafProduct p, int col_
     // the block's part of the result, and the length of the contraction
     int tree = tree_y, first = 0, length, m0 = 0, c0, cols;
     int64_t leaf;
+    DwPart part{};
     if (DW) {
       const int of = (p.outputs + BM - 1) / BM * col_tiles, tile = (int)(blockIdx.x % of);
-      leaf = blockIdx.x / of;
-      if (p.g.trees * (int64_t)p.g.leaves <= THREADS)
-        leaf = leaf_of_rank(p.g, p.g.trees * p.g.leaves, (int)leaf);
-      tree = (int)(leaf / p.g.leaves);
-      length = min(max(p.g.count[leaf], 0), p.g.rows);
-      first = min(max(p.g.begin[leaf], 0), p.g.rows - length);
+      const int id = (int)(blockIdx.x / of);
+      part = p.g.trees * (int64_t)p.g.leaves <= THREADS
+                 ? part_of_rank(p, split, (int)(blockIdx.y * split.slots) + id)
+                 : dw_part<THREADS>(p, split, id);
+      if (part.count < 0) return;
+      tree = part.tree, first = part.first, length = part.count;
+      leaf = 0;
       m0 = tile / col_tiles * BM, c0 = tile % col_tiles * BN, cols = p.inputs;
     } else {
       length = MODE == LEAF_PRODUCT_Y ? p.inputs : p.outputs;
@@ -245,7 +269,7 @@ __global__ __launch_bounds__(THREADS, 1) void k_leaf_big(LeafProduct p, int col_
     int next_rows = 0;  // DW: what put_rows takes next
     // sums of dy's columns cost as much again as what else the matrix instructions hide: only
     // the blocks of the first columns make them
-    const bool sums = DW && p.db && c0 == 0;
+    const bool sums = DW && part.db && c0 == 0;
     // A stage is 16 items: a fragment of rows times the four of columns, for each 16 of the
     // stage's contraction.  Fragments of rows are read three items ahead, the columns' four.
     // During items 0 to 11 the next stage goes from registers to the other buffer, and the
@@ -275,8 +299,8 @@ __global__ __launch_bounds__(THREADS, 1) void k_leaf_big(LeafProduct p, int col_
         if (DW && sums) {
           T e[8];
           __builtin_memcpy(e, &f, 16);
-#pragma unroll
-          for (int k = 0; k < 8; ++k) bias[DW ? i : 0] += (float)e[k];
+          bias[DW ? i : 0] += (((float)e[0] + (float)e[1]) + ((float)e[2] + (float)e[3])) +
+                              (((float)e[4] + (float)e[5]) + ((float)e[6] + (float)e[7]));
         }
         if (share_of(t) >= 0) {
           const int l = share_of(t);
@@ -358,13 +382,12 @@ __global__ __launch_bounds__(THREADS, 1) void k_leaf_big(LeafProduct p, int col_
     // us instead of 32).
     const int col0 = c0 + wn + (lane & 31), row4 = (lane >> 5) * 4;
     if (DW) {
-      float* const dw = p.dw + leaf * p.outputs * (int64_t)p.inputs;
 #pragma unroll
       for (int i = 0; i < FM; ++i) {
         const int mi = m0 + wm + i * 32;
         if (sums && wn == 0) {
           const float b = bias[DW ? i : 0] + __shfl_xor(bias[DW ? i : 0], 32);
-          if (lane < 32 && mi + lane < p.outputs) p.db[leaf * p.outputs + mi + lane] = b;
+          if (lane < 32 && mi + lane < p.outputs) part.db[mi + lane] = b;
         }
 #pragma unroll
         for (int e = 0; e < 16; ++e) {
@@ -372,7 +395,7 @@ __global__ __launch_bounds__(THREADS, 1) void k_leaf_big(LeafProduct p, int col_
           if (m >= p.outputs) continue;
 #pragma unroll
           for (int j = 0; j < FN; ++j)
-            if (col0 + j * 32 < cols) dw[(int64_t)m * cols + col0 + j * 32] = acc[i][j][e];
+            if (col0 + j * 32 < cols) part.dw[(int64_t)m * cols + col0 + j * 32] = acc[i][j][e];
         }
       }
       return;
@@ -415,20 +438,32 @@ __global__ __launch_bounds__(THREADS, 1) void k_leaf_big(LeafProduct p, int col_
 template <typename T>
 void launch(const LeafProduct& p, int what, hipStream_t s) {
   const int cols = what == LEAF_PRODUCT_Y ? p.outputs : p.inputs, ct = (cols + BN - 1) / BN;
-  const dim3 grid((unsigned)leaf_big_blocks(p, what), what == LEAF_PRODUCT_DW ? 1u : (unsigned)p.g.trees);
+  const Split split = what == LEAF_PRODUCT_DW ? leaf_big_split(p) : Split{0, 0};
+  const dim3 grid((unsigned)leaf_big_blocks(p, what),
+                  what == LEAF_PRODUCT_DW && split.rows == 0 ? 1u : (unsigned)p.g.trees);
   if (what == LEAF_PRODUCT_Y)
-    k_leaf_big<T, LEAF_PRODUCT_Y><<<grid, THREADS, 0, s>>>(p, ct);
+    k_leaf_big<T, LEAF_PRODUCT_Y><<<grid, THREADS, 0, s>>>(p, ct, split);
   else if (what == LEAF_PRODUCT_DX)
-    k_leaf_big<T, LEAF_PRODUCT_DX><<<grid, THREADS, 0, s>>>(p, ct);
+    k_leaf_big<T, LEAF_PRODUCT_DX><<<grid, THREADS, 0, s>>>(p, ct, split);
   else
-    k_leaf_big<T, LEAF_PRODUCT_DW><<<grid, THREADS, 0, s>>>(p, ct);
+    k_leaf_big<T, LEAF_PRODUCT_DW><<<grid, THREADS, 0, s>>>(p, ct, split);
 }
 
 }  // namespace
 
+// Rows a block of the maps' gradients sums at most.
+Split leaf_big_split(const LeafProduct& p) {
+  const int64_t rows = CHAIN_ROWS;
+  if (rows >= p.g.rows) return {0, 0};
+  return {(int)rows, row_tiles(p.g, rows)};
+}
+
 int64_t leaf_big_blocks(const LeafProduct& p, int what) {
   const int64_t ct = ((what == LEAF_PRODUCT_Y ? p.outputs : p.inputs) + BN - 1) / BN;
-  if (what == LEAF_PRODUCT_DW) return (p.outputs + BM - 1) / BM * ct * p.g.trees * p.g.leaves;
+  if (what == LEAF_PRODUCT_DW) {
+    const Split split = leaf_big_split(p);
+    return (p.outputs + BM - 1) / BM * ct * (split.rows ? split.slots : (int64_t)p.g.trees * p.g.leaves);
+  }
   return std::min<int64_t>((row_tiles(p.g, BM) * ct + 7) / 8 * 8, 256);  // one a CU
 }
 

@@ -54,8 +54,9 @@ struct El<_Float16> {
 
 // The sums of a stretch of the contraction.  In float32 they start at zero and are added to
 // the whole ones afterwards, so that a rounding is of a short sum's size: a chain over 1000
-// elements was off by ten times as much.  With 16-bit operands the rounding of the result
-// hides that, and the stretch goes on in place.
+// elements was off by ten times as much.  With 16-bit operands the stretch goes on in place:
+// the rounding of y and dx hides that, and the gradients of the maps, float32 whatever
+// their operands, add no more than Split's rows in one chain.
 template <typename T, int M, int N>
 struct Parts {
   f32x4 (&at)[M][N];
@@ -215,6 +216,46 @@ __device__ __forceinline__ int row_at(const LeafGroups& g, int tree, int positio
   return n >= 0 && n < g.rows ? n : -1;
 }
 
+// ---- parts of the maps' gradients --------------------------------------------------------------
+
+// Rows a block sums at most, 0: a leaf's rows are not split.  The sums of a leaf of more rows
+// go to slots in the workspace, [tree][slots][outputs * inputs + outputs], in the order of
+// find_tile's tiles, and k_sum_slots adds them; a leaf of one part has its place in dw.
+struct Split {
+  int rows;
+  int64_t slots;  // a tree
+};
+
+// The longest chain of float32 adds over rows: the running sum's rounding is 8192 terms' at
+// most (600000 rows of the same bfloat16 value in one chain were off by 4 in 1000).
+constexpr int64_t CHAIN_ROWS = 8192;
+
+// What a block sums, and where to.
+struct DwPart {
+  int tree, first, count;  // count -1: nothing
+  float *dw, *db;
+};
+// `rows` from `first` on of a leaf, its slot-th part of the tree's.
+__device__ __forceinline__ DwPart dw_part_of(const LeafProduct& p, const Split& split, int tree, int leaf, int first,
+                                             int rows, int64_t slot) {
+  const int64_t size = (int64_t)p.outputs * p.inputs, at = (int64_t)tree * p.g.leaves + leaf;
+  const bool whole = split.rows == 0 || min(max(p.g.count[at], 0), p.g.rows) <= split.rows;
+  float* const dw = whole ? p.dw + at * size : (float*)p.ws + (tree * split.slots + slot) * (size + p.outputs);
+  return {tree, first, rows, dw, !p.db ? nullptr : whole ? p.db + at * p.outputs : dw + size};
+}
+// Part number `id`: of tree blockIdx.y where leaves are split, else a leaf of the forest.
+template <int THREADS>
+__device__ __forceinline__ DwPart dw_part(const LeafProduct& p, const Split& split, int id) {
+  if (split.rows) {
+    const RowTile rt = find_tile<THREADS>(p.g, blockIdx.y, id, split.rows);
+    if (rt.rows == 0 || rt.leaf < 0) return {0, 0, -1, nullptr, nullptr};
+    return dw_part_of(p, split, blockIdx.y, rt.leaf, rt.first, rt.rows, id);
+  }
+  const int count = min(max(p.g.count[id], 0), p.g.rows);
+  return dw_part_of(p, split, id / p.g.leaves, id % p.g.leaves, min(max(p.g.begin[id], 0), p.g.rows - count), count,
+                    0);
+}
+
 // The results v of column col in rows n[0 .. 4) (-1: none), to the output of one tree or to a
 // tree's plane.  Neighbouring lanes have neighbouring columns, so that a store's lanes fill
 // pieces of a row: lanes of different rows side by side make a request of every lane's bytes
@@ -312,4 +353,7 @@ __device__ __forceinline__ u32x4 cm_frag(const char* tile, int col0, int step, i
 }
 
 }  // namespace mma
+
+mma::Split leaf_big_split(const LeafProduct& p);  // leaf_big.hip: of the maps' gradients
+
 }  // namespace lgbm

@@ -405,42 +405,16 @@ __global__ __launch_bounds__(THREADS) void k_sum_few_trees(const float* planes, 
 
 // ---- gradients of the maps -------------------------------------------------------------------
 
-// Rows a block sums at most, 0: a leaf's rows are not split.  Split sums go to slots in the
-// workspace, [tree][slots][outputs * inputs + outputs], and k_sum_slots adds them.  Leaves
-// differ in size and may be fewer than the CUs, so blocks take about a 2048th of the work (a
-// thousandth is one round of blocks and a few more: ragged leaves of 2M rows, 100 float32
+// Leaves differ in size and may be fewer than the CUs, so blocks take about a 2048th of the
+// work (a thousandth is one round of blocks and a few more: ragged leaves of 2M rows, 100 float32
 // inputs, 10 outputs 382 us instead of 283), or of many tiles a thousandth (40000 x 2001 to
-// 2047 bfloat16: 1370 us instead of 1480); in float32 also no more than 8192 rows, to keep
-// a sum's rounding at that of its slots.
-struct Split {
-  int rows;
-  int64_t slots;  // a tree
-};
+// 2047 bfloat16: 1370 us instead of 1480).
 Split dw_split(const LeafProduct& p, int64_t tiles) {
   const int64_t work = (int64_t)p.g.rows * p.g.trees * tiles;
   int64_t rows = (work / (tiles <= 64 ? 2048 : 1024) + 255) / 256 * 256;
-  rows = std::max<int64_t>(rows, 512);
-  if (p.dtype == LGBM_HIP_DTYPE_F32) rows = std::min<int64_t>(rows, 8192);
+  rows = std::min<int64_t>(std::max<int64_t>(rows, 512), CHAIN_ROWS);
   if (rows >= p.g.rows) return {0, 0};
   return {(int)rows, row_tiles(p.g, rows)};
-}
-
-// What block number `id` of a tile sums, and where to.
-struct DwPart {
-  int tree, first, count;  // count -1: nothing
-  float *dw, *db;
-};
-__device__ __forceinline__ DwPart dw_part(const LeafProduct& p, const Split& split, int id) {
-  const int64_t size = (int64_t)p.outputs * p.inputs;
-  if (split.rows) {
-    const int tree = blockIdx.y;
-    const RowTile rt = find_tile<THREADS>(p.g, tree, id, split.rows);
-    float* const dw = (float*)p.ws + (tree * split.slots + id) * (size + p.outputs);
-    return {tree, rt.first, rt.rows == 0 || rt.leaf < 0 ? -1 : rt.rows, dw, p.db ? dw + size : nullptr};
-  }
-  const int count = min(max(p.g.count[id], 0), p.g.rows);
-  return {id / p.g.leaves, min(max(p.g.begin[id], 0), p.g.rows - count), count, p.dw + id * size,
-          p.db ? p.db + (int64_t)id * p.outputs : nullptr};
 }
 
 // dw[leaf][m][k] = sum over the leaf's rows of dy[row][m] * x[row][k]; db[leaf][m] their sum.
@@ -458,7 +432,7 @@ __global__ __launch_bounds__(THREADS) void k_leaf_dw(LeafProduct p, int m_tiles,
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const int tiles = m_tiles * k_tiles, tile = (int)(blockIdx.x % tiles);
   const int k0 = tile % k_tiles * BN, m0 = tile / k_tiles * BM;
-  const DwPart part_of = dw_part(p, split, (int)(blockIdx.x / tiles));
+  const DwPart part_of = dw_part<THREADS>(p, split, (int)(blockIdx.x / tiles));
   const int tree = part_of.tree, first = part_of.first, count = part_of.count;
   float *const dw = part_of.dw, *const db = part_of.db;
   if (count < 0) return;
@@ -581,7 +555,7 @@ __global__ __launch_bounds__(THREADS) void k_leaf_dw_small(LeafProduct p, Split 
   constexpr int V = El<T>::V, STEP = 4 * V, UNROLL = NB == 8 ? 1 : 2;
   __shared__ f32x4 sums[THREADS / 64][NB + 1][64];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, r = lane & 15, q = lane >> 4;
-  const DwPart part_of = dw_part(p, split, (int)blockIdx.x);
+  const DwPart part_of = dw_part<THREADS>(p, split, (int)blockIdx.x);
   if (part_of.count < 0) return;
   f32x4 acc[1][NB + 1];  // the last: with ones
 #pragma unroll
@@ -649,12 +623,15 @@ __global__ __launch_bounds__(THREADS) void k_leaf_dw_small(LeafProduct p, Split 
   }
 }
 
-// A leaf's slots added in their order, by `parts` blocks a leaf.
+// The slots of a leaf of several parts added in their order, by `parts` blocks a leaf, in
+// float64: a long leaf has hundreds.  A leaf without rows gets its zeros here.
 __global__ __launch_bounds__(THREADS) void k_sum_slots(LeafProduct p, Split split, int parts) {
   __shared__ int before[THREADS / 64];
   const int64_t at = blockIdx.x / parts;  // leaf of the forest
   const int tree = (int)(at / p.g.leaves), leaf = (int)(at - (int64_t)tree * p.g.leaves);
   const int32_t* const counts = p.g.count + (int64_t)tree * p.g.leaves;
+  const int64_t num = ((int64_t)min(max(counts[leaf], 0), p.g.rows) + split.rows - 1) / split.rows;
+  if (num == 1) return;
   int tiles = 0;
   for (int l = threadIdx.x; l < leaf; l += THREADS)
     tiles += (int)(((int64_t)min(max(counts[l], 0), p.g.rows) + split.rows - 1) / split.rows);
@@ -663,19 +640,18 @@ __global__ __launch_bounds__(THREADS) void k_sum_slots(LeafProduct p, Split spli
   if ((threadIdx.x & 63) == 0) before[threadIdx.x >> 6] = tiles;
   __syncthreads();
   const int64_t from = (int64_t)before[0] + before[1] + before[2] + before[3];
-  const int64_t num = ((int64_t)min(max(counts[leaf], 0), p.g.rows) + split.rows - 1) / split.rows;
   const int64_t to = min(from + num, split.slots);
   const int64_t map = (int64_t)p.outputs * p.inputs, size = map + p.outputs;
   const int64_t used = p.db ? size : map;
   const float* const slots = (const float*)p.ws + tree * split.slots * size;
   for (int64_t e = blockIdx.x % parts * (int64_t)THREADS + threadIdx.x; e < used; e += (int64_t)parts * THREADS) {
-    float v = 0.0f;
+    double v = 0.0;
 #pragma unroll 16
-    for (int64_t s = from; s < to; ++s) v += slots[s * size + e];
+    for (int64_t s = from; s < to; ++s) v += (double)slots[s * size + e];
     if (e < map)
-      p.dw[at * map + e] = v;
+      p.dw[at * map + e] = (float)v;
     else
-      p.db[at * p.outputs + (e - map)] = v;
+      p.db[at * p.outputs + (e - map)] = (float)v;
   }
 }
 
@@ -716,6 +692,14 @@ bool wide_tiles(const LeafProduct& p, int cols) {
          (int64_t)p.g.rows / 128 * ((cols + 127) / 128) * p.g.trees >= 256;
 }
 
+// Leaves of one part leave most of the blocks without work (bfloat16, 60000 x 256 to 256 by 300
+// leaves: 88 us of all the kernels by 2^16 blocks, 55 by 2^13).
+void sum_slots(const LeafProduct& p, const Split& split, hipStream_t s) {
+  const int64_t leaves = (int64_t)p.g.trees * p.g.leaves, size = (int64_t)p.outputs * (p.inputs + 1);
+  const int parts = (int)std::max<int64_t>(1, std::min((size + THREADS - 1) / THREADS, (1 << 13) / leaves));
+  k_sum_slots<<<(unsigned)(leaves * parts), THREADS, 0, s>>>(p, split, parts);
+}
+
 template <typename T>
 void launch_dw(const LeafProduct& p, hipStream_t s) {
   const DwShape d = dw_shape(p);
@@ -736,10 +720,7 @@ void launch_dw(const LeafProduct& p, hipStream_t s) {
     k_leaf_dw<T, 128, 16, 4><<<grid, THREADS, 0, s>>>(p, mt, kt, split);
   else
     k_leaf_dw<T, 64, 64, 2><<<grid, THREADS, 0, s>>>(p, mt, kt, split);
-  if (split.rows == 0) return;
-  const int64_t size = (int64_t)p.outputs * (p.inputs + 1);
-  const int parts = (int)std::max<int64_t>(1, std::min((size + THREADS - 1) / THREADS, (1 << 16) / leaves));
-  k_sum_slots<<<(unsigned)(leaves * parts), THREADS, 0, s>>>(p, split, parts);
+  if (split.rows) sum_slots(p, split, s);
 }
 
 template <typename T, bool DX, int BM, int BN>
@@ -761,8 +742,11 @@ void launch_tiles(const LeafProduct& p, int cols, hipStream_t s) {
 template <typename T>
 void launch(const LeafProduct& p, int what, hipStream_t s) {
   if (what == LEAF_PRODUCT_DW) {
-    if (leaf_big_fits(p, what)) return launch_leaf_big(p, what, s);
-    return launch_dw<T>(p, s);
+    if (!leaf_big_fits(p, what)) return launch_dw<T>(p, s);
+    launch_leaf_big(p, what, s);
+    const Split split = leaf_big_split(p);
+    if (split.rows) sum_slots(p, split, s);
+    return;
   }
   const bool dx = what == LEAF_PRODUCT_DX;
   const int cols = dx ? p.inputs : p.outputs;
@@ -815,7 +799,10 @@ size_t leaf_product_workspace(const LeafProduct& p, int what) {
     // whatever the pointers' alignment, which may turn the large tiles down
     const DwShape d = dw_shape(p);
     const Split split = dw_split(p, (int64_t)((p.outputs + d.bm - 1) / d.bm) * ((p.inputs + d.bn - 1) / d.bn));
-    return (size_t)p.g.trees * (size_t)split.slots * (size_t)p.outputs * (size_t)(p.inputs + 1) * 4;
+    LeafProduct any = p;
+    any.x = any.dy = nullptr, any.ldx = any.lddy = 0;
+    const int64_t slots = std::max(split.slots, leaf_big_fits(any, what) ? leaf_big_split(any).slots : 0);
+    return (size_t)p.g.trees * (size_t)slots * (size_t)p.outputs * (size_t)(p.inputs + 1) * 4;
   }
   if (p.g.trees <= 1) return 0;
   return (size_t)p.g.trees * (size_t)p.g.rows * (size_t)(what == LEAF_PRODUCT_DX ? p.inputs : p.outputs) * 4;

@@ -738,3 +738,34 @@ def refused():
         except HipError:
             continue
         raise AssertionError("not refused")
+
+
+def whole_dw(rows, inputs, outputs, trees, leaves, dtype, shape):
+    """Gradients of the maps of whole numbers: every sum is exact, whatever its order, so the
+    result has to be the oracle's bit for bit."""
+    assert 25 * rows <= 2 ** 24
+    rng = np.random.default_rng(rows)
+    leaf = leaves_of(rng, rows, trees, leaves, shape)
+    g = LeafGroups(*(torch.from_numpy(v).to(DEV) for v in oracle.groups(leaf, leaves)))
+    x, dy = oracle.whole_numbers(rng, rows, inputs), oracle.whole_numbers(rng, rows, outputs)
+    up = lambda v: torch.from_numpy(v).to(TYPES[dtype]).to(DEV)
+    dw, db = backend().leaf_product_dw(up(dy), up(x), g)
+    w_want, _, b_want, _ = oracle.product_dw(dy, x, leaf, leaves)
+    assert w_want.any() and np.array_equal(wide(dw), w_want) and np.array_equal(wide(db), b_want)
+
+
+def long_sums(rows, inputs, outputs, dtype):
+    """A leaf of many rows, all alike: x = dy = 1 + 2^-5 makes products of 1 + 2^-4 + 2^-10.
+    Of at most 8192 rows every partial sum is a whole number of 2^-10 and below 2^14, so it is
+    exact in float32's 24 bits, and so are their sums in float64: the result is the exact one,
+    rounded once.  (One chain of float32 adds drops the low bits of every term.)"""
+    dt = TYPES[dtype]
+    g = LeafGroups(torch.arange(rows, dtype=torch.int32, device=DEV)[None],
+                   torch.zeros((1, 1), dtype=torch.int32, device=DEV),
+                   torch.full((1, 1), rows, dtype=torch.int32, device=DEV))
+    x = torch.full((rows, inputs), 1 + 2.0 ** -5, dtype=dt, device=DEV)
+    dy = torch.full((rows, outputs), 1 + 2.0 ** -5, dtype=dt, device=DEV)
+    dw, db = backend().leaf_product_dw(dy, x, g)
+    w_want, b_want = np.float32(rows * (1 + 2.0 ** -5) ** 2), np.float32(rows * (1 + 2.0 ** -5))
+    assert bool((dw == float(w_want)).all()), (w_want, dw.min().item(), dw.max().item())
+    assert bool((db == float(b_want)).all()), (b_want, db.min().item(), db.max().item())

@@ -120,3 +120,12 @@ def scores(x, kind, bias=None, mask=None, mask_rows=None, ids=None, offsets=None
                 s = e / e.sum()
         out[n], size[n] = s, big
     return out, size
+
+
+def whole_numbers(rng, rows, cols):
+    """Whole numbers of -3 .. 5 without 0 and of positive mean.  Products of two are at most
+    25, so float32 sums of up to 2^24 / 25 = 671088 of them are exact in any order, and a
+    gradient of the maps that leaves out or repeats a row differs in every element of its
+    leaf."""
+    v = rng.integers(-3, 5, (rows, cols))
+    return np.where(v >= 0, v + 1, v).astype(np.float64)

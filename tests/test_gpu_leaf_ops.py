@@ -170,3 +170,20 @@ def test_scores_edges(check, dtype):
 def test_together(check, dtype):
     check("together", dtype=dtype)
 
+
+# every form of the maps' gradients, over leaves of one part and of many
+@pytest.mark.parametrize("dtype", ["f32", "bf16", "f16"])
+@pytest.mark.parametrize("rows,inputs,outputs,trees,leaves,shape", [
+    (300000, 61, 10, 1, 3, "lost"), (270001, 140, 3, 2, 5, "skew"), (200000, 90, 1, 1, 1, "one"),
+    (140000, 300, 20, 1, 1, "lost"), (30011, 100, 64, 2, 4, "skew"), (30000, 9, 130, 1, 3, "even"),
+    (300, 70, 20, 3, 5, "lost"), (30000, 200, 264, 1, 7, "skew"), (40000, 200, 192, 2, 100, "skew"),
+    (12000, 192, 200, 5, 60, "one"), (25000, 264, 520, 1, 3, "lost"), (16384, 192, 192, 1, 2, "one")])
+def test_whole_gradients(check, rows, inputs, outputs, trees, leaves, shape, dtype):
+    check("whole_dw", rows=rows, inputs=inputs, outputs=outputs, trees=trees, leaves=leaves, shape=shape,
+          dtype=dtype)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16", "f16"])
+@pytest.mark.parametrize("inputs,outputs", [(192, 192), (100, 64), (64, 10), (140, 10), (10, 64)])
+def test_long_sums(check, inputs, outputs, dtype):
+    check("long_sums", rows=600000, inputs=inputs, outputs=outputs, dtype=dtype)

@@ -242,3 +242,22 @@ def test_oracle_against_loops():
     assert np.allclose(oracle.product_dx(dy, w, leaf, 3)[0], dx)
     got = oracle.product_dw(dy, x, leaf, 3)
     assert np.allclose(got[0], dw) and np.allclose(got[2], db)
+
+
+def test_whole_numbers_show_every_row():
+    """What the GPU's exact gradients are compared with: a row left out, or taken twice, is
+    seen in every element of its leaf, and sums stay within float32's whole numbers."""
+    rng = np.random.default_rng(1)
+    x, dy = oracle.whole_numbers(rng, 400, 7), oracle.whole_numbers(rng, 400, 3)
+    assert np.abs(x).max() == 5 and x.min() == -3 and x.all() and dy.all()
+    leaf = rng.integers(0, 3, (400, 1)).astype(np.int32)
+    dw, _, db, _ = oracle.product_dw(dy, x, leaf, 3)
+    for row in (0, 17, 399):
+        l = leaf[row, 0]
+        lost = leaf.copy()
+        lost[row] = -1
+        w, _, b, _ = oracle.product_dw(dy, x, lost, 3)
+        assert (w[l] != dw[l]).all() and (b[l] != db[l]).all()
+        twice = np.concatenate([np.arange(400), [row]])
+        w, _, b, _ = oracle.product_dw(dy[twice], x[twice], leaf[twice], 3)
+        assert (w[l] != dw[l]).all() and (b[l] != db[l]).all()
