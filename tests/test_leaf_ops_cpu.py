@@ -261,3 +261,16 @@ def test_whole_numbers_show_every_row():
         twice = np.concatenate([np.arange(400), [row]])
         w, _, b, _ = oracle.product_dw(dy[twice], x[twice], leaf[twice], 3)
         assert (w[l] != dw[l]).all() and (b[l] != db[l]).all()
+
+
+@pytest.mark.parametrize("rows,inputs,outputs,dtype", [(100000, 256, 512, 2), (1000000, 256, 256, 3), (60000, 200, 192, 2)])
+def test_gradients_take_the_card(lib, rows, inputs, outputs, dtype):
+    """The rows of one leaf go to about as many blocks as there are CUs, also where large tiles
+    make few of the leaf's map: working memory holds the parts' sums."""
+    need = C.c_size_t(0)
+    m = maps(rows=rows, leaves=1, inputs=inputs, outputs=outputs, dtype=dtype)
+    assert lib.lgbm_hip_leaf_product_workspace(C.byref(m), C.c_int32(2), C.byref(need)) == 0
+    tiles = -(-inputs // 256) * -(-outputs // 256)
+    # parts of at least 512 rows, a slot for the leaf's end and one for the rows in no leaf
+    parts = need.value // (4 * outputs * (inputs + 1)) - 2
+    assert parts * tiles >= min(200, rows // 512 * tiles)
