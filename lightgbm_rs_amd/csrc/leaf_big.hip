@@ -474,11 +474,26 @@ int64_t leaf_big_blocks(const LeafProduct& p, int what) {
 }
 
 // Rows and maps that make whole tiles of 256 x 256 worthwhile, and 16-byte chunks that do not
-// cross a row's end.
+// cross a row's end.  The counts of the leaves are on the device, so the rule takes their
+// average; tables of many small leaves and a few long ones still gain or break even (bfloat16,
+// these tiles and the other kernels, us: 100000 x 512 to 512 by 500 leaves alike y 141, 202, dx 156,
+// 206, dw 218, 371; with sizes as exp(3 N(0, 1)) 168, 192, 183, 188, 484, 510; 40000 x 2048 to 2048
+// by 200 leaves of sizes as exp(N(0, 1)) 677, 781, 699, 696, 1512, 1967).
+//
+// y and dx also need tiles for the CUs, about 72 with half a tile for every leaf's end (bfloat16 by
+// these tiles and by k_leaf_tile's, us):
+//   tiles            y           dx
+//     2..5   400 x 4096 to 200 by two leaves 92, 38; 400 x 200 to 4096 103, 43
+//    39..41  1000 x 2048 to 2048 by two 57, 42 and 64, 41; 400 x 4096 to 4096 by two 96, 61 and 107, 59
+//    63..66  16000 x 4096 to 200 by one 98, 80; 2000 x 2048 to 2048 by one 58, 45 and 66, 43
+//    76..78  4000 x 1024 to 1024 by seven 38, 43 and 43, 42; 16000 x 4096 to 200 by 31 100, 127
+//   127..139 8000 x 1024 to 1024 by one 41, 44 and 45, 42, by seven 41, 64 and 46, 60
 bool leaf_big_fits(const LeafProduct& p, int what) {
   if (p.dtype == LGBM_HIP_DTYPE_F32) return false;
   if (p.inputs % 8 || p.outputs % 8 || p.inputs < 192 || p.outputs < 192) return false;
   if ((int64_t)p.g.rows < 192 * (int64_t)p.g.leaves) return false;
+  const int64_t ct = ((what == LEAF_PRODUCT_Y ? p.outputs : p.inputs) + BN - 1) / BN;
+  if (what != LEAF_PRODUCT_DW && (2 * (int64_t)p.g.rows / BM + p.g.leaves) * ct * p.g.trees < 2 * 72) return false;
   if (p.g.rows * std::max(p.ldx, p.lddy) >> 35 || (int64_t)p.inputs * p.outputs >> 35) return false;  // 64 GB
   auto ok = [](const void* q, int64_t ld) { return (((uintptr_t)q) | (uintptr_t)(ld * 2)) % 16 == 0; };
   if (what == LEAF_PRODUCT_Y) return ok(p.x, p.ldx) && ok(p.w, p.inputs);

@@ -769,3 +769,38 @@ def long_sums(rows, inputs, outputs, dtype):
     w_want, b_want = np.float32(rows * (1 + 2.0 ** -5) ** 2), np.float32(rows * (1 + 2.0 ** -5))
     assert bool((dw == float(w_want)).all()), (w_want, dw.min().item(), dw.max().item())
     assert bool((db == float(b_want)).all()), (b_want, db.min().item(), db.max().item())
+
+
+def odd_tables_large_tiles():
+    """As odd_tables, with rows enough for the large tiles of y and dx."""
+    odd_tables(400, 200, 192, "bf16")
+
+
+def captured_tiles():
+    """y and dx by large tiles replayed from a graph, over tables that change."""
+    be = backend()
+    rng = np.random.default_rng(12)
+    dt = torch.float16
+    x, dy = matrix(rng, 9000, 264, dt), matrix(rng, 9000, 520, dt)
+    w = matrix(rng, 6 * 520, 264, dt).view(6, 520, 264)
+    leaf = torch.from_numpy(leaves_of(rng, 9000, 2, 3, "even")).to(DEV).int()
+
+    def run():
+        g = be.leaf_groups(leaf, 3)
+        return be.leaf_product(x, w, g), be.leaf_product_dx(dy, w, g), *be.leaf_product_dw(dy, x, g)
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):
+        run()
+    torch.cuda.current_stream().wait_stream(s)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = run()
+    for shape in ("lost", "one", "skew"):
+        x.copy_(matrix(rng, 9000, 264, dt))
+        leaf.copy_(torch.from_numpy(leaves_of(rng, 9000, 2, 3, shape)).to(DEV).int())
+        graph.replay()
+        want = run()
+        torch.cuda.synchronize()
+        for a, b in zip(out, want):
+            assert torch.equal(a, b)

@@ -187,3 +187,19 @@ def test_whole_gradients(check, rows, inputs, outputs, trees, leaves, shape, dty
 @pytest.mark.parametrize("inputs,outputs", [(192, 192), (100, 64), (64, 10), (140, 10), (10, 64)])
 def test_long_sums(check, inputs, outputs, dtype):
     check("long_sums", rows=600000, inputs=inputs, outputs=outputs, dtype=dtype)
+
+
+# enough tiles of 256 x 256 for the CUs, or just too few (19000 rows of two leaves: 75; 18000: 71)
+@pytest.mark.parametrize("what", ["product", "grads"])
+@pytest.mark.parametrize("rows,inputs,outputs,trees,leaves,shape,pad,dtype", [
+    (19000, 200, 192, 1, 2, "even", 8, "bf16"), (18000, 200, 192, 1, 2, "even", 8, "bf16"),
+    (9000, 320, 272, 2, 3, "lost", 0, "f16"), (9000, 272, 320, 2, 3, "skew", 16, "bf16"),
+    (5000, 1024, 1032, 1, 4, "one", 0, "bf16"), (3000, 1288, 520, 3, 15, "lost", 8, "f16")])
+def test_large_tiles(check, what, rows, inputs, outputs, trees, leaves, shape, pad, dtype):
+    check(what, rows=rows, inputs=inputs, outputs=outputs, trees=trees, leaves=leaves, shape=shape,
+          pad=pad, dtype=dtype)
+
+
+@pytest.mark.parametrize("name", ["odd_tables_large_tiles", "captured_tiles"])
+def test_large_tiles_plain(check, name):
+    check(name)
