@@ -770,6 +770,10 @@ typedef struct lgbm_leaf_maps {
 #define LGBM_HIP_LEAF_PRODUCT 0
 #define LGBM_HIP_LEAF_PRODUCT_DX 1
 #define LGBM_HIP_LEAF_PRODUCT_DW 2
+/* Working memory.  y and dx of one tree: none; of several: a float32 plane of the output for
+ * each tree, up to 4 GiB of them (a plane at least); beyond that trees are made in runs, and
+ * a float64 plane carries their sums.  dw: parts of a leaf's rows have sums of their own where
+ * one leaf may not fill the device or has more than 8192 rows. */
 int lgbm_hip_leaf_product_workspace(const lgbm_leaf_maps* maps, int32_t what, size_t* bytes);
 /* y[n] = sum over trees t of w[t][leaf] x[n] + bias[t][leaf], in float32 and rounded
  * once.  d_x [num_rows][inputs], d_w [num_trees * num_leaves][outputs][inputs], d_bias

@@ -412,7 +412,7 @@ __global__ __launch_bounds__(THREADS, 1) void k_leaf_big(LeafProduct p, int col_
       for (int e = 0; e < 16; e += 2) {
         const int r = wm + i * 32 + (e >> 2) * 8 + row4 + (e & 3);
         const int n[2] = {row_of[DW ? 0 : r], row_of[DW ? 0 : r + 1]};
-        if (p.g.trees > 1) {
+        if (p.planes) {
 #pragma unroll
           for (int k = 0; k < 2; ++k) {
             if (n[k] < 0) continue;

@@ -264,7 +264,7 @@ __device__ __forceinline__ DwPart dw_part(const LeafProduct& p, const Split& spl
 template <typename T>
 __device__ __forceinline__ void store_rows(const LeafProduct& p, int tree, const int (&n)[4], int col, int cols,
                                            f32x4 v) {
-  if (p.g.trees > 1) {
+  if (p.planes) {
     float* const to = (float*)p.ws + (int64_t)tree * p.g.rows * cols + col;
 #pragma unroll
     for (int e = 0; e < 4; ++e)

@@ -45,6 +45,9 @@ struct LeafProduct {
   float* dw;  // [trees * leaves][outputs][inputs]
   float* db;  // [trees * leaves][outputs], may be null
   void* ws;
+  // product and dx: whether a tree's results go to its float32 plane [rows][columns] in ws,
+  // to be added, instead of to out
+  bool planes;
 };
 
 #define LEAF_PRODUCT_Y 0

@@ -5,7 +5,7 @@
 // is a matrix product of its own, of as many rows as it holds: a block finds its leaf from
 // the counts on the device and gathers its rows through the order.  One tree writes its
 // rows directly; several write float32 planes [tree][row] that k_sum_trees adds, so results
-// never depend on the order of blocks.
+// never depend on the order of blocks.  As many trees at a time as PLANES holds the planes of.
 #include <algorithm>
 #include <type_traits>
 
@@ -349,7 +349,7 @@ __global__ __launch_bounds__(THREADS) void k_leaf_dx_narrow(LeafProduct p, int c
       }
       __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
       __builtin_amdgcn_wave_barrier();
-      if (p.g.trees > 1)
+      if (p.planes)
         store_tile((float*)p.ws + (int64_t)tree * p.g.rows * cols + c0, cols, cols - c0, n[u], mine);
       else
         store_tile((T*)p.out + c0, p.ldo, cols - c0, n[u], mine);
@@ -358,11 +358,25 @@ __global__ __launch_bounds__(THREADS) void k_leaf_dx_narrow(LeafProduct p, int c
   }
 }
 
-// The trees' planes added, rounded once: 64 elements a block, a quarter of the trees a wave;
-// in float64, since a forest has hundreds of trees.
+// The planes of a run of trees added, in float64, since a forest has hundreds; the last run
+// rounds once, the others leave their sums in carry [rows][cols] (null: one run).
+struct Run {
+  double* carry;
+  bool first, last;
+};
+template <int V>
+__device__ __forceinline__ void carry_in(const Run& run, int64_t e, double (&v)[V]) {
+  if (run.first) return;
+  double c[V];
+  __builtin_memcpy(c, run.carry + e, sizeof(c));
+#pragma unroll
+  for (int i = 0; i < V; ++i) v[i] += c[i];
+}
+
+// 64 elements a block, a quarter of the trees a wave.
 template <typename T>
 __global__ __launch_bounds__(THREADS) void k_sum_trees(const float* planes, int64_t rows, int cols,
-                                                       int trees, T* out, int64_t ldo) {
+                                                       int trees, Run run, T* out, int64_t ldo) {
   __shared__ double part[4][64];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const int64_t total = rows * cols;
@@ -376,15 +390,21 @@ __global__ __launch_bounds__(THREADS) void k_sum_trees(const float* planes, int6
     }
     part[wave][lane] = v;
     __syncthreads();
-    if (wave == 0 && e < total)
-      out[e / cols * ldo + e % cols] = (T)(float)(part[0][lane] + part[1][lane] + part[2][lane] + part[3][lane]);
+    if (wave == 0 && e < total) {
+      double sum[1] = {part[0][lane] + part[1][lane] + part[2][lane] + part[3][lane]};
+      carry_in(run, e, sum);
+      if (run.last)
+        out[e / cols * ldo + e % cols] = (T)(float)sum[0];
+      else
+        run.carry[e] = sum[0];
+    }
     __syncthreads();
   }
 }
 // Few trees: a thread an element, or four of rows without gaps.
 template <typename T, int V>
 __global__ __launch_bounds__(THREADS) void k_sum_few_trees(const float* planes, int64_t rows, int cols,
-                                                           int trees, T* out, int64_t ldo) {
+                                                           int trees, Run run, T* out, int64_t ldo) {
   const int64_t total = rows * cols;
   for (int64_t e = (blockIdx.x * (int64_t)THREADS + threadIdx.x) * V; e < total;
        e += (int64_t)gridDim.x * THREADS * V) {
@@ -395,6 +415,11 @@ __global__ __launch_bounds__(THREADS) void k_sum_few_trees(const float* planes, 
       __builtin_memcpy(x, planes + t * total + e, sizeof(x));
 #pragma unroll
       for (int i = 0; i < V; ++i) v[i] += (double)x[i];
+    }
+    carry_in(run, e, v);
+    if (!run.last) {
+      __builtin_memcpy(run.carry + e, v, sizeof(v));
+      continue;
     }
     T o[V];
 #pragma unroll
@@ -732,25 +757,27 @@ void launch_tile(const LeafProduct& p, hipStream_t s) {
 }
 
 template <typename T, bool DX>
-void launch_tiles(const LeafProduct& p, int cols, hipStream_t s) {
+void launch_tiles(const LeafProduct& p, bool wide, hipStream_t s) {
   if constexpr (sizeof(T) == 2) {
-    if (wide_tiles(p, cols)) return launch_tile<T, DX, 128, 128>(p, s);
+    if (wide) return launch_tile<T, DX, 128, 128>(p, s);
   }
   launch_tile<T, DX, 64, 64>(p, s);
 }
 
+// Which kernel makes y or dx; by all the trees, however few of them are made at a time.
+struct Form {
+  bool big, maps, wide;
+};
+Form form_of(const LeafProduct& p, int what) {
+  return {leaf_big_fits(p, what), what == LEAF_PRODUCT_Y && by_maps(p),
+          wide_tiles(p, what == LEAF_PRODUCT_DX ? p.inputs : p.outputs)};
+}
+
 template <typename T>
-void launch(const LeafProduct& p, int what, hipStream_t s) {
-  if (what == LEAF_PRODUCT_DW) {
-    if (!leaf_big_fits(p, what)) return launch_dw<T>(p, s);
-    launch_leaf_big(p, what, s);
-    const Split split = leaf_big_split(p);
-    if (split.rows) sum_slots(p, split, s);
-    return;
-  }
+void launch_product(const LeafProduct& p, int what, const Form& form, hipStream_t s) {
   const bool dx = what == LEAF_PRODUCT_DX;
   const int cols = dx ? p.inputs : p.outputs;
-  if (leaf_big_fits(p, what)) {
+  if (form.big) {
     launch_leaf_big(p, what, s);
   } else if (dx && p.outputs <= 32) {
     const int ct = (cols + 127) / 128;
@@ -760,8 +787,8 @@ void launch(const LeafProduct& p, int what, hipStream_t s) {
     else if constexpr (sizeof(T) == 4)
       k_leaf_dx_narrow<T, 2><<<grid, THREADS, 0, s>>>(p, ct);
   } else if (dx) {
-    launch_tiles<T, true>(p, cols, s);
-  } else if (by_maps(p)) {
+    launch_tiles<T, true>(p, form.wide, s);
+  } else if (form.maps) {
     const int ct = (cols + 15) / 16;
     k_leaf_few<T><<<dim3((unsigned)(row_tiles(p.g, 16) * ct), (unsigned)p.g.trees), THREADS, 0, s>>>(p, ct);
   } else if (cols <= 32) {
@@ -776,19 +803,60 @@ void launch(const LeafProduct& p, int what, hipStream_t s) {
     else
       k_leaf_narrow<T, 2, 4><<<grid, 256, 0, s>>>(p);
   } else {
-    launch_tiles<T, false>(p, cols, s);
+    launch_tiles<T, false>(p, form.wide, s);
   }
-  if (p.g.trees > 1) {
-    const int64_t total = (int64_t)p.g.rows * cols;
-    if (p.g.trees >= 16)
-      k_sum_trees<T><<<(unsigned)std::min<int64_t>((total + 63) / 64, 1 << 20), THREADS, 0, s>>>(
-          (const float*)p.ws, p.g.rows, cols, p.g.trees, (T*)p.out, p.ldo);
+}
+
+// Trees made at a time: as many as have their planes within PLANES, one at least, in runs
+// alike.
+constexpr int64_t PLANES = (int64_t)4 << 30;
+int64_t plane_bytes(const LeafProduct& p, int what) {
+  return (int64_t)p.g.rows * (what == LEAF_PRODUCT_DX ? p.inputs : p.outputs) * 4;
+}
+int run_trees(const LeafProduct& p, int what) {
+  const int64_t most = std::max<int64_t>(1, PLANES / std::max<int64_t>(1, plane_bytes(p, what)));
+  const int64_t runs = (p.g.trees + most - 1) / most;
+  return (int)((p.g.trees + runs - 1) / runs);
+}
+size_t planes_bytes(const LeafProduct& p, int what) {  // the sums carried over stand behind them
+  return ((size_t)run_trees(p, what) * (size_t)plane_bytes(p, what) + 15) / 16 * 16;
+}
+
+template <typename T>
+void launch(const LeafProduct& p, int what, hipStream_t s) {
+  if (what == LEAF_PRODUCT_DW) {
+    if (!leaf_big_fits(p, what)) return launch_dw<T>(p, s);
+    launch_leaf_big(p, what, s);
+    const Split split = leaf_big_split(p);
+    if (split.rows) sum_slots(p, split, s);
+    return;
+  }
+  const Form form = form_of(p, what);
+  if (p.g.trees == 1) return launch_product<T>(p, what, form, s);
+  const int cols = what == LEAF_PRODUCT_DX ? p.inputs : p.outputs, trees = run_trees(p, what);
+  const int64_t total = (int64_t)p.g.rows * cols;
+  double* const carry = trees < p.g.trees ? (double*)((char*)p.ws + planes_bytes(p, what)) : nullptr;
+  for (int t = 0; t < p.g.trees; t += trees) {
+    LeafProduct q = p;
+    const int64_t leaves = (int64_t)t * p.g.leaves;
+    q.planes = true;
+    q.g.trees = std::min(trees, p.g.trees - t);
+    q.g.order += (int64_t)t * p.g.rows, q.g.begin += leaves, q.g.count += leaves;
+    q.w = (const T*)p.w + leaves * p.outputs * p.inputs;
+    if (p.b) q.b = (const T*)p.b + leaves * p.outputs;
+    launch_product<T>(q, what, form, s);
+    const Run run{carry, t == 0, t + trees >= p.g.trees};
+    const float* const planes = (const float*)p.ws;
+    const auto blocks = [&](int64_t elements, int64_t most) { return (unsigned)std::min(elements, most); };
+    if (q.g.trees >= 16)
+      k_sum_trees<T><<<blocks((total + 63) / 64, 1 << 20), THREADS, 0, s>>>(planes, p.g.rows, cols, q.g.trees, run,
+                                                                            (T*)p.out, p.ldo);
     else if (p.ldo == cols && total % 4 == 0)
-      k_sum_few_trees<T, 4><<<(unsigned)std::min<int64_t>((total / 4 + THREADS - 1) / THREADS, 1 << 16), THREADS, 0,
-                              s>>>((const float*)p.ws, p.g.rows, cols, p.g.trees, (T*)p.out, p.ldo);
+      k_sum_few_trees<T, 4><<<blocks((total / 4 + THREADS - 1) / THREADS, 1 << 16), THREADS, 0, s>>>(
+          planes, p.g.rows, cols, q.g.trees, run, (T*)p.out, p.ldo);
     else
-      k_sum_few_trees<T, 1><<<(unsigned)std::min<int64_t>((total + THREADS - 1) / THREADS, 1 << 16), THREADS, 0,
-                              s>>>((const float*)p.ws, p.g.rows, cols, p.g.trees, (T*)p.out, p.ldo);
+      k_sum_few_trees<T, 1><<<blocks((total + THREADS - 1) / THREADS, 1 << 16), THREADS, 0, s>>>(
+          planes, p.g.rows, cols, q.g.trees, run, (T*)p.out, p.ldo);
   }
 }
 
@@ -805,7 +873,7 @@ size_t leaf_product_workspace(const LeafProduct& p, int what) {
     return (size_t)p.g.trees * (size_t)slots * (size_t)p.outputs * (size_t)(p.inputs + 1) * 4;
   }
   if (p.g.trees <= 1) return 0;
-  return (size_t)p.g.trees * (size_t)p.g.rows * (size_t)(what == LEAF_PRODUCT_DX ? p.inputs : p.outputs) * 4;
+  return planes_bytes(p, what) + (run_trees(p, what) < p.g.trees ? 2 * (size_t)plane_bytes(p, what) : 0);
 }
 
 int64_t leaf_product_blocks(const LeafProduct& p, int what) {

@@ -804,3 +804,32 @@ def captured_tiles():
         torch.cuda.synchronize()
         for a, b in zip(out, want):
             assert torch.equal(a, b)
+
+
+def tree_runs(rows, inputs, width, trees, dtype, strided=False):
+    """Planes of more than 4 GiB: trees in runs, the last one shorter.  A row has one input
+    that is not 0, and all are whole numbers, so every sum is exact in the type."""
+    be, dt, leaves = backend(), TYPES[dtype], 5
+    assert trees * rows * width * 4 > 2 ** 32 and trees * 30 <= 2 / torch.finfo(dt).eps
+    gen = torch.Generator(device=DEV).manual_seed(rows)
+    whole = lambda *shape: torch.randint(-5, 6, shape, generator=gen, device=DEV).to(dt)
+    leaf = torch.randint(0, leaves, (rows, trees), generator=gen, device=DEV).int()
+    leaf[torch.rand((rows, trees), generator=gen, device=DEV) < 0.1] = -1
+    g = be.leaf_groups(leaf, leaves)
+    w, b, value = whole(trees * leaves, inputs, width), whole(trees * leaves, width), whole(rows, 1)
+    at = torch.randint(0, inputs, (rows, 1), generator=gen, device=DEV)
+    x = torch.zeros((rows, inputs), dtype=dt, device=DEV).scatter_(1, at, value)
+    room = torch.full((rows, width + 3), 9, dtype=dt, device=DEV) if strided else None
+    out = None if room is None else room[:, 1:1 + width]
+    y = be.leaf_product(x, w.transpose(1, 2).contiguous(), g, bias=b, out=out)
+    want, sums = torch.zeros_like(y), torch.zeros_like(y)
+    none = torch.zeros((), dtype=dt, device=DEV)
+    for t in range(trees):
+        l, there = (leaf[:, t].clamp(min=0) + t * leaves).long(), (leaf[:, t] >= 0)[:, None]
+        want += torch.where(there, value * w[l, at[:, 0]], none)
+        sums += torch.where(there, value * w[l, at[:, 0]] + b[l], none)
+    assert bool(want.any()) and torch.equal(y, sums)
+    if strided:
+        assert bool((room[:, 0] == 9).all()) and bool((room[:, 1 + width:] == 9).all())
+    del y, sums, room, out
+    assert torch.equal(be.leaf_product_dx(x, w, g), want)

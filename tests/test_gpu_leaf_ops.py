@@ -203,3 +203,11 @@ def test_large_tiles(check, what, rows, inputs, outputs, trees, leaves, shape, p
 @pytest.mark.parametrize("name", ["odd_tables_large_tiles", "captured_tiles"])
 def test_large_tiles_plain(check, name):
     check(name)
+
+
+# runs of 4 and 3 trees, 3 and 3 and 1, 1 and 1 and 1, 16 and 16
+@pytest.mark.parametrize("rows,inputs,width,trees,dtype,strided", [
+    (2500000, 1, 96, 7, "bf16", False), (3000001, 3, 101, 7, "f32", True), (2900000, 192, 200, 3, "bf16", False),
+    (3000000, 1, 17, 32, "f32", False), (2800000, 5, 200, 3, "f16", True)])
+def test_trees_in_runs(check, rows, inputs, width, trees, dtype, strided):
+    check("tree_runs", rows=rows, inputs=inputs, width=width, trees=trees, dtype=dtype, strided=strided)

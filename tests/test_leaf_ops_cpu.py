@@ -274,3 +274,17 @@ def test_gradients_take_the_card(lib, rows, inputs, outputs, dtype):
     # parts of at least 512 rows, a slot for the leaf's end and one for the rows in no leaf
     parts = need.value // (4 * outputs * (inputs + 1)) - 2
     assert parts * tiles >= min(200, rows // 512 * tiles)
+
+
+@pytest.mark.parametrize("what,cols", [(0, 10), (1, 100)])
+def test_planes_are_bounded(lib, what, cols):
+    """However many trees there are: planes of 4 GiB, one plane at least, and a float64 one that
+    carries the sums."""
+    need = C.c_size_t(0)
+    for rows, trees in ((1000000, 500), (1000000, 5000), (200000000, 3), (10500000, 100), (7, 65535)):
+        m = maps(rows=rows, trees=trees, inputs=100, outputs=10)
+        assert lib.lgbm_hip_leaf_product_workspace(C.byref(m), C.c_int32(what), C.byref(need)) == 0
+        plane = rows * cols * 4
+        assert plane <= need.value <= max(plane, 2 ** 32) + 2 * plane + 16
+        if trees * plane <= 2 ** 32:
+            assert trees * plane <= need.value <= trees * plane + 16
