@@ -6,7 +6,9 @@ Tensors are on the backend's device; matrices have a row stride (a matrix whose 
 are strided is copied first).  A call queues its work on torch's current stream of that
 device and returns, so calls follow each other like torch's own operations and can be
 captured into a graph.  Gradients are entries of their own: nothing is recorded for
-torch's autograd.
+torch's autograd, so a floating-point tensor that requires gradients is refused while they are
+recorded (call under torch.no_grad(), as the methods of a torch.autograd.Function are, or
+on detached tensors).
 
 Import torch before the first `HipBackend`: torch brings a HIP runtime of its own, which
 the library then shares.  (The other way round torch finds no device.)
@@ -101,6 +103,10 @@ def _dtype(t, what, double=False):
 
 
 def _here(self, **tensors):
+    """Every tensor on the backend's device, and none that autograd would have to record."""
+    for name, t in tensors.items():
+        if t is not None and t.requires_grad and _torch.is_grad_enabled():
+            raise ValueError(f"{name} requires gradients, which this call does not record")
     for name, t in tensors.items():
         if t is not None and (not t.is_cuda or t.get_device() != self.device):
             raise ValueError(f"{name} is on {t.device}: cuda:{self.device} is needed")

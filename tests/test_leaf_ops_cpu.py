@@ -288,3 +288,30 @@ def test_planes_are_bounded(lib, what, cols):
         assert plane <= need.value <= max(plane, 2 ** 32) + 2 * plane + 16
         if trees * plane <= 2 ** 32:
             assert trees * plane <= need.value <= trees * plane + 16
+
+
+def test_python_refuses_what_autograd_would_lose():
+    """A tensor that requires gradients is refused while torch records; without recording, and
+    detached, the call goes on to its next check."""
+    import torch
+    be = Plain()
+    z = torch.zeros
+    i32 = torch.int32
+    g = LeafGroups(z((1, 6), dtype=i32), z((1, 4), dtype=i32), z((1, 4), dtype=i32))
+    calls = [
+        (lambda x, w, dy: be.leaf_product(x, w, g), "x"), (lambda x, w, dy: be.leaf_product(x, w, g), "weight"),
+        (lambda x, w, dy: be.leaf_product(x, w, g, bias=dy[:4]), "bias"),
+        (lambda x, w, dy: be.leaf_product(x, w, g, out=dy), "out"),
+        (lambda x, w, dy: be.leaf_product_dx(dy, w, g), "dy"), (lambda x, w, dy: be.leaf_product_dw(dy, x, g), "x"),
+        (lambda x, w, dy: be.dropout(x, 0.5, 1), "x"), (lambda x, w, dy: be.dropout(x[:, 0], 0.5, 1), "x"),
+        (lambda x, w, dy: be.adjust_scores(x), "scores"), (lambda x, w, dy: be.adjust_scores(x, bias=w[0, 0]), "bias")]
+    holder = {"x": "x", "weight": "w", "bias": None, "out": "dy", "dy": "dy", "scores": "x"}
+    for i, (call, name) in enumerate(calls):
+        t = {"x": z((6, 5)), "w": z((4, 3, 5)), "dy": z((6, 3))}
+        t[holder[name] or ("dy" if i == 2 else "w")].requires_grad_()
+        with pytest.raises(ValueError, match=f"{name} requires gradients"):
+            call(**t)
+        with torch.no_grad(), pytest.raises(ValueError, match="is on cpu"):
+            call(**t)
+        with pytest.raises(ValueError, match="is on cpu"):
+            call(**{k: v.detach() for k, v in t.items()})
