@@ -150,6 +150,14 @@ def _out(out, like, shape):
     return out
 
 
+def _written(*tensors):
+    """Tells autograd of the caller's tensors that were written, as torch's own in-place
+    operations do: a graph that saved one refuses its backward pass."""
+    for t in tensors:
+        if t is not None and not t.is_inference():
+            _torch.autograd.graph.increment_version(t)
+
+
 def _workspace(self, torch, entry, *args):
     """(pointer, bytes, the tensor that holds them) of an entry's working memory."""
     size = C.c_size_t(0)
@@ -215,6 +223,7 @@ def _leaf_product(self, x, weight, groups, bias=None, out=None):
         bias = bias.contiguous()
     _here(self, x=x, weight=weight, bias=bias, out=out)
     m, keep = _maps(self, torch, rows, inputs, outputs, dtype, groups, leaves)
+    given = out
     x, weight, out = _rows(x), weight.contiguous(), _out(out, x, (rows, outputs))
     ws, nbytes, hold = _workspace(self, torch, self.lib.lgbm_hip_leaf_product_workspace,
                                   C.byref(m), _PRODUCT)
@@ -222,6 +231,7 @@ def _leaf_product(self, x, weight, groups, bias=None, out=None):
         self.ctx, C.byref(m), x.data_ptr(), _ld(x), weight.data_ptr(),
         None if bias is None else bias.data_ptr(), out.data_ptr(), _ld(out), ws, nbytes,
         _stream(self, torch)))
+    _written(given)
     return out
 
 
@@ -238,12 +248,14 @@ def _leaf_product_dx(self, dy, weight, groups, out=None):
         raise ValueError("dy and weight differ in type")
     _here(self, dy=dy, weight=weight, out=out)
     m, keep = _maps(self, torch, rows, inputs, outputs, dtype, groups, leaves)
+    given = out
     dy, weight, out = _rows(dy), weight.contiguous(), _out(out, dy, (rows, inputs))
     ws, nbytes, hold = _workspace(self, torch, self.lib.lgbm_hip_leaf_product_workspace,
                                   C.byref(m), _DX)
     self._check(self.lib.lgbm_hip_leaf_product_dx(
         self.ctx, C.byref(m), dy.data_ptr(), _ld(dy), weight.data_ptr(), out.data_ptr(), _ld(out),
         ws, nbytes, _stream(self, torch)))
+    _written(given)
     return out
 
 
@@ -280,6 +292,7 @@ def _leaf_product_dw(self, dy, x, groups, bias=True, out=None, bias_out=None):
     self._check(self.lib.lgbm_hip_leaf_product_dw(
         self.ctx, C.byref(m), dy.data_ptr(), _ld(dy), x.data_ptr(), _ld(x), dw.data_ptr(),
         None if db is None else db.data_ptr(), ws, nbytes, _stream(self, torch)))
+    _written(out, bias_out)
     return dw, db
 
 
@@ -309,6 +322,7 @@ def _dropout(self, x, p, seed, offset=0, by="element", out=None):
     self._check(self.lib.lgbm_hip_dropout(
         self.ctx, src.data_ptr(), _ld(src), x.shape[0], x.shape[1], dtype, p, seed & (2 ** 64 - 1),
         offset & (2 ** 64 - 1), by == "row", dst.data_ptr(), _ld(dst), _stream(self, torch)))
+    _written(out)
     return dst
 
 
@@ -359,6 +373,7 @@ def _adjust_scores(self, scores, kind="raw", bias=None, mask=None, mask_rows=Non
     src = _rows(scores)
     if out is scores and src is not scores:
         raise ValueError("out has strided columns or rows that overlap")
+    given = out
     out = _out(out, scores, (rows, classes))
     at = lambda t: None if t is None else t.data_ptr()
     a = _Scores(at(src), _ld(src), rows, classes, dtype, PREDICT_KINDS[kind],
@@ -368,6 +383,7 @@ def _adjust_scores(self, scores, kind="raw", bias=None, mask=None, mask_rows=Non
     ws, nbytes, hold = _workspace(self, torch, self.lib.lgbm_hip_adjust_scores_workspace, C.byref(a))
     self._check(self.lib.lgbm_hip_adjust_scores(self.ctx, C.byref(a), ws, nbytes,
                                                 _stream(self, torch)))
+    _written(given)
     return out
 
 

@@ -833,3 +833,34 @@ def tree_runs(rows, inputs, width, trees, dtype, strided=False):
         assert bool((room[:, 0] == 9).all()) and bool((room[:, 1 + width:] == 9).all())
     del y, sums, room, out
     assert torch.equal(be.leaf_product_dx(x, w, g), want)
+
+
+def versions():
+    """Tensors that a call writes: a graph of torch's that saved one refuses its backward pass,
+    and one of inference mode is written all the same."""
+    be = backend()
+    z = lambda *shape: torch.ones(shape, device=DEV)
+    g = be.leaf_groups(torch.zeros((6, 1), dtype=torch.int32, device=DEV), 2)
+    x, w, dy = z(6, 5), z(2, 3, 5), z(6, 3)
+    line, mat, scores = z(40), z(6, 5), z(6, 3)
+    for out, call in ((z(6, 3), lambda o: be.leaf_product(x, w, g, out=o)),
+                      (z(6, 5), lambda o: be.leaf_product_dx(dy, w, g, out=o)),
+                      (z(2, 3, 5), lambda o: be.leaf_product_dw(dy, x, g, out=o)),
+                      (z(2, 3), lambda o: be.leaf_product_dw(dy, x, g, bias_out=o)),
+                      (z(6, 5), lambda o: be.dropout(x, 0.5, 1, out=o)), (mat, lambda o: be.dropout(mat, 0.5, 1, out=o)),
+                      (line, lambda o: be.dropout(line, 0.5, 1, out=o)), (z(40), lambda o: be.dropout(line, 0.5, 1, out=o)),
+                      (z(6, 3), lambda o: be.adjust_scores(dy, "transformed", out=o)),
+                      (scores, lambda o: be.adjust_scores(scores, "transformed", out=o))):
+        leaf = torch.ones_like(out).requires_grad_()
+        y = (leaf * out).sum()
+        call(out)
+        try:
+            y.backward()
+        except RuntimeError as e:
+            assert "inplace" in str(e)
+            continue
+        raise AssertionError("a saved tensor was written unseen")
+    assert not x._version and not dy._version and not w._version
+    with torch.inference_mode():
+        v = torch.ones((6, 5), device=DEV)
+        assert be.dropout(v, 1.0, 1, out=v) is v and not bool(v.any())

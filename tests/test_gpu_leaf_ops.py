@@ -211,3 +211,8 @@ def test_large_tiles_plain(check, name):
     (3000000, 1, 17, 32, "f32", False), (2800000, 5, 200, 3, "f16", True)])
 def test_trees_in_runs(check, rows, inputs, width, trees, dtype, strided):
     check("tree_runs", rows=rows, inputs=inputs, width=width, trees=trees, dtype=dtype, strided=strided)
+
+
+@pytest.mark.parametrize("name", ["versions"])
+def test_contracts(check, name):
+    check(name)
