@@ -76,6 +76,7 @@ int queue(lgbm_hip_ctx* c, void* const* stream, F&& work) {
   if (device != own && hipSetDevice(own) != hipSuccess)
     return context_error(c, LGBM_HIP_ERR_HIP, "hipSetDevice");
   const hipStream_t s = stream ? (hipStream_t)*stream : context_stream(c);
+  (void)hipGetLastError();  // an earlier call's
   work(s);
   hipError_t e = hipGetLastError();
   if (e == hipSuccess && !stream) e = hipStreamSynchronize(s);

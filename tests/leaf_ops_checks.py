@@ -864,3 +864,21 @@ def versions():
     with torch.inference_mode():
         v = torch.ones((6, 5), device=DEV)
         assert be.dropout(v, 1.0, 1, out=v) is v and not bool(v.any())
+
+
+def earlier_error():
+    """An error that an earlier call of the program left in the HIP runtime is not this call's."""
+    be = backend()
+    with open("/proc/self/maps") as maps:
+        path = next(line.split()[-1] for line in maps if "libamdhip64" in line)
+    hip = C.CDLL(path)
+    x = torch.ones((4, 5), device=DEV)
+    out = torch.empty_like(x)
+    want = be.dropout(x, 0.5, 1)
+    torch.cuda.synchronize()
+    assert hip.hipSetDevice(C.c_int(99)) != 0  # no such device
+    try:
+        be.dropout(x, 0.5, 1, out=out)
+    finally:
+        hip.hipGetLastError()
+    assert torch.equal(out, want)

@@ -213,6 +213,6 @@ def test_trees_in_runs(check, rows, inputs, width, trees, dtype, strided):
     check("tree_runs", rows=rows, inputs=inputs, width=width, trees=trees, dtype=dtype, strided=strided)
 
 
-@pytest.mark.parametrize("name", ["versions"])
+@pytest.mark.parametrize("name", ["versions", "earlier_error"])
 def test_contracts(check, name):
     check(name)
