@@ -50,9 +50,12 @@ template <typename T>
 __device__ __forceinline__ double exp_of(double v) {
   return exp(v);
 }
-// The larger; a NaN is passed over (it comes back through the sum).
-__device__ __forceinline__ float top_of(float a, float b) { return fmaxf(a, b); }
+// The larger.  A NaN that is one of them comes through in float32, which has an instruction
+// for it; in float64 it is passed over, and found by is_nan beside the maximum.
+__device__ __forceinline__ float top_of(float a, float b) { return __builtin_elementwise_maximum(a, b); }
 __device__ __forceinline__ double top_of(double a, double b) { return fmax(a, b); }
+__device__ __forceinline__ bool is_nan(float) { return false; }
+__device__ __forceinline__ bool is_nan(double a) { return a != a; }
 // s, or -inf where bit e is set.
 __device__ __forceinline__ float unless(uint32_t bits, int e, float s) {
   const uint32_t m = (uint32_t)((int32_t)(bits << (31 - e)) >> 31);
@@ -61,10 +64,13 @@ __device__ __forceinline__ float unless(uint32_t bits, int e, float s) {
 __device__ __forceinline__ double unless(uint32_t bits, int e, double s) {
   return (bits >> e) & 1 ? -INFINITY : s;
 }
-// What the exponentials are relative to: where every class is masked their -inf stays.
+// What the exponentials are relative to.  Where every class is masked their -inf stays; in a
+// row of a NaN no exponential but a masked class's may be 0, so that the NaN of their sum
+// reaches the others.
 template <typename A>
 __device__ __forceinline__ A base_of(A top) {
-  return top == -INFINITY ? (A)0 : top;
+  const A lowest = sizeof(A) == 8 ? (A)-__DBL_MAX__ : (A)-__FLT_MAX__;
+  return top == -INFINITY ? (A)0 : top != top ? lowest : top;
 }
 
 // What a row's scores are adjusted by.
@@ -150,14 +156,16 @@ __global__ __launch_bounds__(THREADS) void k_scores_thread(ScoreArgs a, uint32_t
         }
       }
       A top = -INFINITY;
+      bool nan = false;
       for (int j = 0; j < V; ++j) {
         const A s = adjusted(mine[j], a.ids ? counts[j] : 0, row, bias ? (A)bias[j] : (A)0,
                              (allowed >> j) & 1);
         mine[j] = s;
         top = top_of(top, s);
+        nan |= is_nan(s);
       }
       if (a.kind == LGBM_HIP_PREDICT_TRANSFORMED) {
-        const A base = base_of(top);
+        const A base = base_of(nan ? (A)NAN : top);
         A sum = 0;
         for (int j = 0; j < V; ++j) {
           const A e = exp_of<T>(mine[j] - base);
@@ -194,9 +202,11 @@ enum { WHOLE, PART, FINISH };
 constexpr int CHUNK_BYTES = 32;
 
 // LANES of one row, each with NV vectors of VW neighbouring classes, LANES * NV * VW classes
-// from c0 on.
+// from c0 on.  float64's FINISH is held to the registers of five waves a SIMD (200 x 60000 75
+// us, by the 101 registers that the compiler takes else 79).
 template <typename T, int LANES, int NV, int VW, int MODE>
-__global__ __launch_bounds__(LANES < THREADS ? THREADS : LANES) void k_scores_row(ScoreArgs a, int chunks) {
+__global__ __launch_bounds__(LANES < THREADS ? THREADS : LANES,
+                             MODE == FINISH && sizeof(T) == 8 && LANES <= 512 ? 5 : 1) void k_scores_row(ScoreArgs a, int chunks) {
   typedef typename Wide<T>::type A;
   constexpr int CAP = LANES * NV * VW, TEAMS = LANES < THREADS ? THREADS / LANES : 1;
   __shared__ __align__(16) uint32_t counts[TEAMS * CAP];
@@ -217,8 +227,8 @@ __global__ __launch_bounds__(LANES < THREADS ? THREADS : LANES) void k_scores_ro
     for (int d = 1; d < 64; d <<= 1) v = join(v, (A)__shfl_xor(v, d));
     return v;
   };
-  auto reduce = [&](A v, auto join) {
-    v = of_wave(v, join);
+  // v: already of the wave
+  auto of_block = [&](A v, auto join) {
     if (LANES > 64) {
       __syncthreads();
       if (lane % 64 == 0) shared[lane / 64] = v;
@@ -229,8 +239,13 @@ __global__ __launch_bounds__(LANES < THREADS ? THREADS : LANES) void k_scores_ro
     }
     return v;
   };
-  const auto larger = [](A p, A q) { return top_of(p, q); };
   const auto plus = [](A p, A q) { return p + q; };
+  const auto larger = [](A p, A q) { return top_of(p, q); };
+  // the maximum over a wave, NaN where a lane's `nan` is set
+  auto top_of_wave = [&](A v, bool nan) {
+    v = of_wave(v, larger);
+    return __any(nan) ? (A)NAN : v;
+  };
   const int64_t tasks = a.rows * chunks;
   for (int64_t task = blockIdx.x * (int64_t)TEAMS + team; task < tasks;
        task += (int64_t)gridDim.x * TEAMS) {
@@ -279,6 +294,7 @@ __global__ __launch_bounds__(LANES < THREADS ? THREADS : LANES) void k_scores_ro
       sync();
     }
     A top = -INFINITY;
+    bool nan = false;
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
       const int j = (i * LANES + lane) * VW;
@@ -301,19 +317,30 @@ __global__ __launch_bounds__(LANES < THREADS ? THREADS : LANES) void k_scores_ro
 #pragma unroll
         for (int e = 0; e < VW; ++e) s[i][e] = unless(refused[i], e, s[i][e]);
 #pragma unroll
-      for (int e = 0; e < VW; ++e) top = top_of(top, s[i][e]);
+      for (int e = 0; e < VW; ++e) top = top_of(top, s[i][e]), nan |= is_nan(s[i][e]);
     }
     if (seen) sync();  // the counts are read before the next row's are cleared
     A scale = 1;
     const bool probabilities = a.kind == LGBM_HIP_PREDICT_TRANSFORMED;
     if (probabilities) {
-      A* const parts = (A*)a.ws;  // [rows][chunks]: maximum, sum
-      if (MODE == FINISH) {
-        top = -INFINITY;
-        for (int c = lane; c < chunks; c += LANES) top = top_of(top, parts[(n * chunks + c) * 2]);
+      A* const parts = (A*)a.ws;  // [rows][chunks]: maximum (NaN: of a NaN), sum
+      if (MODE == FINISH) {  // each wave for itself
+        top = -INFINITY, nan = false;
+        for (int c = lane % 64; c < chunks; c += 64) {
+          const A t = parts[(n * chunks + c) * 2];
+          top = top_of(top, t), nan |= is_nan(t);
+        }
       }
       // a part's waves are joined at its end, in one turn of the block
-      top = MODE == PART ? of_wave(top, larger) : reduce(top, larger);
+      top = top_of_wave(top, nan);
+      if (MODE == WHOLE && LANES > 64) {
+        nan = false;
+        top = of_block(top, [&](A p, A q) {
+          nan |= is_nan(p) || is_nan(q);
+          return top_of(p, q);
+        });
+        if (nan) top = NAN;
+      }
       const A base = base_of(top);
       A sum = 0;
 #pragma unroll
@@ -334,16 +361,16 @@ __global__ __launch_bounds__(LANES < THREADS ? THREADS : LANES) void k_scores_ro
         __syncthreads();
         if (lane < 64) {
           A t = lane < LANES / 64 ? shared[lane] : (A)-INFINITY;
-          top = of_wave(t, larger);
+          top = top_of_wave(t, is_nan(t));
           sum = of_wave(lane < LANES / 64 ? sums[lane] * exp_of<A>(t - base_of(top)) : (A)0, plus);
           if (lane == 0) parts[task * 2] = top, parts[task * 2 + 1] = sum;
         }
         continue;
       }
-      sum = reduce(sum, plus);
+      sum = of_block(of_wave(sum, plus), plus);
       scale = 1 / sum;
     }
-    if (!(scale <= 1)) {  // of a NaN, or of no class: 0 stays 0 beside it
+    if (!(scale <= 1)) {  // of a NaN or an infinity, or of no class: 0 stays 0 beside it
 #pragma unroll
       for (int i = 0; i < NV; ++i)
 #pragma unroll

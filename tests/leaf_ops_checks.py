@@ -882,3 +882,30 @@ def earlier_error():
     finally:
         hip.hipGetLastError()
     assert torch.equal(out, want)
+
+
+def scores_nan(classes, dtype):
+    """A NaN that is not masked: the row's probabilities are NaN, also where they would vanish
+    beside the row's largest, but for those of classes at -inf."""
+    dt, rows = TYPES[dtype], 5
+    rng = np.random.default_rng(classes)
+    x = torch.from_numpy(rng.standard_normal((rows, classes))).to(dt)
+    x[:, 1] = -1000  # e^-1000 is 0 in every type
+    x[:, 0], x[:, 2] = -float("inf"), float("inf")
+    x[:4, 2] = 3
+    at = [classes - 1, 3, classes // 2, 0, 4]
+    for n in (0, 1, 2, 4):
+        x[n, at[n]] = float("nan")
+    allowed = rng.random((rows, classes)) < 0.7
+    allowed[:, 1:5] = True
+    for n in (0, 1, 2, 4):
+        allowed[n, at[n]] = True
+    allowed[0, 3] = False
+    bits = np.zeros((rows, (classes + 31) // 32 * 32), bool)
+    bits[:, :classes] = allowed
+    mask = torch.from_numpy(np.packbits(bits, axis=1, bitorder="little").view(np.int32)).to(DEV)
+    p = wide(backend().adjust_scores(x.to(DEV), "transformed", mask=mask))
+    none = ~allowed | np.isneginf(wide(x))
+    for n in (0, 1, 2, 4):
+        assert (p[n, none[n]] == 0).all() and np.isnan(p[n, ~none[n]]).all(), n
+    assert (p[3, none[3]] == 0).all() and p[3, 1] == 0 and abs(p[3].sum() - 1) < 0.05

@@ -216,3 +216,9 @@ def test_trees_in_runs(check, rows, inputs, width, trees, dtype, strided):
 @pytest.mark.parametrize("name", ["versions", "earlier_error"])
 def test_contracts(check, name):
     check(name)
+
+
+@pytest.mark.parametrize("dtype", ["f64", "f32", "bf16", "f16"])
+@pytest.mark.parametrize("classes", [6, 32, 33, 300, 700, 5000, 20000, 100001])
+def test_scores_nan(check, classes, dtype):
+    check("scores_nan", classes=classes, dtype=dtype)
