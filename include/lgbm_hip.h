@@ -727,8 +727,9 @@ int lgbm_hip_predict_early_stop(lgbm_hip_ctx* ctx, const lgbm_hip_model* model, 
  * have to be complete before the call.  Nothing is allocated: working memory is the
  * caller's (d_ws, 16-byte aligned, of the size that the _workspace entry gives; unused
  * after the work is done, and not shared by calls that may run at the same time).
- * Outputs must not overlap inputs unless an entry says so.  Matrices are row-major with a
- * row stride in elements (at least the columns); any alignment of the element type.  The
+ * Outputs must not overlap inputs unless an entry says so; matrices of one row stride may
+ * lie side by side in a table.  Matrices are row-major with a row stride in elements (at
+ * least the columns); any alignment of the element type.  The
  * caller's current device is the same after a call.  Results depend neither on the order
  * in which blocks run nor on the device's number of CUs. */
 #define LGBM_HIP_DTYPE_BF16 2

@@ -38,14 +38,20 @@ int64_t type_size(int32_t dtype) {
 struct Span {
   const void* p;
   int64_t bytes;
+  int64_t row, pitch;  // of a matrix: the bytes of a row, and from row to row
 };
 Span matrix(const void* p, int64_t rows, int64_t cols, int64_t ld, int64_t e) {
-  return {p, rows > 0 ? ((rows - 1) * ld + cols) * e : 0};
+  return {p, rows > 0 ? ((rows - 1) * ld + cols) * e : 0, cols * e, ld * e};
 }
 bool overlap(const Span& a, const Span& b) {
   const uintptr_t x = (uintptr_t)a.p, y = (uintptr_t)b.p;
-  return a.p && b.p && a.bytes > 0 && b.bytes > 0 && x < y + (uintptr_t)b.bytes &&
-         y < x + (uintptr_t)a.bytes;
+  if (!(a.p && b.p && a.bytes > 0 && b.bytes > 0 && x < y + (uintptr_t)b.bytes && y < x + (uintptr_t)a.bytes))
+    return false;
+  if (a.pitch <= 0 || a.pitch != b.pitch) return true;
+  // matrices side by side in one table: where b's row begins within a's pitch
+  const uintptr_t pitch = (uintptr_t)a.pitch;
+  const uintptr_t at = y >= x ? (y - x) % pitch : (pitch - (x - y) % pitch) % pitch;
+  return at < (uintptr_t)a.row || at + (uintptr_t)b.row > pitch;
 }
 bool overlaps(const Span& out, std::initializer_list<Span> in) {
   for (const Span& s : in)

@@ -909,3 +909,25 @@ def scores_nan(classes, dtype):
     for n in (0, 1, 2, 4):
         assert (p[n, none[n]] == 0).all() and np.isnan(p[n, ~none[n]]).all(), n
     assert (p[3, none[3]] == 0).all() and p[3, 1] == 0 and abs(p[3].sum() - 1) < 0.05
+
+
+def side_by_side():
+    """Inputs and outputs as columns of one table."""
+    be = backend()
+    rng = np.random.default_rng(31)
+    table = matrix(rng, 300, 40, torch.float32)
+    x, y, d, p = table[:, :20], table[:, 20:26], table[:, 26:32], table[:, 34:40]
+    kept = table[:, 32:34].clone()
+    leaf = torch.from_numpy(leaves_of(rng, 300, 2, 5, "lost")).to(DEV)
+    g = be.leaf_groups(leaf, 5)
+    w = matrix(rng, 60, 20, torch.float32).view(10, 6, 20)
+    x0 = x.clone()
+    want = be.leaf_product(x0, w, g)
+    assert be.leaf_product(x, w, g, out=y) is y and torch.equal(y, want)
+    be.dropout(y, 0.3, 7, out=d)
+    assert torch.equal(d, be.dropout(want, 0.3, 7))
+    be.adjust_scores(d, "transformed", out=p)
+    assert torch.equal(p, be.adjust_scores(d.clone(), "transformed"))
+    dx = be.leaf_product_dx(p.clone(), w, g)
+    be.leaf_product_dx(p, w, g, out=x)
+    assert torch.equal(x, dx) and torch.equal(y, want) and torch.equal(table[:, 32:34], kept)

@@ -315,3 +315,28 @@ def test_python_refuses_what_autograd_would_lose():
             call(**t)
         with pytest.raises(ValueError, match="is on cpu"):
             call(**{k: v.detach() for k, v in t.items()})
+
+
+@pytest.mark.parametrize("out,ldx,ldo,text", [
+    (A + 32, 16, 16, "null context"), (A - 32, 16, 16, "null context"), (A + 64 * 7 + 32, 16, 16, "null context"),
+    (A + 28, 16, 16, "in place"), (A + 36, 16, 16, "in place"), (A - 28, 16, 16, "in place"),
+    (A - 36, 16, 16, "in place"), (A + 64, 16, 16, "in place"), (A - 64 * 3, 16, 16, "in place"),
+    (A + 32, 16, 24, "in place"), (A + 32, 8, 8, "in place"), (A + 3200, 8, 8, "null context")])
+def test_tables_side_by_side(lib, out, ldx, ldo, text):
+    """Eight columns of a table may go to eight others: rows of one stride overlap where their
+    columns do, other matrices where their memory does."""
+    refused(lib, dropout(lib, out=out, ldx=ldx, ldo=ldo), INVALID, text)
+
+
+def test_products_side_by_side(lib):
+    """x or dy, and y or dx, as columns of one table."""
+    it = calls(lib, maps(), p1=D, ld1=20, out=D + 5 * 4, ldo=20)
+    refused(lib, next(it), INVALID, "null context")
+    it = calls(lib, maps(), p1=D, ld1=20, out=D + 4 * 4, ldo=20)
+    refused(lib, next(it), INVALID, "overlaps")
+    rc = lib.lgbm_hip_adjust_scores(None, C.byref(score_args(ldx=80, ldo=80, out=A + 160)), C.c_void_p(W),
+                                    C.c_size_t(1 << 40), None)
+    refused(lib, rc, INVALID, "null context")
+    rc = lib.lgbm_hip_adjust_scores(None, C.byref(score_args(ldx=80, ldo=80, out=A + 164)), C.c_void_p(W),
+                                    C.c_size_t(1 << 40), None)
+    refused(lib, rc, INVALID, "in place")
