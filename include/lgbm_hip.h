@@ -832,7 +832,7 @@ typedef struct lgbm_score_args {
   const int64_t* d_offsets;   /* [num_rows + 1]: row n's history is ids[offsets[n] ..
                                  offsets[n + 1]) */
   int64_t num_ids;
-  double repetition; /* > 0; 1: none */
+  double repetition; /* > 0, also as a float32 where that is the arithmetic's; 1: none */
   double frequency;
   double presence;
   const float* d_penalties; /* [num_rows][3] (repetition, frequency, presence) instead of

@@ -301,8 +301,11 @@ static int check_scores(lgbm_hip_ctx* c, const lgbm_score_args* a) {
   if (a->d_ids || a->d_offsets || a->num_ids) {
     if (a->num_ids < 0 || !a->d_offsets || (a->num_ids > 0 && !a->d_ids))
       return bad(c, "a history needs ids and offsets");
-    if (!a->d_penalties && !(a->repetition > 0.0 && std::isfinite(a->repetition) &&
-                             std::isfinite(a->frequency) && std::isfinite(a->presence)))
+    // in the type of the arithmetic, where a small repetition may be 0 and a large one infinite
+    const bool wide = a->dtype == LGBM_HIP_DTYPE_F64;
+    const auto of = [&](double v) { return wide ? v : (double)(float)v; };
+    if (!a->d_penalties && !(of(a->repetition) > 0.0 && std::isfinite(of(a->repetition)) &&
+                             std::isfinite(of(a->frequency)) && std::isfinite(of(a->presence))))
       return bad(c, "repetition not positive, or a penalty not finite");
   }
   if (misaligned(a->d_x, e) || misaligned(a->d_out, e) || misaligned(a->d_bias, e) ||

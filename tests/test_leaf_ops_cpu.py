@@ -340,3 +340,12 @@ def test_products_side_by_side(lib):
     rc = lib.lgbm_hip_adjust_scores(None, C.byref(score_args(ldx=80, ldo=80, out=A + 164)), C.c_void_p(W),
                                     C.c_size_t(1 << 40), None)
     refused(lib, rc, INVALID, "in place")
+
+
+@pytest.mark.parametrize("change", [dict(repetition=1e-46), dict(repetition=1e39), dict(frequency=-1e39), dict(presence=1e300)])
+@pytest.mark.parametrize("dtype", [0, 1, 2, 3])
+def test_penalties_in_the_type_of_the_arithmetic(lib, change, dtype):
+    """What is 0 or infinite as a float32 is refused where the arithmetic is float32."""
+    rc = lib.lgbm_hip_adjust_scores(None, C.byref(score_args(**HISTORY, dtype=dtype, **change)), C.c_void_p(W),
+                                    C.c_size_t(1 << 40), None)
+    refused(lib, rc, INVALID, "null context" if dtype == 1 else "not positive, or a penalty not finite")
