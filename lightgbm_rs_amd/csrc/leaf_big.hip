@@ -86,21 +86,20 @@ __device__ __forceinline__ u32x4 cm_frag32(const char* tile, int base, int step,
 // of 2048 to 2048: 824 us in their order, 789).
 __device__ __forceinline__ DwPart part_of_rank(const LeafProduct& p, const Split& split, int rank) {
   __shared__ int fulls[THREADS], ends[THREADS];
-  __shared__ int found[4];  // leaf of the forest, -1: none; first row, rows, slot
-  const int tid = threadIdx.x, leaves = p.g.trees * p.g.leaves, tree0 = tid / p.g.leaves * p.g.leaves;
+  __shared__ int found[3];  // leaf of the forest, -1: none; first row, rows
+  const int tid = threadIdx.x, leaves = p.g.trees * p.g.leaves;
   const int count = tid < leaves ? min(max(p.g.count[tid], 0), p.g.rows) : 0;
   const int full = split.rows ? count / split.rows : 0, end = count - full * split.rows;
   fulls[tid] = full, ends[tid] = end;
   if (tid == 0) found[0] = -1;
   __syncthreads();
-  int longer = 0, before = 0, all = 0, slot = 0;
+  int longer = 0, before = 0, all = 0;
 #pragma unroll 8
   for (int l = 0; l < leaves; ++l) {
     const int f = fulls[l], e = ends[l];
     longer += e > end || (e == end && l < tid);
     all += f;
     before += l < tid ? f : 0;
-    slot += l >= tree0 && l < tid ? f + (e > 0) : 0;
   }
   // a leaf without rows is a part where leaves are not split: its zeros
   const bool in_full = rank >= before && rank < before + full;
@@ -109,14 +108,12 @@ __device__ __forceinline__ DwPart part_of_rank(const LeafProduct& p, const Split
     found[0] = tid;
     found[1] = min(max(p.g.begin[tid], 0), p.g.rows - count) + skip * split.rows;
     found[2] = in_full ? split.rows : end;
-    found[3] = slot + skip;
   }
   __syncthreads();
   const int at = __builtin_amdgcn_readfirstlane(found[0]);
-  // a table whose counts exceed its rows may ask for more slots than there are
-  if (at < 0 || (split.rows && found[3] >= split.slots)) return {0, 0, -1, nullptr, nullptr};
+  if (at < 0) return {0, 0, -1, nullptr, nullptr};
   return dw_part_of(p, split, at / p.g.leaves, at % p.g.leaves, __builtin_amdgcn_readfirstlane(found[1]),
-                    __builtin_amdgcn_readfirstlane(found[2]), __builtin_amdgcn_readfirstlane(found[3]));
+                    __builtin_amdgcn_readfirstlane(found[2]));
 }
 
 // MODE LEAF_PRODUCT_Y: a = x rows [k], b = w[leaf] [col][k]; _DX: a = dy rows [m], b = w[leaf]
@@ -150,7 +147,7 @@ __global__ __launch_bounds__(THREADS, 1) void k_leaf_big(LeafProduct p, int col_
       const int of = (p.outputs + BM - 1) / BM * col_tiles, tile = (int)(blockIdx.x % of);
       const int id = (int)(blockIdx.x / of);
       part = p.g.trees * (int64_t)p.g.leaves <= THREADS
-                 ? part_of_rank(p, split, (int)(blockIdx.y * split.slots) + id)
+                 ? part_of_rank(p, split, (int)(blockIdx.y * split.parts) + id)
                  : dw_part<THREADS>(p, split, id);
       if (part.count < 0) return;
       tree = part.tree, first = part.first, length = part.count;
@@ -438,7 +435,7 @@ __global__ __launch_bounds__(THREADS, 1) void k_leaf_big(LeafProduct p, int col_
 template <typename T>
 void launch(const LeafProduct& p, int what, hipStream_t s) {
   const int cols = what == LEAF_PRODUCT_Y ? p.outputs : p.inputs, ct = (cols + BN - 1) / BN;
-  const Split split = what == LEAF_PRODUCT_DW ? leaf_big_split(p) : Split{0, 0};
+  const Split split = what == LEAF_PRODUCT_DW ? leaf_big_split(p) : Split{0, 0, 0};
   const dim3 grid((unsigned)leaf_big_blocks(p, what),
                   what == LEAF_PRODUCT_DW && split.rows == 0 ? 1u : (unsigned)p.g.trees);
   if (what == LEAF_PRODUCT_Y)
@@ -460,15 +457,14 @@ Split leaf_big_split(const LeafProduct& p) {
   const int64_t tiles = (int64_t)((p.outputs + BM - 1) / BM) * ((p.inputs + BN - 1) / BN);
   const int64_t share = (p.g.rows * (int64_t)p.g.trees * tiles / 256 + BK - 1) / BK * BK;
   const int64_t rows = std::min<int64_t>(std::max<int64_t>(share, 512), CHAIN_ROWS);
-  if (rows >= p.g.rows) return {0, 0};
-  return {(int)rows, row_tiles(p.g, rows)};
+  return split_by(p.g, rows);
 }
 
 int64_t leaf_big_blocks(const LeafProduct& p, int what) {
   const int64_t ct = ((what == LEAF_PRODUCT_Y ? p.outputs : p.inputs) + BN - 1) / BN;
   if (what == LEAF_PRODUCT_DW) {
     const Split split = leaf_big_split(p);
-    return (p.outputs + BM - 1) / BM * ct * (split.rows ? split.slots : (int64_t)p.g.trees * p.g.leaves);
+    return (p.outputs + BM - 1) / BM * ct * (split.rows ? split.parts : (int64_t)p.g.trees * p.g.leaves);
   }
   return std::min<int64_t>((row_tiles(p.g, BM) * ct + 7) / 8 * 8, 256);  // one a CU
 }

@@ -122,9 +122,11 @@ struct RowTile {
   int rows;   // 0: there is no such tile
 };
 
-// Tile number `mt` of a tree: the leaves' rows in tiles of `bm`, then the rows in no leaf.
-// Every thread of the block takes part; counts and begins are held within [0, rows], so
-// that a wrong table cannot reach outside the order.
+// Tile number `mt` of a tree, below MAX_TILES: the leaves' rows in tiles of `bm`, then the rows
+// in no leaf.  Every thread of the block takes part; counts and begins are held within [0,
+// rows], and a leaf's and a wave's tiles to MAX_TILES, so that a wrong table can neither reach
+// outside the order nor have sums that wrap, by which two threads would find the tile.
+constexpr int MAX_TILES = 1 << 24;  // blocks of a launch
 template <int THREADS>
 __device__ RowTile find_tile(const LeafGroups& g, int tree, int mt, int bm) {
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
@@ -142,7 +144,7 @@ __device__ RowTile find_tile(const LeafGroups& g, int tree, int mt, int bm) {
     if (l < g.leaves) c = min(max(count[l], 0), g.rows);
     // of 64 leaves at most 2^6 times 2^31 rows: held back to the rows there are, which
     // only counts that exceed them reach
-    const int tiles = (int)(((int64_t)c + bm - 1) / bm);
+    const int tiles = (int)min(((int64_t)c + bm - 1) / bm, (int64_t)MAX_TILES);
     int incl = tiles, rows = c;
 #pragma unroll
     for (int d = 1; d < 64; d <<= 1) {
@@ -152,7 +154,7 @@ __device__ RowTile find_tile(const LeafGroups& g, int tree, int mt, int bm) {
     }
     __syncthreads();
     if (lane == 63) {
-      wave_tiles[wave] = incl;
+      wave_tiles[wave] = min(incl, MAX_TILES);
       wave_rows[wave] = rows;
     }
     __syncthreads();
@@ -178,7 +180,14 @@ __device__ RowTile find_tile(const LeafGroups& g, int tree, int mt, int bm) {
   return found;
 }
 
-// How many tiles a tree has.
+// A bound of a tree's tiles: whole ones, an end for every leaf and for the rows in none, and
+// no tile without a row.
+__host__ __device__ inline int64_t row_tiles(const LeafGroups& g, int64_t bm) {
+  const int64_t tiles = (g.rows + bm - 1) / bm + g.leaves + 1;
+  return tiles < g.rows ? tiles : g.rows;
+}
+
+// How many tiles a tree has (a wrong table's counts may ask for more than there can be).
 template <int THREADS>
 __device__ int count_tiles(const LeafGroups& g, int tree, int bm) {
   __shared__ int64_t wave_tiles[THREADS / 64], wave_rows[THREADS / 64];
@@ -200,14 +209,7 @@ __device__ int count_tiles(const LeafGroups& g, int tree, int bm) {
 #pragma unroll
   for (int w = 0; w < THREADS / 64; ++w) tiles += wave_tiles[w], rows += wave_rows[w];
   if (rows < g.rows) tiles += (g.rows - rows + bm - 1) / bm;
-  return (int)min(tiles, (int64_t)0x7fffffff);
-}
-
-// A bound of a tree's tiles: whole ones, an end for every leaf and for the rows in none, and
-// no tile without a row.
-inline int64_t row_tiles(const LeafGroups& g, int64_t bm) {
-  const int64_t tiles = (g.rows + bm - 1) / bm + g.leaves + 1;
-  return tiles < g.rows ? tiles : g.rows;
+  return (int)min(tiles, row_tiles(g, bm));
 }
 
 // The row at a position of a tree's order, -1 for an entry outside the matrix.
@@ -218,13 +220,23 @@ __device__ __forceinline__ int row_at(const LeafGroups& g, int tree, int positio
 
 // ---- parts of the maps' gradients --------------------------------------------------------------
 
-// Rows a block sums at most, 0: a leaf's rows are not split.  The sums of a leaf of more rows
-// go to slots in the workspace, [tree][slots][outputs * inputs + outputs], in the order of
-// find_tile's tiles, and k_sum_slots adds them; a leaf of one part has its place in dw.
+// Rows a block sums at most, 0: a leaf's rows are not split.  The parts of a leaf of more rows
+// go to slots in the workspace, [tree][slots][outputs * inputs + outputs], and k_sum_slots
+// adds them; a leaf of one part has its place in dw.  A part's slot follows from where it
+// begins in the order: of the parts that begin in one stretch of `rows` one at most, the first of
+// its leaf, is not the last of another, so two slots for a stretch are enough, whatever the
+// leaves.
 struct Split {
   int rows;
-  int64_t slots;  // a tree
+  int64_t parts, slots;  // of a tree, at most
 };
+inline Split split_by(const LeafGroups& g, int64_t rows) {
+  if (rows >= g.rows) return {0, 0, 0};
+  return {(int)rows, row_tiles(g, rows), 2 * ((g.rows - 1) / rows + 1)};
+}
+__device__ __forceinline__ int64_t slot_of(const Split& split, int first, bool first_of_leaf) {
+  return 2 * (int64_t)(first / split.rows) + first_of_leaf;
+}
 
 // The longest chain of float32 adds over rows: the running sum's rounding is 8192 terms' at
 // most (600000 rows of the same bfloat16 value in one chain were off by 4 in 1000).
@@ -235,13 +247,16 @@ struct DwPart {
   int tree, first, count;  // count -1: nothing
   float *dw, *db;
 };
-// `rows` from `first` on of a leaf, its slot-th part of the tree's.
+// `rows` from `first` on of a leaf.
 __device__ __forceinline__ DwPart dw_part_of(const LeafProduct& p, const Split& split, int tree, int leaf, int first,
-                                             int rows, int64_t slot) {
+                                             int rows) {
   const int64_t size = (int64_t)p.outputs * p.inputs, at = (int64_t)tree * p.g.leaves + leaf;
-  const bool whole = split.rows == 0 || min(max(p.g.count[at], 0), p.g.rows) <= split.rows;
-  float* const dw = whole ? p.dw + at * size : (float*)p.ws + (tree * split.slots + slot) * (size + p.outputs);
-  return {tree, first, rows, dw, !p.db ? nullptr : whole ? p.db + at * p.outputs : dw + size};
+  const int count = min(max(p.g.count[at], 0), p.g.rows);
+  if (split.rows == 0 || count <= split.rows)
+    return {tree, first, rows, p.dw + at * size, p.db ? p.db + at * p.outputs : nullptr};
+  const int64_t slot = slot_of(split, first, first == min(max(p.g.begin[at], 0), p.g.rows - count));
+  float* const dw = (float*)p.ws + (tree * split.slots + slot) * (size + p.outputs);
+  return {tree, first, rows, dw, p.db ? dw + size : nullptr};
 }
 // Part number `id`: of tree blockIdx.y where leaves are split, else a leaf of the forest.
 template <int THREADS>
@@ -249,11 +264,10 @@ __device__ __forceinline__ DwPart dw_part(const LeafProduct& p, const Split& spl
   if (split.rows) {
     const RowTile rt = find_tile<THREADS>(p.g, blockIdx.y, id, split.rows);
     if (rt.rows == 0 || rt.leaf < 0) return {0, 0, -1, nullptr, nullptr};
-    return dw_part_of(p, split, blockIdx.y, rt.leaf, rt.first, rt.rows, id);
+    return dw_part_of(p, split, blockIdx.y, rt.leaf, rt.first, rt.rows);
   }
   const int count = min(max(p.g.count[id], 0), p.g.rows);
-  return dw_part_of(p, split, id / p.g.leaves, id % p.g.leaves, min(max(p.g.begin[id], 0), p.g.rows - count), count,
-                    0);
+  return dw_part_of(p, split, id / p.g.leaves, id % p.g.leaves, min(max(p.g.begin[id], 0), p.g.rows - count), count);
 }
 
 // The results v of column col in rows n[0 .. 4) (-1: none), to the output of one tree or to a

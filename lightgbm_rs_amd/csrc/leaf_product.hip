@@ -438,8 +438,7 @@ Split dw_split(const LeafProduct& p, int64_t tiles) {
   const int64_t work = (int64_t)p.g.rows * p.g.trees * tiles;
   int64_t rows = (work / (tiles <= 64 ? 2048 : 1024) + 255) / 256 * 256;
   rows = std::min<int64_t>(std::max<int64_t>(rows, 512), CHAIN_ROWS);
-  if (rows >= p.g.rows) return {0, 0};
-  return {(int)rows, row_tiles(p.g, rows)};
+  return split_by(p.g, rows);
 }
 
 // dw[leaf][m][k] = sum over the leaf's rows of dy[row][m] * x[row][k]; db[leaf][m] their sum.
@@ -651,28 +650,20 @@ __global__ __launch_bounds__(THREADS) void k_leaf_dw_small(LeafProduct p, Split 
 // The slots of a leaf of several parts added in their order, by `parts` blocks a leaf, in
 // float64: a long leaf has hundreds.  A leaf without rows gets its zeros here.
 __global__ __launch_bounds__(THREADS) void k_sum_slots(LeafProduct p, Split split, int parts) {
-  __shared__ int before[THREADS / 64];
   const int64_t at = blockIdx.x / parts;  // leaf of the forest
-  const int tree = (int)(at / p.g.leaves), leaf = (int)(at - (int64_t)tree * p.g.leaves);
-  const int32_t* const counts = p.g.count + (int64_t)tree * p.g.leaves;
-  const int64_t num = ((int64_t)min(max(counts[leaf], 0), p.g.rows) + split.rows - 1) / split.rows;
-  if (num == 1) return;
-  int tiles = 0;
-  for (int l = threadIdx.x; l < leaf; l += THREADS)
-    tiles += (int)(((int64_t)min(max(counts[l], 0), p.g.rows) + split.rows - 1) / split.rows);
-#pragma unroll
-  for (int d = 1; d < 64; d <<= 1) tiles += __shfl_xor(tiles, d);
-  if ((threadIdx.x & 63) == 0) before[threadIdx.x >> 6] = tiles;
-  __syncthreads();
-  const int64_t from = (int64_t)before[0] + before[1] + before[2] + before[3];
-  const int64_t to = min(from + num, split.slots);
+  const int tree = (int)(at / p.g.leaves);
+  const int count = min(max(p.g.count[at], 0), p.g.rows), begin = min(max(p.g.begin[at], 0), p.g.rows - count);
+  if (count > 0 && count <= split.rows) return;
+  const int more = (int)(((int64_t)count + split.rows - 1) / split.rows) - 1;  // parts behind the first
   const int64_t map = (int64_t)p.outputs * p.inputs, size = map + p.outputs;
   const int64_t used = p.db ? size : map;
   const float* const slots = (const float*)p.ws + tree * split.slots * size;
+  const float* const first = slots + slot_of(split, begin, true) * size;
+  const float* const others = slots + slot_of(split, begin, false) * size;  // two slots a part
   for (int64_t e = blockIdx.x % parts * (int64_t)THREADS + threadIdx.x; e < used; e += (int64_t)parts * THREADS) {
-    double v = 0.0;
+    double v = count > 0 ? (double)first[e] : 0.0;
 #pragma unroll 16
-    for (int64_t s = from; s < to; ++s) v += (double)slots[s * size + e];
+    for (int64_t s = 1; s <= more; ++s) v += (double)others[2 * s * size + e];
     if (e < map)
       p.dw[at * map + e] = (float)v;
     else
@@ -731,7 +722,7 @@ void launch_dw(const LeafProduct& p, hipStream_t s) {
   const int mt = (p.outputs + d.bm - 1) / d.bm, kt = (p.inputs + d.bn - 1) / d.bn;
   const Split split = dw_split(p, (int64_t)mt * kt);
   const int64_t leaves = (int64_t)p.g.trees * p.g.leaves;
-  const dim3 grid = split.rows ? dim3((unsigned)(split.slots * mt * kt), p.g.trees)
+  const dim3 grid = split.rows ? dim3((unsigned)(split.parts * mt * kt), p.g.trees)
                                : dim3((unsigned)((int64_t)mt * kt * leaves));
   if (d.small && p.inputs <= 32)
     k_leaf_dw_small<T, 2><<<grid, THREADS, 0, s>>>(p, split);
@@ -883,7 +874,7 @@ int64_t leaf_product_blocks(const LeafProduct& p, int what) {
     const int64_t tiles = (int64_t)((p.outputs + d.bm - 1) / d.bm) * ((p.inputs + d.bn - 1) / d.bn);
     const Split split = dw_split(p, tiles);
     const int64_t leaves = (int64_t)p.g.trees * p.g.leaves;
-    return split.rows ? std::max(tiles * split.slots, leaves) : tiles * leaves;
+    return split.rows ? std::max(tiles * split.parts, leaves) : tiles * leaves;
   }
   const int64_t cols = what == LEAF_PRODUCT_DX ? p.inputs : p.outputs;
   if (what == LEAF_PRODUCT_DX && p.outputs <= 32) return row_tiles(p.g, 512) * ((cols + 127) / 128);

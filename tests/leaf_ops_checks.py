@@ -931,3 +931,15 @@ def side_by_side():
     dx = be.leaf_product_dx(p.clone(), w, g)
     be.leaf_product_dx(p, w, g, out=x)
     assert torch.equal(x, dx) and torch.equal(y, want) and torch.equal(table[:, 32:34], kept)
+
+
+def odd_counts():
+    """A table of a million leaves that all claim every row: together they would have more than
+    2^32 parts.  The first leaf's gradient is right, the others' are some value."""
+    rows, leaves = 2 ** 26, 2 ** 20 + 300
+    one = torch.ones((rows, 1), device=DEV)
+    g = LeafGroups(torch.arange(rows, dtype=torch.int32, device=DEV)[None],
+                   torch.zeros((1, leaves), dtype=torch.int32, device=DEV),
+                   torch.full((1, leaves), rows, dtype=torch.int32, device=DEV))
+    dw, db = backend().leaf_product_dw(one, one, g)
+    assert dw[0].item() == rows and db[0].item() == rows and bool(dw.isfinite().all())

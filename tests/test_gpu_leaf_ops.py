@@ -213,7 +213,7 @@ def test_trees_in_runs(check, rows, inputs, width, trees, dtype, strided):
     check("tree_runs", rows=rows, inputs=inputs, width=width, trees=trees, dtype=dtype, strided=strided)
 
 
-@pytest.mark.parametrize("name", ["versions", "earlier_error", "side_by_side"])
+@pytest.mark.parametrize("name", ["versions", "earlier_error", "side_by_side", "odd_counts"])
 def test_contracts(check, name):
     check(name)
 

@@ -271,9 +271,20 @@ def test_gradients_take_the_card(lib, rows, inputs, outputs, dtype):
     m = maps(rows=rows, leaves=1, inputs=inputs, outputs=outputs, dtype=dtype)
     assert lib.lgbm_hip_leaf_product_workspace(C.byref(m), C.c_int32(2), C.byref(need)) == 0
     tiles = -(-inputs // 256) * -(-outputs // 256)
-    # parts of at least 512 rows, a slot for the leaf's end and one for the rows in no leaf
-    parts = need.value // (4 * outputs * (inputs + 1)) - 2
+    # two slots for each stretch of the order that is as long as a part, of at least 512 rows
+    parts = need.value // (4 * outputs * (inputs + 1)) // 2
     assert parts * tiles >= min(200, rows // 512 * tiles)
+
+
+@pytest.mark.parametrize("dtype", [0, 2])
+def test_parts_are_few(lib, dtype):
+    """The parts' working memory goes by the rows, not by the leaves, most of which are a part
+    of their own."""
+    need, other = C.c_size_t(0), C.c_size_t(0)
+    for leaves, into in ((1, need), (5000, other)):
+        m = maps(rows=100000, leaves=leaves, inputs=65, outputs=70, dtype=dtype)
+        assert lib.lgbm_hip_leaf_product_workspace(C.byref(m), C.c_int32(2), C.byref(into)) == 0
+    assert 0 < need.value == other.value <= 2 * (100000 // 512 + 1) * 4 * 70 * 66
 
 
 @pytest.mark.parametrize("what,cols", [(0, 10), (1, 100)])
