@@ -480,9 +480,9 @@ __global__ __launch_bounds__(THREADS) void k_leaf_dw(LeafProduct p, int m_tiles,
   for (int i = 0; i < WM / 16; ++i)
 #pragma unroll
     for (int j = 0; j < WN / 16; ++j) acc[i][j] = f32x4{0, 0, 0, 0};
-  f32x4 bias[WM / 16];
+  f32x4 bias[WM / 16][1];
 #pragma unroll
-  for (int i = 0; i < WM / 16; ++i) bias[i] = f32x4{0, 0, 0, 0};
+  for (int i = 0; i < WM / 16; ++i) bias[i][0] = f32x4{0, 0, 0, 0};
   const bool sums = db && k0 == 0 && wave % GN == 0;  // a product with ones
 
   // rows of step s in row_of[s & 1]; the loads of a step are two steps behind its rows
@@ -534,6 +534,7 @@ __global__ __launch_bounds__(THREADS) void k_leaf_dw(LeafProduct p, int m_tiles,
       rows(r0 + 2 * BK);  // into the half whose rows are loaded already
       const char *ta = lds[b], *tb = lds[b] + BM * 128;
       Parts<T, WM / 16, WN / 16> part(acc);
+      Parts<T, WM / 16, 1> bias_part(bias);
 #pragma unroll
       for (int step = 0; step < 2; ++step) {
         u32x4 fa[WM / 16], fb[WN / 16];
@@ -543,13 +544,15 @@ __global__ __launch_bounds__(THREADS) void k_leaf_dw(LeafProduct p, int m_tiles,
         for (int j = 0; j < WN / 16; ++j) fb[j] = cm_frag<T, BN>(tb, (wave % GN) * WN + 16 * j, step, lane);
         if (sums)
 #pragma unroll
-          for (int i = 0; i < WM / 16; ++i) bias[i] = El<T>::mfma(El<T>::ones(), fa[i], bias[i]);
+          for (int i = 0; i < WM / 16; ++i)
+            bias_part.at[i][0] = El<T>::mfma(El<T>::ones(), fa[i], bias_part.at[i][0]);
 #pragma unroll
         for (int i = 0; i < WM / 16; ++i)
 #pragma unroll
           for (int j = 0; j < WN / 16; ++j) part.at[i][j] = El<T>::mfma(fa[i], fb[j], part.at[i][j]);
       }
       part.add_to(acc);
+      if (sums) bias_part.add_to(bias);
       if (more) store(lds[b ^ 1]);
       __syncthreads();
     }
@@ -557,7 +560,7 @@ __global__ __launch_bounds__(THREADS) void k_leaf_dw(LeafProduct p, int m_tiles,
 #pragma unroll
   for (int i = 0; i < WM / 16; ++i) {
     const int mi = m0 + (wave / GN) * WM + i * 16;
-    if (sums && lane < 16 && mi + lane < p.outputs) db[mi + lane] = bias[i][0];
+    if (sums && lane < 16 && mi + lane < p.outputs) db[mi + lane] = bias[i][0][0];
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
       const int m = mi + (lane >> 4) * 4 + e;

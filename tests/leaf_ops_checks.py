@@ -943,3 +943,20 @@ def odd_counts():
                    torch.full((1, leaves), rows, dtype=torch.int32, device=DEV))
     dw, db = backend().leaf_product_dw(one, one, g)
     assert dw[0].item() == rows and db[0].item() == rows and bool(dw.isfinite().all())
+
+
+def short_sums(inputs, outputs):
+    """float32 sums go in stretches of 32 rows that start at zero: with c = 1 + 2^-15, 32 c is
+    a whole number of 2^-10, exact beside sums below 2^14, and within a stretch sums are whole
+    numbers of 2^-15 below 2^6.  So dW and db of x = 1 and dy = c are exact, where a chain of
+    single rows or fours drops the 2^-13 of 4 c beside sums above 2^11."""
+    rows = 3 * 8192
+    g = LeafGroups(torch.arange(rows, dtype=torch.int32, device=DEV)[None],
+                   torch.zeros((1, 1), dtype=torch.int32, device=DEV),
+                   torch.full((1, 1), rows, dtype=torch.int32, device=DEV))
+    x = torch.ones((rows, inputs), device=DEV)
+    dy = torch.full((rows, outputs), 1 + 2.0 ** -15, device=DEV)
+    dw, db = backend().leaf_product_dw(dy, x, g)
+    want = rows * (1 + 2.0 ** -15)
+    assert bool((dw == want).all()), (want, dw.min().item(), dw.max().item())
+    assert bool((db == want).all()), (want, db.min().item(), db.max().item())

@@ -222,3 +222,8 @@ def test_contracts(check, name):
 @pytest.mark.parametrize("classes", [6, 32, 33, 300, 700, 5000, 20000, 100001])
 def test_scores_nan(check, classes, dtype):
     check("scores_nan", classes=classes, dtype=dtype)
+
+
+@pytest.mark.parametrize("inputs,outputs", [(1280, 1280), (2000, 7), (7, 2000), (28, 1), (100, 10)])
+def test_short_sums(check, inputs, outputs):
+    check("short_sums", inputs=inputs, outputs=outputs)
