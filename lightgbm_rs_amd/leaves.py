@@ -354,6 +354,8 @@ def _adjust_scores(self, scores, kind="raw", bias=None, mask=None, mask_rows=Non
             mask = mask[None]
         _shape(mask, (mask.shape[0], (classes + 31) // 32), "mask")
         mask = _typed(mask, "mask", torch.int32)
+        if mask_rows is None and mask.shape[0] == 0 < rows:
+            raise ValueError("a mask table without masks")
     elif mask_rows is not None:
         raise ValueError("mask_rows without mask")
     if mask_rows is not None:

@@ -360,3 +360,15 @@ def test_penalties_in_the_type_of_the_arithmetic(lib, change, dtype):
     rc = lib.lgbm_hip_adjust_scores(None, C.byref(score_args(**HISTORY, dtype=dtype, **change)), C.c_void_p(W),
                                     C.c_size_t(1 << 40), None)
     refused(lib, rc, INVALID, "null context" if dtype == 1 else "not positive, or a penalty not finite")
+
+
+def test_python_refuses_no_masks():
+    """A table of no masks has no memory, which the C entry would take as no table."""
+    import torch
+    be, x = Plain(), torch.zeros((6, 5))
+    with pytest.raises(ValueError, match="without masks"):
+        be.adjust_scores(x, mask=torch.zeros((0, 1), dtype=torch.int32))
+    with pytest.raises(ValueError, match="is on cpu"):
+        be.adjust_scores(x, mask=torch.zeros((0, 1), dtype=torch.int32), mask_rows=torch.zeros(6, dtype=torch.int32))
+    with pytest.raises(ValueError, match="is on cpu"):
+        be.adjust_scores(x[:0], mask=torch.zeros((0, 1), dtype=torch.int32))
