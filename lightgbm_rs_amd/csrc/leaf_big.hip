@@ -101,9 +101,9 @@ __device__ __forceinline__ DwPart part_of_rank(const LeafProduct& p, const Split
     all += f;
     before += l < tid ? f : 0;
   }
-  // a leaf without rows is a part where leaves are not split: its zeros
+  // a leaf without rows is a part: its zeros
   const bool in_full = rank >= before && rank < before + full;
-  if (tid < leaves && (in_full || (rank == all + longer && (end > 0 || split.rows == 0)))) {
+  if (tid < leaves && (in_full || (rank == all + longer && (end > 0 || count == 0)))) {
     const int skip = in_full ? rank - before : full;
     found[0] = tid;
     found[1] = min(max(p.g.begin[tid], 0), p.g.rows - count) + skip * split.rows;
@@ -146,7 +146,7 @@ __global__ __launch_bounds__(THREADS, 1) void k_leaf_big(LeafProduct p, int col_
     if (DW) {
       const int of = (p.outputs + BM - 1) / BM * col_tiles, tile = (int)(blockIdx.x % of);
       const int id = (int)(blockIdx.x / of);
-      part = p.g.trees * (int64_t)p.g.leaves <= THREADS
+      part = leaf_big_ranks(p.g)
                  ? part_of_rank(p, split, (int)(blockIdx.y * split.parts) + id)
                  : dw_part<THREADS>(p, split, id);
       if (part.count < 0) return;

@@ -368,6 +368,9 @@ __device__ __forceinline__ u32x4 cm_frag(const char* tile, int col0, int step, i
 
 }  // namespace mma
 
-mma::Split leaf_big_split(const LeafProduct& p);  // leaf_big.hip: of the maps' gradients
+// leaf_big.hip, gradients of the maps: the parts, and whether they are taken by their length
+// (those of empty leaves, their zeros, with them)
+mma::Split leaf_big_split(const LeafProduct& p);
+__host__ __device__ inline bool leaf_big_ranks(const LeafGroups& g) { return (int64_t)g.trees * g.leaves <= 256; }
 
 }  // namespace lgbm

@@ -651,12 +651,12 @@ __global__ __launch_bounds__(THREADS) void k_leaf_dw_small(LeafProduct p, Split 
 }
 
 // The slots of a leaf of several parts added in their order, by `parts` blocks a leaf, in
-// float64: a long leaf has hundreds.  A leaf without rows gets its zeros here.
-__global__ __launch_bounds__(THREADS) void k_sum_slots(LeafProduct p, Split split, int parts) {
+// float64: a long leaf has hundreds.  `zeros`: and the zeros of leaves without rows.
+__global__ __launch_bounds__(THREADS) void k_sum_slots(LeafProduct p, Split split, int parts, bool zeros) {
   const int64_t at = blockIdx.x / parts;  // leaf of the forest
   const int tree = (int)(at / p.g.leaves);
   const int count = min(max(p.g.count[at], 0), p.g.rows), begin = min(max(p.g.begin[at], 0), p.g.rows - count);
-  if (count > 0 && count <= split.rows) return;
+  if (count <= split.rows && !(count == 0 && zeros)) return;
   const int more = (int)(((int64_t)count + split.rows - 1) / split.rows) - 1;  // parts behind the first
   const int64_t map = (int64_t)p.outputs * p.inputs, size = map + p.outputs;
   const int64_t used = p.db ? size : map;
@@ -713,10 +713,10 @@ bool wide_tiles(const LeafProduct& p, int cols) {
 
 // Leaves of one part leave most of the blocks without work (bfloat16, 60000 x 256 to 256 by 300
 // leaves: 88 us of all the kernels by 2^16 blocks, 55 by 2^13).
-void sum_slots(const LeafProduct& p, const Split& split, hipStream_t s) {
+void sum_slots(const LeafProduct& p, const Split& split, bool zeros, hipStream_t s) {
   const int64_t leaves = (int64_t)p.g.trees * p.g.leaves, size = (int64_t)p.outputs * (p.inputs + 1);
   const int parts = (int)std::max<int64_t>(1, std::min((size + THREADS - 1) / THREADS, (1 << 13) / leaves));
-  k_sum_slots<<<(unsigned)(leaves * parts), THREADS, 0, s>>>(p, split, parts);
+  k_sum_slots<<<(unsigned)(leaves * parts), THREADS, 0, s>>>(p, split, parts, zeros);
 }
 
 template <typename T>
@@ -739,7 +739,7 @@ void launch_dw(const LeafProduct& p, hipStream_t s) {
     k_leaf_dw<T, 128, 16, 4><<<grid, THREADS, 0, s>>>(p, mt, kt, split);
   else
     k_leaf_dw<T, 64, 64, 2><<<grid, THREADS, 0, s>>>(p, mt, kt, split);
-  if (split.rows) sum_slots(p, split, s);
+  if (split.rows) sum_slots(p, split, true, s);
 }
 
 template <typename T, bool DX, int BM, int BN>
@@ -822,7 +822,7 @@ void launch(const LeafProduct& p, int what, hipStream_t s) {
     if (!leaf_big_fits(p, what)) return launch_dw<T>(p, s);
     launch_leaf_big(p, what, s);
     const Split split = leaf_big_split(p);
-    if (split.rows) sum_slots(p, split, s);
+    if (split.rows) sum_slots(p, split, !leaf_big_ranks(p.g), s);
     return;
   }
   const Form form = form_of(p, what);
