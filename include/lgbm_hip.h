@@ -718,6 +718,8 @@ int lgbm_hip_predict_early_stop(lgbm_hip_ctx* ctx, const lgbm_hip_model* model, 
  * These entries group the rows by leaf, apply the maps, give their gradients, drop
  * elements or rows at random, and turn class scores into answers.  None has a counterpart
  * in the reference, which fits linear leaves on the host and has no device path for them.
+ * The maps are dense: a NaN input makes its row's outputs NaN, where lgbm_hip_predict
+ * falls back to the value of a linear leaf whose features have one.
  *
  * All pointers marked d_ are memory of the context's device.  `stream` points to a stream
  * handle (hipStream_t; the handle 0 is the device's default stream) of the HIP runtime
@@ -729,9 +731,9 @@ int lgbm_hip_predict_early_stop(lgbm_hip_ctx* ctx, const lgbm_hip_model* model, 
  * after the work is done, and not shared by calls that may run at the same time).
  * Outputs must not overlap inputs unless an entry says so; matrices of one row stride may
  * lie side by side in a table.  Matrices are row-major with a row stride in elements (at
- * least the columns); any alignment of the element type.  The
- * caller's current device is the same after a call.  Results depend neither on the order
- * in which blocks run nor on the device's number of CUs. */
+ * least the columns); any alignment of the element type.  The caller's current device is
+ * the same after a call.  Results depend neither on the order in which blocks run nor on
+ * the device's number of CUs. */
 #define LGBM_HIP_DTYPE_BF16 2
 #define LGBM_HIP_DTYPE_F16 3
 #define LGBM_HIP_MAX_GROUP_LEAVES 4095 /* of one tree, for lgbm_hip_leaf_groups */
@@ -796,7 +798,8 @@ int lgbm_hip_leaf_product_dw(lgbm_hip_ctx* ctx, const lgbm_leaf_maps* maps, cons
 
 /* out = x with units dropped (0, whatever x holds there) with probability p and the
  * others divided by the share kept.  A unit is an element, numbered row by row, or with
- * by_row a whole row (bagging of [g, h] pairs).  Unit e is kept where 16-bit field e % 8
+ * by_row a whole row ([g, h] pairs; to the learner a dropped pair is a row of zeros, which
+ * still counts in min_data_in_leaf).  Unit e is kept where 16-bit field e % 8
  * (low half first) of Philox4x32-10's block for counter (e / 8, offset) and key seed is at
  * least t = round(65536 p); the share kept is 1 - t / 65536.  The mask is nowhere stored:
  * the gradient is the same call on the outputs' gradient.  dtype as in lgbm_leaf_maps;

@@ -83,7 +83,7 @@ __device__ __forceinline__ u32x4 cm_frag32(const char* tile, int base, int step,
 // The part of the gradients that is the `rank`-th by rows, in a forest of at most THREADS
 // leaves: whole parts first, then the leaves' ends by their length.  So the long blocks begin
 // first, and the short ones fill the end (both gradients of two trees of 15 leaves, 16389 rows
-// of 2048 to 2048: 824 us in their order, 789).
+// of 2048 to 2048: 885 us in their order, 840).
 __device__ __forceinline__ DwPart part_of_rank(const LeafProduct& p, const Split& split, int rank) {
   __shared__ int fulls[THREADS], ends[THREADS];
   __shared__ int found[3];  // leaf of the forest, -1: none; first row, rows

@@ -432,8 +432,9 @@ __global__ __launch_bounds__(THREADS) void k_sum_few_trees(const float* planes, 
 
 // Leaves differ in size and may be fewer than the CUs, so blocks take about a 2048th of the
 // work (a thousandth is one round of blocks and a few more: ragged leaves of 2M rows, 100 float32
-// inputs, 10 outputs 382 us instead of 283), or of many tiles a thousandth (40000 x 2001 to
-// 2047 bfloat16: 1370 us instead of 1480).
+// inputs, 10 outputs 382 us instead of 283), or of many tiles a thousandth, which leaves more
+// leaves whole (float32, by that and by a 2048th: 20000 x 1000 to 1000 by seven leaves alike 622 and 709
+// us, 5000 x 2000 to 2000 by two 580 and 600; ragged 40000 x 600 to 600 by 31 547 and 472).
 Split dw_split(const LeafProduct& p, int64_t tiles) {
   const int64_t work = (int64_t)p.g.rows * p.g.trees * tiles;
   int64_t rows = (work / (tiles <= 64 ? 2048 : 1024) + 255) / 256 * 256;
@@ -443,8 +444,8 @@ Split dw_split(const LeafProduct& p, int64_t tiles) {
 
 // dw[leaf][m][k] = sum over the leaf's rows of dy[row][m] * x[row][k]; db[leaf][m] their sum.
 // BM x BN of a leaf's outputs x inputs a block, 128 bytes' worth of rows a step.  As
-// k_leaf_tile, with both operands read across (20000 x 1000 to 1000 float32 by 7 leaves: 630 us,
-// 63 TFLOP/s; 50000 x 300 to 100 float16 by two trees of 15: 89 us).
+// k_leaf_tile, with both operands read across (20000 x 1000 to 1000 float32 by 7 leaves: 610 us,
+// 66 TFLOP/s; 50000 x 300 to 100 float16 by two trees of 15: 89 us).
 template <typename T, int BM, int BN, int GM>
 __global__ __launch_bounds__(THREADS) void k_leaf_dw(LeafProduct p, int m_tiles, int k_tiles, Split split) {
   constexpr int V = El<T>::V, BK = 8 * V;  // rows a step
@@ -705,7 +706,7 @@ bool by_maps(const LeafProduct& p) {
 // Tiles of 128 x 128, where leaves fill them and there is one for every CU: 16-bit products
 // that are not for leaf_big.hip (40000 x 2001 to 2047 bf16 by 9 leaves: y 690 us instead of
 // 965, dx 945 instead of 1004).  float32 is slower by them (20000 x 1000 to 1000 by 7: 454 us,
-// 423 by 64 x 64), and so are the gradients of the maps (bf16 as above: 2518 us, 1371).
+// 423 by 64 x 64), and so are the gradients of the maps (bf16 as above, rows not split: 2518 us, 1371).
 bool wide_tiles(const LeafProduct& p, int cols) {
   return p.dtype != LGBM_HIP_DTYPE_F32 && cols >= 128 && p.g.rows >= 128 * (int64_t)p.g.leaves &&
          (int64_t)p.g.rows / 128 * ((cols + 127) / 128) * p.g.trees >= 256;
