@@ -54,9 +54,10 @@ struct El<_Float16> {
 
 // The sums of a stretch of the contraction.  In float32 they start at zero and are added to
 // the whole ones afterwards, so that a rounding is of a short sum's size (root mean square
-// error of y, and by one chain: 100 inputs 1.1e-7, 1.8e-7, 1000 inputs 1.5e-7, 5.7e-7).  With 16-bit operands the stretch goes on in place:
-// the rounding of y and dx hides that, and the gradients of the maps, float32 whatever
-// their operands, add no more than Split's rows in one chain.
+// error of y, and by one chain: 100 inputs 1.1e-7, 1.8e-7, 1000 inputs 1.5e-7, 5.7e-7).  With
+// 16-bit operands the stretch goes on in place: the rounding of y and dx hides that, and the
+// gradients of the maps, float32 whatever their operands, add no more than CHAIN_ROWS rows
+// in one chain.
 template <typename T, int M, int N>
 struct Parts {
   f32x4 (&at)[M][N];
