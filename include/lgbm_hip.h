@@ -715,8 +715,9 @@ int lgbm_hip_predict_early_stop(lgbm_hip_ctx* ctx, const lgbm_hip_model* model, 
 
 /* A tree sends every row to a leaf (LGBM_HIP_PREDICT_LEAF), and a leaf may hold a linear
  * map of its own: one output for the linear leaves of a linear tree, several for experts.
- * These entries group the rows by leaf, apply the maps, give their gradients, drop
- * elements or rows at random, and turn class scores into answers.  None has a counterpart
+ * These entries group the rows by leaf, apply the maps, or layers with an activation, give
+ * their gradients, clip gradients by their norm, drop elements or rows at random, and turn
+ * class scores into answers.  None has a counterpart
  * in the reference, which fits linear leaves on the host and has no device path for them.
  * The maps are dense: a NaN input makes its row's outputs NaN, where lgbm_hip_predict
  * falls back to the value of a linear leaf whose features have one.
@@ -795,6 +796,83 @@ int lgbm_hip_leaf_product_dx(lgbm_hip_ctx* ctx, const lgbm_leaf_maps* maps, cons
 int lgbm_hip_leaf_product_dw(lgbm_hip_ctx* ctx, const lgbm_leaf_maps* maps, const void* d_dy,
                              int64_t lddy, const void* d_x, int64_t ldx, float* d_dw, float* d_db,
                              void* d_ws, size_t ws_bytes, void* const* stream);
+
+/* Layers of the leaves: z[t][n] = w[t][leaf] x[n] + bias[t][leaf] and
+ *   y[n] = residual[n] + sum over trees t of f(z[t][n])
+ * in float32 and rounded once, with f the activation, or gated f = the activation of the first
+ * `outputs` elements of z times its other `outputs`.  A tree that has a row in no leaf adds
+ * nothing to it.  RELU max(z, 0); SILU z / (1 + exp(-z)); GELU z (1 + erf(z / sqrt 2)) / 2;
+ * GELU_TANH z (1 + tanh(sqrt(2 / pi) (z + 0.044715 z^3))) / 2; SIGMOID 1 / (1 + exp(-z)). */
+#define LGBM_HIP_ACT_NONE 0
+#define LGBM_HIP_ACT_RELU 1
+#define LGBM_HIP_ACT_SILU 2
+#define LGBM_HIP_ACT_GELU 3
+#define LGBM_HIP_ACT_GELU_TANH 4
+#define LGBM_HIP_ACT_SIGMOID 5
+typedef struct lgbm_leaf_layer {
+  lgbm_leaf_maps maps; /* outputs: those of the layer; a leaf's map has R = outputs rows, 2 *
+                          outputs where gated */
+  int32_t activation;  /* LGBM_HIP_ACT_* */
+  int32_t gated;
+  const void* d_x; /* [num_rows][inputs], row stride ldx */
+  int64_t ldx;
+  const void* d_w;    /* [num_trees * num_leaves][R][inputs], gates first */
+  const void* d_bias; /* [num_trees * num_leaves][R] or NULL */
+  const void* d_residual; /* [num_rows][outputs], row stride ldr, or NULL */
+  int64_t ldr;
+  void* d_y; /* [num_rows][outputs], row stride ldy; may be d_residual with the same stride */
+  int64_t ldy;
+  void* d_z; /* [num_trees][num_rows][R]: z, for the gradients; or NULL */
+  int32_t z_dtype; /* LGBM_HIP_DTYPE_F32, or that of maps: z is rounded to it */
+  int32_t _pad;
+} lgbm_leaf_layer;
+int lgbm_hip_leaf_layer_workspace(const lgbm_leaf_layer* layer, size_t* bytes);
+int lgbm_hip_leaf_layer(lgbm_hip_ctx* ctx, const lgbm_leaf_layer* layer, void* d_ws, size_t ws_bytes,
+                        void* const* stream);
+
+/* The gradients of a layer from dy [num_rows][outputs] and the z that it kept: with dz = f'(z)
+ * dy, rounded to the type, dx[n] = sum over trees of w[t][leaf]^T dz[t][n], dw[leaf] = sum over
+ * the leaf's rows of dz[n] x[n]^T and dbias[leaf] = the sum of dz[n], sums in float32.  The
+ * residual's gradient is dy.  Where f is z itself (LGBM_HIP_ACT_NONE, not gated) dz is dy and
+ * d_z is not read. */
+typedef struct lgbm_leaf_layer_grad {
+  lgbm_leaf_maps maps;
+  int32_t activation;
+  int32_t gated;
+  const void* d_dy; /* [num_rows][outputs], row stride lddy */
+  int64_t lddy;
+  const void* d_z;
+  const void* d_x; /* [num_rows][inputs], for dw */
+  int64_t ldx;
+  const void* d_w; /* for dx */
+  void* d_dx;      /* [num_rows][inputs], row stride lddx, or NULL: not made */
+  int64_t lddx;
+  void* d_dw;       /* [num_trees * num_leaves][R][inputs], or NULL: not made, nor is dbias */
+  void* d_dbias;    /* [num_trees * num_leaves][R], or NULL */
+  int32_t dw_dtype; /* of dw and dbias: that of maps or LGBM_HIP_DTYPE_F32 */
+  int32_t z_dtype;
+} lgbm_leaf_layer_grad;
+int lgbm_hip_leaf_layer_grad_workspace(const lgbm_leaf_layer_grad* grad, size_t* bytes);
+int lgbm_hip_leaf_layer_grad(lgbm_hip_ctx* ctx, const lgbm_leaf_layer_grad* grad, void* d_ws,
+                             size_t ws_bytes, void* const* stream);
+
+/* The 2-norm over all elements of many tensors, and the tensors scaled to a largest norm:
+ *   norm = sqrt(sum of in^2);  out = in * min(1, max_norm / norm).
+ * Sums are float64; norm is a float32 on the device.  A norm that is infinite gives a factor of 0
+ * (infinite elements become NaN), one that is NaN a factor that is NaN.  `grads` is host memory and
+ * is not read after the call. */
+typedef struct lgbm_grad {
+  const void* d_in; /* count elements without gaps */
+  void* d_out;      /* clip: may be d_in; overlaps nothing else.  norm: not used */
+  int64_t count;
+  int32_t dtype; /* LGBM_HIP_DTYPE_F32, _BF16 or _F16 */
+  int32_t _pad;
+} lgbm_grad;
+int lgbm_hip_grad_norm_workspace(const lgbm_grad* grads, int64_t num_grads, size_t* bytes);
+int lgbm_hip_grad_norm(lgbm_hip_ctx* ctx, const lgbm_grad* grads, int64_t num_grads, float* d_norm,
+                       void* d_ws, size_t ws_bytes, void* const* stream);
+int lgbm_hip_clip_grads(lgbm_hip_ctx* ctx, const lgbm_grad* grads, int64_t num_grads, double max_norm,
+                        float* d_norm, void* d_ws, size_t ws_bytes, void* const* stream);
 
 /* out = x with units dropped (0, whatever x holds there) with probability p and the
  * others divided by the share kept.  A unit is an element, numbered row by row, or with

@@ -84,6 +84,7 @@ __device__ __forceinline__ u32x4 cm_frag32(const char* tile, int base, int step,
 // leaves: whole parts first, then the leaves' ends by their length.  So the long blocks begin
 // first, and the short ones fill the end (both gradients of two trees of 15 leaves, 16389 rows
 // of 2048 to 2048: 885 us in their order, 840).
+template <typename T>
 __device__ __forceinline__ DwPart part_of_rank(const LeafProduct& p, const Split& split, int rank) {
   __shared__ int fulls[THREADS], ends[THREADS];
   __shared__ int found[3];  // leaf of the forest, -1: none; first row, rows
@@ -111,8 +112,8 @@ __device__ __forceinline__ DwPart part_of_rank(const LeafProduct& p, const Split
   }
   __syncthreads();
   const int at = __builtin_amdgcn_readfirstlane(found[0]);
-  if (at < 0) return {0, 0, -1, nullptr, nullptr};
-  return dw_part_of(p, split, at / p.g.leaves, at % p.g.leaves, __builtin_amdgcn_readfirstlane(found[1]),
+  if (at < 0) return {0, 0, -1, nullptr, nullptr, false};
+  return dw_part_of<T>(p, split, at / p.g.leaves, at % p.g.leaves, __builtin_amdgcn_readfirstlane(found[1]),
                     __builtin_amdgcn_readfirstlane(found[2]));
 }
 
@@ -120,7 +121,8 @@ __device__ __forceinline__ DwPart part_of_rank(const LeafProduct& p, const Split
 // [m][col]; _DW: a = dy [row][m], b = x [row][k] over a leaf's rows.  Y and DX: one block a
 // CU takes tile after tile, so that what it stores drains while the next tile begins; DW:
 // a block a tile of a part, since leaves differ in length.
-template <typename T, int MODE>
+// NARROW: dw and db of whole leaves are 16-bit.
+template <typename T, int MODE, bool NARROW = false>
 __global__ __launch_bounds__(THREADS, 1) void k_leaf_big(LeafProduct p, int col_tiles, Split split) {
   constexpr bool DW = MODE == LEAF_PRODUCT_DW, ACM = DW, BCM = MODE != LEAF_PRODUCT_Y;
   constexpr int FM = WM / 32, FN = WN / 32, STEPS = BK / 16, ITEMS = STEPS * FM, RING = 4;
@@ -147,9 +149,10 @@ __global__ __launch_bounds__(THREADS, 1) void k_leaf_big(LeafProduct p, int col_
       const int of = (p.outputs + BM - 1) / BM * col_tiles, tile = (int)(blockIdx.x % of);
       const int id = (int)(blockIdx.x / of);
       part = leaf_big_ranks(p.g)
-                 ? part_of_rank(p, split, (int)(blockIdx.y * split.parts) + id)
-                 : dw_part<THREADS>(p, split, id);
+                 ? part_of_rank<T>(p, split, (int)(blockIdx.y * split.parts) + id)
+                 : dw_part<T, THREADS>(p, split, id);
       if (part.count < 0) return;
+      if (!NARROW) part.narrow = false;
       tree = part.tree, first = part.first, length = part.count;
       leaf = 0;
       m0 = tile / col_tiles * BM, c0 = tile % col_tiles * BN, cols = p.inputs;
@@ -191,7 +194,7 @@ __global__ __launch_bounds__(THREADS, 1) void k_leaf_big(LeafProduct p, int col_
     // from LDS, and every lane adds its column.  Columns behind the last only make results
     // that are not stored, so they read the last ones.
     const int half = lane >> 5, op = (lane >> 4) & 1;
-    const T* const base = op ? (const T*)p.x + c0 : (const T*)p.dy + m0;
+    const T* const base = op ? (const T*)p.x + c0 : (const T*)p.dy + tree * p.dy_tree + m0;
     const uint32_t ld_of_op = (uint32_t)(op ? p.ldx : p.lddy) * 2;
     const uint32_t a_col = (uint32_t)(min(m0 + (lane & 31) * 8, p.outputs - 8) - m0) * 2;
     const uint32_t b_col = (uint32_t)(min(c0 + (lane & 31) * 8, cols - 8) - c0) * 2;
@@ -208,7 +211,7 @@ __global__ __launch_bounds__(THREADS, 1) void k_leaf_big(LeafProduct p, int col_
     // The j-th loads of the stage at k0, and their place in its buffer.  The stage's addresses
     // are scalars that the compiler takes as new ones, or it would keep a lane's 32 in
     // registers.
-    const T* const src = (const T*)(MODE == LEAF_PRODUCT_Y ? p.x : p.dy);
+    const T* const src = MODE == LEAF_PRODUCT_Y ? (const T*)p.x : (const T*)p.dy + tree * p.dy_tree;
     const uint64_t zero_at = (uint64_t)(uintptr_t)zeros;
     struct Stage {
       uint64_t a, b;
@@ -384,7 +387,20 @@ __global__ __launch_bounds__(THREADS, 1) void k_leaf_big(LeafProduct p, int col_
         const int mi = m0 + wm + i * 32;
         if (sums && wn == 0) {
           const float b = bias[DW ? i : 0] + __shfl_xor(bias[DW ? i : 0], 32);
-          if (lane < 32 && mi + lane < p.outputs) part.db[mi + lane] = b;
+          if (lane < 32 && mi + lane < p.outputs) put<T>(part, part.db, mi + lane, b);
+        }
+        if (NARROW && part.narrow) {  // pieces of a row as y's
+#pragma unroll
+          for (int e = 0; e < 16; e += 2) {
+            const int m = mi + (e >> 2) * 8 + row4 + (e & 3) + (lane & 1);
+            T* const to = (T*)part.dw + (int64_t)m * cols + (col0 & ~1);
+#pragma unroll
+            for (int j = 0; j < FN; ++j) {
+              const uint32_t v = pair_of<T>(acc[i][j][e], acc[i][j][e + 1]);
+              if (m < p.outputs && col0 + j * 32 < cols) __builtin_memcpy(to + j * 32, &v, 4);
+            }
+          }
+          continue;
         }
 #pragma unroll
         for (int e = 0; e < 16; ++e) {
@@ -392,7 +408,7 @@ __global__ __launch_bounds__(THREADS, 1) void k_leaf_big(LeafProduct p, int col_
           if (m >= p.outputs) continue;
 #pragma unroll
           for (int j = 0; j < FN; ++j)
-            if (col0 + j * 32 < cols) part.dw[(int64_t)m * cols + col0 + j * 32] = acc[i][j][e];
+            if (col0 + j * 32 < cols) ((float*)part.dw)[(int64_t)m * cols + col0 + j * 32] = acc[i][j][e];
         }
       }
       return;
@@ -442,6 +458,8 @@ void launch(const LeafProduct& p, int what, hipStream_t s) {
     k_leaf_big<T, LEAF_PRODUCT_Y><<<grid, THREADS, 0, s>>>(p, ct, split);
   else if (what == LEAF_PRODUCT_DX)
     k_leaf_big<T, LEAF_PRODUCT_DX><<<grid, THREADS, 0, s>>>(p, ct, split);
+  else if (p.narrow)
+    k_leaf_big<T, LEAF_PRODUCT_DW, true><<<grid, THREADS, 0, s>>>(p, ct, split);
   else
     k_leaf_big<T, LEAF_PRODUCT_DW><<<grid, THREADS, 0, s>>>(p, ct, split);
 }

@@ -1,9 +1,12 @@
 // leaf_capi.hip — the C entries of the operators around a forest's leaves
 // (include/lgbm_hip.h): every argument is checked before the device is touched, then the
 // work is queued on the caller's stream, or run to its end on the context's own.
+#include <algorithm>
 #include <cmath>
 #include <cstdint>
 #include <initializer_list>
+#include <new>
+#include <vector>
 
 #include "context.h"
 #include "leaf_ops.h"
@@ -128,11 +131,15 @@ int check_grid(lgbm_hip_ctx* c, const LeafProduct& p, int what) {
                                                    : LGBM_HIP_OK;
 }
 
-Span weights(const lgbm_leaf_maps* m, const void* w, int64_t e) {
-  return {w, (int64_t)m->num_trees * m->num_leaves * m->outputs * m->inputs * e};
+// `rows`: of a leaf's map for each output
+Span weights(const lgbm_leaf_maps* m, const void* w, int64_t e, int64_t rows = 1) {
+  return {w, (int64_t)m->num_trees * m->num_leaves * m->outputs * rows * m->inputs * e};
 }
-Span biases(const lgbm_leaf_maps* m, const void* b, int64_t e) {
-  return {b, (int64_t)m->num_trees * m->num_leaves * m->outputs * e};
+Span biases(const lgbm_leaf_maps* m, const void* b, int64_t e, int64_t rows = 1) {
+  return {b, (int64_t)m->num_trees * m->num_leaves * m->outputs * rows * e};
+}
+Span kept(const lgbm_leaf_maps* m, const void* z, int64_t e, int64_t rows) {
+  return {z, (int64_t)m->num_trees * m->num_rows * m->outputs * rows * e};
 }
 Span order_of(const lgbm_leaf_maps* m) { return {m->d_order, (int64_t)m->num_trees * m->num_rows * 4}; }
 Span table(const lgbm_leaf_maps* m, const int32_t* t) {
@@ -255,6 +262,283 @@ int lgbm_hip_leaf_product_dw(lgbm_hip_ctx* c, const lgbm_leaf_maps* m, const voi
       overlaps(ws, {dy, x, order_of(m), table(m, m->d_begin), table(m, m->d_count)}))
     return bad(c, "dw, db or the workspace overlaps an input or one another");
   return queue(c, stream, [&](hipStream_t s) { launch_leaf_product(p, LEAF_PRODUCT_DW, s); });
+}
+
+// ---- layers ----------------------------------------------------------------------------
+
+static int check_layer(lgbm_hip_ctx* c, const lgbm_leaf_maps* m, int32_t activation, int32_t gated,
+                       int32_t z_dtype) {
+  const int rc = check_maps(c, m);
+  if (rc) return rc;
+  if (activation < LGBM_HIP_ACT_NONE || activation > LGBM_HIP_ACT_SIGMOID) return bad(c, "unknown activation");
+  if (gated != 0 && gated != 1) return bad(c, "gated is neither 0 nor 1");
+  if (z_dtype != m->dtype && z_dtype != LGBM_HIP_DTYPE_F32) return bad(c, "z_dtype is neither the maps' nor f32");
+  const int64_t rows = gated ? 2 : 1;
+  if ((__int128)m->num_trees * m->num_leaves * m->inputs * m->outputs * rows > ((__int128)1 << 48))
+    return beyond(c, "more than 2^48 weights");
+  if (m->outputs * rows > (1 << 24)) return beyond(c, "more than 2^24 rows of a leaf's map");
+  if ((__int128)m->num_trees * m->num_rows * m->outputs * rows > ((__int128)1 << 58))
+    return beyond(c, "more than 2^58 elements of z");
+  return LGBM_HIP_OK;
+}
+
+static LeafProduct layer_of(const lgbm_leaf_layer* a) {
+  LeafProduct p = product_of(&a->maps);
+  p.act = a->activation, p.gated = a->gated != 0;
+  p.x = a->d_x, p.ldx = a->ldx, p.w = a->d_w, p.b = a->d_bias, p.res = a->d_residual, p.ldr = a->ldr;
+  p.out = a->d_y, p.ldo = a->ldy, p.z = a->d_z, p.z_narrow = a->z_dtype != LGBM_HIP_DTYPE_F32;
+  return p;
+}
+
+int lgbm_hip_leaf_layer_workspace(const lgbm_leaf_layer* a, size_t* bytes) {
+  if (!a) return bad(nullptr, "null layer");
+  const int rc = check_layer(nullptr, &a->maps, a->activation, a->gated, a->z_dtype);
+  if (rc) return rc;
+  if (!bytes) return bad(nullptr, "null bytes");
+  *bytes = leaf_product_workspace(layer_of(a), LEAF_LAYER);
+  return LGBM_HIP_OK;
+}
+
+int lgbm_hip_leaf_layer(lgbm_hip_ctx* c, const lgbm_leaf_layer* a, void* d_ws, size_t ws_bytes,
+                        void* const* stream) {
+  if (!a) return bad(c, "null layer");
+  const lgbm_leaf_maps* const m = &a->maps;
+  int rc = check_layer(c, m, a->activation, a->gated, a->z_dtype);
+  if (rc) return rc;
+  const int64_t e = type_size(m->dtype), rows = m->num_rows, of = a->gated ? 2 : 1;
+  if (a->ldx < m->inputs || a->ldy < m->outputs || (a->d_residual && a->ldr < m->outputs) || huge(rows, a->ldx) ||
+      huge(rows, a->ldy) || (a->d_residual && huge(rows, a->ldr)))
+    return bad(c, "row stride smaller than the row, or too large");
+  if (!a->d_w || (rows > 0 && (!a->d_x || !a->d_y))) return bad(c, "null x, w or y");
+  if (misaligned(a->d_x, e) || misaligned(a->d_w, e) || misaligned(a->d_bias, e) || misaligned(a->d_residual, e) ||
+      misaligned(a->d_y, e) || misaligned(a->d_z, type_size(a->z_dtype)))
+    return bad(c, "a pointer is not aligned to its type");
+  LeafProduct p = layer_of(a);
+  p.ws = d_ws;
+  const size_t need = leaf_product_workspace(p, LEAF_LAYER);
+  if ((rc = check_ws(c, d_ws, ws_bytes, need)) || (rc = check_grid(c, p, LEAF_LAYER))) return rc;
+  const Span x = matrix(a->d_x, rows, m->inputs, a->ldx, e), w = weights(m, a->d_w, e, of);
+  const Span b = biases(m, a->d_bias, e, of), z = kept(m, a->d_z, type_size(a->z_dtype), of), ws{d_ws, (int64_t)need};
+  const Span y = matrix(a->d_y, rows, m->outputs, a->ldy, e);
+  const Span r = matrix(a->d_residual, a->d_residual ? rows : 0, m->outputs, a->ldr, e);
+  const Span order = order_of(m), begin = table(m, m->d_begin), count = table(m, m->d_count);
+  if (overlaps(y, {x, w, b, z, order, begin, count, ws}) || overlaps(z, {x, w, b, r, order, begin, count, ws}) ||
+      overlaps(ws, {x, w, b, r, order, begin, count}))
+    return bad(c, "y, z or the workspace overlaps an input or one another");
+  if (!(a->d_y == a->d_residual && a->ldy == a->ldr) && overlap(y, r))
+    return bad(c, "y overlaps the residual other than in place");
+  if (rows == 0) return c ? LGBM_HIP_OK : bad(c, "null context");
+  return queue(c, stream, [&](hipStream_t s) { launch_leaf_product(p, LEAF_LAYER, s); });
+}
+
+// dz is dy itself where the layer is a linear map.
+static bool linear(const lgbm_leaf_layer_grad* a) { return a->activation == LGBM_HIP_ACT_NONE && !a->gated; }
+
+// The products that a layer's gradients are, of dz (at `dz`) in dy's place.
+static LeafProduct layer_grad_of(const lgbm_leaf_layer_grad* a, const void* dz) {
+  LeafProduct p = product_of(&a->maps);
+  if (a->gated) p.outputs *= 2;
+  p.dy = linear(a) ? a->d_dy : dz;
+  p.lddy = linear(a) ? a->lddy : p.outputs;
+  p.dy_tree = linear(a) ? 0 : a->maps.num_rows * p.outputs;
+  p.x = a->d_x, p.ldx = a->ldx, p.w = a->d_w, p.out = a->d_dx, p.ldo = a->lddx, p.dw = a->d_dw, p.db = a->d_dbias;
+  p.narrow = a->dw_dtype != LGBM_HIP_DTYPE_F32;
+  return p;
+}
+
+static int64_t dz_bytes(const lgbm_leaf_layer_grad* a) {
+  if (linear(a)) return 0;
+  const int64_t n = (int64_t)a->maps.num_trees * a->maps.num_rows * a->maps.outputs * (a->gated ? 2 : 1);
+  return (n * type_size(a->maps.dtype) + 255) / 256 * 256;
+}
+
+// dz, then what the products need, one after the other.
+static size_t layer_grad_workspace(const lgbm_leaf_layer_grad* a) {
+  const LeafProduct p = layer_grad_of(a, nullptr);
+  return (size_t)dz_bytes(a) + std::max(a->d_dx ? leaf_product_workspace(p, LEAF_PRODUCT_DX) : 0,
+                                        a->d_dw ? leaf_product_workspace(p, LEAF_PRODUCT_DW) : 0);
+}
+
+static int check_layer_grad(lgbm_hip_ctx* c, const lgbm_leaf_layer_grad* a) {
+  if (!a) return bad(c, "null gradient");
+  const int rc = check_layer(c, &a->maps, a->activation, a->gated, a->z_dtype);
+  if (rc) return rc;
+  if (a->dw_dtype != a->maps.dtype && a->dw_dtype != LGBM_HIP_DTYPE_F32)
+    return bad(c, "dw_dtype is neither the maps' nor f32");
+  if (!a->d_dx && !a->d_dw) return bad(c, "neither dx nor dw is asked for");
+  if (a->d_dbias && !a->d_dw) return bad(c, "dbias without dw");
+  return LGBM_HIP_OK;
+}
+
+int lgbm_hip_leaf_layer_grad_workspace(const lgbm_leaf_layer_grad* a, size_t* bytes) {
+  const int rc = check_layer_grad(nullptr, a);
+  if (rc) return rc;
+  if (!bytes) return bad(nullptr, "null bytes");
+  *bytes = layer_grad_workspace(a);
+  return LGBM_HIP_OK;
+}
+
+int lgbm_hip_leaf_layer_grad(lgbm_hip_ctx* c, const lgbm_leaf_layer_grad* a, void* d_ws, size_t ws_bytes,
+                             void* const* stream) {
+  int rc = check_layer_grad(c, a);
+  if (rc) return rc;
+  const lgbm_leaf_maps* const m = &a->maps;
+  const int64_t e = type_size(m->dtype), rows = m->num_rows, of = a->gated ? 2 : 1;
+  const int64_t we = type_size(a->dw_dtype), ze = type_size(a->z_dtype);
+  if (a->lddy < m->outputs || (a->d_dw && a->ldx < m->inputs) || (a->d_dx && a->lddx < m->inputs) ||
+      huge(rows, a->lddy) || (a->d_dw && huge(rows, a->ldx)) || (a->d_dx && huge(rows, a->lddx)))
+    return bad(c, "row stride smaller than the row, or too large");
+  if ((rows > 0 && (!a->d_dy || (!a->d_z && !linear(a)) || (a->d_dw && !a->d_x))) || (a->d_dx && !a->d_w))
+    return bad(c, "null dy, z, x or w");
+  if (misaligned(a->d_dy, e) || misaligned(a->d_z, ze) || misaligned(a->d_x, e) || misaligned(a->d_w, e) ||
+      misaligned(a->d_dx, e) || misaligned(a->d_dw, we) || misaligned(a->d_dbias, we))
+    return bad(c, "a pointer is not aligned to its type");
+  const size_t need = layer_grad_workspace(a);
+  if ((rc = check_ws(c, d_ws, ws_bytes, need))) return rc;
+  LeafProduct p = layer_grad_of(a, d_ws);
+  p.ws = (char*)d_ws + dz_bytes(a);
+  if (a->d_dx && (rc = check_grid(c, p, LEAF_PRODUCT_DX))) return rc;
+  if (a->d_dw && (rc = check_grid(c, p, LEAF_PRODUCT_DW))) return rc;
+  const Span dy = matrix(a->d_dy, rows, m->outputs, a->lddy, e), z = kept(m, linear(a) ? nullptr : a->d_z, ze, of);
+  const Span x = matrix(a->d_x, a->d_dw ? rows : 0, m->inputs, a->ldx, e);
+  const Span w = weights(m, a->d_dx ? a->d_w : nullptr, e, of), ws{d_ws, (int64_t)need};
+  const Span dx = matrix(a->d_dx, a->d_dx ? rows : 0, m->inputs, a->lddx, e);
+  const Span dw = weights(m, a->d_dw, we, of), db = biases(m, a->d_dbias, we, of);
+  const Span order = order_of(m), begin = table(m, m->d_begin), count = table(m, m->d_count);
+  if (overlaps(dx, {dy, z, x, w, dw, db, order, begin, count, ws}) ||
+      overlaps(dw, {dy, z, x, w, db, order, begin, count, ws}) ||
+      overlaps(db, {dy, z, x, w, order, begin, count, ws}) || overlaps(ws, {dy, z, x, w, order, begin, count}))
+    return bad(c, "an output or the workspace overlaps an input or one another");
+  if (rows == 0 && !a->d_dw) return c ? LGBM_HIP_OK : bad(c, "null context");
+  return queue(c, stream, [&](hipStream_t s) {
+    if (rows > 0 && !linear(a)) {
+      LeafProduct q = product_of(m);
+      q.act = a->activation, q.gated = a->gated != 0;
+      q.dy = a->d_dy, q.lddy = a->lddy, q.z = const_cast<void*>(a->d_z);
+      q.z_narrow = a->z_dtype != LGBM_HIP_DTYPE_F32;
+      launch_layer_dz(q, d_ws, s);
+    }
+    if (rows > 0 && a->d_dx) launch_leaf_product(p, LEAF_PRODUCT_DX, s);
+    if (a->d_dw) launch_leaf_product(p, LEAF_PRODUCT_DW, s);
+  });
+}
+
+// ---- the norm of many tensors ------------------------------------------------------------
+
+// The list as the kernels' launcher takes it; an error code, or LGBM_HIP_OK.
+static int check_grads(lgbm_hip_ctx* c, const lgbm_grad* g, int64_t num, bool clip, std::vector<GradTensor>& list) {
+  if (num < 0 || (num > 0 && !g)) return bad(c, "null or negative list of gradients");
+  if (num > (1 << 24)) return beyond(c, "more than 2^24 gradients");
+  try {
+    list.reserve((size_t)num);
+  } catch (const std::bad_alloc&) {
+    return beyond(c, "no host memory for the list of gradients");
+  }
+  int64_t total = 0;
+  for (int64_t i = 0; i < num; ++i) {
+    if (g[i].dtype != LGBM_HIP_DTYPE_F32 && g[i].dtype != LGBM_HIP_DTYPE_BF16 && g[i].dtype != LGBM_HIP_DTYPE_F16)
+      return bad(c, "dtype is none of f32, bf16 and f16");
+    if (g[i].count < 0) return bad(c, "negative count");
+    if (g[i].count > ((int64_t)1 << 48) || (total += g[i].count) > ((int64_t)1 << 48))
+      return beyond(c, "more than 2^48 elements");
+    if (g[i].count == 0) continue;
+    const int64_t e = type_size(g[i].dtype);
+    if (!g[i].d_in || (clip && !g[i].d_out)) return bad(c, "null gradient");
+    if (misaligned(g[i].d_in, e) || (clip && misaligned(g[i].d_out, e)))
+      return bad(c, "a pointer is not aligned to its type");
+    list.push_back({g[i].d_in, clip ? g[i].d_out : nullptr, g[i].count, g[i].dtype});
+  }
+  return LGBM_HIP_OK;
+}
+
+// Whether a clipped gradient overlaps anything but its own input, or `more`.
+static bool clipped_overlap(const std::vector<GradTensor>& list, std::initializer_list<Span> more, bool& no_memory) {
+  struct Range {
+    uintptr_t from, to;
+    bool out;
+  };
+  std::vector<Range> all;
+  try {
+    all.reserve(2 * list.size() + more.size());
+  } catch (const std::bad_alloc&) {
+    no_memory = true;
+    return false;
+  }
+  const auto put = [&](const void* p, int64_t bytes, bool out) {
+    if (p && bytes > 0) all.push_back({(uintptr_t)p, (uintptr_t)p + (uintptr_t)bytes, out});
+  };
+  for (const GradTensor& t : list) {
+    const int64_t bytes = t.count * type_size(t.dtype);
+    put(t.out, bytes, true);
+    if (t.in != t.out) put(t.in, bytes, false);
+  }
+  for (const Span& s : more) put(s.p, s.bytes, true);
+  // inputs may overlap one another: behind each range's begin, the furthest ends so far
+  const auto before = [](const Range& a, const Range& b) { return a.from < b.from; };
+  if (!std::is_sorted(all.begin(), all.end(), before)) std::sort(all.begin(), all.end(), before);
+  uintptr_t out_end = 0, in_end = 0;
+  for (const Range& r : all) {
+    if (r.from < out_end || (r.out && r.from < in_end)) return true;
+    uintptr_t& end = r.out ? out_end : in_end;
+    end = std::max(end, r.to);
+  }
+  return false;
+}
+
+int lgbm_hip_grad_norm_workspace(const lgbm_grad* g, int64_t num, size_t* bytes) {
+  // sizes and types: pointers may be missing still
+  if (num < 0 || (num > 0 && !g)) return bad(nullptr, "null or negative list of gradients");
+  if (num > (1 << 24)) return beyond(nullptr, "more than 2^24 gradients");
+  if (!bytes) return bad(nullptr, "null bytes");
+  int64_t total = 0;
+  for (int64_t i = 0; i < num; ++i) {
+    if (g[i].count < 0) return bad(nullptr, "negative count");
+    if (g[i].count > ((int64_t)1 << 48) || (total += g[i].count) > ((int64_t)1 << 48))
+      return beyond(nullptr, "more than 2^48 elements");
+  }
+  *bytes = grad_norm_workspace(total, num);
+  return LGBM_HIP_OK;
+}
+
+static int norm_and_clip(lgbm_hip_ctx* c, const lgbm_grad* g, int64_t num, bool clip, double most, float* d_norm,
+                         void* d_ws, size_t ws_bytes, void* const* stream) {
+  std::vector<GradTensor> list;
+  int rc = check_grads(c, g, num, clip, list);
+  if (rc) return rc;
+  if (clip && !(most >= 0.0)) return bad(c, "max_norm is negative or NaN");
+  if (!d_norm) return bad(c, "null norm");
+  if (misaligned(d_norm, 4)) return bad(c, "a pointer is not aligned to its type");
+  int64_t total = 0;
+  for (const GradTensor& t : list) total += t.count;
+  const size_t need = grad_norm_workspace(total, num);
+  if ((rc = check_ws(c, d_ws, ws_bytes, need))) return rc;
+  const Span norm{d_norm, 4}, ws{d_ws, (int64_t)need};
+  if (clip) {
+    bool no_memory = false;
+    if (clipped_overlap(list, {norm, ws}, no_memory))
+      return bad(c, "a clipped gradient, the norm or the workspace overlaps another tensor");
+    if (no_memory) return beyond(c, "no host memory for the list of gradients");
+  } else {
+    bool hit = overlap(norm, ws);
+    for (const GradTensor& t : list) {
+      const Span in{t.in, t.count * type_size(t.dtype)};
+      hit = hit || overlap(norm, in) || overlap(ws, in);
+    }
+    if (hit) return bad(c, "the norm or the workspace overlaps a gradient or one another");
+  }
+  return queue(c, stream, [&](hipStream_t s) {
+    launch_grad_norm(list.data(), (int64_t)list.size(), clip, most, d_norm, d_ws, s);
+  });
+}
+
+int lgbm_hip_grad_norm(lgbm_hip_ctx* c, const lgbm_grad* g, int64_t num, float* d_norm, void* d_ws,
+                       size_t ws_bytes, void* const* stream) {
+  return norm_and_clip(c, g, num, false, 0.0, d_norm, d_ws, ws_bytes, stream);
+}
+
+int lgbm_hip_clip_grads(lgbm_hip_ctx* c, const lgbm_grad* g, int64_t num, double max_norm, float* d_norm, void* d_ws,
+                        size_t ws_bytes, void* const* stream) {
+  return norm_and_clip(c, g, num, true, max_norm, d_norm, d_ws, ws_bytes, stream);
 }
 
 int lgbm_hip_dropout(lgbm_hip_ctx* c, const void* d_x, int64_t ldx, int64_t rows, int64_t cols,

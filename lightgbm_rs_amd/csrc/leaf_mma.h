@@ -246,29 +246,42 @@ constexpr int64_t CHAIN_ROWS = 8192;
 // What a block sums, and where to.
 struct DwPart {
   int tree, first, count;  // count -1: nothing
-  float *dw, *db;
+  void *dw, *db;
+  bool narrow;  // dw and db are 16-bit, else float32
 };
+// Element `at` of a part's dw or db.
+template <typename T>
+__device__ __forceinline__ void put(const DwPart& part, void* to, int64_t at, float v) {
+  if (part.narrow)
+    ((T*)to)[at] = (T)v;
+  else
+    ((float*)to)[at] = v;
+}
 // `rows` from `first` on of a leaf.
+template <typename T>
 __device__ __forceinline__ DwPart dw_part_of(const LeafProduct& p, const Split& split, int tree, int leaf, int first,
                                              int rows) {
   const int64_t size = (int64_t)p.outputs * p.inputs, at = (int64_t)tree * p.g.leaves + leaf;
   const int count = min(max(p.g.count[at], 0), p.g.rows);
-  if (split.rows == 0 || count <= split.rows)
-    return {tree, first, rows, p.dw + at * size, p.db ? p.db + at * p.outputs : nullptr};
+  if (split.rows == 0 || count <= split.rows) {
+    if (sizeof(T) == 2 && p.narrow)
+      return {tree, first, rows, (T*)p.dw + at * size, p.db ? (T*)p.db + at * p.outputs : nullptr, true};
+    return {tree, first, rows, (float*)p.dw + at * size, p.db ? (float*)p.db + at * p.outputs : nullptr, false};
+  }
   const int64_t slot = slot_of(split, first, first == min(max(p.g.begin[at], 0), p.g.rows - count));
   float* const dw = (float*)p.ws + (tree * split.slots + slot) * (size + p.outputs);
-  return {tree, first, rows, dw, p.db ? dw + size : nullptr};
+  return {tree, first, rows, dw, p.db ? dw + size : nullptr, false};
 }
 // Part number `id`: of tree blockIdx.y where leaves are split, else a leaf of the forest.
-template <int THREADS>
+template <typename T, int THREADS>
 __device__ __forceinline__ DwPart dw_part(const LeafProduct& p, const Split& split, int id) {
   if (split.rows) {
     const RowTile rt = find_tile<THREADS>(p.g, blockIdx.y, id, split.rows);
-    if (rt.rows == 0 || rt.leaf < 0) return {0, 0, -1, nullptr, nullptr};
-    return dw_part_of(p, split, blockIdx.y, rt.leaf, rt.first, rt.rows);
+    if (rt.rows == 0 || rt.leaf < 0) return {0, 0, -1, nullptr, nullptr, false};
+    return dw_part_of<T>(p, split, blockIdx.y, rt.leaf, rt.first, rt.rows);
   }
   const int count = min(max(p.g.count[id], 0), p.g.rows);
-  return dw_part_of(p, split, id / p.g.leaves, id % p.g.leaves, min(max(p.g.begin[id], 0), p.g.rows - count), count);
+  return dw_part_of<T>(p, split, id / p.g.leaves, id % p.g.leaves, min(max(p.g.begin[id], 0), p.g.rows - count), count);
 }
 
 // The results v of column col in rows n[0 .. 4) (-1: none), to the output of one tree or to a

@@ -45,7 +45,7 @@ __global__ __launch_bounds__(THREADS) void k_leaf_tile(LeafProduct p, int length
   __syncthreads();
   const int64_t leaf = (int64_t)tree * p.g.leaves + rt.leaf;
   const T* const w = (const T*)p.w + (rt.leaf < 0 ? 0 : leaf * p.outputs * (int64_t)p.inputs);
-  const T* const src = (const T*)(DX ? p.dy : p.x);
+  const T* const src = DX ? (const T*)p.dy + tree * p.dy_tree : (const T*)p.x;
   const int64_t ld = DX ? p.lddy : p.ldx;
   const int m0 = (wave / GN) * WM, n0 = (wave % GN) * WN;
 
@@ -333,7 +333,7 @@ __global__ __launch_bounds__(THREADS) void k_leaf_dx_narrow(LeafProduct p, int c
 #pragma unroll
       for (int s = 0; s < STEPS; ++s) {
         const int m = (s * 4 + q) * V;
-        f[u][s] = load16((const T*)p.dy + (int64_t)max(n[u], 0) * p.lddy + m,
+        f[u][s] = load16((const T*)p.dy + tree * p.dy_tree + (int64_t)max(n[u], 0) * p.lddy + m,
                          n[u] < 0 || rt.leaf < 0 ? 0 : length - m);
       }
 #pragma unroll
@@ -359,11 +359,18 @@ __global__ __launch_bounds__(THREADS) void k_leaf_dx_narrow(LeafProduct p, int c
 }
 
 // The planes of a run of trees added, in float64, since a forest has hundreds; the last run
-// rounds once, the others leave their sums in carry [rows][cols] (null: one run).
+// rounds once, the others leave their sums in carry [rows][cols] (null: one run).  The last
+// adds a layer's residual (null: none).
 struct Run {
   double* carry;
   bool first, last;
+  const void* res;
+  int64_t ldr;
 };
+template <typename T>
+__device__ __forceinline__ double res_at(const Run& run, int64_t row, int64_t col) {
+  return run.res ? (double)(float)((const T*)run.res)[row * run.ldr + col] : 0.0;
+}
 template <int V>
 __device__ __forceinline__ void carry_in(const Run& run, int64_t e, double (&v)[V]) {
   if (run.first) return;
@@ -394,7 +401,7 @@ __global__ __launch_bounds__(THREADS) void k_sum_trees(const float* planes, int6
       double sum[1] = {part[0][lane] + part[1][lane] + part[2][lane] + part[3][lane]};
       carry_in(run, e, sum);
       if (run.last)
-        out[e / cols * ldo + e % cols] = (T)(float)sum[0];
+        out[e / cols * ldo + e % cols] = (T)(float)(sum[0] + res_at<T>(run, e / cols, e % cols));
       else
         run.carry[e] = sum[0];
     }
@@ -421,6 +428,9 @@ __global__ __launch_bounds__(THREADS) void k_sum_few_trees(const float* planes, 
       __builtin_memcpy(run.carry + e, v, sizeof(v));
       continue;
     }
+    if (run.res)
+#pragma unroll
+      for (int i = 0; i < V; ++i) v[i] += res_at<T>(run, (e + i) / cols, (e + i) % cols);
     T o[V];
 #pragma unroll
     for (int i = 0; i < V; ++i) o[i] = (T)(float)v[i];
@@ -457,22 +467,27 @@ __global__ __launch_bounds__(THREADS) void k_leaf_dw(LeafProduct p, int m_tiles,
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const int tiles = m_tiles * k_tiles, tile = (int)(blockIdx.x % tiles);
   const int k0 = tile % k_tiles * BN, m0 = tile / k_tiles * BM;
-  const DwPart part_of = dw_part<THREADS>(p, split, (int)(blockIdx.x / tiles));
+  const DwPart part_of = dw_part<T, THREADS>(p, split, (int)(blockIdx.x / tiles));
   const int tree = part_of.tree, first = part_of.first, count = part_of.count;
-  float *const dw = part_of.dw, *const db = part_of.db;
   if (count < 0) return;
   if (count == 0) {  // the leaf's zeros, in one piece a block
     const int64_t size = (int64_t)p.outputs * p.inputs;
     const int64_t piece = ((size + tiles - 1) / tiles + 3) / 4 * 4, to = min(size, (tile + 1) * piece);
+    const int64_t word = part_of.narrow ? 2 : 4;
     for (int64_t e = tile * piece + tid * 4; e < to; e += THREADS * 4) {
       if (e + 4 <= to) {
         const f32x4 none = {0, 0, 0, 0};
-        __builtin_memcpy(dw + e, &none, 16);
+        char* const at = (char*)part_of.dw + e * word;
+        if (part_of.narrow)
+          __builtin_memcpy(at, &none, 8);
+        else
+          __builtin_memcpy(at, &none, 16);
       } else {
-        for (int64_t k = e; k < to; ++k) dw[k] = 0.0f;
+        for (int64_t k = e; k < to; ++k) put<T>(part_of, part_of.dw, k, 0.0f);
       }
     }
-    for (int m = tile * THREADS + tid; db && m < p.outputs; m += tiles * THREADS) db[m] = 0.0f;
+    for (int m = tile * THREADS + tid; part_of.db && m < p.outputs; m += tiles * THREADS)
+      put<T>(part_of, part_of.db, m, 0.0f);
     return;
   }
 
@@ -484,7 +499,8 @@ __global__ __launch_bounds__(THREADS) void k_leaf_dw(LeafProduct p, int m_tiles,
   f32x4 bias[WM / 16][1];
 #pragma unroll
   for (int i = 0; i < WM / 16; ++i) bias[i][0] = f32x4{0, 0, 0, 0};
-  const bool sums = db && k0 == 0 && wave % GN == 0;  // a product with ones
+  const bool sums = part_of.db && k0 == 0 && wave % GN == 0;  // a product with ones
+  const T* const dy = (const T*)p.dy + tree * p.dy_tree;
 
   // rows of step s in row_of[s & 1]; the loads of a step are two steps behind its rows
   auto rows = [&](int r0) {
@@ -498,7 +514,7 @@ __global__ __launch_bounds__(THREADS) void k_leaf_dw(LeafProduct p, int m_tiles,
       const int at = tid + i * THREADS;
       if (BM * 8 % THREADS != 0 && at >= BM * 8) break;
       const int n = of[at / CA], m = m0 + at % CA * V;
-      ra[i] = load16((const T*)p.dy + (int64_t)max(n, 0) * p.lddy + m, n < 0 ? 0 : p.outputs - m);
+      ra[i] = load16(dy + (int64_t)max(n, 0) * p.lddy + m, n < 0 ? 0 : p.outputs - m);
     }
 #pragma unroll
     for (int i = 0; i < BCH; ++i) {
@@ -561,14 +577,15 @@ __global__ __launch_bounds__(THREADS) void k_leaf_dw(LeafProduct p, int m_tiles,
 #pragma unroll
   for (int i = 0; i < WM / 16; ++i) {
     const int mi = m0 + (wave / GN) * WM + i * 16;
-    if (sums && lane < 16 && mi + lane < p.outputs) db[mi + lane] = bias[i][0][0];
+    if (sums && lane < 16 && mi + lane < p.outputs) put<T>(part_of, part_of.db, mi + lane, bias[i][0][0]);
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
       const int m = mi + (lane >> 4) * 4 + e;
 #pragma unroll
       for (int j = 0; j < WN / 16; ++j) {
         const int k = k0 + (wave % GN) * WN + j * 16 + (lane & 15);
-        if (m < p.outputs && k < p.inputs) dw[(int64_t)m * p.inputs + k] = acc[i][j][e];
+        if (m < p.outputs && k < p.inputs)
+          put<T>(part_of, part_of.dw, (int64_t)m * p.inputs + k, acc[i][j][e]);
       }
     }
   }
@@ -583,13 +600,13 @@ __global__ __launch_bounds__(THREADS) void k_leaf_dw_small(LeafProduct p, Split 
   constexpr int V = El<T>::V, STEP = 4 * V, UNROLL = NB == 8 ? 1 : 2;
   __shared__ f32x4 sums[THREADS / 64][NB + 1][64];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, r = lane & 15, q = lane >> 4;
-  const DwPart part_of = dw_part<THREADS>(p, split, (int)blockIdx.x);
+  const DwPart part_of = dw_part<T, THREADS>(p, split, (int)blockIdx.x);
   if (part_of.count < 0) return;
   f32x4 acc[1][NB + 1];  // the last: with ones
 #pragma unroll
   for (int j = 0; j <= NB; ++j) acc[0][j] = f32x4{0, 0, 0, 0};
   // columns behind the last only make results that are not stored
-  const T* const dy = (const T*)p.dy + min(r, p.outputs - 1);
+  const T* const dy = (const T*)p.dy + part_of.tree * p.dy_tree + min(r, p.outputs - 1);
   const T* x[NB];
 #pragma unroll
   for (int j = 0; j < NB; ++j) x[j] = (const T*)p.x + min(j * 16 + r, p.inputs - 1);
@@ -641,19 +658,22 @@ __global__ __launch_bounds__(THREADS) void k_leaf_dw_small(LeafProduct p, Split 
 #pragma unroll
     for (int w = 1; w < THREADS / 64; ++w) v += sums[w][j][lane];
     if (j == NB) {
-      if (part_of.db && lane < p.outputs && lane < 16) part_of.db[lane] = v[0];
+      if (part_of.db && lane < p.outputs && lane < 16) put<T>(part_of, part_of.db, lane, v[0]);
       continue;
     }
     const int k = j * 16 + r;
 #pragma unroll
     for (int e = 0; e < 4; ++e)
-      if (q * 4 + e < p.outputs && k < p.inputs) part_of.dw[(q * 4 + e) * p.inputs + k] = v[e];
+      if (q * 4 + e < p.outputs && k < p.inputs)
+        put<T>(part_of, part_of.dw, (q * 4 + e) * p.inputs + k, v[e]);
   }
 }
 
 // The slots of a leaf of several parts added in their order, by `parts` blocks a leaf, in
 // float64: a long leaf has hundreds.  `zeros`: and the zeros of leaves without rows.
+template <typename T>
 __global__ __launch_bounds__(THREADS) void k_sum_slots(LeafProduct p, Split split, int parts, bool zeros) {
+  const DwPart to{0, 0, 0, p.dw, p.db, sizeof(T) == 2 && p.narrow};
   const int64_t at = blockIdx.x / parts;  // leaf of the forest
   const int tree = (int)(at / p.g.leaves);
   const int count = min(max(p.g.count[at], 0), p.g.rows), begin = min(max(p.g.begin[at], 0), p.g.rows - count);
@@ -669,9 +689,9 @@ __global__ __launch_bounds__(THREADS) void k_sum_slots(LeafProduct p, Split spli
 #pragma unroll 16
     for (int64_t s = 1; s <= more; ++s) v += (double)others[2 * s * size + e];
     if (e < map)
-      p.dw[at * map + e] = (float)v;
+      put<T>(to, to.dw, at * map + e, (float)v);
     else
-      p.db[at * p.outputs + (e - map)] = (float)v;
+      put<T>(to, to.db, at * p.outputs + (e - map), (float)v);
   }
 }
 
@@ -714,10 +734,11 @@ bool wide_tiles(const LeafProduct& p, int cols) {
 
 // Leaves of one part leave most of the blocks without work (bfloat16, 60000 x 256 to 256 by 300
 // leaves: 88 us of all the kernels by 2^16 blocks, 55 by 2^13).
+template <typename T>
 void sum_slots(const LeafProduct& p, const Split& split, bool zeros, hipStream_t s) {
   const int64_t leaves = (int64_t)p.g.trees * p.g.leaves, size = (int64_t)p.outputs * (p.inputs + 1);
   const int parts = (int)std::max<int64_t>(1, std::min((size + THREADS - 1) / THREADS, (1 << 13) / leaves));
-  k_sum_slots<<<(unsigned)(leaves * parts), THREADS, 0, s>>>(p, split, parts, zeros);
+  k_sum_slots<T><<<(unsigned)(leaves * parts), THREADS, 0, s>>>(p, split, parts, zeros);
 }
 
 template <typename T>
@@ -740,7 +761,7 @@ void launch_dw(const LeafProduct& p, hipStream_t s) {
     k_leaf_dw<T, 128, 16, 4><<<grid, THREADS, 0, s>>>(p, mt, kt, split);
   else
     k_leaf_dw<T, 64, 64, 2><<<grid, THREADS, 0, s>>>(p, mt, kt, split);
-  if (split.rows) sum_slots(p, split, true, s);
+  if (split.rows) sum_slots<T>(p, split, true, s);
 }
 
 template <typename T, bool DX, int BM, int BN>
@@ -823,11 +844,17 @@ void launch(const LeafProduct& p, int what, hipStream_t s) {
     if (!leaf_big_fits(p, what)) return launch_dw<T>(p, s);
     launch_leaf_big(p, what, s);
     const Split split = leaf_big_split(p);
-    if (split.rows) sum_slots(p, split, !leaf_big_ranks(p.g), s);
+    if (split.rows) sum_slots<T>(p, split, !leaf_big_ranks(p.g), s);
     return;
   }
-  const Form form = form_of(p, what);
-  if (p.g.trees == 1) return launch_product<T>(p, what, form, s);
+  const Form form = what == LEAF_LAYER ? Form{} : form_of(p, what);
+  const auto make = [&](const LeafProduct& q) {
+    if (what == LEAF_LAYER)
+      launch_leaf_layer(q, p.g.trees, s);
+    else
+      launch_product<T>(q, what, form, s);
+  };
+  if (p.g.trees == 1) return make(p);
   const int cols = what == LEAF_PRODUCT_DX ? p.inputs : p.outputs, trees = run_trees(p, what);
   const int64_t total = (int64_t)p.g.rows * cols;
   double* const carry = trees < p.g.trees ? (double*)((char*)p.ws + planes_bytes(p, what)) : nullptr;
@@ -837,10 +864,12 @@ void launch(const LeafProduct& p, int what, hipStream_t s) {
     q.planes = true;
     q.g.trees = std::min(trees, p.g.trees - t);
     q.g.order += (int64_t)t * p.g.rows, q.g.begin += leaves, q.g.count += leaves;
-    q.w = (const T*)p.w + leaves * p.outputs * p.inputs;
-    if (p.b) q.b = (const T*)p.b + leaves * p.outputs;
-    launch_product<T>(q, what, form, s);
-    const Run run{carry, t == 0, t + trees >= p.g.trees};
+    q.w = (const T*)p.w + leaves * p.map_rows() * p.inputs;
+    if (p.b) q.b = (const T*)p.b + leaves * p.map_rows();
+    if (p.dy) q.dy = (const T*)p.dy + t * p.dy_tree;
+    if (p.z) q.z = p.z_of<T>(t);
+    make(q);
+    const Run run{carry, t == 0, t + trees >= p.g.trees, p.res, p.ldr};
     const float* const planes = (const float*)p.ws;
     const auto blocks = [&](int64_t elements, int64_t most) { return (unsigned)std::min(elements, most); };
     if (q.g.trees >= 16)
@@ -872,6 +901,7 @@ size_t leaf_product_workspace(const LeafProduct& p, int what) {
 }
 
 int64_t leaf_product_blocks(const LeafProduct& p, int what) {
+  if (what == LEAF_LAYER) return leaf_layer_blocks(p);
   if (leaf_big_fits(p, what)) return leaf_big_blocks(p, what);
   if (what == LEAF_PRODUCT_DW) {
     const DwShape d = dw_shape(p);

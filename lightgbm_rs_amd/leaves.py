@@ -1,6 +1,6 @@
 """The operators around a forest's leaves, as methods of `HipBackend` over torch tensors:
-rows grouped by leaf, the leaves' linear maps and their gradients, dropout and class scores
-(include/lgbm_hip.h has the definitions).
+rows grouped by leaf, the leaves' linear maps and layers and their gradients, clipping of
+gradients, dropout and class scores (include/lgbm_hip.h has the definitions).
 
 Tensors are on the backend's device; matrices have a row stride (a matrix whose columns
 are strided is copied first).  A call queues its work on torch's current stream of that
@@ -45,6 +45,32 @@ class _Scores(C.Structure):
                 ("ldo", C.c_int64)]
 
 
+class _Layer(C.Structure):
+    """`lgbm_leaf_layer`."""
+
+    _fields_ = [("maps", _Maps), ("activation", C.c_int32), ("gated", C.c_int32), ("x", C.c_void_p),
+                ("ldx", C.c_int64), ("w", C.c_void_p), ("bias", C.c_void_p),
+                ("residual", C.c_void_p), ("ldr", C.c_int64), ("y", C.c_void_p),
+                ("ldy", C.c_int64), ("z", C.c_void_p), ("z_dtype", C.c_int32), ("_pad", C.c_int32)]
+
+
+class _LayerGrad(C.Structure):
+    """`lgbm_leaf_layer_grad`."""
+
+    _fields_ = [("maps", _Maps), ("activation", C.c_int32), ("gated", C.c_int32),
+                ("dy", C.c_void_p), ("lddy", C.c_int64), ("z", C.c_void_p), ("x", C.c_void_p),
+                ("ldx", C.c_int64), ("w", C.c_void_p), ("dx", C.c_void_p), ("lddx", C.c_int64),
+                ("dw", C.c_void_p), ("dbias", C.c_void_p), ("dw_dtype", C.c_int32),
+                ("z_dtype", C.c_int32)]
+
+
+# `lgbm_grad`
+_GRAD = np.dtype([("in", np.uint64), ("out", np.uint64), ("count", np.int64), ("dtype", np.int32),
+                  ("_pad", np.int32)])
+
+ACTIVATIONS = {"none": 0, "relu": 1, "silu": 2, "gelu": 3, "gelu_tanh": 4, "sigmoid": 5}
+
+
 class LeafGroups(NamedTuple):
     """The rows of every leaf: order int32 [trees, rows], begin and count int32 [trees,
     leaves] (each leaf's range of its tree's order)."""
@@ -79,6 +105,13 @@ def _module():
                 ("leaf_product", (p, p, p, i64, p, p, p, i64, p, size, p)),
                 ("leaf_product_dx", (p, p, p, i64, p, p, i64, p, size, p)),
                 ("leaf_product_dw", (p, p, p, i64, p, i64, p, p, p, size, p)),
+                ("leaf_layer_workspace", (p, p)),
+                ("leaf_layer", (p, p, p, size, p)),
+                ("leaf_layer_grad_workspace", (p, p)),
+                ("leaf_layer_grad", (p, p, p, size, p)),
+                ("grad_norm_workspace", (p, i64, p)),
+                ("grad_norm", (p, p, i64, p, p, size, p)),
+                ("clip_grads", (p, p, i64, C.c_double, p, p, size, p)),
                 ("dropout", (p, p, i64, i64, i64, i32, C.c_double, u64, u64, i32, p, i64, p)),
                 ("adjust_scores_workspace", (p, p)),
                 ("adjust_scores", (p, p, p, size, p))):
@@ -296,6 +329,199 @@ def _leaf_product_dw(self, dy, x, groups, bias=True, out=None, bias_out=None):
     return dw, db
 
 
+def _activation(name):
+    if name not in ACTIVATIONS:
+        raise ValueError(f"activation is none of {', '.join(ACTIVATIONS)}")
+    return ACTIVATIONS[name]
+
+
+def _leaf_layer(self, x, weight, groups, bias=None, activation="none", gated=False, residual=None,
+                keep=False, out=None):
+    """y[n] = residual[n] + sum over trees of f(z[t, n]), z[t, n] = weight[t, leaf] x[n] +
+    bias[t, leaf] (`lgbm_hip_leaf_layer`).  f is the activation ("none", "relu", "silu", "gelu",
+    "gelu_tanh" or "sigmoid"), or with `gated` the activation of z's first half times its second.
+
+    x [rows, inputs], weight [trees * leaves, R, inputs], bias [trees * leaves, R] or None,
+    residual [rows, outputs] or None, all float32, bfloat16 or float16; R is outputs, gated 2 *
+    outputs.  Returns y [rows, outputs], or with `keep` (y, z [trees, rows, R]) for
+    `leaf_layer_grad`: z in float32, or of a type given as `keep`, which may be x's.  out may be
+    residual."""
+    torch = _module()
+    if x.dim() != 2 or weight.dim() != 3:
+        raise ValueError("x has to be [rows, inputs], weight [leaves, outputs, inputs]")
+    act, dtype, (rows, inputs) = _activation(activation), _dtype(x, "x"), x.shape
+    leaves, full = weight.shape[:2]
+    _shape(weight, (leaves, full, inputs), "weight")
+    if gated and full % 2:
+        raise ValueError("a gated layer's maps have an even number of rows")
+    outputs = full // 2 if gated else full
+    for name, t, shape in (("weight", weight, weight.shape), ("bias", bias, (leaves, full)),
+                           ("residual", residual, (rows, outputs))):
+        if t is None:
+            continue
+        if t.dtype != x.dtype:
+            raise ValueError(f"x and {name} differ in type")
+        _shape(t, shape, name)
+    _here(self, x=x, weight=weight, bias=bias, residual=residual, out=out)
+    m, hold_maps = _maps(self, torch, rows, inputs, outputs, dtype, groups, leaves)
+    given, inplace = out, out is not None and out is residual
+    x, weight = _rows(x), weight.contiguous()
+    bias = None if bias is None else bias.contiguous()
+    out = _out(out, x, (rows, outputs))
+    if residual is not None and not inplace:
+        residual = _rows(residual)
+    ztype = torch.float32 if isinstance(keep, bool) else keep
+    if ztype not in (torch.float32, x.dtype):
+        raise ValueError(f"keep is {keep}: True, float32 or {x.dtype} is needed")
+    z = None if keep is False else x.new_empty((m.num_trees, rows, full), dtype=ztype)
+    at = lambda t: None if t is None else t.data_ptr()
+    a = _Layer(m, act, bool(gated), at(x), _ld(x), at(weight), at(bias), at(residual),
+               0 if residual is None else _ld(residual), at(out), _ld(out), at(z), _DTYPES[ztype], 0)
+    ws, nbytes, hold = _workspace(self, torch, self.lib.lgbm_hip_leaf_layer_workspace, C.byref(a))
+    self._check(self.lib.lgbm_hip_leaf_layer(self.ctx, C.byref(a), ws, nbytes, _stream(self, torch)))
+    _written(given)
+    return out if z is None else (out, z)
+
+
+def _leaf_layer_grad(self, dy, z, x, weight, groups, activation="none", gated=False, bias=True,
+                     inputs=True, maps=True, out=None, weight_out=None, bias_out=None):
+    """The gradients of `leaf_layer` (`lgbm_hip_leaf_layer_grad`) from dy [rows, outputs] and the
+    z that it kept (None for a layer that is neither gated nor has an activation): (dx [rows,
+    inputs], dw as weight, dbias [trees * leaves, R]).  Left out and None: dx without `inputs`,
+    dw and dbias without `maps`, dbias without `bias`.  dw and dbias have the type of x; a
+    weight_out of float32 takes them in that (bias_out has weight_out's type).  The gradient of
+    the residual is dy."""
+    torch = _module()
+    if dy.dim() != 2 or x.dim() != 2 or weight.dim() != 3:
+        raise ValueError("dy has to be [rows, outputs], x [rows, inputs], weight [leaves, outputs, inputs]")
+    act, dtype, (rows, cols) = _activation(activation), _dtype(x, "x"), x.shape
+    leaves, full = weight.shape[:2]
+    _shape(weight, (leaves, full, cols), "weight")
+    if gated and full % 2:
+        raise ValueError("a gated layer's maps have an even number of rows")
+    outputs = full // 2 if gated else full
+    _shape(dy, (rows, outputs), "dy")
+    if not inputs and not maps:
+        raise ValueError("neither inputs nor maps")
+    bias = bias and maps
+    for name, t, asked in (("out", out, inputs), ("weight_out", weight_out, maps),
+                           ("bias_out", bias_out, bias)):
+        if t is not None and not asked:
+            raise ValueError(f"{name} for a gradient that is not asked for")
+    linear = act == 0 and not gated
+    if z is None and not linear:
+        raise ValueError("z is needed (leaf_layer with keep=True)")
+    z = None if linear else z
+    for name, t in (("dy", dy), ("weight", weight)):
+        if t.dtype != x.dtype:
+            raise ValueError(f"x and {name} differ in type")
+    ztype = torch.float32 if z is None else z.dtype
+    if ztype not in (torch.float32, x.dtype):
+        raise ValueError(f"z is {ztype}: float32 or {x.dtype} is needed")
+    _here(self, dy=dy, z=z, x=x, weight=weight, out=out, weight_out=weight_out, bias_out=bias_out)
+    m, hold_maps = _maps(self, torch, rows, cols, outputs, dtype, groups, leaves)
+    if z is not None:
+        _shape(z, (m.num_trees, rows, full), "z")
+        z = z.contiguous()
+    wtype = x.dtype if weight_out is None else weight_out.dtype
+    if wtype not in (x.dtype, torch.float32):
+        raise ValueError(f"weight_out is {wtype}: {x.dtype} or float32 is needed")
+    for name, t, shape in (("weight_out", weight_out, weight.shape), ("bias_out", bias_out, (leaves, full))):
+        if t is not None:
+            _shape(t, shape, name)
+            if t.dtype != wtype or not t.is_contiguous():
+                raise ValueError(f"{name} has to be contiguous {wtype}")
+    given = (out, weight_out, bias_out)
+    dy, x = _rows(dy), _rows(x)
+    dx = _out(out, x, (rows, cols)) if inputs else None
+    dw, db = weight_out, bias_out
+    if maps and dw is None:
+        dw = x.new_empty(weight.shape)
+    if bias and db is None:
+        db = x.new_empty((leaves, full), dtype=wtype)
+    weight = weight.contiguous()
+    at = lambda t: None if t is None else t.data_ptr()
+    a = _LayerGrad(m, act, bool(gated), at(dy), _ld(dy), at(z), at(x), _ld(x), at(weight), at(dx),
+                   0 if dx is None else _ld(dx), at(dw), at(db), _DTYPES[wtype], _DTYPES[ztype])
+    ws, nbytes, hold = _workspace(self, torch, self.lib.lgbm_hip_leaf_layer_grad_workspace, C.byref(a))
+    self._check(self.lib.lgbm_hip_leaf_layer_grad(self.ctx, C.byref(a), ws, nbytes, _stream(self, torch)))
+    _written(*given)
+    return dx, dw, db
+
+
+def _dense(t):
+    """Whether t's elements lie side by side in some order of its dimensions."""
+    if t.is_contiguous():
+        return True
+    step = 1
+    for stride, size in sorted((st, n) for st, n in zip(t.stride(), t.shape) if n != 1):
+        if stride != step:
+            return False
+        step *= size
+    return True
+
+
+def _grad_list(self, tensors, out):
+    """The list as an array of `lgbm_grad`."""
+    torch = _module()
+    a = np.zeros(len(tensors), _GRAD)
+    for name, ts, field in (("tensors", tensors, "in"), ("out", out, "out")):
+        if ts is None:
+            continue
+        if not all(map(torch.Tensor.is_contiguous, ts)) and not all(map(_dense, ts)):
+            raise ValueError(f"a tensor of {name} has gaps")
+        if torch.is_grad_enabled() and any(t.requires_grad for t in ts):
+            raise ValueError(f"{name} require gradients, which this call does not record")
+        for d in {t.device for t in ts}:
+            if d.type != "cuda" or d.index != self.device:
+                raise ValueError(f"a tensor of {name} is on {d}: cuda:{self.device} is needed")
+        a[field] = list(map(torch.Tensor.data_ptr, ts))
+    types = [t.dtype for t in tensors]
+    for dtype in set(types):
+        if dtype not in _DTYPES or dtype == torch.float64:
+            raise ValueError(f"a tensor is {dtype}: a floating-point type of at most 32 bits is needed")
+    a["dtype"] = [_DTYPES[d] for d in types]
+    a["count"] = list(map(torch.Tensor.numel, tensors))
+    return a
+
+
+def _norm_of(self, tensors, out, max_norm):
+    torch = _module()
+    a = _grad_list(self, tensors, out)
+    norm = torch.empty((), dtype=torch.float32, device=f"cuda:{self.device}")
+    ws, nbytes, hold = _workspace(self, torch, self.lib.lgbm_hip_grad_norm_workspace, a.ctypes.data, len(a))
+    if out is None:
+        self._check(self.lib.lgbm_hip_grad_norm(self.ctx, a.ctypes.data, len(a), norm.data_ptr(), ws,
+                                                nbytes, _stream(self, torch)))
+    else:
+        self._check(self.lib.lgbm_hip_clip_grads(self.ctx, a.ctypes.data, len(a), max_norm,
+                                                 norm.data_ptr(), ws, nbytes, _stream(self, torch)))
+        _written(*out)
+    return norm
+
+
+def _grad_norm(self, tensors):
+    """The 2-norm over all elements of a list of tensors (`lgbm_hip_grad_norm`), float32,
+    bfloat16 or float16, without gaps: a float32 tensor of no dimensions."""
+    return _norm_of(self, list(tensors), None, 0.0)
+
+
+def _clip_grads(self, tensors, max_norm, out=None):
+    """The tensors times min(1, max_norm / norm), norm their 2-norm over all elements
+    (`lgbm_hip_clip_grads`), in place, or in the tensors of the list `out`.  Returns the norm, a
+    float32 tensor of no dimensions; nothing waits for it."""
+    tensors = list(tensors)
+    if out is not None:
+        out = list(out)
+        if len(out) != len(tensors):
+            raise ValueError("out and the tensors differ in number")
+        if ([t.shape for t in out] != [t.shape for t in tensors]
+                or [t.dtype for t in out] != [t.dtype for t in tensors]
+                or [t.stride() for t in out] != [t.stride() for t in tensors]):
+            raise ValueError("out and the tensors differ in shape, type or strides")
+    return _norm_of(self, tensors, tensors if out is None else out, float(max_norm))
+
+
 def _dropout(self, x, p, seed, offset=0, by="element", out=None):
     """x with elements, or with by="row" whole rows, dropped with probability p and the
     others divided by the share kept (`lgbm_hip_dropout`): the mask follows from seed and
@@ -393,6 +619,10 @@ HipBackend.leaf_groups = _leaf_groups
 HipBackend.leaf_product = _leaf_product
 HipBackend.leaf_product_dx = _leaf_product_dx
 HipBackend.leaf_product_dw = _leaf_product_dw
+HipBackend.leaf_layer = _leaf_layer
+HipBackend.leaf_layer_grad = _leaf_layer_grad
+HipBackend.grad_norm = _grad_norm
+HipBackend.clip_grads = _clip_grads
 HipBackend.dropout = _dropout
 HipBackend.adjust_scores = _adjust_scores
 

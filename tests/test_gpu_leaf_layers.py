@@ -1,0 +1,124 @@
+"""Layers of a forest's leaves, their gradients and the clipping of gradients on the GPU, alone
+and together, on streams and in graphs.  The checks are in leaf_layer_checks.py; they run in one
+child process, which imports torch first."""
+import os
+import subprocess
+import sys
+
+import pytest
+
+from tests.test_gpu_leaf_ops import Worker
+
+pytestmark = pytest.mark.gpu
+HERE = os.path.dirname(os.path.abspath(__file__))
+
+
+class LayerWorker(Worker):
+    def __init__(self):
+        self.p = subprocess.Popen([sys.executable, "-u", os.path.join(HERE, "leaf_layer_worker.py")],
+                                  stdin=subprocess.PIPE, stdout=subprocess.PIPE, text=True)
+        self.answer()
+
+
+@pytest.fixture(scope="module")
+def check():
+    w = LayerWorker()
+    yield w
+    w.close()
+
+
+ACTS = ["none", "relu", "silu", "gelu", "gelu_tanh", "sigmoid"]
+
+# rows, inputs, outputs, trees, leaves, leaves' sizes, pad: one of each; around 8, 16, 32, 64, 128
+# and 256; few and many rows a leaf; several trees; odd strides and addresses; rows in no leaf
+SHAPES = [
+    (1, 1, 1, 1, 1, "one", 0), (5, 3, 2, 1, 3, "even", 1), (64, 28, 1, 20, 31, "even", 0),
+    (17, 16, 16, 1, 1, "one", 0), (100, 33, 17, 2, 7, "lost", 3), (257, 64, 64, 1, 4, "skew", 8),
+    (300, 100, 10, 1, 31, "even", 0), (129, 128, 130, 1, 2, "even", 8), (500, 200, 96, 3, 5, "lost", 0),
+    (16, 520, 300, 1, 31, "even", 0), (1, 1000, 260, 2, 1, "one", 0), (64, 1030, 264, 1, 1, "one", 1),
+    (1000, 70, 257, 1, 3, "skew", 1), (700, 256, 256, 1, 2, "one", 0), (2000, 13, 3, 5, 63, "skew", 0),
+    (40, 2000, 1, 1, 7, "even", 0), (600, 530, 20, 1, 2, "skew", 0), (33, 600, 40, 1, 1, "lost", 1)]
+
+
+@pytest.mark.parametrize("gated", [False, True])
+@pytest.mark.parametrize("dtype", ["f32", "bf16", "f16"])
+@pytest.mark.parametrize("shape", SHAPES)
+def test_layer(check, shape, dtype, gated):
+    i = SHAPES.index(shape)
+    rows, inputs, outputs, trees, leaves, sizes, pad = shape
+    check("layer", rows=rows, inputs=inputs, outputs=outputs, trees=trees, leaves=leaves, dtype=dtype,
+          shape=sizes, pad=pad, act=ACTS[(i + gated) % 6], gated=gated, bias=i % 4 != 3, residual=i % 3 != 1)
+
+
+@pytest.mark.parametrize("gated", [False, True])
+@pytest.mark.parametrize("dtype", ["f32", "bf16", "f16"])
+@pytest.mark.parametrize("shape", SHAPES)
+def test_grads(check, shape, dtype, gated):
+    i = SHAPES.index(shape)
+    rows, inputs, outputs, trees, leaves, sizes, pad = shape
+    check("grads", rows=rows, inputs=inputs, outputs=outputs, trees=trees, leaves=leaves, dtype=dtype,
+          shape=sizes, pad=pad, act=ACTS[(i + 2 * gated) % 6], gated=gated, kept="narrow" if i % 5 == 0 else None)
+
+
+# every activation by every kernel
+@pytest.mark.parametrize("gated", [False, True])
+@pytest.mark.parametrize("act", ACTS)
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+def test_activations(check, dtype, act, gated):
+    for rows, inputs, outputs, leaves in ((90, 40, 6, 2), (12, 600, 50, 3), (200, 72, 80, 2)):
+        check("layer", rows=rows, inputs=inputs, outputs=outputs, leaves=leaves, dtype=dtype, act=act, gated=gated)
+        check("grads", rows=rows, inputs=inputs, outputs=outputs, leaves=leaves, dtype=dtype, act=act, gated=gated)
+
+
+# large tiles of 16-bit types: whole and ragged, rows off 16 bytes, several trees
+@pytest.mark.parametrize("gated", [False, True])
+@pytest.mark.parametrize("rows,inputs,outputs,trees,leaves,dtype,shape,pad", [
+    (4000, 256, 1024, 1, 2, "bf16", "skew", 0), (9001, 264, 520, 1, 3, "f16", "lost", 8),
+    (3000, 328, 776, 2, 3, "bf16", "even", 0), (5000, 200, 512, 1, 2, "bf16", "one", 1),
+    (2600, 1000, 1288, 1, 1, "f16", "lost", 8)])
+def test_large(check, rows, inputs, outputs, trees, leaves, dtype, shape, pad, gated):
+    args = dict(rows=rows, inputs=inputs, outputs=outputs, trees=trees, leaves=leaves, dtype=dtype,
+                shape=shape, pad=pad, gated=gated)
+    check("layer", act="gelu", residual=not gated, **args)
+    check("grads", act="silu", **args)
+
+
+@pytest.mark.parametrize("trees", [1, 3])
+@pytest.mark.parametrize("gated", [False, True])
+@pytest.mark.parametrize("act", ["none", "silu", "gelu", "gelu_tanh", "sigmoid"])
+def test_differences(check, act, gated, trees):
+    check("differences", act=act, gated=gated, trees=trees)
+
+
+def test_extreme_values(check):
+    check("extreme")
+
+
+def test_empty_tables(check):
+    check("kernels_of_layers")
+
+
+def test_linear_layers_are_products(check):
+    check("as_products")
+
+
+@pytest.mark.parametrize("sizes,dtypes,flat", [
+    ([1], ["f32"], False), ([7, 0, 1], ["bf16", "f32"], False), ([4096, 4095, 4097], ["f16"], True),
+    ([100003, 5, 70000], ["f32", "bf16", "f16"], False), ([13] * 300, ["bf16"], True),
+    ([1000, 0] * 128 + [9], ["f32"], True), ([20000003, 3], ["bf16"], True), ([9000001] * 2, ["f32", "f16"], False)])
+@pytest.mark.parametrize("factor", [0.25, 1.5])
+def test_clip(check, sizes, dtypes, flat, factor):
+    check("clip", sizes=sizes, dtypes=dtypes, flat=flat, factor=factor)
+
+
+def test_clip_special_values(check):
+    check("clip_special")
+
+
+def test_refused(check):
+    check("refused")
+
+
+@pytest.mark.parametrize("dtype,trees", [("f32", 1), ("bf16", 1), ("f16", 2), ("bf16", 3)])
+def test_block(check, dtype, trees):
+    check("block", dtype=dtype, trees=trees)
