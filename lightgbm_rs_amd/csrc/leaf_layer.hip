@@ -5,6 +5,7 @@
 // (unless it is kept for the gradients) nor the two halves of a gated layer go through memory.
 // Several trees write float32 planes that are added together with r.
 #include <algorithm>
+#include <type_traits>
 
 #include "leaf_layer.h"
 
@@ -125,6 +126,237 @@ __global__ __launch_bounds__(THREADS) void k_layer_tile(LeafProduct p, int col_t
   }
 }
 
+// ---- few rows a leaf ------------------------------------------------------------------------------
+
+// Bound by reading the maps: a block makes 16 RB rows by 16 results of a leaf (32 rows of its map
+// where gated); its waves take every WAVES-th stretch of the inputs, and their sums are added in
+// LDS in the waves' order.  A wave's stretch is BYTES of every row, side by side in the lanes (a
+// matrix instruction takes 16 rows side by side: loads in its order touch a line for every lane),
+// and goes through LDS to the lanes that need it, the next stretch on its way.
+template <typename T, bool GATED, int RB, int WAVES, int BYTES>
+__attribute__((amdgpu_waves_per_eu(1, 4))) __global__ __launch_bounds__(WAVES * 64) void k_layer_few(LeafProduct p, int col_tiles) {
+  constexpr int V = El<T>::V, NB = GATED ? 2 : 1, PART = BYTES / (int)sizeof(T), STEPS = BYTES / 64;
+  constexpr int CH = BYTES / 16, PER = 64 / CH;  // chunks a row, rows a load
+  constexpr int XLOADS = 16 * RB / PER, LOADS = XLOADS + 16 * NB / PER, STAGE = 16 * (RB + NB) * BYTES;
+  constexpr int PITCH = 16 * NB + 4, SUMS = 16 * RB * PITCH * 4;
+  __shared__ __align__(16) char lds[WAVES * (STAGE > SUMS ? STAGE : SUMS)];
+  __shared__ int32_t row_of[16 * RB];
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, r = lane & 15, q = lane >> 4;
+  const int tree = blockIdx.y, length = p.inputs, cols = p.outputs;
+  const int c0 = (int)(blockIdx.x % col_tiles) * 16;
+  const RowTile rt = find_tile<WAVES * 64>(p.g, tree, blockIdx.x / col_tiles, 16 * RB);
+  if (rt.rows == 0) return;
+  const int64_t leaf = rt.leaf < 0 ? -1 : (int64_t)tree * p.g.leaves + rt.leaf;
+  if (tid < 16 * RB) row_of[tid] = tid < rt.rows ? row_at(p.g, tree, rt.first + tid) : -1;
+  __syncthreads();
+  f32x4 acc[RB][NB];
+#pragma unroll
+  for (int i = 0; i < RB; ++i)
+#pragma unroll
+    for (int j = 0; j < NB; ++j) acc[i][j] = f32x4{0, 0, 0, 0};
+  if (leaf >= 0) {
+    char* const mine = lds + wave * STAGE;
+    const int chunk = lane % CH;
+    // rows in the order of the stage: x's, the gates', the other half's
+    const T* from[LOADS];
+    int to[LOADS];
+#pragma unroll
+    for (int i = 0; i < LOADS; ++i) {
+      const int row = i * PER + lane / CH;
+      if (i < XLOADS)
+        from[i] = (const T*)p.x + (int64_t)max(row_of[row], 0) * p.ldx;
+      else
+        from[i] = (const T*)p.w + (leaf * p.map_rows() + (row - 16 * RB) / 16 * cols + min(c0 + row % 16, cols - 1)) *
+                                      (int64_t)length;
+      from[i] += chunk * V;
+      to[i] = row * BYTES + ((chunk ^ row) & (CH - 1)) * 16;
+    }
+    u32x4 ahead[LOADS];
+    const auto load = [&](int k0) {
+      if (k0 + PART <= length) {
+#pragma unroll
+        for (int i = 0; i < LOADS; ++i) ahead[i] = load16(from[i] + k0);
+      } else if (k0 < length) {
+#pragma unroll
+        for (int i = 0; i < LOADS; ++i) ahead[i] = load16(from[i] + k0, length - k0 - chunk * V);
+      }
+    };
+    load(wave * PART);
+    for (int k0 = wave * PART; k0 < length; k0 += WAVES * PART) {
+#pragma unroll
+      for (int i = 0; i < LOADS; ++i) *reinterpret_cast<u32x4*>(mine + to[i]) = ahead[i];
+      __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+      __builtin_amdgcn_wave_barrier();
+      load(k0 + WAVES * PART);
+      Parts<T, RB, NB> part(acc);
+#pragma unroll
+      for (int u = 0; u < STEPS; ++u) {
+        const auto frag = [&](int row0) {
+          const int row = row0 + r;
+          return *reinterpret_cast<const u32x4*>(mine + row * BYTES + (((u * 4 + q) ^ row) & (CH - 1)) * 16);
+        };
+        u32x4 fw[NB];
+#pragma unroll
+        for (int j = 0; j < NB; ++j) fw[j] = frag(16 * (RB + j));
+#pragma unroll
+        for (int i = 0; i < RB; ++i) {
+          const u32x4 fx = frag(16 * i);
+#pragma unroll
+          for (int j = 0; j < NB; ++j) part.at[i][j] = El<T>::mfma(fx, fw[j], part.at[i][j]);
+        }
+      }
+      part.add_to(acc);
+      __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+      __builtin_amdgcn_wave_barrier();
+    }
+    __syncthreads();
+  }
+  float* const sums = reinterpret_cast<float*>(lds);
+#pragma unroll
+  for (int i = 0; i < RB; ++i)
+#pragma unroll
+    for (int j = 0; j < NB; ++j)
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        sums[wave * (SUMS / 4) + (i * 16 + q * 4 + e) * PITCH + j * 16 + r] = acc[i][j][e];
+  __syncthreads();
+  // eight results a thread
+  for (int at = tid; at < 16 * RB * 2; at += WAVES * 64) {
+    const int row = at >> 1, col = (at & 1) * 8;
+    float a[8] = {}, u[8] = {};
+#pragma unroll
+    for (int v = 0; v < WAVES; ++v)
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        a[j] += sums[v * (SUMS / 4) + row * PITCH + col + j];
+        if (GATED) u[j] += sums[v * (SUMS / 4) + row * PITCH + 16 + col + j];
+      }
+    layer_end<T, GATED>(p, tree, leaf, row_of[row], c0 + col, a, u);
+  }
+}
+
+// ---- few outputs ----------------------------------------------------------------------------------
+
+// Up to 16 NB outputs of a leaf: bound by reading x, which no wave shares with another, so lanes
+// load their fragments straight from memory, UNROLL steps at a time and without a barrier; maps
+// come from the caches.  A wave takes ROUNDS times 32 rows; blocks of one wave where leaves hold
+// few rows.  Sums stay in registers to the end: lane r of 16 has column r of the outputs.
+template <typename T, bool GATED, int NB, int WAVES>
+__global__ __launch_bounds__(WAVES * 64) void k_layer_narrow(LeafProduct p) {
+  constexpr int V = El<T>::V, UNROLL = 4, ROUNDS = 2, BM = WAVES * 32 * ROUNDS, M = GATED ? 2 * NB : NB;
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, r = lane & 15, q = lane >> 4;
+  const int tree = blockIdx.y, length = p.inputs, cols = p.outputs, rows = p.map_rows();
+  const RowTile rt = find_tile<WAVES * 64>(p.g, tree, blockIdx.x, BM);
+  if (rt.rows == 0) return;
+  const int64_t leaf = (int64_t)tree * p.g.leaves + rt.leaf;
+  const T* const w = (const T*)p.w + (rt.leaf < 0 ? 0 : leaf * rows * (int64_t)length);
+  // group j of 16 map rows: outputs 16 (j % NB) on, of the gates or the second half
+  const T* wrow[M];
+  float b[M];
+#pragma unroll
+  for (int j = 0; j < M; ++j) {
+    const int at = j / NB * cols + min(j % NB * 16 + r, cols - 1);
+    wrow[j] = w + (int64_t)at * length;
+    b[j] = p.b && rt.leaf >= 0 ? (float)((const T*)p.b)[leaf * rows + at] : 0.0f;
+  }
+  int n[ROUNDS][2];
+#pragma unroll
+  for (int t = 0; t < ROUNDS; ++t)
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const int at = (t * WAVES + wave) * 32 + i * 16 + r;
+      n[t][i] = at < rt.rows ? row_at(p.g, tree, rt.first + at) : -1;
+    }
+#pragma unroll
+  for (int t = 0; t < ROUNDS; ++t) {
+    if ((t * WAVES + wave) * 32 >= rt.rows) break;
+    // the rows of a lane's results, and what they have already
+    int of[2][4];
+    float res[2][NB][4];
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      rows_of(n[t][i], lane, of[i]);
+#pragma unroll
+      for (int j = 0; j < NB; ++j)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const int col = j * 16 + r;
+          const bool has = p.res && !p.planes && of[i][e] >= 0 && col < cols;
+          res[i][j][e] = has ? (float)((const T*)p.res)[of[i][e] * p.ldr + col] : 0.0f;
+        }
+    }
+    f32x4 acc[2][M];
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+#pragma unroll
+      for (int j = 0; j < M; ++j) acc[i][j] = f32x4{b[j], b[j], b[j], b[j]};
+    if (rt.leaf >= 0) {
+      const T* xrow[2];
+#pragma unroll
+      for (int i = 0; i < 2; ++i) xrow[i] = (const T*)p.x + (int64_t)max(n[t][i], 0) * p.ldx;
+      const auto stretch = [&](int k0, auto whole) {
+        u32x4 fa[UNROLL][2], fb[UNROLL][M];
+#pragma unroll
+        for (int u = 0; u < UNROLL; ++u) {
+          const int k = k0 + (u * 4 + q) * V;
+#pragma unroll
+          for (int i = 0; i < 2; ++i) fa[u][i] = whole ? load16(xrow[i] + k) : load16(xrow[i] + k, length - k);
+#pragma unroll
+          for (int j = 0; j < M; ++j) fb[u][j] = whole ? load16(wrow[j] + k) : load16(wrow[j] + k, length - k);
+        }
+        Parts<T, 2, M> part(acc);
+#pragma unroll
+        for (int u = 0; u < UNROLL; ++u) {
+          if (k0 + u * 4 * V >= length) break;
+#pragma unroll
+          for (int i = 0; i < 2; ++i)
+#pragma unroll
+            for (int j = 0; j < M; ++j) part.at[i][j] = El<T>::mfma(fa[u][i], fb[u][j], part.at[i][j]);
+        }
+        part.add_to(acc);
+      };
+      int k0 = 0;
+      for (; k0 + 4 * V * UNROLL <= length; k0 += 4 * V * UNROLL) stretch(k0, std::true_type());
+      if (k0 < length) stretch(k0, std::false_type());
+    }
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+#pragma unroll
+      for (int j = 0; j < NB; ++j) {
+        const int col = j * 16 + r;
+        float a[4], f[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) a[e] = acc[i][j][e];
+        if (p.z) {
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            if (of[i][e] < 0 || col >= cols) continue;
+            const int64_t at = (int64_t)of[i][e] * rows + col;
+            if (sizeof(T) == 2 && p.z_narrow) {
+              T* const z = (T*)p.z_of<T>(tree) + at;
+              z[0] = (T)a[e];
+              if (GATED) z[cols] = (T)acc[i][GATED ? NB + j : 0][e];
+            } else {
+              float* const z = (float*)p.z_of<T>(tree) + at;
+              z[0] = a[e];
+              if (GATED) z[cols] = acc[i][GATED ? NB + j : 0][e];
+            }
+          }
+        }
+        activate<T>(p.act, a, f);
+        f32x4 v;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          v[e] = GATED ? f[e] * acc[i][GATED ? NB + j : 0][e] : f[e];
+          if (rt.leaf < 0) v[e] = 0.0f;
+          v[e] += res[i][j][e];
+        }
+        store_rows<T>(p, tree, of[i], col, cols, v);
+      }
+    }
+  }
+}
+
 // ---- the gradient of z ----------------------------------------------------------------------------
 
 // dz = dy f'(z), or where gated dy f'(z_gate) z_up and dy f(z_gate): eight neighbouring results a
@@ -157,6 +389,16 @@ __global__ __launch_bounds__(THREADS) void k_layer_dz(LeafProduct p, int64_t pie
 
 // ---- which kernel ---------------------------------------------------------------------------------
 
+// Leaves of 16 rows at most, on average.
+bool few_rows_a_leaf(const LeafProduct& p) { return p.g.rows <= 16 * (int64_t)p.g.leaves; }
+
+// Rows a block of k_layer_few, in units of 16, 0: not for it.
+int few_rows(const LeafProduct& p) {
+  const int64_t rows = (p.g.rows + p.g.leaves - 1) / p.g.leaves;
+  if (p.inputs < 512) return 0;
+  return rows <= 16 ? 1 : rows <= 32 ? 2 : rows <= 128 ? 4 : 0;
+}
+
 // Tiles of 128 x 128, as for the linear maps (wide_tiles).
 bool wide_tiles(const LeafProduct& p, int trees) {
   const int rows = p.map_rows();
@@ -172,8 +414,34 @@ void launch_tile(const LeafProduct& p, hipStream_t s) {
   k_layer_tile<T, GATED, BM, BN, 2><<<grid, THREADS, 0, s>>>(p, ct);
 }
 
+template <typename T, bool GATED, int RB>
+void launch_few(const LeafProduct& p, hipStream_t s) {
+  const int ct = (p.outputs + 15) / 16;
+  const dim3 grid((unsigned)(row_tiles(p.g, 16 * RB) * ct), (unsigned)p.g.trees);
+  // 256 bytes a row of few rows, 128 of many (64 rows of 4096 bfloat16 inputs to 4096: 16.1 and
+  // 14.7 us; one row to 4096 gated: 13.6 and 14.1)
+  k_layer_few<T, GATED, RB, 4, RB == 1 ? 256 : 128><<<grid, 256, 0, s>>>(p, ct);
+}
+
 template <typename T, bool GATED>
 void launch(const LeafProduct& p, int trees, hipStream_t s) {
+  const int few = few_rows(p);
+  if (few == 1) return launch_few<T, GATED, 1>(p, s);
+  if (few == 2) return launch_few<T, GATED, 2>(p, s);
+  if (few == 4) return launch_few<T, GATED, 4>(p, s);
+  if (p.outputs <= 32) {
+    const bool one = few_rows_a_leaf(p);
+    const dim3 grid((unsigned)row_tiles(p.g, one ? 64 : 256), (unsigned)p.g.trees);
+    if (p.outputs <= 16 && one)
+      k_layer_narrow<T, GATED, 1, 1><<<grid, 64, 0, s>>>(p);
+    else if (p.outputs <= 16)
+      k_layer_narrow<T, GATED, 1, 4><<<grid, 256, 0, s>>>(p);
+    else if (one)
+      k_layer_narrow<T, GATED, 2, 1><<<grid, 64, 0, s>>>(p);
+    else
+      k_layer_narrow<T, GATED, 2, 4><<<grid, 256, 0, s>>>(p);
+    return;
+  }
   if constexpr (sizeof(T) == 2) {
     if (wide_tiles(p, trees)) return launch_tile<T, GATED, 128, 128>(p, s);
   }
@@ -193,6 +461,7 @@ void launch_dz(const LeafProduct& p, void* dz, hipStream_t s) {
 }  // namespace
 
 int64_t leaf_layer_blocks(const LeafProduct& p) {
+  if (const int few = few_rows(p)) return row_tiles(p.g, 16 * few) * ((p.outputs + 15) / 16);
   const int64_t cb = p.gated ? 32 : 64;
   return row_tiles(p.g, 64) * ((p.outputs + cb - 1) / cb);
 }
