@@ -39,36 +39,40 @@ __device__ __forceinline__ float sigmoid_of(float z) {
   return inverse<T>(1.0f + exp_of<T>(-z));
 }
 
-// N values of an activation.
+// Activations by the code that makes them.
+enum ActClass { ACT_LINE, ACT_SIGMOID, ACT_ERF };
+__host__ __device__ inline ActClass act_class(int act) {
+  return act <= LGBM_HIP_ACT_RELU ? ACT_LINE : act == LGBM_HIP_ACT_GELU ? ACT_ERF : ACT_SIGMOID;
+}
+
+// N values of an activation.  SILU, GELU_TANH ((1 + tanh v) / 2 = sigmoid(2 v)) and SIGMOID are
+// sigmoids of z (c1 + c3 z^2), times z or not; the square is held back, or it would be infinite
+// where c3 is 0.
+template <typename T, ActClass CLASS, int N>
+__device__ __forceinline__ void activate_as(int act, const float (&z)[N], float (&f)[N]) {
+  if (CLASS == ACT_LINE) {
+    const float least = act == LGBM_HIP_ACT_RELU ? 0.0f : -__builtin_inff();
+#pragma unroll
+    for (int i = 0; i < N; ++i) f[i] = z[i] < least ? 0.0f : z[i];  // a NaN stays
+  } else if (CLASS == ACT_ERF) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) f[i] = 0.5f * z[i] * (1.0f + erf_of<T>(z[i] * SQRT_HALF));
+  } else {
+    const bool cubic = act == LGBM_HIP_ACT_GELU_TANH, alone = act == LGBM_HIP_ACT_SIGMOID;
+    const float c1 = cubic ? 2.0f * TANH_SCALE : 1.0f, c3 = cubic ? 2.0f * TANH_SCALE * TANH_CUBE : 0.0f;
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      const float p = sigmoid_of<T>(z[i] * fmaf(c3, fminf(z[i] * z[i], 1e6f), c1));
+      f[i] = alone ? p : z[i] * p;
+    }
+  }
+}
 template <typename T, int N>
 __device__ __forceinline__ void activate(int act, const float (&z)[N], float (&f)[N]) {
-  switch (act) {
-    case LGBM_HIP_ACT_RELU:
-#pragma unroll
-      for (int i = 0; i < N; ++i) f[i] = z[i] < 0.0f ? 0.0f : z[i];  // a NaN stays
-      return;
-    case LGBM_HIP_ACT_SILU:
-#pragma unroll
-      for (int i = 0; i < N; ++i) f[i] = z[i] * sigmoid_of<T>(z[i]);
-      return;
-    case LGBM_HIP_ACT_GELU:
-#pragma unroll
-      for (int i = 0; i < N; ++i) f[i] = 0.5f * z[i] * (1.0f + erf_of<T>(z[i] * SQRT_HALF));
-      return;
-    case LGBM_HIP_ACT_GELU_TANH:  // (1 + tanh u) / 2 = sigmoid(2 u)
-#pragma unroll
-      for (int i = 0; i < N; ++i) {
-        const float u = 2.0f * TANH_SCALE * (z[i] + TANH_CUBE * z[i] * z[i] * z[i]);
-        f[i] = z[i] * sigmoid_of<T>(u);
-      }
-      return;
-    case LGBM_HIP_ACT_SIGMOID:
-#pragma unroll
-      for (int i = 0; i < N; ++i) f[i] = sigmoid_of<T>(z[i]);
-      return;
-    default:
-#pragma unroll
-      for (int i = 0; i < N; ++i) f[i] = z[i];
+  switch (act_class(act)) {
+    case ACT_LINE: return activate_as<T, ACT_LINE>(act, z, f);
+    case ACT_ERF: return activate_as<T, ACT_ERF>(act, z, f);
+    default: activate_as<T, ACT_SIGMOID>(act, z, f);
   }
 }
 
@@ -138,29 +142,16 @@ __device__ __forceinline__ void store8(T* p, int valid, const float (&v)[8]) {
   }
 }
 
-// Eight neighbouring results of row n (-1: none) of a layer, from column col on: a is the map's
-// sums (where gated the gates') and u the second half's.  leaf < 0: the row is in no leaf,
-// nothing is added to it and its z is 0.
-template <typename T, bool GATED>
-__device__ __forceinline__ void layer_end(const LeafProduct& p, int tree, int64_t leaf, int n, int col, float (&a)[8],
-                                          float (&u)[8]) {
+// Eight neighbouring results of row n (-1: none) of a layer, from column col on: a is z (where
+// gated the gates') and u its second half, r what the row has already.  lost: the row is in no
+// leaf, nothing is added to it.  CLASS: the activation's, where it is known.
+template <typename T, bool GATED, int CLASS = -1>
+__device__ __forceinline__ void layer_end(const LeafProduct& p, int tree, bool lost, int n, int col,
+                                          const float (&a)[8], const float (&u)[8], const float (&r)[8]) {
   const int cols = p.outputs, valid = min(8, cols - col);
   if (n < 0 || valid <= 0) return;
-  const int64_t rows = GATED ? 2 * (int64_t)cols : cols;
-  if (p.b && leaf >= 0) {
-    const T* const b = (const T*)p.b + leaf * rows + col;
-    float v[8];
-    load8(b, valid, v);
-#pragma unroll
-    for (int j = 0; j < 8; ++j) a[j] += v[j];
-    if (GATED) {
-      load8(b + cols, valid, v);
-#pragma unroll
-      for (int j = 0; j < 8; ++j) u[j] += v[j];
-    }
-  }
   if (p.z) {
-    const int64_t at = n * rows + col;
+    const int64_t at = n * (GATED ? 2 * (int64_t)cols : cols) + col;
     if (sizeof(T) == 2 && p.z_narrow) {
       T* const z = (T*)p.z_of<T>(tree) + at;
       store8(z, valid, a);
@@ -172,23 +163,51 @@ __device__ __forceinline__ void layer_end(const LeafProduct& p, int tree, int64_
     }
   }
   float f[8];
-  activate<T>(p.act, a, f);
+  if constexpr (CLASS >= 0)
+    activate_as<T, (ActClass)CLASS>(p.act, a, f);
+  else
+    activate<T>(p.act, a, f);
 #pragma unroll
   for (int j = 0; j < 8; ++j) {
     if (GATED) f[j] *= u[j];
-    if (leaf < 0) f[j] = 0.0f;
+    if (lost) f[j] = 0.0f;
+    f[j] += r[j];
   }
-  if (p.planes) {
+  if (p.planes)
     store8((float*)p.ws + ((int64_t)tree * p.g.rows + n) * cols + col, valid, f);
-    return;
-  }
-  if (p.res) {
-    float r[8];
-    load8((const T*)p.res + (int64_t)n * p.ldr + col, valid, r);
+  else
+    store8((T*)p.out + (int64_t)n * p.ldo + col, valid, f);
+}
+
+// Bias of eight neighbouring results of a leaf (-1: none) of the map's half `half`; what row n has
+// already in eight columns.  Zeros where there is none.
+template <typename T>
+__device__ __forceinline__ void bias8(const LeafProduct& p, int64_t leaf, int half, int col, float (&v)[8]) {
+  const bool has = p.b && leaf >= 0;
+  const T* const b = (const T*)p.b + (has ? leaf * p.map_rows() + half * p.outputs + col : 0);
+  load8(b, has ? p.outputs - col : 0, v);
+}
+template <typename T>
+__device__ __forceinline__ void residual8(const LeafProduct& p, int n, int col, float (&v)[8]) {
+  const bool has = p.res && !p.planes && n >= 0;
+  load8((const T*)p.res + (has ? (int64_t)n * p.ldr + col : 0), has ? p.outputs - col : 0, v);
+}
+
+// The same from the map's sums.
+template <typename T, bool GATED>
+__device__ __forceinline__ void layer_end_of_sums(const LeafProduct& p, int tree, int64_t leaf, int n, int col,
+                                                  float (&a)[8], float (&u)[8]) {
+  float r[8], b[8];
+  residual8<T>(p, n, col, r);
+  bias8<T>(p, leaf, 0, col, b);
 #pragma unroll
-    for (int j = 0; j < 8; ++j) f[j] += r[j];
+  for (int j = 0; j < 8; ++j) a[j] += b[j];
+  if (GATED) {
+    bias8<T>(p, leaf, 1, col, b);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) u[j] += b[j];
   }
-  store8((T*)p.out + (int64_t)n * p.ldo + col, valid, f);
+  layer_end<T, GATED>(p, tree, leaf < 0, n, col, a, u, r);
 }
 
 // The row of a leaf's map that column r of a tile holds, whose waves hold WN columns each: where

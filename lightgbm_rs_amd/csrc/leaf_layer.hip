@@ -119,7 +119,7 @@ __global__ __launch_bounds__(THREADS) void k_layer_tile(LeafProduct p, int col_t
       float a[8], u[8];
       __builtin_memcpy(a, mine + row * PITCH + col, sizeof(a));
       if (GATED) __builtin_memcpy(u, mine + row * PITCH + WN / 2 + col, sizeof(u));
-      layer_end<T, GATED>(p, tree, leaf, row_of[m0 + i * 16 + row], c0 + (wave % GN) * CW + col, a, u);
+      layer_end_of_sums<T, GATED>(p, tree, leaf, row_of[m0 + i * 16 + row], c0 + (wave % GN) * CW + col, a, u);
     }
     __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
     __builtin_amdgcn_wave_barrier();
@@ -231,7 +231,7 @@ __attribute__((amdgpu_waves_per_eu(1, 4))) __global__ __launch_bounds__(WAVES * 
         a[j] += sums[v * (SUMS / 4) + row * PITCH + col + j];
         if (GATED) u[j] += sums[v * (SUMS / 4) + row * PITCH + 16 + col + j];
       }
-    layer_end<T, GATED>(p, tree, leaf, row_of[row], c0 + col, a, u);
+    layer_end_of_sums<T, GATED>(p, tree, leaf, row_of[row], c0 + col, a, u);
   }
 }
 
@@ -389,6 +389,12 @@ __global__ __launch_bounds__(THREADS) void k_layer_dz(LeafProduct p, int64_t pie
 
 // ---- which kernel ---------------------------------------------------------------------------------
 
+// The large tiles of leaf_big.hip, by all the trees, however few of them are made at a time.
+bool big_tiles(LeafProduct p, int trees) {
+  p.g.trees = trees;
+  return leaf_big_fits(p, LEAF_LAYER);
+}
+
 // Leaves of 16 rows at most, on average.
 bool few_rows_a_leaf(const LeafProduct& p) { return p.g.rows <= 16 * (int64_t)p.g.leaves; }
 
@@ -425,6 +431,7 @@ void launch_few(const LeafProduct& p, hipStream_t s) {
 
 template <typename T, bool GATED>
 void launch(const LeafProduct& p, int trees, hipStream_t s) {
+  if (big_tiles(p, trees)) return launch_leaf_big(p, LEAF_LAYER, s);
   const int few = few_rows(p);
   if (few == 1) return launch_few<T, GATED, 1>(p, s);
   if (few == 2) return launch_few<T, GATED, 2>(p, s);
@@ -461,6 +468,7 @@ void launch_dz(const LeafProduct& p, void* dz, hipStream_t s) {
 }  // namespace
 
 int64_t leaf_layer_blocks(const LeafProduct& p) {
+  if (leaf_big_fits(p, LEAF_LAYER)) return leaf_big_blocks(p, LEAF_LAYER);
   if (const int few = few_rows(p)) return row_tiles(p.g, 16 * few) * ((p.outputs + 15) / 16);
   const int64_t cb = p.gated ? 32 : 64;
   return row_tiles(p.g, 64) * ((p.outputs + cb - 1) / cb);
