@@ -25,7 +25,7 @@ namespace {
 
 using namespace mma;
 
-constexpr int THREADS = 256, BM = 256, BN = 256, BK = 64, WM = 128, WN = 128;
+constexpr int THREADS = 256, BM = BIG_ROWS, BN = 256, BK = 64, WM = 128, WN = 128;
 constexpr int A_BYTES = BM * BK * 2, STAGE = (BM + BN) * BK * 2;
 constexpr int LOADS = 8;  // of 1 KB a wave, operand and stage
 
@@ -143,6 +143,7 @@ __global__ __launch_bounds__(THREADS, 1) void k_leaf_big(LeafProduct p, int col_
   int tiles = 0, share = 0;
   if (!DW) {
     tiles = count_tiles<THREADS>(p.g, tree_y, BM) * col_tiles;
+    if (p.rest) tiles = in_rounds(tiles);
     share = (tiles + 7) / 8;
   }
   // The tile of a slot, its rows in row_of[buf]; rows 0: there is none.
@@ -563,13 +564,6 @@ __global__ __launch_bounds__(THREADS, 1) void k_leaf_big(LeafProduct p, int col_
   }
 }
 
-// Tiles along the columns of a result; a gated layer's has half as many results.
-int64_t col_tiles_of(const LeafProduct& p, int what) {
-  const int64_t cols = what == LEAF_PRODUCT_Y || what == LEAF_LAYER ? p.outputs : p.inputs;
-  const int64_t of = what == LEAF_LAYER && p.gated ? BN / 2 : BN;
-  return (cols + of - 1) / of;
-}
-
 template <typename T, int LAYER>
 void launch_layer(const LeafProduct& p, const dim3& grid, int ct, hipStream_t s) {
   const Split none{0, 0, 0};
@@ -582,7 +576,7 @@ void launch_layer(const LeafProduct& p, const dim3& grid, int ct, hipStream_t s)
 
 template <typename T>
 void launch(const LeafProduct& p, int what, hipStream_t s) {
-  const int ct = (int)col_tiles_of(p, what);
+  const int ct = (int)leaf_big_cols(p, what);
   const Split split = what == LEAF_PRODUCT_DW ? leaf_big_split(p) : Split{0, 0, 0};
   const dim3 grid((unsigned)leaf_big_blocks(p, what),
                   what == LEAF_PRODUCT_DW && split.rows == 0 ? 1u : (unsigned)p.g.trees);
@@ -614,13 +608,20 @@ Split leaf_big_split(const LeafProduct& p) {
   return split_by(p.g, rows);
 }
 
+// A gated layer's tile has half as many results.
+int64_t leaf_big_cols(const LeafProduct& p, int what) {
+  const int64_t cols = what == LEAF_PRODUCT_Y || what == LEAF_LAYER ? p.outputs : p.inputs;
+  const int64_t of = what == LEAF_LAYER && p.gated ? BN / 2 : BN;
+  return (cols + of - 1) / of;
+}
+
 int64_t leaf_big_blocks(const LeafProduct& p, int what) {
-  const int64_t ct = col_tiles_of(p, what);
+  const int64_t ct = leaf_big_cols(p, what);
   if (what == LEAF_PRODUCT_DW) {
     const Split split = leaf_big_split(p);
     return (p.outputs + BM - 1) / BM * ct * (split.rows ? split.parts : (int64_t)p.g.trees * p.g.leaves);
   }
-  return std::min<int64_t>((row_tiles(p.g, BM) * ct + 7) / 8 * 8, 256);  // one a CU
+  return std::min<int64_t>((row_tiles(p.g, BM) * ct + 7) / 8 * 8, BIG_BLOCKS);  // one a CU
 }
 
 // Rows and maps that make whole tiles of 256 x 256 worthwhile, and 16-byte chunks that do not
@@ -644,7 +645,7 @@ bool leaf_big_fits(const LeafProduct& p, int what) {
   // a layer's outputs may end anywhere
   if (p.inputs % 8 || (what != LEAF_LAYER && rows % 8) || p.inputs < 192 || rows < 192) return false;
   if ((int64_t)p.g.rows < 192 * (int64_t)p.g.leaves) return false;
-  const int64_t ct = col_tiles_of(p, what);
+  const int64_t ct = leaf_big_cols(p, what);
   if (what != LEAF_PRODUCT_DW && (2 * (int64_t)p.g.rows / BM + p.g.leaves) * ct * p.g.trees < 2 * 72) return false;
   if (p.g.rows * std::max(p.ldx, p.lddy) >> 35 || (int64_t)p.inputs * rows >> 35) return false;  // 64 GB
   auto ok = [](const void* q, int64_t ld) { return (((uintptr_t)q) | (uintptr_t)(ld * 2)) % 16 == 0; };

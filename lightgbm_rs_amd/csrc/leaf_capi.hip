@@ -343,6 +343,7 @@ static LeafProduct layer_grad_of(const lgbm_leaf_layer_grad* a, const void* dz) 
   p.dy_tree = linear(a) ? 0 : a->maps.num_rows * p.outputs;
   p.x = a->d_x, p.ldx = a->ldx, p.w = a->d_w, p.out = a->d_dx, p.ldo = a->lddx, p.dw = a->d_dw, p.db = a->d_dbias;
   p.narrow = a->dw_dtype != LGBM_HIP_DTYPE_F32;
+  p.rest = true;
   return p;
 }
 

@@ -24,7 +24,8 @@ constexpr int THREADS = 256;
 // last ones; only the end of the contraction needs zeros.  The sums of 16 rows of a wave go
 // through LDS to eight neighbouring results a lane, so that z, r and y are read and written by
 // 16 bytes.
-template <typename T, bool GATED, int BM, int BN, int GM>
+// REST: the quarters of large tiles behind their last whole round, of which a row has col_tiles.
+template <typename T, bool GATED, int BM, int BN, int GM, bool REST = false>
 __global__ __launch_bounds__(THREADS) void k_layer_tile(LeafProduct p, int col_tiles) {
   constexpr int V = El<T>::V, BK = 8 * V;  // elements of the contraction a step
   constexpr int GN = 4 / GM, WM = BM / GM, WN = BN / GN, CW = GATED ? WN / 2 : WN;
@@ -35,9 +36,11 @@ __global__ __launch_bounds__(THREADS) void k_layer_tile(LeafProduct p, int col_t
   __shared__ __align__(16) int32_t row_of[BM];
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const int tree = blockIdx.y, length = p.inputs, cols = p.outputs;
-  const int mt = blockIdx.x / col_tiles, c0 = (blockIdx.x % col_tiles) * (GATED ? BN / 2 : BN);
-  const RowTile rt = find_tile<THREADS>(p.g, tree, mt, BM);
-  if (rt.rows == 0) return;
+  constexpr int CB = GATED ? BN / 2 : BN;
+  int c0 = (blockIdx.x % col_tiles) * CB;
+  const RowTile rt = REST ? rest_tile<THREADS>(p.g, tree, col_tiles, CB, &c0)
+                          : find_tile<THREADS>(p.g, tree, blockIdx.x / col_tiles, BM);
+  if (rt.rows == 0 || (REST && c0 >= cols)) return;
   for (int r = tid; r < BM; r += THREADS) row_of[r] = r < rt.rows ? row_at(p.g, tree, rt.first + r) : -1;
   __syncthreads();
   const int64_t leaf = rt.leaf < 0 ? -1 : (int64_t)tree * p.g.leaves + rt.leaf;
@@ -420,6 +423,16 @@ void launch_tile(const LeafProduct& p, hipStream_t s) {
   k_layer_tile<T, GATED, BM, BN, 2><<<grid, THREADS, 0, s>>>(p, ct);
 }
 
+// Large tiles, and what is behind their last whole round.
+template <typename T, bool GATED>
+void launch_big(LeafProduct p, hipStream_t s) {
+  const int ct = (int)leaf_big_cols(p, LEAF_LAYER);
+  p.rest = row_tiles(p.g, BIG_ROWS) * ct > BIG_BLOCKS;
+  launch_leaf_big(p, LEAF_LAYER, s);
+  if (p.rest)
+    k_layer_tile<T, GATED, 128, 128, 2, true><<<dim3(REST_BLOCKS, (unsigned)p.g.trees), THREADS, 0, s>>>(p, ct);
+}
+
 template <typename T, bool GATED, int RB>
 void launch_few(const LeafProduct& p, hipStream_t s) {
   const int ct = (p.outputs + 15) / 16;
@@ -431,7 +444,6 @@ void launch_few(const LeafProduct& p, hipStream_t s) {
 
 template <typename T, bool GATED>
 void launch(const LeafProduct& p, int trees, hipStream_t s) {
-  if (big_tiles(p, trees)) return launch_leaf_big(p, LEAF_LAYER, s);
   const int few = few_rows(p);
   if (few == 1) return launch_few<T, GATED, 1>(p, s);
   if (few == 2) return launch_few<T, GATED, 2>(p, s);
@@ -450,6 +462,7 @@ void launch(const LeafProduct& p, int trees, hipStream_t s) {
     return;
   }
   if constexpr (sizeof(T) == 2) {
+    if (big_tiles(p, trees)) return launch_big<T, GATED>(p, s);
     if (wide_tiles(p, trees)) return launch_tile<T, GATED, 128, 128>(p, s);
   }
   launch_tile<T, GATED, 64, 64>(p, s);

@@ -213,6 +213,27 @@ __device__ int count_tiles(const LeafGroups& g, int tree, int bm) {
   return (int)min(tiles, row_tiles(g, bm));
 }
 
+// Large tiles of 256 x 256 are made in rounds of a launch's BIG_BLOCKS blocks.  The tiles behind
+// the last whole round, where they are half a round at most, are better made by four blocks each
+// of 128 x 128, which that round has CUs for: how many tiles are made in rounds.
+constexpr int BIG_ROWS = 256, BIG_BLOCKS = 256;
+__host__ __device__ inline int in_rounds(int tiles) {
+  const int rest = tiles % BIG_BLOCKS;
+  return tiles > BIG_BLOCKS && rest <= BIG_BLOCKS / 2 ? tiles - rest : tiles;
+}
+constexpr int REST_BLOCKS = BIG_BLOCKS / 2 * 4;  // of a tree
+// The rows and the first column of a block's quarter of such a tile of 2 `cols` columns, of which
+// a row of tiles has col_tiles; rows 0: there is none.
+template <int THREADS>
+__device__ RowTile rest_tile(const LeafGroups& g, int tree, int col_tiles, int cols, int* c0) {
+  const int tiles = count_tiles<THREADS>(g, tree, BIG_ROWS) * col_tiles;
+  const int id = in_rounds(tiles) + (int)(blockIdx.x >> 2), down = blockIdx.x >> 1 & 1;
+  *c0 = (id % col_tiles * 2 + (int)(blockIdx.x & 1)) * cols;
+  if (id >= tiles) return {-1, 0, 0};
+  const RowTile t = find_tile<THREADS>(g, tree, id / col_tiles, BIG_ROWS);
+  return {t.leaf, t.first + down * (BIG_ROWS / 2), min(max(t.rows - down * (BIG_ROWS / 2), 0), BIG_ROWS / 2)};
+}
+
 // The row at a position of a tree's order, -1 for an entry outside the matrix.
 __device__ __forceinline__ int row_at(const LeafGroups& g, int tree, int position) {
   const int n = g.order[(int64_t)tree * g.rows + position];

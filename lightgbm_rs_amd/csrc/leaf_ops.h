@@ -51,6 +51,9 @@ struct LeafProduct {
   // product, layer and dx: whether a tree's results go to its float32 plane [rows][columns] in
   // ws, to be added, instead of to out
   bool planes;
+  // layer, and dx of its gradient: whether the large tiles behind their last whole round go to
+  // smaller ones
+  bool rest;
   // layer: out[n] = res[n] + sum over trees of act(z), or of act(z's first half) times its
   // second half where gated; z = W x + b has map_rows() elements, `outputs` those of the layer
   int32_t act;
@@ -83,6 +86,7 @@ void launch_layer_dz(const LeafProduct& p, void* dz, hipStream_t s);
 // leaf_big.hip: 16-bit products of large tiles
 bool leaf_big_fits(const LeafProduct& p, int what);
 int64_t leaf_big_blocks(const LeafProduct& p, int what);
+int64_t leaf_big_cols(const LeafProduct& p, int what);  // tiles along the columns of a result
 void launch_leaf_big(const LeafProduct& p, int what, hipStream_t s);
 
 // ---- the norm of many tensors ------------------------------------------------------------

@@ -28,7 +28,8 @@ constexpr int THREADS = 256;
 // the last ones; only the end of the contraction needs zeros.  Bound by the matrix
 // instructions and, in 16 bits, by LDS (20000 x 1000 to 1000 float32 by 7 leaves: 99 TFLOP/s of
 // the 142 to 155 of a library product; 40000 x 2001 to 2047 bfloat16 by 9: 483).
-template <typename T, bool DX, int BM, int BN, int GM>
+// REST: the quarters of large tiles behind their last whole round, of which a row has col_tiles.
+template <typename T, bool DX, int BM, int BN, int GM, bool REST = false>
 __global__ __launch_bounds__(THREADS) void k_leaf_tile(LeafProduct p, int length, int cols,
                                                        int col_tiles) {
   constexpr int V = El<T>::V, BK = 8 * V;  // elements of the contraction a step
@@ -38,9 +39,10 @@ __global__ __launch_bounds__(THREADS) void k_leaf_tile(LeafProduct p, int length
   __shared__ __align__(16) int32_t row_of[BM];
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const int tree = blockIdx.y;
-  const int mt = blockIdx.x / col_tiles, c0 = (blockIdx.x % col_tiles) * BN;
-  const RowTile rt = find_tile<THREADS>(p.g, tree, mt, BM);
-  if (rt.rows == 0) return;
+  int c0 = (blockIdx.x % col_tiles) * BN;
+  const RowTile rt = REST ? rest_tile<THREADS>(p.g, tree, col_tiles, BN, &c0)
+                          : find_tile<THREADS>(p.g, tree, blockIdx.x / col_tiles, BM);
+  if (rt.rows == 0 || (REST && c0 >= cols)) return;
   for (int r = tid; r < BM; r += THREADS) row_of[r] = r < rt.rows ? row_at(p.g, tree, rt.first + r) : -1;
   __syncthreads();
   const int64_t leaf = (int64_t)tree * p.g.leaves + rt.leaf;
@@ -794,7 +796,15 @@ void launch_product(const LeafProduct& p, int what, const Form& form, hipStream_
   const bool dx = what == LEAF_PRODUCT_DX;
   const int cols = dx ? p.inputs : p.outputs;
   if (form.big) {
-    launch_leaf_big(p, what, s);
+    const int ct = (int)leaf_big_cols(p, what);
+    LeafProduct q = p;
+    q.rest = p.rest && row_tiles(p.g, BIG_ROWS) * ct > BIG_BLOCKS;
+    launch_leaf_big(q, what, s);
+    if constexpr (sizeof(T) == 2) {
+      if (dx && q.rest)
+        k_leaf_tile<T, true, 128, 128, 2, true>
+            <<<dim3(REST_BLOCKS, (unsigned)p.g.trees), THREADS, 0, s>>>(q, p.outputs, cols, ct);
+    }
   } else if (dx && p.outputs <= 32) {
     const int ct = (cols + 127) / 128;
     const dim3 grid((unsigned)(row_tiles(p.g, 512) * ct), (unsigned)p.g.trees);
