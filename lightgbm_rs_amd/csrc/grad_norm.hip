@@ -20,7 +20,7 @@
 namespace lgbm {
 namespace {
 
-constexpr int THREADS = 256, LIST = 128, FINAL = 1024;
+constexpr int THREADS = 256, LIST = 128, FINAL = 1024, FEW = 16;
 
 // first[i]: the launch's block that begins tensor i.  count: elements times four, and the type
 // (0: float32, 1: bfloat16, 2: float16).
@@ -60,7 +60,7 @@ __device__ __forceinline__ double squares(const T* in, int64_t from, int64_t to)
       sum[j & 1] = fma(d, d, sum[j & 1]);
     }
   };
-  int64_t i = from + threadIdx.x * V;
+  int64_t i = from + threadIdx.x % THREADS * V;
   for (; i + (UNROLL - 1) * (int64_t)THREADS * V + V <= to; i += UNROLL * (int64_t)THREADS * V) {
     T v[UNROLL][V];
 #pragma unroll
@@ -95,16 +95,26 @@ __device__ __forceinline__ double block_sum(double v) {
   return v;
 }
 
-__global__ __launch_bounds__(THREADS) void k_squares(List l, int64_t chunk, double* sums) {
-  const Chunk c = chunk_of(l, blockIdx.x, chunk);
-  double v;
+// A thread's part of a chunk's sum.
+__device__ __forceinline__ double squares_of(const List& l, int block, int64_t chunk) {
+  const Chunk c = chunk_of(l, block, chunk);
   switch (l.count[c.tensor] & 3) {
-    case 0: v = squares((const float*)l.in[c.tensor], c.from, c.to); break;
-    case 1: v = squares((const __bf16*)l.in[c.tensor], c.from, c.to); break;
-    default: v = squares((const _Float16*)l.in[c.tensor], c.from, c.to);
+    case 0: return squares((const float*)l.in[c.tensor], c.from, c.to);
+    case 1: return squares((const __bf16*)l.in[c.tensor], c.from, c.to);
+    default: return squares((const _Float16*)l.in[c.tensor], c.from, c.to);
   }
-  v = block_sum<THREADS>(v);
+}
+
+__global__ __launch_bounds__(THREADS) void k_squares(List l, int64_t chunk, double* sums) {
+  const double v = block_sum<THREADS>(squares_of(l, blockIdx.x, chunk));
   if (threadIdx.x == 0) sums[blockIdx.x] = v;
+}
+
+__device__ __forceinline__ void put_norm(double sum, double most, float* norm, float* scale) {
+  const double v = sqrt(sum);
+  *norm = (float)v;
+  // a norm that is NaN gives a scale that is
+  if (scale) *scale = v <= most ? 1.0f : (float)(most / v);
 }
 
 // The norm, and the scale in front of the sums.
@@ -112,12 +122,17 @@ __global__ __launch_bounds__(FINAL) void k_norm(const double* sums, int64_t n, d
                                                 float* scale) {
   double v = 0;
   for (int64_t i = threadIdx.x; i < n; i += FINAL) v += sums[i];
-  v = sqrt(block_sum<FINAL>(v));
-  if (threadIdx.x == 0) {
-    *norm = (float)v;
-    // a norm that is NaN gives a scale that is
-    if (scale) *scale = v <= most ? 1.0f : (float)(most / v);
-  }
+  v = block_sum<FINAL>(v);
+  if (threadIdx.x == 0) put_norm(v, most, norm, scale);
+}
+
+// Both for a list of few chunks: one block, whose parts of THREADS take a chunk each.
+__global__ __launch_bounds__(FINAL) void k_norm_of_few(List l, int64_t chunk, int chunks, double most, float* norm,
+                                                       float* scale) {
+  double v = 0;
+  for (int i = threadIdx.x / THREADS; i < chunks; i += FINAL / THREADS) v += squares_of(l, i, chunk);
+  v = block_sum<FINAL>(v);
+  if (threadIdx.x == 0) put_norm(v, most, norm, scale);
 }
 
 template <typename T>
@@ -197,11 +212,18 @@ void launch_grad_norm(const GradTensor* t, int64_t num, bool clip, double most, 
   float* const scale = clip ? (float*)ws : nullptr;
   double* const sums = (double*)ws + 2;
   int64_t chunks = 0;
+  int64_t most_chunks = 0;
+  for (int64_t i = 0; i < num; ++i) most_chunks += chunks_of(t[i], chunk);
   lists(t, num, chunk, [&](const List& l, int64_t done, int64_t blocks) {
+    if (most_chunks <= FEW && blocks == most_chunks) {
+      k_norm_of_few<<<1, FINAL, 0, s>>>(l, chunk, (int)blocks, most, norm, scale);
+      chunks = -1;
+      return;
+    }
     k_squares<<<(unsigned)blocks, THREADS, 0, s>>>(l, chunk, sums + done);
     chunks = done + blocks;
   });
-  k_norm<<<1, FINAL, 0, s>>>(sums, chunks, most, norm, scale);
+  if (chunks >= 0) k_norm<<<1, FINAL, 0, s>>>(sums, chunks, most, norm, scale);
   if (!clip) return;
   lists(t, num, chunk, [&](const List& l, int64_t, int64_t blocks) {
     k_scale<<<(unsigned)blocks, THREADS, 0, s>>>(l, chunk, scale);

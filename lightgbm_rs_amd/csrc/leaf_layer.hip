@@ -24,7 +24,7 @@ constexpr int THREADS = 256;
 // last ones; only the end of the contraction needs zeros.  The sums of 16 rows of a wave go
 // through LDS to eight neighbouring results a lane, so that z, r and y are read and written by
 // 16 bytes.
-// REST: the quarters of large tiles behind their last whole round, of which a row has col_tiles.
+// REST: the parts of large tiles behind their last whole round, of which a row has col_tiles.
 template <typename T, bool GATED, int BM, int BN, int GM, bool REST = false>
 __global__ __launch_bounds__(THREADS) void k_layer_tile(LeafProduct p, int col_tiles) {
   constexpr int V = El<T>::V, BK = 8 * V;  // elements of the contraction a step
@@ -57,18 +57,26 @@ __global__ __launch_bounds__(THREADS) void k_layer_tile(LeafProduct p, int col_t
     u32x4 ra[ACH], rb[BCH];
     const T *arow[ACH], *brow[BCH];
 #pragma unroll
-    for (int i = 0; i < ACH; ++i) arow[i] = (const T*)p.x + (int64_t)max(row_of[(tid + i * THREADS) >> 3], 0) * p.ldx;
+    for (int i = 0; i < ACH; ++i)
+      arow[i] = (const T*)p.x + (int64_t)max(row_of[(tid + i * THREADS) >> 3], 0) * p.ldx + (tid & 7) * V;
 #pragma unroll
-    for (int i = 0; i < BCH; ++i) brow[i] = w + (int64_t)map_row<GATED, WN>((tid + i * THREADS) >> 3, c0, cols) * length;
-    auto load = [&](int k0) {
-      const int k = k0 + (tid & 7) * V;
-      const bool whole = k0 + BK <= length;
+    for (int i = 0; i < BCH; ++i)
+      brow[i] = w + (int64_t)map_row<GATED, WN>((tid + i * THREADS) >> 3, c0, cols) * length + (tid & 7) * V;
+    const auto load = [&](int k0) {
+      if (k0 + BK <= length) {
 #pragma unroll
-      for (int i = 0; i < ACH; ++i) ra[i] = whole ? load16(arow[i] + k) : load16(arow[i] + k, length - k);
+        for (int i = 0; i < ACH; ++i) ra[i] = load16(arow[i] + k0);
 #pragma unroll
-      for (int i = 0; i < BCH; ++i) rb[i] = whole ? load16(brow[i] + k) : load16(brow[i] + k, length - k);
+        for (int i = 0; i < BCH; ++i) rb[i] = load16(brow[i] + k0);
+      } else if (k0 < length) {
+        const int valid = length - k0 - (tid & 7) * V;
+#pragma unroll
+        for (int i = 0; i < ACH; ++i) ra[i] = load16(arow[i] + k0, valid);
+#pragma unroll
+        for (int i = 0; i < BCH; ++i) rb[i] = load16(brow[i] + k0, valid);
+      }
     };
-    auto store = [&](char* buf) {
+    const auto store = [&](char* buf) {
 #pragma unroll
       for (int i = 0; i < ACH; ++i) {
         const int at = tid + i * THREADS;
@@ -85,7 +93,7 @@ __global__ __launch_bounds__(THREADS) void k_layer_tile(LeafProduct p, int col_t
     __syncthreads();
     for (int k0 = 0, b = 0; k0 < length; k0 += BK, b ^= 1) {
       const bool more = k0 + BK < length;
-      if (more) load(k0 + BK);
+      load(k0 + BK);
       const char *ta = lds + b * STAGE, *tb = ta + BM * 128;
       Parts<T, WM / 16, WN / 16> part(acc);
 #pragma unroll
@@ -430,7 +438,7 @@ void launch_big(LeafProduct p, hipStream_t s) {
   p.rest = row_tiles(p.g, BIG_ROWS) * ct > BIG_BLOCKS;
   launch_leaf_big(p, LEAF_LAYER, s);
   if (p.rest)
-    k_layer_tile<T, GATED, 128, 128, 2, true><<<dim3(REST_BLOCKS, (unsigned)p.g.trees), THREADS, 0, s>>>(p, ct);
+    k_layer_tile<T, GATED, PART_ROWS, PART_ROWS, 2, true><<<dim3(REST_BLOCKS, (unsigned)p.g.trees), THREADS, 0, s>>>(p, ct);
 }
 
 template <typename T, bool GATED, int RB>

@@ -214,24 +214,25 @@ __device__ int count_tiles(const LeafGroups& g, int tree, int bm) {
 }
 
 // Large tiles of 256 x 256 are made in rounds of a launch's BIG_BLOCKS blocks.  The tiles behind
-// the last whole round, where they are half a round at most, are better made by four blocks each
-// of 128 x 128, which that round has CUs for: how many tiles are made in rounds.
-constexpr int BIG_ROWS = 256, BIG_BLOCKS = 256;
+// the last whole round, where they are half a round at most, are better made by PARTS x PARTS
+// blocks each, which that round has CUs for: how many tiles are made in rounds.
+constexpr int BIG_ROWS = 256, BIG_BLOCKS = 256, PARTS = 4, PART_ROWS = BIG_ROWS / PARTS;
 __host__ __device__ inline int in_rounds(int tiles) {
   const int rest = tiles % BIG_BLOCKS;
   return tiles > BIG_BLOCKS && rest <= BIG_BLOCKS / 2 ? tiles - rest : tiles;
 }
-constexpr int REST_BLOCKS = BIG_BLOCKS / 2 * 4;  // of a tree
-// The rows and the first column of a block's quarter of such a tile of 2 `cols` columns, of which
-// a row of tiles has col_tiles; rows 0: there is none.
+constexpr int REST_BLOCKS = BIG_BLOCKS / 2 * PARTS * PARTS;  // of a tree
+// The rows and the first column of a block's part of such a tile of PARTS times `cols` columns, of
+// which a row of tiles has col_tiles; rows 0: there is none.
 template <int THREADS>
 __device__ RowTile rest_tile(const LeafGroups& g, int tree, int col_tiles, int cols, int* c0) {
   const int tiles = count_tiles<THREADS>(g, tree, BIG_ROWS) * col_tiles;
-  const int id = in_rounds(tiles) + (int)(blockIdx.x >> 2), down = blockIdx.x >> 1 & 1;
-  *c0 = (id % col_tiles * 2 + (int)(blockIdx.x & 1)) * cols;
+  const int id = in_rounds(tiles) + (int)blockIdx.x / (PARTS * PARTS), part = (int)blockIdx.x % (PARTS * PARTS);
+  *c0 = (id % col_tiles * PARTS + part % PARTS) * cols;
   if (id >= tiles) return {-1, 0, 0};
   const RowTile t = find_tile<THREADS>(g, tree, id / col_tiles, BIG_ROWS);
-  return {t.leaf, t.first + down * (BIG_ROWS / 2), min(max(t.rows - down * (BIG_ROWS / 2), 0), BIG_ROWS / 2)};
+  const int down = part / PARTS * PART_ROWS;
+  return {t.leaf, t.first + down, min(max(t.rows - down, 0), PART_ROWS)};
 }
 
 // The row at a position of a tree's order, -1 for an entry outside the matrix.

@@ -28,7 +28,7 @@ constexpr int THREADS = 256;
 // the last ones; only the end of the contraction needs zeros.  Bound by the matrix
 // instructions and, in 16 bits, by LDS (20000 x 1000 to 1000 float32 by 7 leaves: 99 TFLOP/s of
 // the 142 to 155 of a library product; 40000 x 2001 to 2047 bfloat16 by 9: 483).
-// REST: the quarters of large tiles behind their last whole round, of which a row has col_tiles.
+// REST: the parts of large tiles behind their last whole round, of which a row has col_tiles.
 template <typename T, bool DX, int BM, int BN, int GM, bool REST = false>
 __global__ __launch_bounds__(THREADS) void k_leaf_tile(LeafProduct p, int length, int cols,
                                                        int col_tiles) {
@@ -802,7 +802,7 @@ void launch_product(const LeafProduct& p, int what, const Form& form, hipStream_
     launch_leaf_big(q, what, s);
     if constexpr (sizeof(T) == 2) {
       if (dx && q.rest)
-        k_leaf_tile<T, true, 128, 128, 2, true>
+        k_leaf_tile<T, true, PART_ROWS, PART_ROWS, 2, true>
             <<<dim3(REST_BLOCKS, (unsigned)p.g.trees), THREADS, 0, s>>>(q, p.outputs, cols, ct);
     }
   } else if (dx && p.outputs <= 32) {

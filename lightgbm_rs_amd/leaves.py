@@ -14,6 +14,7 @@ Import torch before the first `HipBackend`: torch brings a HIP runtime of its ow
 the library then shares.  (The other way round torch finds no device.)
 """
 import ctypes as C
+import operator
 from typing import Any, NamedTuple
 
 import numpy as np
@@ -67,6 +68,8 @@ class _LayerGrad(C.Structure):
 # `lgbm_grad`
 _GRAD = np.dtype([("in", np.uint64), ("out", np.uint64), ("count", np.int64), ("dtype", np.int32),
                   ("_pad", np.int32)])
+
+_GET_DTYPE, _GET_REQUIRES_GRAD = operator.attrgetter("dtype"), operator.attrgetter("requires_grad")
 
 ACTIVATIONS = {"none": 0, "relu": 1, "silu": 2, "gelu": 3, "gelu_tanh": 4, "sigmoid": 5}
 
@@ -462,26 +465,31 @@ def _dense(t):
 
 
 def _grad_list(self, tensors, out):
-    """The list as an array of `lgbm_grad`."""
+    """The list as an array of `lgbm_grad`.  A model has hundreds of tensors: each of these is one
+    pass over them without Python code."""
     torch = _module()
-    a = np.zeros(len(tensors), _GRAD)
+    T, n = torch.Tensor, len(tensors)
+    types = list(map(_GET_DTYPE, tensors))
+    a = np.zeros(n, _GRAD)
     for name, ts, field in (("tensors", tensors, "in"), ("out", out, "out")):
-        if ts is None:
+        if ts is None or (field == "out" and ts is tensors):
             continue
-        if not all(map(torch.Tensor.is_contiguous, ts)) and not all(map(_dense, ts)):
+        if not all(map(T.is_contiguous, ts)) and not all(map(_dense, ts)):
             raise ValueError(f"a tensor of {name} has gaps")
-        if torch.is_grad_enabled() and any(t.requires_grad for t in ts):
-            raise ValueError(f"{name} require gradients, which this call does not record")
-        for d in {t.device for t in ts}:
-            if d.type != "cuda" or d.index != self.device:
-                raise ValueError(f"a tensor of {name} is on {d}: cuda:{self.device} is needed")
-        a[field] = list(map(torch.Tensor.data_ptr, ts))
-    types = [t.dtype for t in tensors]
+        if torch.is_grad_enabled() and any(map(_GET_REQUIRES_GRAD, ts)):
+            raise ValueError(f"a tensor of {name} requires gradients, which this call does not record")
+        for d in set(map(T.get_device, ts)):
+            if d != self.device:
+                raise ValueError(f"a tensor of {name} is on {'cpu' if d < 0 else f'cuda:{d}'}: "
+                                 f"cuda:{self.device} is needed")
+        a[field] = np.fromiter(map(T.data_ptr, ts), np.uint64, n)
+    if out is tensors:
+        a["out"] = a["in"]
     for dtype in set(types):
         if dtype not in _DTYPES or dtype == torch.float64:
             raise ValueError(f"a tensor is {dtype}: a floating-point type of at most 32 bits is needed")
-    a["dtype"] = [_DTYPES[d] for d in types]
-    a["count"] = list(map(torch.Tensor.numel, tensors))
+    a["dtype"] = _DTYPES[types[0]] if len(set(types)) == 1 else [_DTYPES[d] for d in types]
+    a["count"] = np.fromiter(map(T.numel, tensors), np.int64, n)
     return a
 
 
@@ -496,7 +504,10 @@ def _norm_of(self, tensors, out, max_norm):
     else:
         self._check(self.lib.lgbm_hip_clip_grads(self.ctx, a.ctypes.data, len(a), max_norm,
                                                  norm.data_ptr(), ws, nbytes, _stream(self, torch)))
-        _written(*out)
+        try:
+            torch.autograd.graph.increment_version(out)
+        except RuntimeError:  # a tensor of inference mode has no version
+            _written(*out)
     return norm
 
 
@@ -515,9 +526,9 @@ def _clip_grads(self, tensors, max_norm, out=None):
         out = list(out)
         if len(out) != len(tensors):
             raise ValueError("out and the tensors differ in number")
-        if ([t.shape for t in out] != [t.shape for t in tensors]
-                or [t.dtype for t in out] != [t.dtype for t in tensors]
-                or [t.stride() for t in out] != [t.stride() for t in tensors]):
+        T = _module().Tensor
+        # (tensors without gaps of as many elements and the same strides have the same shape)
+        if any(list(map(of, tensors)) != list(map(of, out)) for of in (T.numel, _GET_DTYPE, T.stride)):
             raise ValueError("out and the tensors differ in shape, type or strides")
     return _norm_of(self, tensors, tensors if out is None else out, float(max_norm))
 
