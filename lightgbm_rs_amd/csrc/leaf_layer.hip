@@ -409,11 +409,18 @@ bool big_tiles(LeafProduct p, int trees) {
 // Leaves of 16 rows at most, on average.
 bool few_rows_a_leaf(const LeafProduct& p) { return p.g.rows <= 16 * (int64_t)p.g.leaves; }
 
-// Rows a block of k_layer_few, in units of 16, 0: not for it.
+// Rows a block of k_layer_few, in units of 16, 0: not for it.  Few outputs of so few rows that
+// k_layer_narrow's blocks would leave CUs without work, as for the linear maps (by_maps); leaves of
+// 32 rows at most, on average; and 64 x 64 tiles that are fewer than about 320 (us by it and by those
+// tiles: 4096 bfloat16 inputs to 4096, one leaf, 64 rows 16.7 and 42.5, 256 rows 38 and 43.5, 384
+// rows 52 and 47; to 2048 gated, 256 rows 25 and 44; float32, 256 rows 115 and 120, 512 rows 206
+// and 174; 48 rows a leaf, 4096 to 4096 by seven leaves 93 and 73, 600 to 100 by 127 24 and 20).
 int few_rows(const LeafProduct& p) {
-  const int64_t rows = (p.g.rows + p.g.leaves - 1) / p.g.leaves;
+  if (p.inputs >= 128 && p.outputs <= 32 && (int64_t)p.g.rows * ((p.outputs + 15) / 16) < 49152) return 1;
   if (p.inputs < 512) return 0;
-  return rows <= 16 ? 1 : rows <= 32 ? 2 : rows <= 128 ? 4 : 0;
+  const int64_t rows = (p.g.rows + p.g.leaves - 1) / p.g.leaves;
+  if (rows <= 32) return rows <= 16 ? 1 : 2;
+  return ((int64_t)p.g.rows / 64 + p.g.leaves) * ((p.map_rows() + 63) / 64) <= 320 ? 4 : 0;
 }
 
 // Tiles of 128 x 128, as for the linear maps (wide_tiles).
