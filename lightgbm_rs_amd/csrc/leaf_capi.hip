@@ -452,36 +452,40 @@ static int check_grads(lgbm_hip_ctx* c, const lgbm_grad* g, int64_t num, bool cl
   return LGBM_HIP_OK;
 }
 
-// Whether a clipped gradient overlaps anything but its own input, or `more`.
+// Whether a clipped gradient overlaps anything but its own input, or `more`.  Views of one buffer
+// come in its order, so the lists are mostly sorted.
 static bool clipped_overlap(const std::vector<GradTensor>& list, std::initializer_list<Span> more, bool& no_memory) {
   struct Range {
     uintptr_t from, to;
-    bool out;
   };
-  std::vector<Range> all;
+  std::vector<Range> in, out;
   try {
-    all.reserve(2 * list.size() + more.size());
+    in.reserve(list.size());
+    out.reserve(list.size() + more.size());
   } catch (const std::bad_alloc&) {
     no_memory = true;
     return false;
   }
-  const auto put = [&](const void* p, int64_t bytes, bool out) {
-    if (p && bytes > 0) all.push_back({(uintptr_t)p, (uintptr_t)p + (uintptr_t)bytes, out});
-  };
+  const auto range = [](const void* p, int64_t bytes) { return Range{(uintptr_t)p, (uintptr_t)p + (uintptr_t)bytes}; };
   for (const GradTensor& t : list) {
     const int64_t bytes = t.count * type_size(t.dtype);
-    put(t.out, bytes, true);
-    if (t.in != t.out) put(t.in, bytes, false);
+    out.push_back(range(t.out, bytes));
+    if (t.in != t.out) in.push_back(range(t.in, bytes));
   }
-  for (const Span& s : more) put(s.p, s.bytes, true);
-  // inputs may overlap one another: behind each range's begin, the furthest ends so far
+  for (const Span& s : more)
+    if (s.p && s.bytes > 0) out.push_back(range(s.p, s.bytes));
   const auto before = [](const Range& a, const Range& b) { return a.from < b.from; };
-  if (!std::is_sorted(all.begin(), all.end(), before)) std::sort(all.begin(), all.end(), before);
-  uintptr_t out_end = 0, in_end = 0;
-  for (const Range& r : all) {
-    if (r.from < out_end || (r.out && r.from < in_end)) return true;
-    uintptr_t& end = r.out ? out_end : in_end;
-    end = std::max(end, r.to);
+  for (std::vector<Range>* v : {&in, &out})
+    if (!std::is_sorted(v->begin(), v->end(), before)) std::sort(v->begin(), v->end(), before);
+  for (size_t k = 1; k < out.size(); ++k)
+    if (out[k].from < out[k - 1].to) return true;
+  // inputs may overlap one another: of those that begin in front of an output's end, the
+  // furthest end
+  size_t at = 0;
+  uintptr_t end = 0;
+  for (const Range& o : out) {
+    for (; at < in.size() && in[at].from < o.to; ++at) end = std::max(end, in[at].to);
+    if (end > o.from) return true;
   }
   return false;
 }

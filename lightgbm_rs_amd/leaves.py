@@ -465,15 +465,22 @@ def _dense(t):
 
 
 def _grad_list(self, tensors, out):
-    """The list as an array of `lgbm_grad`.  A model has hundreds of tensors: each of these is one
-    pass over them without Python code."""
+    """The list as an array of `lgbm_grad`, and of the tensors of `out` (None: the norm alone) as
+    their outputs.  A model has hundreds of tensors: each of these is one pass over them without
+    Python code."""
     torch = _module()
     T, n = torch.Tensor, len(tensors)
-    types = list(map(_GET_DTYPE, tensors))
+    count, types = list(map(T.numel, tensors)), list(map(_GET_DTYPE, tensors))
     a = np.zeros(n, _GRAD)
-    for name, ts, field in (("tensors", tensors, "in"), ("out", out, "out")):
-        if ts is None or (field == "out" and ts is tensors):
-            continue
+    lists = [("tensors", "in", tensors)]
+    if out is not None and out is not tensors:
+        lists.append(("out", "out", out))
+        # tensors without gaps of as many elements and the same strides have the same shape
+        if (count != list(map(T.numel, out)) or types != list(map(_GET_DTYPE, out))
+                or list(map(T.dim, tensors)) != list(map(T.dim, out))
+                or (max(map(T.dim, out), default=0) > 1 and list(map(T.stride, tensors)) != list(map(T.stride, out)))):
+            raise ValueError("out and the tensors differ in shape, type or strides")
+    for name, field, ts in lists:
         if not all(map(T.is_contiguous, ts)) and not all(map(_dense, ts)):
             raise ValueError(f"a tensor of {name} has gaps")
         if torch.is_grad_enabled() and any(map(_GET_REQUIRES_GRAD, ts)):
@@ -482,32 +489,33 @@ def _grad_list(self, tensors, out):
             if d != self.device:
                 raise ValueError(f"a tensor of {name} is on {'cpu' if d < 0 else f'cuda:{d}'}: "
                                  f"cuda:{self.device} is needed")
-        a[field] = np.fromiter(map(T.data_ptr, ts), np.uint64, n)
+        a[field] = list(map(T.data_ptr, ts))
     if out is tensors:
         a["out"] = a["in"]
-    for dtype in set(types):
+    kinds = set(types)
+    for dtype in kinds:
         if dtype not in _DTYPES or dtype == torch.float64:
             raise ValueError(f"a tensor is {dtype}: a floating-point type of at most 32 bits is needed")
-    a["dtype"] = _DTYPES[types[0]] if len(set(types)) == 1 else [_DTYPES[d] for d in types]
-    a["count"] = np.fromiter(map(T.numel, tensors), np.int64, n)
+    a["dtype"] = _DTYPES[types[0]] if len(kinds) == 1 else [_DTYPES[d] for d in types]
+    a["count"] = count
     return a
 
 
 def _norm_of(self, tensors, out, max_norm):
     torch = _module()
     a = _grad_list(self, tensors, out)
+    at, n = a.ctypes.data, len(a)
     norm = torch.empty((), dtype=torch.float32, device=f"cuda:{self.device}")
-    ws, nbytes, hold = _workspace(self, torch, self.lib.lgbm_hip_grad_norm_workspace, a.ctypes.data, len(a))
+    ws, nbytes, hold = _workspace(self, torch, self.lib.lgbm_hip_grad_norm_workspace, at, n)
+    stream = _stream(self, torch)
     if out is None:
-        self._check(self.lib.lgbm_hip_grad_norm(self.ctx, a.ctypes.data, len(a), norm.data_ptr(), ws,
-                                                nbytes, _stream(self, torch)))
-    else:
-        self._check(self.lib.lgbm_hip_clip_grads(self.ctx, a.ctypes.data, len(a), max_norm,
-                                                 norm.data_ptr(), ws, nbytes, _stream(self, torch)))
-        try:
-            torch.autograd.graph.increment_version(out)
-        except RuntimeError:  # a tensor of inference mode has no version
-            _written(*out)
+        self._check(self.lib.lgbm_hip_grad_norm(self.ctx, at, n, norm.data_ptr(), ws, nbytes, stream))
+        return norm
+    self._check(self.lib.lgbm_hip_clip_grads(self.ctx, at, n, max_norm, norm.data_ptr(), ws, nbytes, stream))
+    try:
+        torch.autograd.graph.increment_version(out)
+    except RuntimeError:  # a tensor of inference mode has no version
+        _written(*out)
     return norm
 
 
@@ -522,15 +530,10 @@ def _clip_grads(self, tensors, max_norm, out=None):
     (`lgbm_hip_clip_grads`), in place, or in the tensors of the list `out`.  Returns the norm, a
     float32 tensor of no dimensions; nothing waits for it."""
     tensors = list(tensors)
-    if out is not None:
-        out = list(out)
-        if len(out) != len(tensors):
-            raise ValueError("out and the tensors differ in number")
-        T = _module().Tensor
-        # (tensors without gaps of as many elements and the same strides have the same shape)
-        if any(list(map(of, tensors)) != list(map(of, out)) for of in (T.numel, _GET_DTYPE, T.stride)):
-            raise ValueError("out and the tensors differ in shape, type or strides")
-    return _norm_of(self, tensors, tensors if out is None else out, float(max_norm))
+    out = tensors if out is None else list(out)
+    if len(out) != len(tensors):
+        raise ValueError("out and the tensors differ in number")
+    return _norm_of(self, tensors, out, float(max_norm))
 
 
 def _dropout(self, x, p, seed, offset=0, by="element", out=None):

@@ -363,3 +363,121 @@ def as_products():
         dw, db = be.leaf_product_dw(c.dy, c.x, c.groups)
         got = c.grad(None, weight_out=torch.empty_like(dw), bias_out=torch.empty_like(db))
         assert torch.equal(got[0], dx) and torch.equal(got[1], dw) and torch.equal(got[2], db)
+
+
+def far_offsets():
+    """Rows whose y and z lie behind 2^31 elements and 2^32 bytes: the last ones, from torch."""
+    be = backend()
+    rows, K, H = 1100000, 16, 2048
+    gen = torch.Generator(device=DEV).manual_seed(0)
+    x = torch.randn((rows, K), generator=gen, device=DEV).bfloat16()
+    w = torch.randn((2, H, K), generator=gen, device=DEV).bfloat16()
+    leaf = torch.randint(0, 2, (rows, 1), generator=gen, device=DEV).int()
+    g = be.leaf_groups(leaf, 2)
+    y, z = be.leaf_layer(x, w, g, activation="relu", keep=True)
+    assert z.numel() > 2 ** 31
+    dx, dw, _ = be.leaf_layer_grad(y, z, x, w, g, activation="relu", bias=False)
+    for at in (0, rows // 2, rows - 300):
+        n = slice(at, at + 300)
+        want = (x[n].double()[:, None, :] @ w[leaf[n, 0].long()].double().transpose(1, 2).contiguous())[:, 0]
+        assert (z[0, n].double() - want).abs().max() <= 2 * (K + 3) * U * 16 * K
+        assert (y[n].double() - want.clamp(min=0)).abs().max() <= 2.0 ** -8 * want.abs().max()
+        # y, and dz = y where z > 0, are bfloat16 here already; dx adds 2048 of them
+        dz = torch.where(z[0, n] > 0, y[n].double(), 0.0)
+        back = (dz[:, None, :] @ w[leaf[n, 0].long()].double())[:, 0]
+        size = (dz.abs()[:, None, :] @ w[leaf[n, 0].long()].double().abs())[:, 0]
+        assert bool(((dx[n].double() - back).abs() <= 2.0 ** -8 * back.abs() + 2 * (H + 2) * U * size).all())
+
+
+def runs_of_planes():
+    """More trees than have their planes in the working memory at a time: z, y and dx against
+    the same forest, a few trees a call."""
+    be = backend()
+    rows, K, H, trees, leaves = 150000, 8, 64, 130, 3
+    gen = torch.Generator(device=DEV).manual_seed(0)
+    x = torch.randn((rows, K), generator=gen, device=DEV)
+    w = torch.randn((trees * leaves, H, K), generator=gen, device=DEV)
+    b = torch.randn((trees * leaves, H), generator=gen, device=DEV)
+    r, dy = (torch.randn((rows, H), generator=gen, device=DEV) for _ in range(2))
+    leaf = torch.randint(-1, leaves, (rows, trees), generator=gen, device=DEV).int()
+    g = be.leaf_groups(leaf, leaves)
+    assert rows * H * 4 * trees > 2 ** 32
+    y, z = be.leaf_layer(x, w, g, bias=b, activation="sigmoid", residual=r, keep=True)
+    dx, dw, db = be.leaf_layer_grad(dy, z, x, w, g, activation="sigmoid")
+    want, back = r.double(), torch.zeros((rows, K), device=DEV, dtype=torch.float64)
+    for t in range(0, trees, 13):
+        few = LeafGroups(*(v[t:t + 13].contiguous() for v in g))
+        at = slice(t * leaves, (t + 13) * leaves)
+        part, kept = be.leaf_layer(x, w[at], few, bias=b[at], activation="sigmoid", keep=True)
+        assert torch.equal(kept, z[t:t + 13])
+        dxp, dwp, dbp = be.leaf_layer_grad(dy, kept, x, w[at], few, activation="sigmoid")
+        # (a forest of fewer trees splits its leaves' rows otherwise, so dw is not bit for bit that)
+        n = torch.nonzero(leaf[:, t] == 1)[:, 0]
+        p = z[t, n].double().sigmoid()
+        dz = dy[n].double() * p * (1 - p)
+        # dz is off by slope_error's 16 U (1 + |z|) |dy| (|z| < 18 here is held at 18) and its own
+        # rounding; a chain of at most 8192 float32 adds by 2 (8192 + 2) U of the terms' size
+        off = dy[n].double().abs() * 16 * U * 19 + 5 * U * dz.abs() + 2 * (8192 + 2) * U * dz.abs()
+        assert bool(((dw[t * leaves + 1] - dz.t() @ x[n].double()).abs() <= off.t() @ x[n].double().abs()).all())
+        assert bool(((db[t * leaves + 1] - dz.sum(0)).abs() <= off.sum(0)).all())
+        want += part
+        back += dxp
+    # every part is rounded to float32 once, and so is the whole
+    assert bool(((y - want).abs() <= U * (11 * 13 + want.abs())).all())
+    scale = 11 * U * 13 * H * 6 * 6
+    assert (dx - back).abs().max() <= scale
+
+
+def streams():
+    """Calls on two streams at once, and one whose inputs another stream made."""
+    be = backend()
+    c = [Case(1500, 70, 50, 2, 5, "f32", act="gelu", seed=1), Case(900, 256, 300, 1, 3, "bf16", act="silu", gated=True, seed=2)]
+    want = [v.layer(keep=True) for v in c]
+    ways = [torch.cuda.Stream(), torch.cuda.Stream()]
+    for turn in range(5):
+        for s in ways:
+            s.wait_stream(torch.cuda.current_stream())
+        got = [None, None]
+        for i, s in enumerate(ways):
+            with torch.cuda.stream(s):
+                y, z = c[i].layer(keep=True)
+                got[i] = (y, z, *c[i].grad(z), be.grad_norm([y, z.to(y.dtype)]))
+        for s in ways:
+            torch.cuda.current_stream().wait_stream(s)
+        for i in range(2):
+            again = c[i].grad(want[i][1])
+            for a, b in zip(got[i], (*want[i], *again)):
+                assert torch.equal(a, b), (turn, i)
+
+
+def graph_of_norms():
+    """A clip captured and replayed over new gradients, long lists among them."""
+    be = backend()
+    flat = torch.zeros(300007, device=DEV)
+    ts = list(flat.split([1000] * 300 + [7]))
+    other = torch.zeros(5000, dtype=torch.bfloat16, device=DEV)
+    out = [torch.empty_like(t) for t in ts + [other]]
+    graph = torch.cuda.CUDAGraph()
+    be.clip_grads(ts + [other], 3.0, out=out)
+    torch.cuda.synchronize()
+    with torch.cuda.graph(graph):
+        norm = be.clip_grads(ts + [other], 3.0, out=out)
+    for turn in range(4):
+        flat.copy_(torch.randn(flat.shape, device=DEV) * 10.0 ** (turn - 3))
+        other.copy_(torch.randn(other.shape, device=DEV))
+        graph.replay()
+        torch.cuda.synchronize()
+        got, held = norm.clone(), [o.clone() for o in out]
+        assert torch.equal(got, be.clip_grads(ts + [other], 3.0, out=out))
+        for a, b in zip(held, out):
+            assert torch.equal(a, b), turn
+
+
+def inference():
+    """Tensors of inference mode, which have no version to count."""
+    be = backend()
+    with torch.inference_mode():
+        t = [torch.ones(10, device=DEV), torch.ones(6, device=DEV)]
+        assert float(be.clip_grads(t, 2.0)) == 4.0 and bool((t[0] == 0.5).all())
+        c = Case(50, 20, 10, act="gelu")
+        near(c.layer(out=torch.empty((50, 10), device=DEV)), c.y, c.y_off, "y")

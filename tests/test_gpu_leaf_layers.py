@@ -83,6 +83,23 @@ def test_large(check, rows, inputs, outputs, trees, leaves, dtype, shape, pad, g
     check("grads", act="silu", **args)
 
 
+# more large tiles than a round of blocks: whole rounds and what is behind them, of y (or dx, whose
+# columns are the inputs), with ends of rows and columns, rows in no leaf, two trees
+@pytest.mark.parametrize("rows,inputs,outputs,trees,leaves,dtype,shape,gated", [
+    (5200, 200, 6200, 1, 1, "bf16", "one", False), (5003, 208, 3140, 1, 3, "f16", "lost", True),
+    (2600, 200, 6200, 2, 2, "bf16", "lost", False), (2570, 200, 3200, 1, 1, "bf16", "one", True)])
+def test_rounds_of_large_tiles(check, rows, inputs, outputs, trees, leaves, dtype, shape, gated):
+    check("layer", rows=rows, inputs=inputs, outputs=outputs, trees=trees, leaves=leaves, dtype=dtype,
+          shape=shape, gated=gated, act="gelu_tanh")
+
+
+@pytest.mark.parametrize("rows,inputs,outputs,trees,leaves,dtype,shape,gated", [
+    (5200, 6200, 200, 1, 1, "bf16", "one", False), (2600, 6208, 104, 2, 2, "f16", "lost", True)])
+def test_rounds_of_large_tiles_of_dx(check, rows, inputs, outputs, trees, leaves, dtype, shape, gated):
+    check("grads", rows=rows, inputs=inputs, outputs=outputs, trees=trees, leaves=leaves, dtype=dtype,
+          shape=shape, gated=gated, act="silu")
+
+
 @pytest.mark.parametrize("trees", [1, 3])
 @pytest.mark.parametrize("gated", [False, True])
 @pytest.mark.parametrize("act", ["none", "silu", "gelu", "gelu_tanh", "sigmoid"])
@@ -122,3 +139,23 @@ def test_refused(check):
 @pytest.mark.parametrize("dtype,trees", [("f32", 1), ("bf16", 1), ("f16", 2), ("bf16", 3)])
 def test_block(check, dtype, trees):
     check("block", dtype=dtype, trees=trees)
+
+
+def test_offsets_beyond_32_bits(check):
+    check("far_offsets")
+
+
+def test_runs_of_planes(check):
+    check("runs_of_planes")
+
+
+def test_streams(check):
+    check("streams")
+
+
+def test_graph_of_norms(check):
+    check("graph_of_norms")
+
+
+def test_inference_mode(check):
+    check("inference")
