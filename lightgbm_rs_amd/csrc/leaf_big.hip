@@ -1,5 +1,5 @@
-// leaf_big.hip — the leaves' linear maps in 16 bits where leaves hold hundreds of rows and
-// wide maps: bound by the matrix cores.
+// leaf_big.hip — the leaves' linear maps and layers in 16 bits where leaves hold hundreds of rows
+// and wide maps: bound by the matrix cores.
 //
 // A block of four waves makes 256 x 256 of a result, a wave 128 x 128 of it in registers (a
 // smaller wave tile reads LDS for as long as it multiplies).  64 elements of the
@@ -15,6 +15,13 @@
 // the matrix instructions are 0.85 at full clock, LDS 0.64, and 19 us around them.  40007
 // ragged rows of 2000 in 31 leaves to 2048: 417 us, 787 TFLOP/s, six rounds of tiles of which
 // the last is 0.4 full and the leaves' ends leave a tenth empty.
+//
+// Layers: 40007 such rows to 2048 gated outputs 812 us, eleven rounds of 32 stages (62 us: the
+// clock is at 1.7 to 1.8 GHz then, and 2000 inputs are no whole lines) and about 15 us around
+// them; 16389 x 4096 to 2048 with a residual 313 us (880 TFLOP/s; a library product alone 323 to
+// 332), two rounds of 113 us for 64 stages and 25 around them, in which all blocks read the
+// residual and write at once (64 MB, 13 us at the memory's rate), and what is left over by parts,
+// 47 us.  What a layer adds to its sums is vector instructions of one wave a SIMD: 256 results a lane.
 #include <algorithm>
 #include <type_traits>
 
@@ -349,10 +356,12 @@ __global__ __launch_bounds__(THREADS, 1) void k_leaf_big(LeafProduct p, int col_
       ahead[2 * j + 1] = load_b(g, 0, j);
     }
   };
-  // A tile goes out through LDS, where the waves have read their last stage: 32 rows of a wave at
-  // a time, then eight neighbouring results a lane, by 16 bytes.  A lane has the same columns
+  // A layer's tile, and 16-bit dw, go out through LDS, where the waves have read their last stage
+  // (what slower waves still read there is of no stage): 32 rows of a wave at a time, then eight neighbouring results a lane, by 16 bytes.  A lane has the same columns
   // throughout.  before(i): loads that rows 32 i on need, kept in LDS by keep(at) and found there
-  // by end(row, at, a, u): the results of a row, and a gated layer's other factors.
+  // by end(row, at, a, u): the results of a row, and a gated layer's other factors.  A rolled loop,
+  // or registers spill: with activations in the registers' order 27 us a tile of 256 x 256 instead
+  // of 25, and 15 instead of 13 of a gated one.
   constexpr int CW = LAYER == 2 ? WN / 2 : WN, ACROSS = CW / 8, DOWN = 64 / ACROSS, TURNS = 32 / DOWN;
   constexpr int PITCH = WN + 4, STRIP = 32 * PITCH * 4, KEPT = TURNS * 1024;
   const int out_row = lane / ACROSS, out_col = (wave & 1) * CW + lane % ACROSS * 8;
@@ -456,8 +465,8 @@ __global__ __launch_bounds__(THREADS, 1) void k_leaf_big(LeafProduct p, int col_
       for (int k0 = 0; k0 < length; k0 += BK, cur ^= 1) stage(k0, lds[cur], lds[cur ^ 1]);
     }
 
-    // A lane has column lane % 32 of each 32 x 32, so that a store's lanes fill 64 or 128 bytes
-    // of a row (by 16 bytes of 64 rows, gradients of maps of 4096 x 4096 over 512 rows took 66
+    // Linear maps and float32 dw go out from the registers.  A lane has column lane % 32 of each
+    // 32 x 32, so that a store's lanes fill 64 or 128 bytes of a row (by 16 bytes of 64 rows, gradients of maps of 4096 x 4096 over 512 rows took 66
     // us instead of 32).
     if (DW) {
       const int col0 = c0 + wn + (lane & 31), row4 = (lane >> 5) * 4;
@@ -570,6 +579,7 @@ void launch_layer(const LeafProduct& p, const dim3& grid, int ct, hipStream_t s)
   switch (act_class(p.act)) {
     case ACT_LINE: k_leaf_big<T, LEAF_PRODUCT_Y, LAYER, ACT_LINE><<<grid, THREADS, 0, s>>>(p, ct, none); break;
     case ACT_ERF: k_leaf_big<T, LEAF_PRODUCT_Y, LAYER, ACT_ERF><<<grid, THREADS, 0, s>>>(p, ct, none); break;
+    case ACT_CUBIC: k_leaf_big<T, LEAF_PRODUCT_Y, LAYER, ACT_CUBIC><<<grid, THREADS, 0, s>>>(p, ct, none); break;
     default: k_leaf_big<T, LEAF_PRODUCT_Y, LAYER, ACT_SIGMOID><<<grid, THREADS, 0, s>>>(p, ct, none);
   }
 }

@@ -10,10 +10,11 @@ namespace mma {
 // exp, 1 / v and erf: the library's in float32.  Where results are rounded to 16 bits the
 // instructions' own (an ulp or two), and erf by Abramowitz and Stegun, "Handbook of
 // Mathematical Functions", 7.1.26, which is off by 1.5e-7 at most.
+constexpr float SQRT_HALF = 0.70710678f, TANH_SCALE = 0.79788456f, TANH_CUBE = 0.044715f, LOG2_E = 1.44269504f;
 template <typename T>
 __device__ __forceinline__ float exp_of(float v) {
   if constexpr (sizeof(T) == 4) return expf(v);
-  return __builtin_amdgcn_exp2f(v * 1.44269504f);
+  return __builtin_amdgcn_exp2f(v * LOG2_E);
 }
 template <typename T>
 __device__ __forceinline__ float inverse(float v) {
@@ -32,38 +33,34 @@ __device__ __forceinline__ float erf_of(float v) {
   return copysignf(1.0f - s * t * exp_of<T>(-a * a), v);
 }
 
-constexpr float SQRT_HALF = 0.70710678f, TANH_SCALE = 0.79788456f, TANH_CUBE = 0.044715f;
-
+// The sigmoid of z c, c a constant; in 16 bits the exponential's base goes into c.
 template <typename T>
-__device__ __forceinline__ float sigmoid_of(float z) {
-  return inverse<T>(1.0f + exp_of<T>(-z));
+__device__ __forceinline__ float sigmoid_of(float z, float c = 1.0f) {
+  if constexpr (sizeof(T) == 4) return 1.0f / (1.0f + expf(-(z * c)));
+  return inverse<T>(1.0f + __builtin_amdgcn_exp2f(z * (c * -LOG2_E)));
 }
 
 // Activations by the code that makes them.
-enum ActClass { ACT_LINE, ACT_SIGMOID, ACT_ERF };
+enum ActClass { ACT_LINE, ACT_SIGMOID, ACT_CUBIC, ACT_ERF };
 __host__ __device__ inline ActClass act_class(int act) {
-  return act <= LGBM_HIP_ACT_RELU ? ACT_LINE : act == LGBM_HIP_ACT_GELU ? ACT_ERF : ACT_SIGMOID;
+  if (act <= LGBM_HIP_ACT_RELU) return ACT_LINE;
+  return act == LGBM_HIP_ACT_GELU ? ACT_ERF : act == LGBM_HIP_ACT_GELU_TANH ? ACT_CUBIC : ACT_SIGMOID;
 }
 
-// N values of an activation.  SILU, GELU_TANH ((1 + tanh v) / 2 = sigmoid(2 v)) and SIGMOID are
-// sigmoids of z (c1 + c3 z^2), times z or not; the square is held back, or it would be infinite
-// where c3 is 0.
+// N values of an activation.  GELU_TANH: (1 + tanh v) / 2 = sigmoid(2 v).
 template <typename T, ActClass CLASS, int N>
 __device__ __forceinline__ void activate_as(int act, const float (&z)[N], float (&f)[N]) {
-  if (CLASS == ACT_LINE) {
-    const float least = act == LGBM_HIP_ACT_RELU ? 0.0f : -__builtin_inff();
 #pragma unroll
-    for (int i = 0; i < N; ++i) f[i] = z[i] < least ? 0.0f : z[i];  // a NaN stays
-  } else if (CLASS == ACT_ERF) {
-#pragma unroll
-    for (int i = 0; i < N; ++i) f[i] = 0.5f * z[i] * (1.0f + erf_of<T>(z[i] * SQRT_HALF));
-  } else {
-    const bool cubic = act == LGBM_HIP_ACT_GELU_TANH, alone = act == LGBM_HIP_ACT_SIGMOID;
-    const float c1 = cubic ? 2.0f * TANH_SCALE : 1.0f, c3 = cubic ? 2.0f * TANH_SCALE * TANH_CUBE : 0.0f;
-#pragma unroll
-    for (int i = 0; i < N; ++i) {
-      const float p = sigmoid_of<T>(z[i] * fmaf(c3, fminf(z[i] * z[i], 1e6f), c1));
-      f[i] = alone ? p : z[i] * p;
+  for (int i = 0; i < N; ++i) {
+    if (CLASS == ACT_LINE) {
+      f[i] = act == LGBM_HIP_ACT_RELU && z[i] < 0.0f ? 0.0f : z[i];  // a NaN stays
+    } else if (CLASS == ACT_ERF) {
+      f[i] = 0.5f * z[i] * (1.0f + erf_of<T>(z[i] * SQRT_HALF));
+    } else if (CLASS == ACT_CUBIC) {
+      f[i] = z[i] * sigmoid_of<T>(z[i] * fmaf(TANH_CUBE, z[i] * z[i], 1.0f), 2.0f * TANH_SCALE);
+    } else {
+      const float p = sigmoid_of<T>(z[i]);
+      f[i] = act == LGBM_HIP_ACT_SIGMOID ? p : z[i] * p;
     }
   }
 }
@@ -72,6 +69,7 @@ __device__ __forceinline__ void activate(int act, const float (&z)[N], float (&f
   switch (act_class(act)) {
     case ACT_LINE: return activate_as<T, ACT_LINE>(act, z, f);
     case ACT_ERF: return activate_as<T, ACT_ERF>(act, z, f);
+    case ACT_CUBIC: return activate_as<T, ACT_CUBIC>(act, z, f);
     default: activate_as<T, ACT_SIGMOID>(act, z, f);
   }
 }
