@@ -357,8 +357,8 @@ __global__ __launch_bounds__(THREADS, 1) void k_leaf_big(LeafProduct p, int col_
     }
   };
   // A layer's tile, and 16-bit dw, go out through LDS, where the waves have read their last stage
-  // (what slower waves still read there is of no stage): 32 rows of a wave at a time, then eight neighbouring results a lane, by 16 bytes.  A lane has the same columns
-  // throughout.  before(i): loads that rows 32 i on need, kept in LDS by keep(at) and found there
+  // (what slower waves still read there is of no stage): 32 rows of a wave at a time, then eight
+  // neighbouring results a lane, by 16 bytes.  A lane has the same columns throughout.  before(i): loads that rows 32 i on need, kept in LDS by keep(at) and found there
   // by end(row, at, a, u): the results of a row, and a gated layer's other factors.  A rolled loop,
   // or registers spill: with activations in the registers' order 27 us a tile of 256 x 256 instead
   // of 25, and 15 instead of 13 of a gated one.
