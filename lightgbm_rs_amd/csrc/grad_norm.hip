@@ -4,8 +4,8 @@
 // norm = sqrt(sum of g^2); out = g * min(1, most / norm).  Squares are added in float64: those of
 // float32 gradients reach over twice its exponents' range, and hundreds of millions of terms over
 // its digits.  Bound by memory: every element is read once for the norm and once more for its
-// scaling, and written once (400M elements, half of them bfloat16: 271 us, 4.4 TB/s, and 536 us, 4.5
-// TB/s, of the 4.9 that a copy reaches).
+// scaling, and written once (400M elements, half of them bfloat16: 243 us, 4.9 TB/s, and 546 us,
+// 4.4 TB/s, of the 4.9 that a copy reaches).
 //
 // The tensors' pointers go to the kernels by value, LIST of them a launch, so nothing is copied
 // to the device and a call can be captured.  A tensor is cut into chunks, a block each, whose
@@ -136,7 +136,12 @@ __global__ __launch_bounds__(FINAL) void k_norm_of_few(List l, int64_t chunk, in
   if (threadIdx.x == 0) put_norm(v, most, norm, scale);
 }
 
-template <typename T>
+// 16 bytes, as elements of 2 or 4 lie in memory.
+typedef unsigned int vec16 __attribute__((ext_vector_type(4), aligned(2)));
+
+// PASS: what is written goes by the caches, and the next kernel finds no lines in them that have
+// to be written back first.
+template <bool PASS, typename T>
 __device__ __forceinline__ void scale_chunk(const T* in, T* out, int64_t from, int64_t to, float scale) {
   constexpr int V = 16 / (int)sizeof(T), UNROLL = 4;
   if (scale == 1.0f && in == out) return;
@@ -149,7 +154,12 @@ __device__ __forceinline__ void scale_chunk(const T* in, T* out, int64_t from, i
     for (int u = 0; u < UNROLL; ++u) {
 #pragma unroll
       for (int j = 0; j < V; ++j) v[u][j] = (T)((float)v[u][j] * scale);
-      __builtin_memcpy(out + i + u * THREADS * V, v[u], 16);
+      vec16 x;
+      __builtin_memcpy(&x, v[u], 16);
+      if constexpr (PASS)
+        __builtin_nontemporal_store(x, (vec16*)(out + i + u * THREADS * V));
+      else
+        *(vec16*)(out + i + u * THREADS * V) = x;
     }
   }
   for (; i < to; i += (int64_t)THREADS * V)
@@ -157,15 +167,16 @@ __device__ __forceinline__ void scale_chunk(const T* in, T* out, int64_t from, i
 }
 
 // The chunks from the last to the first: what was read last is still in the caches.
+template <bool PASS>
 __global__ __launch_bounds__(THREADS) void k_scale(List l, int64_t chunk, const float* scale) {
   const Chunk c = chunk_of(l, gridDim.x - 1 - blockIdx.x, chunk);
   const float s = *scale;
   const void* const in = l.in[c.tensor];
   void* const out = l.out[c.tensor];
   switch (l.count[c.tensor] & 3) {
-    case 0: scale_chunk((const float*)in, (float*)out, c.from, c.to, s); break;
-    case 1: scale_chunk((const __bf16*)in, (__bf16*)out, c.from, c.to, s); break;
-    default: scale_chunk((const _Float16*)in, (_Float16*)out, c.from, c.to, s);
+    case 0: scale_chunk<PASS>((const float*)in, (float*)out, c.from, c.to, s); break;
+    case 1: scale_chunk<PASS>((const __bf16*)in, (__bf16*)out, c.from, c.to, s); break;
+    default: scale_chunk<PASS>((const _Float16*)in, (_Float16*)out, c.from, c.to, s);
   }
 }
 
@@ -226,8 +237,16 @@ void launch_grad_norm(const GradTensor* t, int64_t num, bool clip, double most, 
   });
   if (chunks >= 0) k_norm<<<1, FINAL, 0, s>>>(sums, chunks, most, norm, scale);
   if (!clip) return;
+  // past the caches where the list is more than half of the memory's cache of 256 MB (400M elements,
+  // 1.2 GB: 825 us a clip through them, 787 past them, of which the next call's k_squares has 37)
+  int64_t bytes = 0;
+  for (int64_t i = 0; i < num; ++i) bytes += t[i].count * (t[i].dtype == LGBM_HIP_DTYPE_F32 ? 4 : 2);
+  const bool pass = bytes > ((int64_t)128 << 20);
   lists(t, num, chunk, [&](const List& l, int64_t, int64_t blocks) {
-    k_scale<<<(unsigned)blocks, THREADS, 0, s>>>(l, chunk, scale);
+    if (pass)
+      k_scale<true><<<(unsigned)blocks, THREADS, 0, s>>>(l, chunk, scale);
+    else
+      k_scale<false><<<(unsigned)blocks, THREADS, 0, s>>>(l, chunk, scale);
   });
 }
 

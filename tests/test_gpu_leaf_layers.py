@@ -128,6 +128,12 @@ def test_clip(check, sizes, dtypes, flat, factor):
     check("clip", sizes=sizes, dtypes=dtypes, flat=flat, factor=factor)
 
 
+@pytest.mark.parametrize("sizes,dtypes,flat", [
+    ([40000003, 0, 5], ["f32"], False), ([70000001, 4096, 1], ["bf16"], True), ([35000001] * 2, ["f16", "f32"], False)])
+def test_clip_beyond_the_cache(check, sizes, dtypes, flat):
+    check("clip", sizes=sizes, dtypes=dtypes, flat=flat, factor=0.25)
+
+
 def test_clip_special_values(check):
     check("clip_special")
 
