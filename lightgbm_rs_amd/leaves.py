@@ -464,6 +464,14 @@ def _dense(t):
     return True
 
 
+def _alike(T, ts, us):
+    """Whether each of ts has the shape of its one of us, and the same strides where they matter."""
+    if list(map(T.size, ts)) != list(map(T.size, us)):
+        return False
+    return list(map(T.stride, ts)) == list(map(T.stride, us)) or all(
+        n == 1 or a == b for t, u in zip(ts, us) if t.numel() for n, a, b in zip(t.shape, t.stride(), u.stride()))
+
+
 def _grad_list(self, tensors, out):
     """The list as an array of `lgbm_grad`, and of the tensors of `out` (None: the norm alone) as
     their outputs.  A model has hundreds of tensors: each of these is one pass over them without
@@ -475,10 +483,10 @@ def _grad_list(self, tensors, out):
     lists = [("tensors", "in", tensors)]
     if out is not None and out is not tensors:
         lists.append(("out", "out", out))
-        # tensors without gaps of as many elements and the same strides have the same shape
-        if (count != list(map(T.numel, out)) or types != list(map(_GET_DTYPE, out))
-                or list(map(T.dim, tensors)) != list(map(T.dim, out))
-                or (max(map(T.dim, out), default=0) > 1 and list(map(T.stride, tensors)) != list(map(T.stride, out)))):
+        # tensors of one dimension without gaps and of as many elements have the same shape
+        dims = list(map(T.dim, out))
+        if (count != list(map(T.numel, out)) or types != list(map(_GET_DTYPE, out)) or list(map(T.dim, tensors)) != dims
+                or (max(dims, default=0) > 1 and not _alike(T, tensors, out))):
             raise ValueError("out and the tensors differ in shape, type or strides")
     for name, field, ts in lists:
         if not all(map(T.is_contiguous, ts)) and not all(map(_dense, ts)):

@@ -216,6 +216,17 @@ def test_python_refuses():
             call()
 
 
+def test_clip_outputs_by_shape():
+    import torch
+    be, z = Plain(), torch.zeros
+    # strides of dimensions of one element do not matter, shapes do, also where strides are the same
+    for t, out, text in [(z((1, 6)), z((6, 1)).t(), "is on cpu"), (z((3, 0, 2)), z((2, 0, 3)).permute(2, 1, 0), "is on cpu"),
+                         (z((2, 3)), z(6).as_strided((1, 6), (3, 1)), "differ"), (z((2, 3)), z((3, 2)).t(), "differ"),
+                         (z(1), z(()), "differ"), (z((6,)), z((6, 1)), "differ")]:
+        with pytest.raises(ValueError, match=text):
+            be.clip_grads([t, z(4)], 1.0, out=[out, z(4)])
+
+
 def test_python_refuses_what_autograd_would_lose():
     import torch
     be, z = Plain(), torch.zeros
