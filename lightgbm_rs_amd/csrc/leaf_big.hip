@@ -18,10 +18,10 @@
 //
 // Layers: 40007 such rows to 2048 gated outputs 812 us, eleven rounds of 32 stages (62 us: the
 // clock is at 1.7 to 1.8 GHz then, and 2000 inputs are no whole lines) and about 15 us around
-// them; 16389 x 4096 to 2048 with a residual 313 us (880 TFLOP/s; a library product alone 323 to
+// them; 16389 x 4096 to 2048 with a residual 303 us (907 TFLOP/s; a library product alone 323 to
 // 332), two rounds of 113 us for 64 stages and 25 around them, in which all blocks read the
 // residual and write at once (64 MB, 13 us at the memory's rate), and what is left over by parts,
-// 47 us.  What a layer adds to its sums is vector instructions of one wave a SIMD: 256 results a lane.
+// 37 us.  What a layer adds to its sums is vector instructions of one wave a SIMD: 256 results a lane.
 #include <algorithm>
 #include <type_traits>
 

@@ -19,7 +19,7 @@ constexpr int THREADS = 256;
 // ---- tiles through LDS ------------------------------------------------------------------------
 
 // BM rows by BN rows of a leaf's map a block (half of that many results where gated), 128 bytes
-// of the contraction a step through LDS, GM x 4 / GM waves.  Rows and columns that a tile has
+// of the contraction a step through LDS (16 bits: loaded two steps ahead), GM x 4 / GM waves.  Rows and columns that a tile has
 // more than the layer only make results that are not stored, so their loads are those of the
 // last ones; only the end of the contraction needs zeros.  The sums of 16 rows of a wave go
 // through LDS to eight neighbouring results a lane, so that z, r and y are read and written by
@@ -31,6 +31,10 @@ __global__ __launch_bounds__(THREADS) void k_layer_tile(LeafProduct p, int col_t
   constexpr int V = El<T>::V, BK = 8 * V;  // elements of the contraction a step
   constexpr int GN = 4 / GM, WM = BM / GM, WN = BN / GN, CW = GATED ? WN / 2 : WN;
   constexpr int ACH = BM * 8 / THREADS, BCH = BN * 8 / THREADS;
+  // steps between a load and its use (us by one and two: the parts behind 16389 x 4096 bfloat16 to
+  // 2048 47 and 37, 64 rows a leaf, 2048 to 2048 by 31 leaves 89 and 83; float32's, of 32 inputs,
+  // 84 and 86)
+  constexpr int AHEAD = sizeof(T) == 2 ? 2 : 1;
   constexpr int PITCH = WN + 4, STRIP = 16 * PITCH * 4;
   constexpr int STAGE = (BM + BN) * 128, LDS = 2 * STAGE > 4 * STRIP ? 2 * STAGE : 4 * STRIP;
   __shared__ __align__(16) char lds[LDS];
@@ -55,7 +59,7 @@ __global__ __launch_bounds__(THREADS) void k_layer_tile(LeafProduct p, int col_t
     for (int j = 0; j < WN / 16; ++j) acc[i][j] = f32x4{0, 0, 0, 0};
 
   if (leaf >= 0) {
-    u32x4 ra[ACH], rb[BCH];
+    u32x4 ra[AHEAD][ACH], rb[AHEAD][BCH];  // of even and odd steps
     const T *arow[ACH], *brow[BCH];
 #pragma unroll
     for (int i = 0; i < ACH; ++i)
@@ -63,38 +67,40 @@ __global__ __launch_bounds__(THREADS) void k_layer_tile(LeafProduct p, int col_t
 #pragma unroll
     for (int i = 0; i < BCH; ++i)
       brow[i] = w + (int64_t)map_row<GATED, WN>((tid + i * THREADS) >> 3, c0, cols) * length + (tid & 7) * V;
-    const auto load = [&](int k0) {
+    const auto load = [&](int k0, auto set) {
+      constexpr int S = decltype(set)::value;
       if (k0 + BK <= length) {
 #pragma unroll
-        for (int i = 0; i < ACH; ++i) ra[i] = load16(arow[i] + k0);
+        for (int i = 0; i < ACH; ++i) ra[S][i] = load16(arow[i] + k0);
 #pragma unroll
-        for (int i = 0; i < BCH; ++i) rb[i] = load16(brow[i] + k0);
+        for (int i = 0; i < BCH; ++i) rb[S][i] = load16(brow[i] + k0);
       } else if (k0 < length) {
         const int valid = length - k0 - (tid & 7) * V;
 #pragma unroll
-        for (int i = 0; i < ACH; ++i) ra[i] = load16(arow[i] + k0, valid);
+        for (int i = 0; i < ACH; ++i) ra[S][i] = load16(arow[i] + k0, valid);
 #pragma unroll
-        for (int i = 0; i < BCH; ++i) rb[i] = load16(brow[i] + k0, valid);
+        for (int i = 0; i < BCH; ++i) rb[S][i] = load16(brow[i] + k0, valid);
       }
     };
-    const auto store = [&](char* buf) {
+    const auto store = [&](char* buf, auto set) {
+      constexpr int S = decltype(set)::value;
 #pragma unroll
       for (int i = 0; i < ACH; ++i) {
         const int at = tid + i * THREADS;
-        *reinterpret_cast<u32x4*>(buf + kc_at(at >> 3, at & 7)) = ra[i];
+        *reinterpret_cast<u32x4*>(buf + kc_at(at >> 3, at & 7)) = ra[S][i];
       }
 #pragma unroll
       for (int i = 0; i < BCH; ++i) {
         const int at = tid + i * THREADS;
-        *reinterpret_cast<u32x4*>(buf + BM * 128 + kc_at(at >> 3, at & 7)) = rb[i];
+        *reinterpret_cast<u32x4*>(buf + BM * 128 + kc_at(at >> 3, at & 7)) = rb[S][i];
       }
     };
-    load(0);
-    store(lds);
-    __syncthreads();
-    for (int k0 = 0, b = 0; k0 < length; k0 += BK, b ^= 1) {
+    const std::integral_constant<int, 0> even;
+    const std::integral_constant<int, AHEAD - 1> odd;
+    // the step at k0, whose loads were `set`, in half b of the LDS
+    const auto step_at = [&](int k0, int b, auto set, auto other) {
       const bool more = k0 + BK < length;
-      load(k0 + BK);
+      load(k0 + AHEAD * BK, set);
       const char *ta = lds + b * STAGE, *tb = ta + BM * 128;
       Parts<T, WM / 16, WN / 16> part(acc);
 #pragma unroll
@@ -111,8 +117,20 @@ __global__ __launch_bounds__(THREADS) void k_layer_tile(LeafProduct p, int col_t
           for (int j = 0; j < WN / 16; ++j) part.at[i][j] = El<T>::mfma(fa[i], fb[j], part.at[i][j]);
       }
       part.add_to(acc);
-      if (more) store(lds + (b ^ 1) * STAGE);
+      if (more) store(lds + (b ^ 1) * STAGE, other);
       __syncthreads();
+    };
+    load(0, even);
+    if (AHEAD == 2) load(BK, odd);
+    store(lds, even);
+    __syncthreads();
+    if constexpr (AHEAD == 2) {
+      for (int k0 = 0; k0 < length; k0 += 2 * BK) {
+        step_at(k0, 0, even, odd);
+        if (k0 + BK < length) step_at(k0 + BK, 1, odd, even);
+      }
+    } else {
+      for (int k0 = 0, b = 0; k0 < length; k0 += BK, b ^= 1) step_at(k0, b, even, even);
     }
   }
 
