@@ -481,3 +481,28 @@ def inference():
         assert float(be.clip_grads(t, 2.0)) == 4.0 and bool((t[0] == 0.5).all())
         c = Case(50, 20, 10, act="gelu")
         near(c.layer(out=torch.empty((50, 10), device=DEV)), c.y, c.y_off, "y")
+
+
+def _of_one_input(z, dtype, outputs, inputs):
+    """x [rows, inputs] and weights [1, outputs, inputs] whose products are z [rows], exactly."""
+    x = torch.zeros((len(z), inputs), dtype=TYPES[dtype], device=DEV)
+    x[:, 0] = torch.from_numpy(z).to(DEV).to(x.dtype)
+    w = torch.zeros((1, outputs, inputs), dtype=x.dtype, device=DEV)
+    w[:, :, 0] = 1
+    return x, w
+
+
+def gelu_tails(dtype, rows, inputs, outputs):
+    """gelu and its slope relative to their values, as far as the type holds them."""
+    be, far = backend(), 5.4 if dtype == "f16" else 12.8
+    z = np.concatenate([-np.linspace(0.01, far, rows - rows // 4), np.linspace(0.0, 9.0, rows // 4)])
+    x, w = _of_one_input(np.random.default_rng(0).permutation(z), dtype, outputs, inputs)
+    g = be.leaf_groups(torch.zeros((rows, 1), dtype=torch.int32, device=DEV), 1)
+    value, off, slope, slope_off = oracle.gelu_tails(wide(x[:, 0]), dtype == "f32")
+    y = be.leaf_layer(x, w, g, activation="gelu")
+    near(y[:, 0], value, off, "gelu")
+    assert torch.equal(y, y[:, :1].expand(rows, outputs))
+    # dz itself: one output, whose map is a one
+    dx, _, _ = be.leaf_layer_grad(torch.ones_like(x[:, :1]), x[None, :, :1].contiguous(), x, w[:, :1].contiguous(), g,
+                                  activation="gelu", maps=False)
+    near(dx[:, 0], slope, slope_off, "slope")

@@ -143,3 +143,20 @@ def clip(grads, limit):
     norm = math.sqrt(math.fsum(float((g * g).sum()) for g in grads))
     scale = 1.0 if norm <= limit else limit / norm
     return norm, scale, [g * scale for g in grads]
+
+
+# The normal distribution's tails keep their digits by erfc, where 1 + erf has none left.
+_erfc = np.vectorize(math.erfc, otypes=[np.float64])
+
+
+def gelu_tails(z, wide):
+    """(gelu, its bound, its slope, its bound) of z as it is, relative to the values also far out.
+
+    P = erfc(-z / sqrt 2) / 2.  float32: z / sqrt 2 is off by 2 U, which moves erfc by 2 U (z^2 + 1)
+    at most; erfc by 16 ulp (what OpenCL asks of it), the products by a few U.  16 bits (`wide`
+    false): the polynomial by 5e-6, its roundings by 48 U, the exponential's argument by 3 U z^2 / 2 and
+    the instruction by 2 U.  The slope adds z times the density, whose argument is off as much."""
+    p = 0.5 * _erfc(-z / math.sqrt(2))
+    d = np.abs(z) * np.exp(-z * z / 2) / math.sqrt(2 * math.pi)
+    rel = (40 + 3 * z * z) * U if wide else 5e-6 + (56 + 3 * z * z) * U
+    return z * p, rel * np.abs(z * p), p + np.copysign(d, z), rel * (p + d)

@@ -165,3 +165,11 @@ def test_graph_of_norms(check):
 
 def test_inference_mode(check):
     check("inference")
+
+
+# by the kernels of few outputs, few rows, tiles of 64 x 64 and of 128 x 128, and large tiles
+@pytest.mark.parametrize("rows,inputs,outputs", [
+    (1500, 4, 3), (40, 600, 50), (700, 8, 70), (17000, 100, 256), (17000, 200, 600)])
+@pytest.mark.parametrize("dtype", ["f32", "bf16", "f16"])
+def test_gelu_tails(check, dtype, rows, inputs, outputs):
+    check("gelu_tails", dtype=dtype, rows=rows, inputs=inputs, outputs=outputs)

@@ -1,6 +1,7 @@
 """Layers of a forest's leaves and the clipping of gradients without a GPU: what the C entries
 and the Python methods refuse, the sizes of working memory, and the oracle of the GPU tests."""
 import ctypes as C
+import math
 import os
 import re
 
@@ -286,3 +287,15 @@ def test_oracle_clip():
     norm, scale, out = oracle.clip([np.array([3.0]), np.array([[0.0, -4.0]])], 2.5)
     assert norm == 5.0 and scale == 0.5 and out[1][0, 1] == -2.0
     assert oracle.clip([np.array([3.0])], 3.0)[1] == 1.0
+
+
+def test_polynomial_of_erfc():
+    """The kernels' polynomial for 16-bit types is off by 4e-8 and 5e-6 of itself at most, where float32 holds it."""
+    text = open(os.path.join(ROOT, "lightgbm_rs_amd", "csrc", "leaf_layer.h")).read()
+    rate = float(re.search(r"BELOW_RATE = ([\d.]+)f", text).group(1))
+    powers = [float(v) for v in re.findall(r"-?[\d.]+(?=f)", re.search(r"BELOW\[7\] = \{(.*?)\}", text, re.S).group(1))]
+    a = np.linspace(0.0, 9.2, 20001)
+    t = 1 / (1 + rate * a)
+    got = 2 * np.exp(-a * a) * sum(c * t ** (k + 1) for k, c in enumerate(powers))
+    want = np.array([math.erfc(v) for v in a])
+    assert len(powers) == 7 and np.abs(got - want).max() < 4e-8 and (np.abs(got - want) / want).max() < 5e-6
