@@ -108,10 +108,13 @@ __device__ __forceinline__ void slope_of(int act, float z, float& f, float& d) {
       d = p + c * 2.0f * p * (1.0f - p) * TANH_SCALE * (1.0f + 3.0f * TANH_CUBE * c * c);
       return;
     }
-    case LGBM_HIP_ACT_SIGMOID:
-      f = sigmoid_of<T>(c);
-      d = f * (1.0f - f);
+    case LGBM_HIP_ACT_SIGMOID: {
+      // 1 - f has no digits left where f is near one, e / (1 + e)^2 keeps them
+      const float e = exp_of<T>(-fabsf(c)), r = inverse<T>(1.0f + e);
+      f = c >= 0.0f ? r : e * r;
+      d = e * r * r;
       return;
+    }
     default:
       f = z;
       d = 1.0f;

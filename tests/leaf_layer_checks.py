@@ -506,3 +506,15 @@ def gelu_tails(dtype, rows, inputs, outputs):
     dx, _, _ = be.leaf_layer_grad(torch.ones_like(x[:, :1]), x[None, :, :1].contiguous(), x, w[:, :1].contiguous(), g,
                                   activation="gelu", maps=False)
     near(dx[:, 0], slope, slope_off, "slope")
+
+
+def sigmoid_slope_tails(dtype):
+    """The sigmoid's slope relative to its value, on either side, where 1 - p has few digits left or none."""
+    be, far = backend(), 15.0 if dtype == "f16" else 80.0
+    x, w = _of_one_input(np.linspace(-far, far, 2001), dtype, 1, 4)
+    g = be.leaf_groups(torch.zeros((2001, 1), dtype=torch.int32, device=DEV), 1)
+    slope, off = oracle.sigmoid_slope_tails(wide(x[:, 0]))
+    for kept in (True, x.dtype):
+        _, z = be.leaf_layer(x, w, g, activation="sigmoid", keep=kept)
+        dx, _, _ = be.leaf_layer_grad(torch.ones_like(x[:, :1]), z, x, w, g, activation="sigmoid", maps=False)
+        near(dx[:, 0], slope, off, "slope")

@@ -160,3 +160,11 @@ def gelu_tails(z, wide):
     d = np.abs(z) * np.exp(-z * z / 2) / math.sqrt(2 * math.pi)
     rel = (40 + 3 * z * z) * U if wide else 5e-6 + (56 + 3 * z * z) * U
     return z * p, rel * np.abs(z * p), p + np.copysign(d, z), rel * (p + d)
+
+
+def sigmoid_slope_tails(z):
+    """(the sigmoid's slope, its bound) of z as it is, relative to it also far out: with e = exp(-|z|) it is
+    e / (1 + e)^2, whose exponential is off by 2 U |z| (its argument) and 6 U, the quotient by a few U."""
+    e = np.exp(-np.abs(z))
+    d = e / (1 + e) ** 2
+    return d, (16 + 2 * np.abs(z)) * U * d

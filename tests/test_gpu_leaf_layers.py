@@ -173,3 +173,8 @@ def test_inference_mode(check):
 @pytest.mark.parametrize("dtype", ["f32", "bf16", "f16"])
 def test_gelu_tails(check, dtype, rows, inputs, outputs):
     check("gelu_tails", dtype=dtype, rows=rows, inputs=inputs, outputs=outputs)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16", "f16"])
+def test_sigmoid_slope_tails(check, dtype):
+    check("sigmoid_slope_tails", dtype=dtype)
