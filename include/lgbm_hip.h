@@ -858,9 +858,10 @@ int lgbm_hip_leaf_layer_grad(lgbm_hip_ctx* ctx, const lgbm_leaf_layer_grad* grad
 
 /* The 2-norm over all elements of many tensors, and the tensors scaled to a largest norm:
  *   norm = sqrt(sum of in^2);  out = in * min(1, max_norm / norm).
- * Sums are float64; norm is a float32 on the device.  A norm that is infinite gives a factor of 0
- * (infinite elements become NaN), one that is NaN a factor that is NaN.  `grads` is host memory and
- * is not read after the call. */
+ * Sums are float64.  d_norm is a float32 on the device, infinite where the norm is beyond its range;
+ * the factor is that of the norm itself, with float32's digits however small it is.  A norm that is
+ * infinite (an element is) gives a factor of 0 (infinite elements become NaN), one that is NaN a
+ * factor that is NaN.  `grads` is host memory and is not read after the call. */
 typedef struct lgbm_grad {
   const void* d_in; /* count elements without gaps */
   void* d_out;      /* clip: may be d_in; overlaps nothing else.  norm: not used */

@@ -111,16 +111,32 @@ __global__ __launch_bounds__(THREADS) void k_squares(List l, int64_t chunk, doub
   if (threadIdx.x == 0) sums[blockIdx.x] = v;
 }
 
-__device__ __forceinline__ void put_norm(double sum, double most, float* norm, float* scale) {
+// What a gradient is multiplied by: first by one factor, then by the other.  The second is 1 unless
+// the scale is below float32's normal numbers, where a single factor would have few digits or none;
+// the product with the first is then in their range wherever that with both is not zero.
+struct Scale {
+  float first, second;
+};
+
+__device__ __forceinline__ void put_norm(double sum, double most, float* norm, Scale* scale) {
   const double v = sqrt(sum);
   *norm = (float)v;
+  if (!scale) return;
   // a norm that is NaN gives a scale that is
-  if (scale) *scale = v <= most ? 1.0f : (float)(most / v);
+  const double s = v <= most ? 1.0 : most / v;
+  Scale of{(float)s, 1.0f};
+  if (s > 0.0 && s < 0x1p-126) {
+    int e;
+    const double m = frexp(s, &e);  // (a scale below 2^-300 makes zeros of all that float32 holds)
+    const int half = max(e, -300) / 2;
+    of = {(float)ldexp(m, e - half), ldexpf(1.0f, half)};
+  }
+  *scale = of;
 }
 
 // The norm, and the scale in front of the sums.
 __global__ __launch_bounds__(FINAL) void k_norm(const double* sums, int64_t n, double most, float* norm,
-                                                float* scale) {
+                                                Scale* scale) {
   double v = 0;
   for (int64_t i = threadIdx.x; i < n; i += FINAL) v += sums[i];
   v = block_sum<FINAL>(v);
@@ -129,7 +145,7 @@ __global__ __launch_bounds__(FINAL) void k_norm(const double* sums, int64_t n, d
 
 // Both for a list of few chunks: one block, whose parts of THREADS take a chunk each.
 __global__ __launch_bounds__(FINAL) void k_norm_of_few(List l, int64_t chunk, int chunks, double most, float* norm,
-                                                       float* scale) {
+                                                       Scale* scale) {
   double v = 0;
   for (int i = threadIdx.x / THREADS; i < chunks; i += FINAL / THREADS) v += squares_of(l, i, chunk);
   v = block_sum<FINAL>(v);
@@ -142,9 +158,9 @@ typedef unsigned int vec16 __attribute__((ext_vector_type(4), aligned(2)));
 // PASS: what is written goes by the caches, and the next kernel finds no lines in them that have
 // to be written back first.
 template <bool PASS, typename T>
-__device__ __forceinline__ void scale_chunk(const T* in, T* out, int64_t from, int64_t to, float scale) {
+__device__ __forceinline__ void scale_chunk(const T* in, T* out, int64_t from, int64_t to, Scale scale) {
   constexpr int V = 16 / (int)sizeof(T), UNROLL = 4;
-  if (scale == 1.0f && in == out) return;
+  if (scale.first == 1.0f && in == out) return;
   int64_t i = from + threadIdx.x * V;
   for (; i + (UNROLL - 1) * (int64_t)THREADS * V + V <= to; i += UNROLL * (int64_t)THREADS * V) {
     T v[UNROLL][V];
@@ -153,7 +169,7 @@ __device__ __forceinline__ void scale_chunk(const T* in, T* out, int64_t from, i
 #pragma unroll
     for (int u = 0; u < UNROLL; ++u) {
 #pragma unroll
-      for (int j = 0; j < V; ++j) v[u][j] = (T)((float)v[u][j] * scale);
+      for (int j = 0; j < V; ++j) v[u][j] = (T)((float)v[u][j] * scale.first * scale.second);
       vec16 x;
       __builtin_memcpy(&x, v[u], 16);
       if constexpr (PASS)
@@ -163,14 +179,14 @@ __device__ __forceinline__ void scale_chunk(const T* in, T* out, int64_t from, i
     }
   }
   for (; i < to; i += (int64_t)THREADS * V)
-    for (int j = 0; j < V && i + j < to; ++j) out[i + j] = (T)((float)in[i + j] * scale);
+    for (int j = 0; j < V && i + j < to; ++j) out[i + j] = (T)((float)in[i + j] * scale.first * scale.second);
 }
 
 // The chunks from the last to the first: what was read last is still in the caches.
 template <bool PASS>
-__global__ __launch_bounds__(THREADS) void k_scale(List l, int64_t chunk, const float* scale) {
+__global__ __launch_bounds__(THREADS) void k_scale(List l, int64_t chunk, const Scale* scale) {
   const Chunk c = chunk_of(l, gridDim.x - 1 - blockIdx.x, chunk);
-  const float s = *scale;
+  const Scale s = *scale;
   const void* const in = l.in[c.tensor];
   void* const out = l.out[c.tensor];
   switch (l.count[c.tensor] & 3) {
@@ -221,7 +237,7 @@ void launch_grad_norm(const GradTensor* t, int64_t num, bool clip, double most, 
   int64_t total = 0;
   for (int64_t i = 0; i < num; ++i) total += t[i].count;
   const int64_t chunk = chunk_size(total);
-  float* const scale = clip ? (float*)ws : nullptr;
+  Scale* const scale = clip ? (Scale*)ws : nullptr;
   double* const sums = (double*)ws + 2;
   int64_t chunks = 0;
   int64_t most_chunks = 0;

@@ -518,3 +518,22 @@ def sigmoid_slope_tails(dtype):
         _, z = be.leaf_layer(x, w, g, activation="sigmoid", keep=kept)
         dx, _, _ = be.leaf_layer_grad(torch.ones_like(x[:, :1]), z, x, w, g, activation="sigmoid", maps=False)
         near(dx[:, 0], slope, off, "slope")
+
+
+def clip_beyond_float32():
+    """Finite gradients whose norm float32 does not hold, and scales below its normal numbers."""
+    be = backend()
+    for sizes, value, dtypes in (([4], 3e38, ["f32"]), ([300000, 7], 3e38, ["f32", "bf16"]), ([100], 1e38, ["bf16"]),
+                                 ([5000], 1.0, ["f32"])):
+        for limit in (1.0, 1e-3, 1e-12, 1e-30, 1e-38, 3e-41):
+            ts = [torch.full((n,), value, device=DEV).to(TYPES[dtypes[i % len(dtypes)]]) for i, n in enumerate(sizes)]
+            ts[0][0] = -value / 3
+            norm, _, want = oracle.clip([wide(t) for t in ts], limit)
+            out = [torch.empty_like(t) for t in ts]
+            got = float(be.clip_grads(ts, limit, out=out))
+            assert got == math.inf if norm > 3.5e38 else abs(got - norm) <= 2 * U * norm, (got, norm)
+            for o, w in zip(out, want):
+                # the scale's rounding, the product's and, where that is subnormal, the first factor's
+                near(o, w, 3 * U * np.abs(w), (value, limit))
+            be.clip_grads(ts, limit)
+            assert all(torch.equal(t, o) for t, o in zip(ts, out))

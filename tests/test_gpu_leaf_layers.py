@@ -178,3 +178,7 @@ def test_gelu_tails(check, dtype, rows, inputs, outputs):
 @pytest.mark.parametrize("dtype", ["f32", "bf16", "f16"])
 def test_sigmoid_slope_tails(check, dtype):
     check("sigmoid_slope_tails", dtype=dtype)
+
+
+def test_clip_beyond_float32(check):
+    check("clip_beyond_float32")
