@@ -8,7 +8,8 @@ device and returns, so calls follow each other like torch's own operations and c
 captured into a graph.  Gradients are entries of their own: nothing is recorded for
 torch's autograd, so a floating-point tensor that requires gradients is refused while they are
 recorded (call under torch.no_grad(), as the methods of a torch.autograd.Function are, or
-on detached tensors).
+on detached tensors).  So is one with a tangent of forward-mode differentiation, which
+torch.no_grad() does not turn off (detach it, or call from such a method).
 
 Import torch before the first `HipBackend`: torch brings a HIP runtime of its own, which
 the library then shares.  (The other way round torch finds no device.)
@@ -138,11 +139,25 @@ def _dtype(t, what, double=False):
     return code
 
 
+def _tangents():
+    """Whether tensors may have a tangent: inside forward-mode differentiation."""
+    return getattr(_torch.autograd.forward_ad, "_current_level", 0) >= 0
+
+
+def _has_tangent(t):
+    return _torch.autograd.forward_ad.unpack_dual(t).tangent is not None
+
+
 def _here(self, **tensors):
-    """Every tensor on the backend's device, and none that autograd would have to record."""
+    """Every tensor on the backend's device, and none that autograd would have to record or to
+    carry a tangent through."""
     for name, t in tensors.items():
         if t is not None and t.requires_grad and _torch.is_grad_enabled():
             raise ValueError(f"{name} requires gradients, which this call does not record")
+    if _tangents():
+        for name, t in tensors.items():
+            if t is not None and _has_tangent(t):
+                raise ValueError(f"{name} has a tangent, which this call does not carry on")
     for name, t in tensors.items():
         if t is not None and (not t.is_cuda or t.get_device() != self.device):
             raise ValueError(f"{name} is on {t.device}: cuda:{self.device} is needed")
@@ -493,6 +508,8 @@ def _grad_list(self, tensors, out):
             raise ValueError(f"a tensor of {name} has gaps")
         if torch.is_grad_enabled() and any(map(_GET_REQUIRES_GRAD, ts)):
             raise ValueError(f"a tensor of {name} requires gradients, which this call does not record")
+        if _tangents() and any(map(_has_tangent, ts)):
+            raise ValueError(f"a tensor of {name} has a tangent, which this call does not carry on")
         for d in set(map(T.get_device, ts)):
             if d != self.device:
                 raise ValueError(f"a tensor of {name} is on {'cpu' if d < 0 else f'cuda:{d}'}: "

@@ -299,3 +299,44 @@ def test_polynomial_of_erfc():
     got = 2 * np.exp(-a * a) * sum(c * t ** (k + 1) for k, c in enumerate(powers))
     want = np.array([math.erfc(v) for v in a])
     assert len(powers) == 7 and np.abs(got - want).max() < 4e-8 and (np.abs(got - want) / want).max() < 5e-6
+
+
+def test_python_refuses_tangents():
+    """Forward-mode differentiation would go on without the tangent of the output: refused, also under
+    no_grad, which does not turn it off; the primal, and what a Function's methods get, go on."""
+    import torch
+    from torch.autograd import forward_ad
+    be, z = Plain(), torch.zeros
+    g = LeafGroups(*(z(s, dtype=torch.int32) for s in ((1, 6), (1, 4), (1, 4))))
+    calls = [(lambda x, w, dy: be.leaf_layer(x, w, g), "x"), (lambda x, w, dy: be.leaf_layer(x, w, g), "w"),
+             (lambda x, w, dy: be.leaf_layer(x, w, g, residual=dy), "dy"),
+             (lambda x, w, dy: be.leaf_layer_grad(dy, None, x, w, g), "dy"),
+             (lambda x, w, dy: be.leaf_layer_grad(dy, dy[None], x, w, g, activation="silu"), "x"),
+             (lambda x, w, dy: be.grad_norm([x, dy]), "dy"), (lambda x, w, dy: be.clip_grads([w], 1.0), "w"),
+             (lambda x, w, dy: be.clip_grads([w], 1.0, out=[z((4, 2, 5))]), "w"),
+             (lambda x, w, dy: be.leaf_product(x, w, g), "x"), (lambda x, w, dy: be.leaf_product_dx(dy, w, g), "w"),
+             (lambda x, w, dy: be.leaf_product_dw(dy, x, g), "x"), (lambda x, w, dy: be.dropout(x, 0.5, 1), "x"),
+             (lambda x, w, dy: be.dropout(x[:, 0], 0.5, 1), "x"), (lambda x, w, dy: be.adjust_scores(x, bias=w[0, 0]), "w")]
+
+    class Through(torch.autograd.Function):
+        @staticmethod
+        def forward(ctx, call, x, w, dy):
+            call(x, w, dy)
+
+    for call, name in calls:
+        t = {"x": z((6, 5)), "w": z((4, 2, 5)), "dy": z((6, 2))}
+        with forward_ad.dual_level():
+            with pytest.raises(ValueError, match="is on cpu"):
+                call(**t)
+            t[name] = forward_ad.make_dual(t[name], torch.ones_like(t[name]))
+            with pytest.raises(ValueError, match="has a tangent"):
+                call(**t)
+            with torch.no_grad(), pytest.raises(ValueError, match="has a tangent"):
+                call(**t)
+            with pytest.raises(ValueError, match="is on cpu"):
+                Through.apply(call, t["x"], t["w"], t["dy"])
+            with pytest.raises(ValueError, match="is on cpu"):
+                call(**{k: v.detach() for k, v in t.items()})
+            t[name] = forward_ad.unpack_dual(t[name]).primal
+            with pytest.raises(ValueError, match="is on cpu"):
+                call(**t)
