@@ -137,8 +137,9 @@ template <typename T, int MODE, int LAYER = 0, ActClass CLASS = ACT_LINE, bool N
 __global__ __launch_bounds__(THREADS, 1) void k_leaf_big(LeafProduct p, int col_tiles, Split split) {
   constexpr bool DW = MODE == LEAF_PRODUCT_DW, ACM = DW, BCM = MODE != LEAF_PRODUCT_Y;
   constexpr int FM = WM / 32, FN = WN / 32, STEPS = BK / 16, ITEMS = STEPS * FM, RING = 4;
-  // dx is slower so (16389 rows of 2048 to 2048, two trees of 15 leaves: 379 us, 397 by EARLY)
-  constexpr bool EARLY = MODE == LEAF_PRODUCT_Y;
+  // the linear maps are slower so, since registers spill: dx of 16389 rows of 2048 to 2048, two trees
+  // of 15 leaves, 379 us and 397 by EARLY, y of 300000 rows of 256 to 256 by two leaves 121 and 128
+  constexpr bool EARLY = MODE == LEAF_PRODUCT_Y && LAYER != 0;
   constexpr int TURN = ITEMS - 2, CB = LAYER == 2 ? BN / 2 : BN;
   __shared__ __align__(1024) char lds[2][STAGE];
   __shared__ int32_t row_of[EARLY ? 2 : 1][DW ? 1 : BM];
