@@ -60,7 +60,7 @@ def test_grads(check, shape, dtype, gated):
           shape=sizes, pad=pad, act=ACTS[(i + 2 * gated) % 6], gated=gated, kept="narrow" if i % 5 == 0 else None)
 
 
-# every activation by every kernel
+# every activation by the kernels of few outputs, of few rows and of 64 x 64 tiles (the others: below)
 @pytest.mark.parametrize("gated", [False, True])
 @pytest.mark.parametrize("act", ACTS)
 @pytest.mark.parametrize("dtype", ["f32", "bf16"])
@@ -182,3 +182,44 @@ def test_sigmoid_slope_tails(check, dtype):
 
 def test_clip_beyond_float32(check):
     check("clip_beyond_float32")
+
+
+# the forms of the kernels between those: two groups of rows a leaf of few rows, 17 to 32 outputs of many
+# rows, and 128 x 128 tiles of 16-bit types (rows off 16 bytes, or inputs that are no whole ones)
+FORMS = [(200, 600, 50, 1, 8, "even", 0), (250, 520, 130, 2, 9, "lost", 1), (700, 60, 24, 1, 3, "skew", 0),
+         (900, 100, 32, 3, 4, "lost", 3), (9000, 130, 512, 1, 2, "skew", 1), (4700, 72, 520, 2, 3, "lost", 3)]
+
+
+@pytest.mark.parametrize("gated", [False, True])
+@pytest.mark.parametrize("dtype", ["f32", "bf16", "f16"])
+@pytest.mark.parametrize("shape", FORMS)
+def test_forms(check, shape, dtype, gated):
+    i = FORMS.index(shape)
+    rows, inputs, outputs, trees, leaves, sizes, pad = shape
+    args = dict(rows=rows, inputs=inputs, outputs=outputs // 2 if gated and outputs > 500 else outputs, trees=trees,
+                leaves=leaves, dtype=dtype, shape=sizes, pad=pad, gated=gated)
+    for act in (ACTS[i], ACTS[(i + 3) % 6]):
+        check("layer", act=act, residual=i % 3 != 1, bias=i % 4 != 3, **args)
+    check("grads", act=ACTS[(i + 2) % 6], kept="narrow" if i % 2 else None, **args)
+
+
+# large tiles: y, z and the gradients of every activation, alone, beside a residual, and of two trees
+@pytest.mark.parametrize("gated", [False, True])
+@pytest.mark.parametrize("act", ACTS)
+@pytest.mark.parametrize("dtype", ["bf16", "f16"])
+def test_large_by_activation(check, dtype, act, gated):
+    i = ACTS.index(act) + gated
+    args = dict(rows=5000, inputs=200, outputs=520 if gated else 1032, dtype=dtype, act=act, gated=gated, pad=i % 2 * 8)
+    check("layer", leaves=2, shape="skew", residual=i % 2 == 0, bias=i % 3 != 1, **args)
+    check("grads", leaves=2, shape="lost", **args)
+    check("layer", trees=2, leaves=3, shape="lost", **dict(args, rows=2500))
+
+
+# the large cases above whose gradients begin from silu's z: that z, and y
+@pytest.mark.parametrize("gated", [False, True])
+@pytest.mark.parametrize("rows,inputs,outputs,trees,leaves,dtype,shape,pad", [
+    (4000, 256, 1024, 1, 2, "bf16", "skew", 0), (9001, 264, 520, 1, 3, "f16", "lost", 8),
+    (3000, 328, 776, 2, 3, "bf16", "even", 0), (2600, 1000, 1288, 1, 1, "f16", "lost", 8)])
+def test_large_silu(check, rows, inputs, outputs, trees, leaves, dtype, shape, pad, gated):
+    check("layer", rows=rows, inputs=inputs, outputs=outputs, trees=trees, leaves=leaves, dtype=dtype,
+          shape=shape, pad=pad, gated=gated, act="silu", residual=not gated)
