@@ -214,14 +214,22 @@ __device__ int count_tiles(const LeafGroups& g, int tree, int bm) {
 }
 
 // Large tiles of 256 x 256 are made in rounds of a launch's BIG_BLOCKS blocks.  The tiles behind
-// the last whole round, where they are half a round at most, are better made by PARTS x PARTS
-// blocks each, which that round has CUs for: how many tiles are made in rounds.
+// the last whole round, where they are a quarter of a round at most, are better made by PARTS x PARTS
+// blocks each, which that round has CUs for: how many tiles are made in rounds.  (us, bfloat16, 2048
+// inputs to 2048 by one leaf, one whole round and more; all by large tiles, and the rest by parts)
+//   tiles behind     a layer       a gated one    dx
+//     8 to 32     133, 101..105    121, 96..98    129, 107..113
+//          48     132, 111         121, 105       130, 114
+//          64     133, 117         121, 111       130, 117
+//          80     133, 128         121, 123       131, 146
+//         128     133, 148         121, 142       131, 151
 constexpr int BIG_ROWS = 256, BIG_BLOCKS = 256, PARTS = 4, PART_ROWS = BIG_ROWS / PARTS;
+constexpr int MOST_REST = BIG_BLOCKS / 4;
 __host__ __device__ inline int in_rounds(int tiles) {
   const int rest = tiles % BIG_BLOCKS;
-  return tiles > BIG_BLOCKS && rest <= BIG_BLOCKS / 2 ? tiles - rest : tiles;
+  return tiles > BIG_BLOCKS && rest <= MOST_REST ? tiles - rest : tiles;
 }
-constexpr int REST_BLOCKS = BIG_BLOCKS / 2 * PARTS * PARTS;  // of a tree
+constexpr int REST_BLOCKS = MOST_REST * PARTS * PARTS;  // of a tree
 // The rows and the first column of a block's part of such a tile of PARTS times `cols` columns, of
 // which a row of tiles has col_tiles; rows 0: there is none.
 template <int THREADS>

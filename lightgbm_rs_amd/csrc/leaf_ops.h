@@ -52,7 +52,8 @@ struct LeafProduct {
   // ws, to be added, instead of to out
   bool planes;
   // layer, and dx of its gradient: whether the large tiles behind their last whole round go to
-  // smaller ones
+  // smaller ones (not product and dx of the linear maps, whose results stay what they were: smaller
+  // tiles add in another order)
   bool rest;
   // layer: out[n] = res[n] + sum over trees of act(z), or of act(z's first half) times its
   // second half where gated; z = W x + b has map_rows() elements, `outputs` those of the layer

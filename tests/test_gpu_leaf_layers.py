@@ -223,3 +223,15 @@ def test_large_by_activation(check, dtype, act, gated):
 def test_large_silu(check, rows, inputs, outputs, trees, leaves, dtype, shape, pad, gated):
     check("layer", rows=rows, inputs=inputs, outputs=outputs, trees=trees, leaves=leaves, dtype=dtype,
           shape=shape, pad=pad, gated=gated, act="silu", residual=not gated)
+
+
+# as many tiles behind a whole round as go to smaller ones, the next number that does not, and an end of one row
+@pytest.mark.parametrize("rows,inputs,outputs,gated", [
+    (5120, 200, 4096, False), (5376, 200, 4096, False), (5121, 200, 2040, True), (5120, 208, 2048, True)])
+def test_rounds_to_their_limit(check, rows, inputs, outputs, gated):
+    check("layer", rows=rows, inputs=inputs, outputs=outputs, dtype="bf16", shape="one", gated=gated, act="silu")
+
+
+@pytest.mark.parametrize("rows", [5120, 5376])
+def test_rounds_of_dx_to_their_limit(check, rows):
+    check("grads", rows=rows, inputs=4096, outputs=200, dtype="f16", shape="one", act="gelu")
