@@ -802,7 +802,9 @@ int lgbm_hip_leaf_product_dw(lgbm_hip_ctx* ctx, const lgbm_leaf_maps* maps, cons
  * in float32 and rounded once, with f the activation, or gated f = the activation of the first
  * `outputs` elements of z times its other `outputs`.  A tree that has a row in no leaf adds
  * nothing to it.  RELU max(z, 0); SILU z / (1 + exp(-z)); GELU z (1 + erf(z / sqrt 2)) / 2;
- * GELU_TANH z (1 + tanh(sqrt(2 / pi) (z + 0.044715 z^3))) / 2; SIGMOID 1 / (1 + exp(-z)). */
+ * GELU_TANH z (1 + tanh(sqrt(2 / pi) (z + 0.044715 z^3))) / 2; SIGMOID 1 / (1 + exp(-z)).  Where
+ * float32 holds z as minus infinity SILU and both GELUs are NaN, as these formulas are; their slopes
+ * there, and where a kept 16-bit z is infinite, are those of the limits. */
 #define LGBM_HIP_ACT_NONE 0
 #define LGBM_HIP_ACT_RELU 1
 #define LGBM_HIP_ACT_SILU 2

@@ -4,8 +4,8 @@
 // norm = sqrt(sum of g^2); out = g * min(1, most / norm).  Squares are added in float64: those of
 // float32 gradients reach over twice its exponents' range, and hundreds of millions of terms over
 // its digits.  Bound by memory: every element is read once for the norm and once more for its
-// scaling, and written once (400M elements, half of them bfloat16: 243 us, 4.9 TB/s, and 546 us,
-// 4.4 TB/s, of the 4.9 that a copy reaches).
+// scaling, and written once (400M elements, half of them bfloat16, to other tensors: 243 us, 4.9
+// TB/s, and 546 us, 4.4 TB/s, of the 4.9 that a copy reaches).
 //
 // The tensors' pointers go to the kernels by value, LIST of them a launch, so nothing is copied
 // to the device and a call can be captured.  A tensor is cut into chunks, a block each, whose
@@ -182,7 +182,8 @@ __device__ __forceinline__ void scale_chunk(const T* in, T* out, int64_t from, i
     for (int j = 0; j < V && i + j < to; ++j) out[i + j] = (T)((float)in[i + j] * scale.first * scale.second);
 }
 
-// The chunks from the last to the first: what was read last is still in the caches.
+// The chunks of a launch from the last to the first: what a list of one launch read last is still in
+// the caches.  (Lists of more than LIST tensors are several launches, which go forward.)
 template <bool PASS>
 __global__ __launch_bounds__(THREADS) void k_scale(List l, int64_t chunk, const Scale* scale) {
   const Chunk c = chunk_of(l, gridDim.x - 1 - blockIdx.x, chunk);
@@ -196,7 +197,10 @@ __global__ __launch_bounds__(THREADS) void k_scale(List l, int64_t chunk, const 
   }
 }
 
-// Elements a chunk: a list in about 4096 of them, whole turns of a block's vectors.
+// Elements a chunk: a list in about 4096 of them, multiples of a float32 turn of a block's vectors.
+// In 16 bits a turn is twice that: where chunks are odd multiples, as in all lists of up to 16.8M
+// elements, the last half turn of each goes through the loops' ends, which k_scale makes by single
+// elements (10M bfloat16: 8.3 and 21.1 us; 10M float32, twice the bytes, 8.7 and 13.5).
 int64_t chunk_size(int64_t total) {
   constexpr int64_t TURN = THREADS * 16;
   return std::max<int64_t>(TURN, (total / 4096 + TURN - 1) / TURN * TURN);
@@ -253,8 +257,11 @@ void launch_grad_norm(const GradTensor* t, int64_t num, bool clip, double most, 
   });
   if (chunks >= 0) k_norm<<<1, FINAL, 0, s>>>(sums, chunks, most, norm, scale);
   if (!clip) return;
-  // past the caches where the list is more than half of the memory's cache of 256 MB (400M elements,
-  // 1.2 GB: 825 us a clip through them, 787 past them, of which the next call's k_squares has 37)
+  // past the caches where the list is more than half of the memory's cache of 256 MB (us of k_squares
+  // and k_scale, eight float32 tensors to others, through the caches and past them: 96 MB 45.3 and
+  // 44.6, 128 MB 58.5 and 57.9, 160 MB 76.5 and 71.8, 256 MB 138 and 113, 768 MB 425 and 400, most of it
+  // the next call's k_squares; in place, where stores hit lines that were just read, it is all one: 160
+  // MB 72.4 and 72.4, 384 MB 187 and 185, 768 MB 428 and 425)
   int64_t bytes = 0;
   for (int64_t i = 0; i < num; ++i) bytes += t[i].count * (t[i].dtype == LGBM_HIP_DTYPE_F32 ? 4 : 2);
   const bool pass = bytes > ((int64_t)128 << 20);

@@ -359,10 +359,11 @@ __global__ __launch_bounds__(THREADS, 1) void k_leaf_big(LeafProduct p, int col_
   };
   // A layer's tile, and 16-bit dw, go out through LDS, where the waves have read their last stage
   // (what slower waves still read there is of no stage): 32 rows of a wave at a time, then eight
-  // neighbouring results a lane, by 16 bytes.  A lane has the same columns throughout.  before(i): loads that rows 32 i on need, kept in LDS by keep(at) and found there
-  // by end(row, at, a, u): the results of a row, and a gated layer's other factors.  A rolled loop,
-  // or registers spill: with activations in the registers' order 27 us a tile of 256 x 256 instead
-  // of 25, and 15 instead of 13 of a gated one.
+  // neighbouring results a lane, by 16 bytes.  A lane has the same columns throughout.
+  // before(i): loads that rows 32 i on need, kept in LDS by keep(at) and found there by end(row,
+  // at, a, u): the results of a row, and a gated layer's other factors.  A rolled loop, or registers
+  // spill: with activations in the registers' order 27 us a tile of 256 x 256 instead of 25, and 15
+  // instead of 13 of a gated one.
   constexpr int CW = LAYER == 2 ? WN / 2 : WN, ACROSS = CW / 8, DOWN = 64 / ACROSS, TURNS = 32 / DOWN;
   constexpr int PITCH = WN + 4, STRIP = 32 * PITCH * 4, KEPT = TURNS * 1024;
   const int out_row = lane / ACROSS, out_col = (wave & 1) * CW + lane % ACROSS * 8;
@@ -467,8 +468,8 @@ __global__ __launch_bounds__(THREADS, 1) void k_leaf_big(LeafProduct p, int col_
     }
 
     // Linear maps and float32 dw go out from the registers.  A lane has column lane % 32 of each
-    // 32 x 32, so that a store's lanes fill 64 or 128 bytes of a row (by 16 bytes of 64 rows, gradients of maps of 4096 x 4096 over 512 rows took 66
-    // us instead of 32).
+    // 32 x 32, so that a store's lanes fill 64 or 128 bytes of a row (by 16 bytes of 64 rows,
+    // gradients of maps of 4096 x 4096 over 512 rows took 66 us instead of 32).
     if (DW) {
       const int col0 = c0 + wn + (lane & 31), row4 = (lane >> 5) * 4;
 #pragma unroll
